@@ -42,6 +42,15 @@ typedef enum mk_status {
 #define MK_FLAG_HISTORY_FULL      0x100u /* mk_decode_commit: the row's history buffer is full, the token was not appended;
                                            sampling: history_len[b] exceeded min(history_ld, 65535) and was clamped to it */
 
+#define MK_FLAG_PLAN_INVALID      0x200u /* mk_kv_plan_step: a length, a count of pages or the table's width is out of range */
+#define MK_FLAG_NO_ROOM           0x400u /* mk_kv_plan_step: the step's tokens passed max_tokens, the sequence sits this one out */
+#define MK_FLAG_NO_PAGES          0x800u /* mk_kv_plan_step: not enough free pages, the sequence sits this one out */
+
+/* Types of the arrays that may hold other than fp32. */
+#define MK_FP32 0
+#define MK_BF16 1
+#define MK_FP16 2
+
 /* Field for field mako::gen::SamplingParams (src/gen/sampler.hpp:12-20). temperature <= 0 selects greedy. */
 typedef struct mk_sampling_params {
     float temperature;
@@ -246,6 +255,104 @@ int mk_rank_force(mk_sampler* s, const float* logits, uint64_t ld, uint32_t batc
 int mk_decode_commit(mk_sampler* s, uint32_t batch, const int32_t* sampled, const int32_t* forced, int32_t* history,
                      uint64_t history_ld, uint32_t history_cap, int32_t* history_len, int32_t* next_input,
                      int32_t* committed, uint32_t* flags, void* stream);
+
+/* ---- the round around the sampler (no counterpart in the reference, whose engines run on another device) ---------------- */
+
+/* A language model's head and the low-rank adapters that requests bring to it. weight, down, up and the hidden states are of
+ * one type, MK_BF16 or MK_FP16, start on 16-byte boundaries and are contiguous; dim and rank are multiples of 8. */
+typedef struct mk_head {
+    const void* weight; /* device [n_vocab][dim] */
+    const void* down;   /* device [n_adapters][rank][dim]; unread where n_adapters == 0 */
+    const void* up;     /* device [n_adapters][n_vocab][rank] */
+    const float* scale; /* device [n_adapters], or NULL: 1 each */
+    uint32_t n_vocab, dim;
+    uint32_t n_adapters, rank; /* rank <= 128 */
+    int type;
+} mk_head;
+
+/* The rows that the sampler reads, from the hidden states behind the model's last norm:
+ *   logits[t][v] = sum_k weight[v][k] hidden[t][k] + scale[a] sum_r up[a][v][r] (sum_k down[a][r][k] hidden[t][k]),  a = adapter[t].
+ * adapter [rows] names each row's adapter, in any order; one outside [0, n_adapters) and a NULL array mean none. Products are
+ * exact, sums are in fp32, the inner sums stay in fp32 between the two projections. rows is at most the handle's max_batch,
+ * n_vocab at most its n_vocab; hidden_ld is a multiple of 8; columns behind n_vocab of a logits row are left as they are. No
+ * row's values reach another row. Calls on one handle must not overlap (they share its scratch). */
+int mk_head_logits(mk_sampler* s, const mk_head* head, const void* hidden, uint64_t hidden_ld, const int32_t* adapter,
+                   uint32_t rows, float* logits, uint64_t ld, void* stream);
+
+/* A speculative round of n_seq sequences of up to n_pos - 1 drafts each, as mk_sampler_spec_round lays it out: row
+ * s*n_pos + j of logits is the target's after the drafts before j, row s*(n_pos - 1) + j of draft_logits the drafter's that
+ * drafts[s][j] was drawn from. All of these rows are of one type, MK_FP32, MK_BF16 or MK_FP16, and start at any element. */
+typedef struct mk_spec_rows {
+    const void* logits;            /* device [n_seq * n_pos][ld] */
+    uint64_t ld;
+    const void* draft_logits;      /* device [n_seq * (n_pos - 1)][draft_ld], or NULL: the drafts are certain (lookup, argmax) */
+    uint64_t draft_ld;
+    int type;
+    uint32_t n_seq, n_pos, n_vocab;
+    const int32_t* drafts;         /* device [n_seq][n_pos - 1]; the first one outside [0, n_vocab) ends its sequence's drafts */
+    const float* u;                /* device [n_seq][n_pos + 1], the uniforms as mk_sampler_spec_round takes them */
+    const float* temperature;      /* device [n_seq], or NULL: temperature_all. Not above 0: the largest logit alone, lowest id */
+    const float* draft_temperature;/* device [n_seq], or NULL: the target's */
+    float temperature_all;
+    const uint32_t* mask;          /* device [n_seq * n_pos][mask_ld] allowed tokens of the target's rows, or NULL */
+    uint64_t mask_ld;
+    int mask_drafts;               /* not 0: the drafter's row of a position drew under the same mask */
+} mk_spec_rows;
+
+/* Verifies a round against whole distributions, untruncated ones included (mk_sampler_verify_pq_batch draws the draft itself
+ * and keeps lists of at most 4096 candidates). With P = softmax(target row / temperature) and Q = softmax(drafter's row /
+ * its temperature), or all of Q on the draft: draft j is kept iff u[s][j] Q(d) < P(d); at the first one refused the token is
+ * drawn from max(0, P - Q) with u[s][j + 1]; where no draft is refused it is drawn from P of the position behind the last one
+ * with that position's u[s][j]. A draw is the first token, by id, at which the running sum is above u times the whole; weights
+ * and running sums of a draw are in 64 bits. Where max(0, P - Q) is nothing, P is drawn from.
+ * NaN and masked logits weigh nothing; where the largest is +inf, its first place weighs all. A row in which nothing weighs
+ * anything refuses its draft, and gives next_token -1 and MK_FLAG_NO_CANDIDATE (with MK_FLAG_ALL_MASKED where its mask allows
+ * no token). Outputs, device: n_kept[n_seq], next_token[n_seq]; optional tokens[n_seq][n_pos] (the kept drafts, next_token,
+ * -1 behind), logprob[n_seq][n_pos] (the logarithm of P at those tokens, 0 behind), flags[n_seq]. n_seq is at most the
+ * handle's max_batch. mk_spec_commit takes n_kept and next_token on from here. */
+int mk_spec_verify(mk_sampler* s, const mk_spec_rows* rows, int32_t* n_kept, int32_t* next_token, int32_t* tokens,
+                   float* logprob, uint32_t* flags, void* stream);
+
+/* A paged cache's pages: which ones each sequence holds, in order, and a list of those that no one holds (a stack: the top is
+ * free_list[n_free - 1]). All device; a plan updates them in place. */
+typedef struct mk_kv_pages {
+    int32_t* block_table; /* [n_seq][table_ld], table_cols used */
+    uint64_t table_ld;
+    uint32_t table_cols;
+    int32_t* n_pages;     /* [n_seq] pages held */
+    int32_t* free_list;   /* [free_cap] */
+    uint32_t free_cap;
+    int32_t* n_free;      /* [1] */
+    uint32_t page_size;   /* tokens a page, any number above 0 */
+} mk_kv_pages;
+
+/* What the next forward pass is handed. All device, each optional. */
+typedef struct mk_kv_plan {
+    int32_t* query_start; /* [n_seq + 1] running sum of the tokens of the pass */
+    int32_t* kv_len;      /* [n_seq] tokens in the cache once the pass has run */
+    int32_t* positions;   /* [max_tokens] of each token of the pass in its sequence */
+    int64_t* slots;       /* [max_tokens] where its key and value go: page * page_size + place in the page */
+    int32_t* token_seq;   /* [max_tokens] its sequence */
+    uint32_t* flags;      /* [n_seq] MK_FLAG_PLAN_INVALID, MK_FLAG_NO_ROOM, MK_FLAG_NO_PAGES */
+    uint32_t max_tokens;
+} mk_kv_plan;
+
+/* Plans a pass from the sequences' lengths, on the device: cache_len[s] tokens are in the cache (after a speculative round:
+ * the kept ones), n_new[s] come with the pass (NULL: none). Every sequence ends up with exactly the pages that
+ * cache_len + n_new need: those above are given back (their table entries become -1), missing ones are taken. A sequence of
+ * 0 + 0 tokens gives all of its pages back. In detail, sequences counted in order:
+ *   - one with a negative number, more pages than table_cols, a need above table_cols or above 2^31 - 1 tokens is invalid: it
+ *     is left alone, kv_len 0 (MK_FLAG_PLAN_INVALID);
+ *   - one with new tokens, of which with those of all valid sequences before it there are more than max_tokens, is left alone
+ *     (MK_FLAG_NO_ROOM);
+ *   - pages given back go on top of the list, the first of them topmost (where they would pass free_cap none is given back);
+ *   - pages are taken from the top, by sequence; one whose pages, with those of the sequences before it, are more than the
+ *     list holds is left alone (MK_FLAG_NO_PAGES).
+ * A sequence that is left alone keeps its pages and has no tokens in the pass. Places behind the last token get position 0,
+ * slot -1, sequence -1, so that a pass of max_tokens rows, captured once, runs on any plan. An n_free outside [0, free_cap] is
+ * taken as the nearest of the two. Table entries are taken as they are. */
+int mk_kv_plan_step(mk_sampler* s, const mk_kv_pages* pages, const int32_t* cache_len, const int32_t* n_new, uint32_t n_seq,
+                    const mk_kv_plan* plan, void* stream);
 
 /* Vocab-parallel sampling, step 1 of 2 (no counterpart in the reference, which runs on one device): each shard
  * writes one record per row — its maximum, its sum of exp((l - max)/T) and its `k` best candidates (<= 64) — of

@@ -25,6 +25,11 @@ FLAG_OVERFLOW = 0x010
 FLAG_VP_TRUNCATED = 0x020
 FLAG_TIMEOUT = 0x040
 FLAG_HISTORY_FULL = 0x100
+FLAG_PLAN_INVALID = 0x200
+FLAG_NO_ROOM = 0x400
+FLAG_NO_PAGES = 0x800
+
+FP32, BF16, FP16 = 0, 1, 2
 
 OVERLAP_OFF, OVERLAP_LAUNCH, OVERLAP_STABLE_SIDE_INPUTS = 0, 1, 2
 
@@ -73,6 +78,66 @@ class SampleOutC(C.Structure):
     ]
 
 
+class HeadC(C.Structure):
+    _fields_ = [
+        ("weight", C.c_void_p),
+        ("down", C.c_void_p),
+        ("up", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("n_vocab", C.c_uint32),
+        ("dim", C.c_uint32),
+        ("n_adapters", C.c_uint32),
+        ("rank", C.c_uint32),
+        ("type", C.c_int),
+    ]
+
+
+class SpecRowsC(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("ld", C.c_uint64),
+        ("draft_logits", C.c_void_p),
+        ("draft_ld", C.c_uint64),
+        ("type", C.c_int),
+        ("n_seq", C.c_uint32),
+        ("n_pos", C.c_uint32),
+        ("n_vocab", C.c_uint32),
+        ("drafts", C.c_void_p),
+        ("u", C.c_void_p),
+        ("temperature", C.c_void_p),
+        ("draft_temperature", C.c_void_p),
+        ("temperature_all", C.c_float),
+        ("mask", C.c_void_p),
+        ("mask_ld", C.c_uint64),
+        ("mask_drafts", C.c_int),
+    ]
+
+
+class KvPagesC(C.Structure):
+    _fields_ = [
+        ("block_table", C.c_void_p),
+        ("table_ld", C.c_uint64),
+        ("table_cols", C.c_uint32),
+        ("n_pages", C.c_void_p),
+        ("free_list", C.c_void_p),
+        ("free_cap", C.c_uint32),
+        ("n_free", C.c_void_p),
+        ("page_size", C.c_uint32),
+    ]
+
+
+class KvPlanC(C.Structure):
+    _fields_ = [
+        ("query_start", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("token_seq", C.c_void_p),
+        ("flags", C.c_void_p),
+        ("max_tokens", C.c_uint32),
+    ]
+
+
 class MakoError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"mako_b200 error {code}: {message}")
@@ -113,6 +178,9 @@ def _load() -> C.CDLL:
                                         C.c_float, vp, vp, vp, vp]
     lib.mk_rank_force.argtypes = [vp, vp, C.c_uint64, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, vp, vp]
     lib.mk_decode_commit.argtypes = [vp, C.c_uint32, vp, vp, vp, C.c_uint64, C.c_uint32, vp, vp, vp, vp, vp]
+    lib.mk_head_logits.argtypes = [vp, C.POINTER(HeadC), vp, C.c_uint64, vp, C.c_uint32, vp, C.c_uint64, vp]
+    lib.mk_spec_verify.argtypes = [vp, C.POINTER(SpecRowsC), vp, vp, vp, vp, vp, vp]
+    lib.mk_kv_plan_step.argtypes = [vp, C.POINTER(KvPagesC), vp, vp, C.c_uint32, C.POINTER(KvPlanC), vp]
     lib.mk_vp_record_bytes.restype = C.c_uint32
     lib.mk_vp_record_bytes.argtypes = [C.c_uint32]
     lib.mk_sampler_vp_local.argtypes = [vp, C.POINTER(RowsC), C.c_uint32, vp, vp]

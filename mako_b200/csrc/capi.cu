@@ -1,6 +1,7 @@
 // C ABI of the library (declared in include/mako_b200.h): argument checks, scratch ownership, kernel launches.
 // No allocation happens after mk_sampler_create, except the host-buffer entry point, which sizes its device staging on
 // first use. There is no CPU fallback anywhere: without a CUDA device every entry point fails.
+#include "round_ops.h"
 #include "row_pipeline.h"
 
 #include <cmath>
@@ -69,6 +70,7 @@ struct mk_sampler {
     // small batches: every row split over many CTAs; twice, for the two row sets of p/q verification
     mk::SplitPart* split_parts = nullptr; // [2][kSplitMaxRows][kMaxSlices]
     uint32_t* split_tickets = nullptr;    // [2][kSplitMaxRows], zero between launches
+    float* head_inner = nullptr;            // [max_batch][kHeadMaxRank]: mk_head_logits' down projections
     int split = 1;                          // 0: every batch runs as one CTA per row
 };
 
@@ -325,6 +327,7 @@ int mk_sampler_create(mk_sampler** out, int device, uint32_t n_vocab, uint32_t m
         {(void**)&s->p_flags, b * 4},
         {(void**)&s->q_flags, b * 4},
         {(void**)&s->p_tok, b * 4},
+        {(void**)&s->head_inner, b * mk::kHeadMaxRank * 4},
     };
     auto up = [](size_t x) { return (x + 255u) & ~(size_t)255u; };
     size_t bytes = 0;
@@ -650,6 +653,98 @@ int mk_spec_commit(mk_sampler* s, uint32_t n_seq, uint32_t n_pos, const int32_t*
     DeviceGuard g(s->device);
     MK_CUDA(mk::launch_spec_commit(n_seq, n_pos, drafts, n_kept, next_token, history, history_ld, history_cap,
                                    history_len, next_input, flags, (cudaStream_t)stream));
+    return MK_OK;
+}
+
+// ---- the round around the sampler -----------------------------------------------------------------------------------
+
+int mk_head_logits(mk_sampler* s, const mk_head* head, const void* hidden, uint64_t hidden_ld, const int32_t* adapter,
+                   uint32_t rows, float* logits, uint64_t ld, void* stream)
+{
+    if (!s || !head || !head->weight)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: null argument");
+    mk_head h = *head;
+    if (!adapter)
+        h.n_adapters = 0; // no row has one
+    if (h.type != MK_BF16 && h.type != MK_FP16)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: type %d is neither MK_BF16 nor MK_FP16", h.type);
+    if (h.n_vocab == 0 || h.n_vocab > s->n_vocab || rows > s->max_batch)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: n_vocab %u (the handle's: %u), rows %u (max_batch %u)", h.n_vocab,
+                    s->n_vocab, rows, s->max_batch);
+    if (h.dim == 0 || (h.dim & 7u) || hidden_ld < h.dim || (hidden_ld & 7u) || ld < h.n_vocab)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: dim %u and hidden_ld %llu are multiples of 8, ld %llu", h.dim,
+                    (unsigned long long)hidden_ld, (unsigned long long)ld);
+    if (h.n_adapters && (!h.down || !h.up || h.rank == 0 || (h.rank & 7u) || h.rank > mk::kHeadMaxRank))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: adapters of rank %u (a multiple of 8, at most %u) need down and up",
+                    h.rank, mk::kHeadMaxRank);
+    auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
+    if (off(h.weight) || off(hidden) || (h.n_adapters && (off(h.down) || off(h.up))))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: weight, hidden, down and up start on 16-byte boundaries");
+    if (rows == 0)
+        return MK_OK;
+    if (!hidden || !logits)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: null argument");
+    DeviceGuard g(s->device);
+    MK_CUDA(mk::launch_head_logits(h, hidden, hidden_ld, adapter, rows, s->head_inner, logits, ld, (cudaStream_t)stream));
+    return MK_OK;
+}
+
+int mk_spec_verify(mk_sampler* s, const mk_spec_rows* r, int32_t* n_kept, int32_t* next_token, int32_t* tokens, float* logprob,
+                   uint32_t* flags, void* stream)
+{
+    if (!s || !r)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: null argument");
+    if (r->type != MK_FP32 && r->type != MK_BF16 && r->type != MK_FP16)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: type %d is none of MK_FP32, MK_BF16, MK_FP16", r->type);
+    if (r->n_vocab == 0 || r->n_vocab > s->n_vocab || r->n_seq > s->max_batch || r->n_pos == 0)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: n_vocab %u (the handle's: %u), n_seq %u (max_batch %u), n_pos %u",
+                    r->n_vocab, s->n_vocab, r->n_seq, s->max_batch, r->n_pos);
+    if (r->ld < r->n_vocab || (r->draft_logits && r->draft_ld < r->n_vocab))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: ld %llu, draft_ld %llu below n_vocab %u", (unsigned long long)r->ld,
+                    (unsigned long long)r->draft_ld, r->n_vocab);
+    if (r->mask && r->mask_ld < (uint64_t)(r->n_vocab + 31) / 32)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: mask_ld %llu smaller than ceil(n_vocab/32)",
+                    (unsigned long long)r->mask_ld);
+    if (!r->temperature && !std::isfinite(r->temperature_all))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: the temperature must be finite");
+    if (r->n_seq == 0)
+        return MK_OK;
+    if (!r->logits || !r->u || !n_kept || !next_token || (r->n_pos > 1 && !r->drafts))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: logits, drafts, u, n_kept and next_token are required");
+    DeviceGuard g(s->device);
+    mk::SpecVerifyArgs a;
+    a.r = *r;
+    a.n_kept = n_kept;
+    a.next_token = next_token;
+    a.tokens = tokens;
+    a.logprob = logprob;
+    a.flags = flags;
+    MK_CUDA(mk::launch_spec_verify(a, (cudaStream_t)stream));
+    return MK_OK;
+}
+
+int mk_kv_plan_step(mk_sampler* s, const mk_kv_pages* pages, const int32_t* cache_len, const int32_t* n_new, uint32_t n_seq,
+                    const mk_kv_plan* plan, void* stream)
+{
+    if (!s || !pages || !plan)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: null argument");
+    if (!pages->n_free || (pages->free_cap && !pages->free_list) || pages->free_cap > 0x7fffffffu)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: n_free and a free_list of free_cap %u pages are required", pages->free_cap);
+    if (n_seq && (!cache_len || !pages->n_pages || (pages->table_cols && !pages->block_table)))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: cache_len, n_pages and block_table are required");
+    if (pages->page_size == 0 || pages->table_ld < pages->table_cols || pages->table_cols > 0x7fffffffu)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: page_size %u, table_ld %llu, table_cols %u", pages->page_size,
+                    (unsigned long long)pages->table_ld, pages->table_cols);
+    if (plan->max_tokens > 0x7fffffffu || n_seq > 0x7ffffffeu)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: max_tokens %u, n_seq %u", plan->max_tokens, n_seq);
+    DeviceGuard g(s->device);
+    mk::KvPlanArgs a;
+    a.p = *pages;
+    a.o = *plan;
+    a.cache_len = cache_len;
+    a.n_new = n_new;
+    a.n_seq = n_seq;
+    MK_CUDA(mk::launch_kv_plan(a, (cudaStream_t)stream));
     return MK_OK;
 }
 

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import RowsC, SampleOutC, check, lib
+from ._lib import HeadC, KvPagesC, KvPlanC, RowsC, SampleOutC, SpecRowsC, check, lib
 from .params import SamplingParams
 
 
@@ -98,6 +98,36 @@ class SampleResult:
     cand_q: Optional[torch.Tensor] = None
     accepted: Optional[torch.Tensor] = None
     draft_token: Optional[torch.Tensor] = None
+
+
+@dataclass
+class SpecVerifyResult:
+    n_kept: torch.Tensor
+    next_token: torch.Tensor
+    tokens: torch.Tensor
+    logprob: torch.Tensor
+    flags: torch.Tensor
+
+
+@dataclass
+class KvPlan:
+    """What a forward pass over a paged cache is handed (mk_kv_plan): query_start [S + 1], kv_len [S], positions [T], token_seq
+    [T], flags [S] int32 and slots [T] int64, T being the most tokens a pass may have."""
+    query_start: torch.Tensor
+    kv_len: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    token_seq: torch.Tensor
+    flags: torch.Tensor
+
+    @classmethod
+    def empty(cls, n_seq: int, max_tokens: int, device="cuda") -> "KvPlan":
+        i32 = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
+        return cls(i32(n_seq + 1), i32(n_seq), i32(max_tokens), torch.empty(max_tokens, dtype=torch.int64, device=device),
+                   i32(max_tokens), i32(n_seq))
+
+
+_TYPE = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 
 
 class BatchSampler:
@@ -317,6 +347,100 @@ class BatchSampler:
         check(lib.mk_spec_commit(self._h, n_seq, n_drafts + 1, drafts.data_ptr(), n_kept.data_ptr(),
                                  next_token.data_ptr(), history.data_ptr(), history.stride(0), history.shape[1],
                                  history_len.data_ptr(), _ptr(next_input), _ptr(flags), _stream_ptr(self.device)))
+
+    # -- the round around the sampler -----------------------------------------------------------------------------
+    def head_logits(self, hidden, weight, *, adapter=None, down=None, up=None, scale=None, out=None) -> torch.Tensor:
+        """The model's head with the requests' low-rank adapters beside it (mk_head_logits): hidden [T, D], weight [V, D],
+        down [N, R, D], up [N, V, R] bf16 or fp16, adapter [T] int32 (-1: none), scale [N] float32. Returns the rows that the
+        sampler reads, [T, V] float32 (`out` where given)."""
+        (rows, dim), v = hidden.shape, weight.shape[0]
+        assert hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.stride(1) == 1
+        assert weight.dtype == hidden.dtype and weight.is_contiguous() and weight.shape[1] == dim
+        h = HeadC()
+        h.weight, h.n_vocab, h.dim, h.type = weight.data_ptr(), v, dim, _TYPE[hidden.dtype]
+        if adapter is not None:
+            assert adapter.dtype == torch.int32 and adapter.is_contiguous() and adapter.numel() == rows
+            n, rank, _ = down.shape
+            assert down.dtype == up.dtype == hidden.dtype and down.is_contiguous() and up.is_contiguous()
+            assert down.shape == (n, rank, dim) and up.shape == (n, v, rank)
+            h.down, h.up, h.n_adapters, h.rank = down.data_ptr(), up.data_ptr(), n, rank
+            if scale is not None:
+                assert scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == n
+                h.scale = scale.data_ptr()
+        if out is None:
+            out = torch.empty((rows, v), dtype=torch.float32, device=hidden.device)
+        assert out.dtype == torch.float32 and out.shape == (rows, v) and out.stride(1) == 1
+        check(lib.mk_head_logits(self._h, C.byref(h), hidden.data_ptr(), hidden.stride(0), _ptr(adapter), rows, out.data_ptr(),
+                                 out.stride(0), _stream_ptr(self.device)))
+        return out
+
+    def spec_verify(self, logits, drafts, u, temperature, *, draft_logits=None, draft_temperature=None, mask=None,
+                    mask_drafts: bool = False) -> SpecVerifyResult:
+        """A speculative round against whole distributions (mk_spec_verify): logits [S * n_pos, V], drafts [S, n_pos - 1] int32
+        (negative: no more drafts), u [S, n_pos + 1], temperature a number or [S] float32, draft_logits [S * (n_pos - 1), V] of
+        the target's type or None for drafts that are certain, mask [S * n_pos, words]. Returns n_kept [S], next_token [S],
+        tokens [S, n_pos], logprob [S, n_pos], flags [S]."""
+        n_seq, n_drafts = drafts.shape
+        n_pos, v = n_drafts + 1, logits.shape[1]
+        assert logits.is_cuda and logits.shape[0] == n_seq * n_pos and logits.stride(1) == 1
+        assert drafts.dtype == torch.int32 and drafts.is_contiguous()
+        assert u.shape == (n_seq, n_pos + 1) and u.dtype == torch.float32 and u.is_contiguous()
+        r = SpecRowsC()
+        r.logits, r.ld, r.type = logits.data_ptr(), logits.stride(0), _TYPE[logits.dtype]
+        r.n_seq, r.n_pos, r.n_vocab = n_seq, n_pos, v
+        r.drafts, r.u = drafts.data_ptr(), u.data_ptr()
+        if draft_logits is not None:
+            assert draft_logits.dtype == logits.dtype and draft_logits.shape == (n_seq * n_drafts, v)
+            assert draft_logits.stride(1) == 1
+            r.draft_logits, r.draft_ld = draft_logits.data_ptr(), draft_logits.stride(0)
+        if isinstance(temperature, torch.Tensor):
+            assert temperature.dtype == torch.float32 and temperature.shape == (n_seq,) and temperature.is_contiguous()
+            r.temperature = temperature.data_ptr()
+        else:
+            r.temperature_all = temperature
+        if draft_temperature is not None:
+            assert draft_temperature.dtype == torch.float32 and draft_temperature.shape == (n_seq,)
+            assert draft_temperature.is_contiguous()
+            r.draft_temperature = draft_temperature.data_ptr()
+        if mask is not None:
+            assert mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos and mask.stride(1) == 1
+            r.mask, r.mask_ld, r.mask_drafts = mask.data_ptr(), mask.stride(0), int(mask_drafts)
+        i32 = torch.empty(n_seq * (n_pos + 3), dtype=torch.int32, device=self.device)
+        kept, nxt, flags, tokens = i32.split([n_seq, n_seq, n_seq, n_seq * n_pos])
+        logprob = torch.empty((n_seq, n_pos), dtype=torch.float32, device=self.device)
+        check(lib.mk_spec_verify(self._h, C.byref(r), kept.data_ptr(), nxt.data_ptr(), tokens.data_ptr(), logprob.data_ptr(),
+                                 flags.data_ptr(), _stream_ptr(self.device)))
+        return SpecVerifyResult(kept, nxt, tokens.view(n_seq, n_pos), logprob, flags)
+
+    def kv_plan(self, block_table, n_pages, free_list, n_free, cache_len, n_new=None, *, page_size: int,
+                out: Optional[KvPlan] = None) -> Optional[KvPlan]:
+        """Pages, positions and slots of the next forward pass from the sequences' lengths, on the device (mk_kv_plan_step):
+        block_table [S, columns], n_pages [S], free_list [P] and n_free [1] int32 are updated in place; cache_len [S] tokens are
+        in the cache, n_new [S] come with the pass (None: pages above the need go back, and that is all). Fills and returns
+        `out` (KvPlan.empty)."""
+        n_seq, cols = block_table.shape
+        for t in (block_table, n_pages, free_list, n_free, cache_len):
+            assert t.is_cuda and t.dtype == torch.int32
+        assert block_table.stride(1) == 1 and n_pages.is_contiguous() and cache_len.is_contiguous() and free_list.is_contiguous()
+        assert n_pages.numel() == cache_len.numel() == n_seq and n_free.numel() == 1
+        p, o = KvPagesC(), KvPlanC()
+        p.block_table, p.table_ld, p.table_cols = block_table.data_ptr(), block_table.stride(0), cols
+        p.n_pages, p.free_list, p.free_cap = n_pages.data_ptr(), free_list.data_ptr(), free_list.numel()
+        p.n_free, p.page_size = n_free.data_ptr(), page_size
+        if n_new is not None:
+            assert n_new.dtype == torch.int32 and n_new.is_contiguous() and n_new.numel() == n_seq and out is not None
+        if out is not None:
+            t = out.positions.numel()
+            for x, n in ((out.query_start, n_seq + 1), (out.kv_len, n_seq), (out.positions, t), (out.token_seq, t),
+                         (out.flags, n_seq)):
+                assert x.dtype == torch.int32 and x.numel() == n and x.is_contiguous()
+            assert out.slots.dtype == torch.int64 and out.slots.numel() == t and out.slots.is_contiguous()
+            o.query_start, o.kv_len, o.positions = out.query_start.data_ptr(), out.kv_len.data_ptr(), out.positions.data_ptr()
+            o.slots, o.token_seq, o.flags = out.slots.data_ptr(), out.token_seq.data_ptr(), out.flags.data_ptr()
+            o.max_tokens = t
+        check(lib.mk_kv_plan_step(self._h, C.byref(p), cache_len.data_ptr(), _ptr(n_new), n_seq, C.byref(o),
+                                  _stream_ptr(self.device)))
+        return out
 
     def vp_local(self, shard_logits, params, k: int, records: torch.Tensor, *, id_offset: int, history=None,
                  history_len=None, mask=None, bias=None) -> torch.Tensor:
