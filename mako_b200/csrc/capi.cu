@@ -70,7 +70,7 @@ struct mk_sampler {
     // small batches: every row split over many CTAs; twice, for the two row sets of p/q verification
     mk::SplitPart* split_parts = nullptr; // [2][kSplitMaxRows][kMaxSlices]
     uint32_t* split_tickets = nullptr;    // [2][kSplitMaxRows], zero between launches
-    float* head_inner = nullptr;            // [max_batch][kHeadMaxRank]: mk_head_logits' down projections
+    float* head_inner = nullptr;            // [max_batch][kHeadMaxRank] and [2][max_batch] behind them: mk_head_logits' scratch
     int split = 1;                          // 0: every batch runs as one CTA per row
 };
 
@@ -327,7 +327,7 @@ int mk_sampler_create(mk_sampler** out, int device, uint32_t n_vocab, uint32_t m
         {(void**)&s->p_flags, b * 4},
         {(void**)&s->q_flags, b * 4},
         {(void**)&s->p_tok, b * 4},
-        {(void**)&s->head_inner, b * mk::kHeadMaxRank * 4},
+        {(void**)&s->head_inner, b * (mk::kHeadMaxRank + 2) * 4},
     };
     auto up = [](size_t x) { return (x + 255u) & ~(size_t)255u; };
     size_t bytes = 0;
@@ -677,6 +677,9 @@ int mk_head_logits(mk_sampler* s, const mk_head* head, const void* hidden, uint6
     if (h.n_adapters && (!h.down || !h.up || h.rank == 0 || (h.rank & 7u) || h.rank > mk::kHeadMaxRank))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: adapters of rank %u (a multiple of 8, at most %u) need down and up",
                     h.rank, mk::kHeadMaxRank);
+    if (h.n_adapters && (uint64_t)rows * h.dim * 2u > s->max_batch * mk::row_scratch_words(scratch_cap(s->n_vocab)) * 4u)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: %u rows of dim %u and adapters need a handle of more columns or rows", rows,
+                    h.dim);
     auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
     if (off(h.weight) || off(hidden) || (h.n_adapters && (off(h.down) || off(h.up))))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: weight, hidden, down and up start on 16-byte boundaries");
@@ -685,7 +688,12 @@ int mk_head_logits(mk_sampler* s, const mk_head* head, const void* hidden, uint6
     if (!hidden || !logits)
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_head_logits: null argument");
     DeviceGuard g(s->device);
-    MK_CUDA(mk::launch_head_logits(h, hidden, hidden_ld, adapter, rows, s->head_inner, logits, ld, (cudaStream_t)stream));
+    // the rows in the order of their adapters lie where a sample call has its candidates: 16 bytes a column of the handle
+    mk::HeadScratch x;
+    x.hidden = s->scratch;
+    x.inner = s->head_inner;
+    x.ints = reinterpret_cast<int32_t*>(s->head_inner + (size_t)s->max_batch * mk::kHeadMaxRank);
+    MK_CUDA(mk::launch_head_logits(h, hidden, hidden_ld, adapter, rows, x, logits, ld, (cudaStream_t)stream));
     return MK_OK;
 }
 

@@ -1,6 +1,21 @@
-// The head with the requests' low-rank adapters beside it (mk_head_logits in include/mako_b200.h), as two launches: the rows'
-// down projections, then tiles of the logits with the up projections added before they are written.
+// The head with the requests' low-rank adapters beside it (mk_head_logits in include/mako_b200.h):
+//     logits[t][v] = weight[v] . hidden[t] + up[a][v] . inner[t],   inner[t] = scale[a] (down[a] hidden[t]),   a = adapter[t]
+// Two launches. The first brings the rows into the order of their adapters (a copy of the hidden states, a few MB at most) and
+// forms `inner`, a CTA per row. The second streams the weight matrix once past the rows: it is what bounds a decode step (1.06 GB
+// at 129280 x 4096), so every CTA has an equal share of the vocabulary, a run of columns of the logits in steps of 16, and keeps
+// as much of it on the way as shared memory holds.
+//
+// A tile is 128 vocabulary rows (the MMA's M, a lane of tensor memory each) by the batch's rows (its N, padded to 16). Batches of
+// few rows take two or four vocabulary tiles side by side, so that the hidden states' tile, which comes from L2 every time, is
+// read once for all of them. Warp 0 copies tiles in, warp 1 issues the MMAs, eight warps drain tensor memory.
+//
+// Precision: the tensor core's fp32 accumulator truncates, 1.0e-6 of the result for every 1024 terms, all of it towards zero
+// (measured against 64 bits). So a run of 512 terms goes into one of two accumulators and is added in registers, rounding to
+// nearest, while the next run goes into the other. `inner` stays in fp32; its products with `up` are FMAs of the draining warps,
+// 16 ranks at a time between the runs: rows of one adapter stand side by side, so that a lane's piece of `up` is loaded once for
+// all of them. (As MMAs they would want `inner` cut to 16 bits, and one adapter's infinite weight would reach other rows as 0 x inf.)
 #include "round_ops.h"
+#include "tcgen05.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -8,94 +23,541 @@
 namespace mk {
 namespace {
 
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+constexpr uint32_t kBlockK = 64;                   // elements of the contraction in a tile: 128 bytes
+constexpr uint32_t kRunBlocks = 8;                 // tiles that go into one accumulator
+constexpr uint32_t kTileV = 128, kGroupV = 16;     // vocabulary rows of a tile; of a CTA's share, a multiple
+constexpr uint32_t kTileBytes = kTileV * kBlockK * 2;
+constexpr uint32_t kDrainWarps = 8, kFirstDrain = 4, kHeadThreads = 32 * (kFirstDrain + kDrainWarps);
+constexpr uint32_t kRankStep = 16;                  // ranks that a lane holds of `up` at a time
+constexpr uint32_t kMaxColumns = 256;              // of one accumulator: vocabulary tiles x rows
+constexpr uint32_t kMaxStages = 16;
+constexpr uint32_t kRingBytes = 206 * 1024;
 
-// inner[row][r] = scale * down[a][r] . hidden[row], a warp each.
+__device__ __forceinline__ float2 pair_to_float(__nv_bfloat162 x) { return __bfloat1622float2(x); }
+__device__ __forceinline__ float2 pair_to_float(__half2 x) { return __half22float2(x); }
+template <typename T>
+struct Type;
+template <>
+struct Type<__nv_bfloat16> {
+    using pair = __nv_bfloat162;
+    static constexpr bool bf16 = true;
+};
+template <>
+struct Type<__half> {
+    using pair = __half2;
+    static constexpr bool bf16 = false;
+};
+
+// Eight elements as four pairs of floats.
+template <typename T>
+__device__ __forceinline__ void load8(float2 (&x)[4], const T* p)
+{
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        x[i] = pair_to_float(*reinterpret_cast<const typename Type<T>::pair*>(&w[i]));
+}
+
+// Where the rows go when they stand in the order of their adapters (rows without one last), and what the adapters' down
+// projections leave of them. All indexed by the new place.
+struct HeadOrder {
+    void* hidden;   // [rows][dim]
+    int32_t* row;   // which row stands here
+    int32_t* adapter; // its adapter, or -1
+    float* inner;   // [rows][kHeadMaxRank]; zeros where there is no adapter
+};
+
+// A CTA per row: its place is the number of rows that come before it; two dot products at a time per warp.
 template <typename T>
 __global__ void __launch_bounds__(256) head_inner_kernel(const mk_head h, const T* hidden, uint64_t hidden_ld,
-                                                         const int32_t* adapter, float* inner)
+                                                         const int32_t* adapter, uint32_t rows, const HeadOrder o)
 {
-    const uint32_t row = blockIdx.x, r = blockIdx.y * 8u + threadIdx.x / 32u, lane = threadIdx.x & 31u;
-    const int32_t a = adapter[row];
-    if (a < 0 || (uint32_t)a >= h.n_adapters || r >= h.rank)
-        return;
-    const T* x = hidden + row * hidden_ld;
-    const T* w = static_cast<const T*>(h.down) + ((size_t)a * h.rank + r) * h.dim;
-    float sum = 0.0f;
-    for (uint32_t i = lane; i < h.dim; i += 32)
-        sum = fmaf(to_float(x[i]), to_float(w[i]), sum);
-#pragma unroll
-    for (uint32_t d = 16; d; d >>= 1)
-        sum += __shfl_xor_sync(~0u, sum, d);
+    griddep_launch_dependents();
+    __shared__ uint32_t s_before[8];
+    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, w = tid / 32u;
+    auto key = [&](uint32_t i) {
+        const uint32_t a = (uint32_t)adapter[i];
+        return a < h.n_adapters ? a : ~0u;
+    };
+    const uint32_t a = key(row);
+    uint32_t before = 0;
+    for (uint32_t i = tid; i < rows; i += 256u) {
+        const uint32_t b = key(i);
+        before += b < a || (b == a && i < row);
+    }
+    before = __reduce_add_sync(~0u, before);
     if (lane == 0)
-        inner[(size_t)row * kHeadMaxRank + r] = (h.scale ? h.scale[a] : 1.0f) * sum;
-}
-
-// 64 columns of 16 rows a CTA; a thread has four columns of one row.
-template <typename T>
-__global__ void __launch_bounds__(256) head_tile_kernel(const mk_head h, const T* hidden, uint64_t hidden_ld,
-                                                        const int32_t* adapter, uint32_t rows, const float* inner, float* logits,
-                                                        uint64_t ld)
-{
-    __shared__ float s_x[16][33], s_w[64][33];
-    const uint32_t v0 = blockIdx.x * 64u, t0 = blockIdx.y * 16u, tx = threadIdx.x & 15u, ty = threadIdx.x >> 4;
-    const T* weight = static_cast<const T*>(h.weight);
-    float acc[4] = {};
-    for (uint32_t k0 = 0; k0 < h.dim; k0 += 32) {
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < 16 * 32; i += 256) {
-            const uint32_t t = t0 + i / 32, k = k0 + i % 32;
-            s_x[i / 32][i % 32] = t < rows && k < h.dim ? to_float(hidden[t * hidden_ld + k]) : 0.0f;
-        }
-        for (uint32_t i = threadIdx.x; i < 64 * 32; i += 256) {
-            const uint32_t v = v0 + i / 32, k = k0 + i % 32;
-            s_w[i / 32][i % 32] = v < h.n_vocab && k < h.dim ? to_float(weight[(size_t)v * h.dim + k]) : 0.0f;
-        }
-        __syncthreads();
-        for (uint32_t k = 0; k < 32; ++k)
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c)
-                acc[c] = fmaf(s_x[ty][k], s_w[tx + 16 * c][k], acc[c]);
+        s_before[w] = before;
+    __syncthreads();
+    uint32_t place = 0;
+    for (int i = 0; i < 8; ++i)
+        place += s_before[i];
+    const T* x = hidden + row * hidden_ld;
+    T* to = static_cast<T*>(o.hidden) + (size_t)place * h.dim;
+    for (uint32_t i = tid * 8u; i < h.dim; i += 256u * 8u)
+        *reinterpret_cast<uint4*>(to + i) = __ldg(reinterpret_cast<const uint4*>(x + i));
+    if (tid == 0) {
+        o.row[place] = (int32_t)row;
+        o.adapter[place] = (int32_t)a;
     }
-    const uint32_t t = t0 + ty;
-    if (t >= rows)
+    float* out = o.inner + (size_t)place * kHeadMaxRank;
+    if (a == ~0u) {
+        if (tid < kHeadMaxRank)
+            out[tid] = 0.0f;
         return;
-    const int32_t a = h.n_adapters ? adapter[t] : -1;
-    for (uint32_t c = 0; c < 4; ++c) {
-        const uint32_t v = v0 + tx + 16 * c;
-        if (v >= h.n_vocab)
-            continue;
-        if (a >= 0 && (uint32_t)a < h.n_adapters) {
-            const T* up = static_cast<const T*>(h.up) + ((size_t)a * h.n_vocab + v) * h.rank;
-            float d = 0.0f;
-            for (uint32_t r = 0; r < h.rank; ++r)
-                d = fmaf(inner[(size_t)t * kHeadMaxRank + r], to_float(up[r]), d);
-            acc[c] += d;
+    }
+    const float scale = h.scale ? h.scale[a] : 1.0f;
+    for (uint32_t r = 2u * w; r < h.rank; r += 16u) { // (the rank is even)
+        const T* d = static_cast<const T*>(h.down) + ((size_t)a * h.rank + r) * h.dim;
+        float2 sum[2][4] = {};
+#pragma unroll 4
+        for (uint32_t i = lane * 8u; i < h.dim; i += 256u) {
+            float2 p[4], q0[4], q1[4];
+            load8(p, x + i);
+            load8(q0, d + i);
+            load8(q1, d + h.dim + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                sum[0][k] = fma2(p[k], q0[k], sum[0][k]);
+                sum[1][k] = fma2(p[k], q1[k], sum[1][k]);
+            }
         }
-        logits[t * ld + v] = acc[c];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float y = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                y += sum[j][k].x + sum[j][k].y;
+#pragma unroll
+            for (uint32_t k = 16; k; k >>= 1)
+                y += __shfl_xor_sync(~0u, y, k);
+            if (lane == 0)
+                out[r + j] = scale * y;
+        }
     }
 }
 
-template <typename T>
-cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, const int32_t* adapter, uint32_t rows, float* inner,
-                   float* logits, uint64_t ld, cudaStream_t stream)
+struct HeadArgs {
+    mk_head h;
+    HeadOrder order; // of no meaning without adapters
+    float* logits;
+    uint64_t ld;
+    uint32_t rows;
+    uint32_t n;            // rows of a tile, a multiple of 16
+    uint32_t side;         // vocabulary tiles side by side: side * n <= kMaxColumns
+    uint32_t w_slots, x_slots;
+};
+
+struct HeadShared {
+    uint64_t w_full[kMaxStages], w_empty[kMaxStages], x_full[kMaxStages], x_empty[kMaxStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    int failed;
+    int32_t row[kMaxColumns], adapter[kMaxColumns]; // of the tile's columns
+    float4 inner[kMaxColumns][kRankStep / 4];
+};
+
+// A ring's place: slot and the parity its barriers complete with next.
+struct Place {
+    uint32_t slot = 0, parity = 0;
+    __device__ void next(uint32_t n)
+    {
+        if (++slot == n) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
+};
+
+// Waits, but not for ever: a wait that runs out, in any warp, ends all.
+__device__ __forceinline__ bool await(HeadShared& s, uint64_t* bar, uint32_t parity)
 {
-    const T* x = static_cast<const T*>(hidden);
+    for (uint32_t i = 0; i < (1u << 17); ++i) {
+        if (mbar_try_wait(bar, parity))
+            return true;
+        if (*reinterpret_cast<volatile int*>(&s.failed))
+            return false;
+    }
+    *reinterpret_cast<volatile int*>(&s.failed) = 1;
+    return false;
+}
+
+// Columns: of one accumulator that a draining thread has, half of all. Its lane is a vocabulary row.
+template <typename T, int Columns>
+__device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t v_from, uint32_t v_to)
+{
+    const uint32_t tid = threadIdx.x - 32u * kFirstDrain, w = tid / 32u, lane = tid & 31u, c0 = (w / 4u) * Columns;
+    const uint32_t quarter = w & 3u; // of the lanes, the one that this warp may read
+    const uint32_t k_blocks = (a.h.dim + kBlockK - 1) / kBlockK, runs = (k_blocks + kRunBlocks - 1) / kRunBlocks;
+    const uint32_t steps = a.h.n_adapters ? (a.h.rank + kRankStep - 1) / kRankStep : 0u;
+    const uint32_t tmem = s.tmem + ((quarter * 32u) << 16) + c0;
+    const T* up = static_cast<const T*>(a.h.up);
+    float acc[Columns];
+    uint32_t buf = 0, parity = 0;
+    bool alive = true;
+    griddep_wait(); // for the rows' order and `inner`
+    for (uint32_t t0 = 0; t0 < a.rows; t0 += a.n) {
+        named_barrier(1, kDrainWarps * 32);
+        if (tid < a.n) {
+            const bool real = t0 + tid < a.rows;
+            s.row[tid] = !real ? -1 : steps ? a.order.row[t0 + tid] : (int32_t)(t0 + tid);
+            s.adapter[tid] = real && steps ? a.order.adapter[t0 + tid] : -1;
+        }
+        named_barrier(1, kDrainWarps * 32);
+        uint32_t turns[Columns / 32]; // columns whose adapter or vocabulary tile is another than the one's before
+#pragma unroll
+        for (int k = 0; k < Columns / 32; ++k) {
+            const uint32_t c = c0 + 32u * k + lane, t = c % a.n;
+            turns[k] = __ballot_sync(~0u, c == c0 || t == 0 || s.adapter[t] != s.adapter[t - 1u]);
+        }
+        for (uint32_t v0 = v_from; v0 < v_to; v0 += a.side * kTileV) {
+#pragma unroll
+            for (int i = 0; i < Columns; ++i)
+                acc[i] = 0.0f;
+            uint32_t step = 0;
+            for (uint32_t run = 0; run < runs; ++run) {
+                alive = alive && await(s, &s.acc_full[buf], parity); // a warp that gave up still meets the others' barriers
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < Columns; i += 32) {
+                    float x[32];
+                    tmem_load32(x, tmem + buf * kMaxColumns + i);
+                    tmem_wait(x);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        acc[i + k] += x[k];
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&s.acc_empty[buf]);
+                buf ^= 1u;
+                parity ^= buf == 0;
+                // this run's part of the adapters' ranks
+                for (; step < ((run + 1u) * steps + runs - 1u) / runs; ++step) {
+                    const uint32_t r = step * kRankStep, left = a.h.rank - r;
+                    if (steps > 1 || (v0 == v_from && run == 0)) {
+                        named_barrier(1, kDrainWarps * 32); // the step before has been used
+                        for (uint32_t i = tid; i < a.n * (kRankStep / 4); i += kDrainWarps * 32) {
+                            const uint32_t t = i / (kRankStep / 4), q = i % (kRankStep / 4);
+                            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (t0 + t < a.rows && q * 4u < left)
+                                y = __ldg(reinterpret_cast<const float4*>(a.order.inner + (size_t)(t0 + t) * kHeadMaxRank + r) + q);
+                            s.inner[t][q] = y;
+                        }
+                        named_barrier(1, kDrainWarps * 32);
+                    }
+                    uint32_t g = c0 / a.n, t = c0 % a.n;
+                    asm volatile("" : "+r"(g), "+r"(t)); // (the columns' places are counted up, not kept in registers for all of them)
+                    float2 x[kRankStep / 2];
+#pragma unroll
+                    for (int k = 0; k < Columns; ++k) {
+                        if (turns[k / 32] >> (k % 32) & 1u) {
+                            const int32_t ad = s.adapter[t];
+                            const uint32_t v = v0 + g * kTileV + quarter * 32u + lane;
+#pragma unroll
+                            for (int i = 0; i < (int)kRankStep / 2; ++i)
+                                x[i] = make_float2(0.0f, 0.0f);
+                            if (ad >= 0 && g < a.side && v < a.h.n_vocab) {
+                                const T* p = up + ((size_t)ad * a.h.n_vocab + v) * a.h.rank + r;
+                                load8(*reinterpret_cast<float2(*)[4]>(&x[0]), p);
+                                if (left > 8u)
+                                    load8(*reinterpret_cast<float2(*)[4]>(&x[4]), p + 8);
+                            }
+                        }
+                        float2 d = make_float2(0.0f, 0.0f);
+#pragma unroll
+                        for (int i = 0; i < (int)kRankStep / 4; ++i) {
+                            const float4 y = s.inner[t][i];
+                            d = fma2(x[2 * i], make_float2(y.x, y.y), d);
+                            d = fma2(x[2 * i + 1], make_float2(y.z, y.w), d);
+                        }
+                        acc[k] += d.x + d.y;
+                        if (++t == a.n) {
+                            t = 0;
+                            ++g;
+                        }
+                    }
+                }
+            }
+            uint32_t g = c0 / a.n, t = c0 % a.n;
+            asm volatile("" : "+r"(g), "+r"(t));
+#pragma unroll
+            for (int k = 0; k < Columns; ++k) {
+                const uint32_t v = v0 + g * kTileV + quarter * 32u + lane;
+                const int32_t row = s.row[t];
+                if (g < a.side && v < v_to && row >= 0)
+                    a.logits[(size_t)row * a.ld + v] = acc[k];
+                if (++t == a.n) {
+                    t = 0;
+                    ++g;
+                }
+            }
+        }
+    }
+}
+
+// A CTA's rings and its share of the vocabulary: [v_from, v_end) is copied, [v_from, v_to) is written.
+struct Share {
+    unsigned char *ring, *x_ring;
+    uint32_t x_bytes, k_blocks, v_from, v_end, v_to;
+};
+
+__device__ __forceinline__ void produce(const HeadArgs& a, HeadShared& s, const Share& c, const CUtensorMap* w_map,
+                                        const CUtensorMap* w_small, const CUtensorMap* x_map)
+{
+    const uint64_t once = l2_evict_first(), often = l2_evict_last();
+    Place w, x;
+    bool ok = true;
+    auto copy_w = [&](uint32_t k, uint32_t v) {
+        if (!(ok = ok && await(s, &s.w_empty[w.slot], w.parity ^ 1u)))
+            return;
+        unsigned char* to = c.ring + w.slot * kTileBytes;
+        const uint32_t left = c.v_end - v;
+        if (left >= kTileV) {
+            mbar_arrive_expect_tx(&s.w_full[w.slot], kTileBytes);
+            tma_load_2d(to, w_map, (int32_t)(k * kBlockK), (int32_t)v, &s.w_full[w.slot], once);
+        } else { // the share's end, in steps of 16 rows; what lies behind them in the slot has no part
+            mbar_arrive_expect_tx(&s.w_full[w.slot], left * kBlockK * 2);
+            for (uint32_t i = 0; i < left; i += kGroupV)
+                tma_load_2d(to + i * kBlockK * 2, w_small, (int32_t)(k * kBlockK), (int32_t)(v + i), &s.w_full[w.slot], once);
+        }
+        w.next(a.w_slots);
+    };
+    auto copy_x = [&](uint32_t k, uint32_t t0) {
+        if (!(ok = ok && await(s, &s.x_empty[x.slot], x.parity ^ 1u)))
+            return;
+        mbar_arrive_expect_tx(&s.x_full[x.slot], c.x_bytes);
+        tma_load_2d(c.x_ring + x.slot * c.x_bytes, x_map, (int32_t)(k * kBlockK), (int32_t)t0, &s.x_full[x.slot], often);
+        x.next(a.x_slots);
+    };
+    // the c.ring's first weights are under way before the rows' order is waited for
+    const uint32_t ahead = min(min(a.w_slots / a.side, a.x_slots), c.k_blocks);
+    for (uint32_t k = 0; k < ahead; ++k)
+        for (uint32_t v = c.v_from; v < c.v_end && v < c.v_from + a.side * kTileV; v += kTileV)
+            copy_w(k, v);
+    griddep_wait();
+    for (uint32_t t0 = 0; t0 < a.rows && ok; t0 += a.n)
+        for (uint32_t v0 = c.v_from; v0 < c.v_end && ok; v0 += a.side * kTileV)
+            for (uint32_t k = 0; k < c.k_blocks && ok; ++k) {
+                copy_x(k, t0);
+                if (t0 != 0 || v0 != c.v_from || k >= ahead)
+                    for (uint32_t v = v0; v < c.v_end && v < v0 + a.side * kTileV; v += kTileV)
+                        copy_w(k, v);
+            }
+}
+
+template <typename T>
+__device__ __forceinline__ void issue(const HeadArgs& a, HeadShared& s, const Share& c)
+{
+                const uint32_t desc = mma_f16_desc(Type<T>::bf16, a.n);
+                Place w, x;
+                uint32_t buf = 0, parity = 0;
+                bool ok = true;
+                for (uint32_t t0 = 0; t0 < a.rows && ok; t0 += a.n)
+                    for (uint32_t v0 = c.v_from; v0 < c.v_end && ok; v0 += a.side * kTileV)
+                        for (uint32_t k = 0; k < c.k_blocks && ok; ++k) {
+                            if (k % kRunBlocks == 0) {
+                                if (!(ok = await(s, &s.acc_empty[buf], parity ^ 1u)))
+                                    break;
+                                tc_fence_after();
+                            }
+                            if (!(ok = await(s, &s.x_full[x.slot], x.parity)))
+                                break;
+                            const uint64_t b = smem_tile_desc(c.x_ring + x.slot * c.x_bytes);
+                            uint32_t g = 0;
+                            for (uint32_t v = v0; v < c.v_end && v < v0 + a.side * kTileV; v += kTileV, ++g) {
+                                if (!(ok = await(s, &s.w_full[w.slot], w.parity)))
+                                    break;
+                                tc_fence_after();
+                                const uint64_t d = smem_tile_desc(c.ring + w.slot * kTileBytes);
+    #pragma unroll
+                                for (uint32_t i = 0; i < kBlockK / 16; ++i)
+                                    mma_f16(s.tmem + buf * kMaxColumns + g * a.n, d + 2 * i, b + 2 * i, desc, k % kRunBlocks != 0 || i != 0);
+                                mma_commit(&s.w_empty[w.slot]);
+                                w.next(a.w_slots);
+                            }
+                            mma_commit(&s.x_empty[x.slot]);
+                            x.next(a.x_slots);
+                            if (k % kRunBlocks == kRunBlocks - 1 || k + 1 == c.k_blocks) {
+                                mma_commit(&s.acc_full[buf]);
+                                buf ^= 1u;
+                                parity ^= buf == 0;
+                            }
+                        }
+}
+
+template <typename T, int Columns>
+__global__ void __launch_bounds__(kHeadThreads, 1)
+    head_kernel(const HeadArgs a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap w_small,
+                const __grid_constant__ CUtensorMap x_map)
+{
+    extern __shared__ unsigned char raw[];
+    __shared__ HeadShared s;
+    const uint32_t warp = threadIdx.x / 32u, groups = (a.h.n_vocab + kGroupV - 1) / kGroupV;
+    Share c;
+    c.ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
+    c.x_ring = c.ring + a.w_slots * kTileBytes;
+    c.x_bytes = a.n * kBlockK * 2;
+    c.k_blocks = (a.h.dim + kBlockK - 1) / kBlockK;
+    c.v_from = (uint32_t)((uint64_t)groups * blockIdx.x / gridDim.x) * kGroupV;
+    c.v_end = (uint32_t)((uint64_t)groups * (blockIdx.x + 1) / gridDim.x) * kGroupV;
+    c.v_to = min(c.v_end, a.h.n_vocab);
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kMaxStages; ++i) {
+            mbar_init(&s.w_full[i], 1);
+            mbar_init(&s.w_empty[i], 1);
+            mbar_init(&s.x_full[i], 1);
+            mbar_init(&s.x_empty[i], 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(&s.acc_full[i], 1);
+            mbar_init(&s.acc_empty[i], kDrainWarps);
+        }
+        s.failed = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1)
+        tmem_alloc_all(&s.tmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // 168 registers a thread at launch: 128 threads give up what 256 that drain take (128 x 40 + 256 x 232 = 384 x 168)
+    if (warp >= kFirstDrain) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        drain<T, Columns>(a, s, c.v_from, c.v_to);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (threadIdx.x == 0)
+            produce(a, s, c, &w_map, &w_small, &x_map);
+        else if (threadIdx.x == 32)
+            issue<T>(a, s, c);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (s.failed) { // never seen: copies and products in flight end within this, and the share's logits say what happened
+        for (int i = 0; i < 2000; ++i)
+            __nanosleep(1000);
+        for (uint32_t t = 0; t < a.rows; ++t)
+            for (uint32_t v = c.v_from + threadIdx.x; v < c.v_to; v += kHeadThreads)
+                a.logits[(size_t)t * a.ld + v] = __int_as_float(0x7fc00000);
+        __syncthreads();
+    }
+    if (warp == 1)
+        tmem_free_all(s.tmem);
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+cudaError_t encoder(EncodeTiled& f)
+{
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q);
+    f = reinterpret_cast<EncodeTiled>(p);
+    return e != cudaSuccess ? e : p && q == cudaDriverEntryPointSuccess ? cudaSuccess : cudaErrorNotSupported;
+}
+
+// A row-major matrix of 16-bit elements in boxes of 64 elements by `box` rows.
+bool encode(EncodeTiled f, CUtensorMap* map, bool bf16, const void* base, uint64_t cols, uint64_t rows, uint64_t ld, uint32_t box)
+{
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * 2};
+    const cuuint32_t boxes[2] = {kBlockK, box}, steps[2] = {1, 1};
+    return f(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides,
+             boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int Columns>
+cudaError_t launch_tiles(const HeadArgs& a, uint32_t grid, bool behind_inner, const CUtensorMap* maps, cudaStream_t stream)
+{
+    const size_t smem = kRingBytes + 1024;
+    static const bool split_fits = [] { // the registers that the warps share out among themselves are those of the launch
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, head_kernel<T, Columns>) == cudaSuccess && f.numRegs == 168;
+    }();
+    if (!split_fits)
+        return cudaErrorInvalidKernelImage;
+    cudaError_t e = cudaFuncSetAttribute(head_kernel<T, Columns>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess)
+        return e;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(kHeadThreads);
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = attr;
+    c.numAttrs = behind_inner ? 1 : 0;
+    return cudaLaunchKernelEx(&c, head_kernel<T, Columns>, a, maps[0], maps[1], maps[2]);
+}
+
+template <typename T>
+cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, const int32_t* adapter, uint32_t rows,
+                   const HeadScratch& scratch, float* logits, uint64_t ld, cudaStream_t stream)
+{
+    EncodeTiled f;
+    cudaError_t e = encoder(f);
+    if (e != cudaSuccess)
+        return e;
+    HeadArgs a;
+    a.h = h;
+    a.order.hidden = scratch.hidden;
+    a.order.row = scratch.ints;
+    a.order.adapter = scratch.ints + rows;
+    a.order.inner = scratch.inner;
+    a.logits = logits;
+    a.ld = ld;
+    a.rows = rows;
+    const uint32_t tiles = (rows + kMaxColumns - 1) / kMaxColumns;
+    a.n = ((rows + tiles - 1) / tiles + 15u) & ~15u;
+    a.side = a.n <= kMaxColumns / 4 ? 4u : a.n <= kMaxColumns / 2 ? 2u : 1u;
+    const uint32_t x_bytes = a.n * kBlockK * 2;
+    a.x_slots = a.w_slots = 0; // as deep a ring of steps of the contraction as fits
+    for (uint32_t x = 2, best = 0; x <= kMaxStages && x * x_bytes < kRingBytes; ++x) {
+        uint32_t w = (kRingBytes - x * x_bytes) / kTileBytes;
+        w = w > kMaxStages ? kMaxStages : w;
+        const uint32_t deep = w < x * a.side ? w : x * a.side;
+        if (deep > best) {
+            best = deep;
+            a.x_slots = x;
+            a.w_slots = w;
+        }
+    }
+    CUtensorMap maps[3];
+    constexpr bool bf16 = Type<T>::bf16;
+    if (!encode(f, &maps[0], bf16, h.weight, h.dim, h.n_vocab, h.dim, kTileV) ||
+        !encode(f, &maps[1], bf16, h.weight, h.dim, h.n_vocab, h.dim, kGroupV) ||
+        !encode(f, &maps[2], bf16, h.n_adapters ? scratch.hidden : hidden, h.dim, rows, h.n_adapters ? h.dim : hidden_ld, a.n))
+        return cudaErrorInvalidValue;
     if (h.n_adapters)
-        head_inner_kernel<T><<<dim3(rows, (h.rank + 7) / 8), 256, 0, stream>>>(h, x, hidden_ld, adapter, inner);
-    head_tile_kernel<T><<<dim3((h.n_vocab + 63) / 64, (rows + 15) / 16), 256, 0, stream>>>(h, x, hidden_ld, adapter, rows, inner,
-                                                                                         logits, ld);
-    return cudaGetLastError();
+        head_inner_kernel<T><<<rows, 256, 0, stream>>>(h, static_cast<const T*>(hidden), hidden_ld, adapter, rows, a.order);
+    e = cudaGetLastError();
+    if (e != cudaSuccess)
+        return e;
+    const uint32_t groups = (h.n_vocab + kGroupV - 1) / kGroupV, grid = groups < 148u ? groups : 148u;
+    const uint32_t half = (a.side * a.n + 1) / 2;
+    const bool behind = h.n_adapters != 0;
+    return half <= 32 ? launch_tiles<T, 32>(a, grid, behind, maps, stream)
+           : half <= 64 ? launch_tiles<T, 64>(a, grid, behind, maps, stream)
+           : half <= 96 ? launch_tiles<T, 96>(a, grid, behind, maps, stream)
+                        : launch_tiles<T, 128>(a, grid, behind, maps, stream);
 }
 
 } // namespace
 
 cudaError_t launch_head_logits(const mk_head& h, const void* hidden, uint64_t hidden_ld, const int32_t* adapter, uint32_t rows,
-                               float* inner, float* logits, uint64_t ld, cudaStream_t stream)
+                               const HeadScratch& scratch, float* logits, uint64_t ld, cudaStream_t stream)
 {
-    return h.type == MK_BF16 ? launch<__nv_bfloat16>(h, hidden, hidden_ld, adapter, rows, inner, logits, ld, stream)
-                             : launch<__half>(h, hidden, hidden_ld, adapter, rows, inner, logits, ld, stream);
+    return h.type == MK_BF16 ? launch<__nv_bfloat16>(h, hidden, hidden_ld, adapter, rows, scratch, logits, ld, stream)
+                             : launch<__half>(h, hidden, hidden_ld, adapter, rows, scratch, logits, ld, stream);
 }
 
 } // namespace mk

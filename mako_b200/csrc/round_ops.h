@@ -9,9 +9,15 @@
 namespace mk {
 
 constexpr uint32_t kHeadMaxRank = 128;
-// inner: [rows][rank] fp32 scratch, what the adapters' down projections leave.
+// What a call with adapters needs of the handle, for its rows: `hidden` [rows][dim] of the matrices' type on a 16-byte boundary,
+// `ints` [2][rows], `inner` [rows][kHeadMaxRank].
+struct HeadScratch {
+    void* hidden;
+    int32_t* ints;
+    float* inner;
+};
 cudaError_t launch_head_logits(const mk_head& h, const void* hidden, uint64_t hidden_ld, const int32_t* adapter, uint32_t rows,
-                               float* inner, float* logits, uint64_t ld, cudaStream_t stream);
+                               const HeadScratch& scratch, float* logits, uint64_t ld, cudaStream_t stream);
 
 struct SpecVerifyArgs {
     mk_spec_rows r;
