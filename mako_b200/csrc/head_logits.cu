@@ -29,9 +29,10 @@ constexpr uint32_t kTileV = 128, kGroupV = 16;     // vocabulary rows of a tile;
 constexpr uint32_t kTileBytes = kTileV * kBlockK * 2;
 constexpr uint32_t kDrainWarps = 8, kFirstDrain = 4, kHeadThreads = 32 * (kFirstDrain + kDrainWarps);
 constexpr uint32_t kRankStep = 16;                  // ranks that a lane holds of `up` at a time
+constexpr uint32_t kDeltas = 16;                   // columns that the adapters' part is formed for at a time
 constexpr uint32_t kMaxColumns = 256;              // of one accumulator: vocabulary tiles x rows
 constexpr uint32_t kMaxStages = 16;
-constexpr uint32_t kRingBytes = 206 * 1024;
+constexpr uint32_t kRingBytes = 190 * 1024;
 
 __device__ __forceinline__ float2 pair_to_float(__nv_bfloat162 x) { return __bfloat1622float2(x); }
 __device__ __forceinline__ float2 pair_to_float(__half2 x) { return __half22float2(x); }
@@ -156,6 +157,7 @@ struct HeadShared {
     int failed;
     int32_t row[kMaxColumns], adapter[kMaxColumns]; // of the tile's columns
     float4 inner[kMaxColumns][kRankStep / 4];
+    float delta[kDrainWarps][kDeltas][32]; // each thread's own; kept here because registers take no running index
 };
 
 // A ring's place: slot and the parity its barriers complete with next.
@@ -170,15 +172,17 @@ struct Place {
     }
 };
 
-// Waits, but not for ever: a wait that runs out, in any warp, ends all.
+// Waits, but not for ever: one that lasts two seconds, in any warp, ends all. (Probes without a suspend-time hint: with one of
+// 20 us a step of the contraction took 0.65 us whatever its size.)
 __device__ __forceinline__ bool await(HeadShared& s, uint64_t* bar, uint32_t parity)
 {
-    for (uint32_t i = 0; i < (1u << 17); ++i) {
-        if (mbar_try_wait(bar, parity))
+    if (mbar_try(bar, parity))
+        return true;
+    const long long from = clock64();
+    do {
+        if (mbar_try(bar, parity))
             return true;
-        if (*reinterpret_cast<volatile int*>(&s.failed))
-            return false;
-    }
+    } while (clock64() - from < (1ll << 32) && !*reinterpret_cast<volatile int*>(&s.failed));
     *reinterpret_cast<volatile int*>(&s.failed) = 1;
     return false;
 }
@@ -191,6 +195,8 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
     const uint32_t quarter = w & 3u; // of the lanes, the one that this warp may read
     const uint32_t k_blocks = (a.h.dim + kBlockK - 1) / kBlockK, runs = (k_blocks + kRunBlocks - 1) / kRunBlocks;
     const uint32_t steps = a.h.n_adapters ? (a.h.rank + kRankStep - 1) / kRankStep : 0u;
+    constexpr uint32_t blocks = Columns / kDeltas;
+    const uint32_t units = steps * blocks;
     const uint32_t tmem = s.tmem + ((quarter * 32u) << 16) + c0;
     const T* up = static_cast<const T*>(a.h.up);
     float acc[Columns];
@@ -215,7 +221,7 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
 #pragma unroll
             for (int i = 0; i < Columns; ++i)
                 acc[i] = 0.0f;
-            uint32_t step = 0;
+            uint32_t unit = 0;
             for (uint32_t run = 0; run < runs; ++run) {
                 alive = alive && await(s, &s.acc_full[buf], parity); // a warp that gave up still meets the others' barriers
                 tc_fence_after();
@@ -234,11 +240,13 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
                     mbar_arrive(&s.acc_empty[buf]);
                 buf ^= 1u;
                 parity ^= buf == 0;
-                // this run's part of the adapters' ranks
-                for (; step < ((run + 1u) * steps + runs - 1u) / runs; ++step) {
-                    const uint32_t r = step * kRankStep, left = a.h.rank - r;
-                    if (steps > 1 || (v0 == v_from && run == 0)) {
-                        named_barrier(1, kDrainWarps * 32); // the step before has been used
+                // this run's part of the adapters' work, which is 16 ranks of 16 columns at a time
+                for (const uint32_t until = ((run + 1u) * units + runs - 1u) / runs; unit < until;) {
+                    const uint32_t r = unit / blocks * kRankStep, left = a.h.rank - r, from = unit % blocks;
+                    const uint32_t to = min(blocks, from + until - unit);
+                    unit += to - from;
+                    if (from == 0 && (steps > 1 || v0 == v_from)) {
+                        named_barrier(1, kDrainWarps * 32); // the ranks before these have been used
                         for (uint32_t i = tid; i < a.n * (kRankStep / 4); i += kDrainWarps * 32) {
                             const uint32_t t = i / (kRankStep / 4), q = i % (kRankStep / 4);
                             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -248,14 +256,16 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
                         }
                         named_barrier(1, kDrainWarps * 32);
                     }
-                    uint32_t g = c0 / a.n, t = c0 % a.n;
-                    asm volatile("" : "+r"(g), "+r"(t)); // (the columns' places are counted up, not kept in registers for all of them)
-                    float2 x[kRankStep / 2];
 #pragma unroll
-                    for (int k = 0; k < Columns; ++k) {
-                        if (turns[k / 32] >> (k % 32) & 1u) {
+                    for (int block = 0; block < (int)blocks; ++block) {
+                        if ((uint32_t)block < from || (uint32_t)block >= to)
+                            continue;
+                        uint32_t g = (c0 + block * kDeltas) / a.n, t = c0 + block * kDeltas - g * a.n, c = 0;
+                        const uint32_t turn = (turns[block / 2] >> (block % 2 * 16)) | 1u;
+                        while (c < kDeltas) {
                             const int32_t ad = s.adapter[t];
                             const uint32_t v = v0 + g * kTileV + quarter * 32u + lane;
+                            float2 x[kRankStep / 2];
 #pragma unroll
                             for (int i = 0; i < (int)kRankStep / 2; ++i)
                                 x[i] = make_float2(0.0f, 0.0f);
@@ -265,19 +275,29 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
                                 if (left > 8u)
                                     load8(*reinterpret_cast<float2(*)[4]>(&x[4]), p + 8);
                             }
-                        }
-                        float2 d = make_float2(0.0f, 0.0f);
+                            const uint32_t later = (turn >> c) >> 1;
+                            const uint32_t end = later ? min(c + (uint32_t)__ffs(later), kDeltas) : kDeltas;
+                            const float4(*y)[kRankStep / 4] = &s.inner[t];
+                            t += end - c;
+#pragma unroll 2
+                            for (; c < end; ++c, ++y) {
+                                float2 d = make_float2(0.0f, 0.0f), e = make_float2(0.0f, 0.0f);
 #pragma unroll
-                        for (int i = 0; i < (int)kRankStep / 4; ++i) {
-                            const float4 y = s.inner[t][i];
-                            d = fma2(x[2 * i], make_float2(y.x, y.y), d);
-                            d = fma2(x[2 * i + 1], make_float2(y.z, y.w), d);
+                                for (int i = 0; i < (int)kRankStep / 4; ++i) {
+                                    const float4 z = (*y)[i];
+                                    d = fma2(x[2 * i], make_float2(z.x, z.y), d);
+                                    e = fma2(x[2 * i + 1], make_float2(z.z, z.w), e);
+                                }
+                                s.delta[w][c][lane] = (d.x + e.x) + (d.y + e.y);
+                            }
+                            if (t == a.n) {
+                                t = 0;
+                                ++g;
+                            }
                         }
-                        acc[k] += d.x + d.y;
-                        if (++t == a.n) {
-                            t = 0;
-                            ++g;
-                        }
+#pragma unroll
+                        for (int k = 0; k < (int)kDeltas; ++k)
+                            acc[block * (int)kDeltas + k] += s.delta[w][k][lane];
                     }
                 }
             }
