@@ -291,7 +291,7 @@ typedef struct mk_spec_rows {
     uint32_t n_seq, n_pos, n_vocab;
     const int32_t* drafts;         /* device [n_seq][n_pos - 1]; the first one outside [0, n_vocab) ends its sequence's drafts */
     const float* u;                /* device [n_seq][n_pos + 1], the uniforms as mk_sampler_spec_round takes them */
-    const float* temperature;      /* device [n_seq], or NULL: temperature_all. Not above 0: the largest logit alone, lowest id */
+    const float* temperature;      /* device [n_seq], or NULL: temperature_all. Not above 0 or not finite: the largest logit alone, lowest id */
     const float* draft_temperature;/* device [n_seq], or NULL: the target's */
     float temperature_all;
     const uint32_t* mask;          /* device [n_seq * n_pos][mask_ld] allowed tokens of the target's rows, or NULL */
