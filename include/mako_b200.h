@@ -291,7 +291,7 @@ typedef struct mk_spec_rows {
     uint32_t n_seq, n_pos, n_vocab;
     const int32_t* drafts;         /* device [n_seq][n_pos - 1]; the first one outside [0, n_vocab) ends its sequence's drafts */
     const float* u;                /* device [n_seq][n_pos + 1], the uniforms as mk_sampler_spec_round takes them */
-    const float* temperature;      /* device [n_seq], or NULL: temperature_all. Not above 0 or not finite: the largest logit alone, lowest id */
+    const float* temperature;      /* device [n_seq], or NULL: temperature_all. Not above 0, or 1e30 and more: the largest logit alone, lowest id */
     const float* draft_temperature;/* device [n_seq], or NULL: the target's */
     float temperature_all;
     const uint32_t* mask;          /* device [n_seq * n_pos][mask_ld] allowed tokens of the target's rows, or NULL */
@@ -309,7 +309,9 @@ typedef struct mk_spec_rows {
  * anything refuses its draft, and gives next_token -1 and MK_FLAG_NO_CANDIDATE (with MK_FLAG_ALL_MASKED where its mask allows
  * no token). Outputs, device: n_kept[n_seq], next_token[n_seq]; optional tokens[n_seq][n_pos] (the kept drafts, next_token,
  * -1 behind), logprob[n_seq][n_pos] (the logarithm of P at those tokens, 0 behind), flags[n_seq]. n_seq is at most the
- * handle's max_batch. mk_spec_commit takes n_kept and next_token on from here. */
+ * handle's max_batch, and n_seq * (n_pos + 1) at most 33 times that. Rows are read in whole 16-byte blocks, as mk_rows says.
+ * Calls on one handle must not overlap (they share its scratch and counters). mk_spec_commit takes n_kept and next_token on
+ * from here. */
 int mk_spec_verify(mk_sampler* s, const mk_spec_rows* rows, int32_t* n_kept, int32_t* next_token, int32_t* tokens,
                    float* logprob, uint32_t* flags, void* stream);
 
@@ -326,7 +328,7 @@ typedef struct mk_kv_pages {
     uint32_t page_size;   /* tokens a page, any number above 0 */
 } mk_kv_pages;
 
-/* What the next forward pass is handed. All device, each optional. */
+/* What the next forward pass is handed. All device, each optional; positions, slots and token_seq need query_start. */
 typedef struct mk_kv_plan {
     int32_t* query_start; /* [n_seq + 1] running sum of the tokens of the pass */
     int32_t* kv_len;      /* [n_seq] tokens in the cache once the pass has run */
@@ -350,7 +352,7 @@ typedef struct mk_kv_plan {
  *     list holds is left alone (MK_FLAG_NO_PAGES).
  * A sequence that is left alone keeps its pages and has no tokens in the pass. Places behind the last token get position 0,
  * slot -1, sequence -1, so that a pass of max_tokens rows, captured once, runs on any plan. An n_free outside [0, free_cap] is
- * taken as the nearest of the two. Table entries are taken as they are. */
+ * taken as the nearest of the two. Table entries are taken as they are. At most 8192 sequences. */
 int mk_kv_plan_step(mk_sampler* s, const mk_kv_pages* pages, const int32_t* cache_len, const int32_t* n_new, uint32_t n_seq,
                     const mk_kv_plan* plan, void* stream);
 

@@ -71,6 +71,10 @@ struct mk_sampler {
     mk::SplitPart* split_parts = nullptr; // [2][kSplitMaxRows][kMaxSlices]
     uint32_t* split_tickets = nullptr;    // [2][kSplitMaxRows], zero between launches
     float* head_inner = nullptr;            // [max_batch][kHeadMaxRank] and [2][max_batch] behind them: mk_head_logits' scratch
+    // mk_spec_verify: [max_batch][kSpecPositions], and so many times the slices of a row
+    mk::SpecState* spec_states = nullptr;
+    mk::SpecPart* spec_parts = nullptr;
+    uint32_t* spec_words = nullptr;         // zero between calls
     int split = 1;                          // 0: every batch runs as one CTA per row
 };
 
@@ -306,12 +310,13 @@ int mk_sampler_create(mk_sampler** out, int device, uint32_t n_vocab, uint32_t m
     // One allocation, shared out: as one for each array they were most of what creating a handle takes.
     const size_t b = max_batch, row_bytes = mk::row_scratch_words(scratch_cap(n_vocab)) * 4;
     const size_t split_rows_max = 2u * (size_t)mk::kSplitMaxRows;
-    const size_t zero_bytes = (mk::kDraftPickMaxSeq + 1) * sizeof(unsigned long long) + split_rows_max * 4;
+    const size_t spec_rows = b * mk::kSpecPositions;
+    const size_t zero_bytes = (mk::kDraftPickMaxSeq + 1) * sizeof(unsigned long long) + (split_rows_max + spec_rows + 2) * 4;
     struct Share {
         void** to;
         size_t bytes;
     } const shares[] = {
-        {(void**)&s->pick_best, zero_bytes}, // maxima and ticket counter of the drafter picks, then the split rows' tickets
+        {(void**)&s->pick_best, zero_bytes}, // maxima and ticket counter of the drafter picks, the split rows' tickets, mk_spec_verify's counters
         {(void**)&s->split_parts, split_rows_max * mk::kMaxSlices * sizeof(mk::SplitPart)},
         {(void**)&s->scratch, b * row_bytes},
         {(void**)&s->scratch_pq, b * row_bytes},
@@ -327,6 +332,8 @@ int mk_sampler_create(mk_sampler** out, int device, uint32_t n_vocab, uint32_t m
         {(void**)&s->p_flags, b * 4},
         {(void**)&s->q_flags, b * 4},
         {(void**)&s->p_tok, b * 4},
+        {(void**)&s->spec_states, spec_rows * sizeof(mk::SpecState)},
+        {(void**)&s->spec_parts, spec_rows * mk::spec_slices(n_vocab) * sizeof(mk::SpecPart)},
         {(void**)&s->head_inner, b * (mk::kHeadMaxRank + 2) * 4},
     };
     auto up = [](size_t x) { return (x + 255u) & ~(size_t)255u; };
@@ -341,6 +348,7 @@ int mk_sampler_create(mk_sampler** out, int device, uint32_t n_vocab, uint32_t m
             at += up(x.bytes);
         }
         s->split_tickets = reinterpret_cast<uint32_t*>(s->pick_best + mk::kDraftPickMaxSeq + 1);
+        s->spec_words = s->split_tickets + split_rows_max;
     }
     if (e == cudaSuccess)
         e = cudaStreamCreateWithFlags(&s->own_stream, cudaStreamNonBlocking);
@@ -707,6 +715,9 @@ int mk_spec_verify(mk_sampler* s, const mk_spec_rows* r, int32_t* n_kept, int32_
     if (r->n_vocab == 0 || r->n_vocab > s->n_vocab || r->n_seq > s->max_batch || r->n_pos == 0)
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: n_vocab %u (the handle's: %u), n_seq %u (max_batch %u), n_pos %u",
                     r->n_vocab, s->n_vocab, r->n_seq, s->max_batch, r->n_pos);
+    if ((uint64_t)r->n_seq * (r->n_pos + 1ull) > (uint64_t)s->max_batch * mk::kSpecPositions)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: n_seq %u of n_pos %u: (n_pos + 1) n_seq is above %u max_batch (%u)", r->n_seq,
+                    r->n_pos, mk::kSpecPositions, s->max_batch);
     if (r->ld < r->n_vocab || (r->draft_logits && r->draft_ld < r->n_vocab))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_spec_verify: ld %llu, draft_ld %llu below n_vocab %u", (unsigned long long)r->ld,
                     (unsigned long long)r->draft_ld, r->n_vocab);
@@ -727,6 +738,13 @@ int mk_spec_verify(mk_sampler* s, const mk_spec_rows* r, int32_t* n_kept, int32_
     a.tokens = tokens;
     a.logprob = logprob;
     a.flags = flags;
+    a.parts = s->spec_parts;
+    a.states = s->spec_states;
+    a.counter = s->spec_words;
+    a.failed = s->spec_words + 1;
+    a.tickets = s->spec_words + 2;
+    a.ended = a.tickets + (size_t)r->n_seq * r->n_pos;
+    a.slices = mk::spec_slices(r->n_vocab);
     MK_CUDA(mk::launch_spec_verify(a, (cudaStream_t)stream));
     return MK_OK;
 }
@@ -743,8 +761,11 @@ int mk_kv_plan_step(mk_sampler* s, const mk_kv_pages* pages, const int32_t* cach
     if (pages->page_size == 0 || pages->table_ld < pages->table_cols || pages->table_cols > 0x7fffffffu)
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: page_size %u, table_ld %llu, table_cols %u", pages->page_size,
                     (unsigned long long)pages->table_ld, pages->table_cols);
-    if (plan->max_tokens > 0x7fffffffu || n_seq > 0x7ffffffeu)
-        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: max_tokens %u, n_seq %u", plan->max_tokens, n_seq);
+    if (plan->max_tokens > 0x7fffffffu || n_seq > mk::kPlanMaxSeq)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: max_tokens %u, n_seq %u (at most %u)", plan->max_tokens, n_seq,
+                    mk::kPlanMaxSeq);
+    if ((plan->positions || plan->slots || plan->token_seq) && !plan->query_start)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_plan_step: positions, slots and token_seq need query_start");
     DeviceGuard g(s->device);
     mk::KvPlanArgs a;
     a.p = *pages;

@@ -19,14 +19,38 @@ struct HeadScratch {
 cudaError_t launch_head_logits(const mk_head& h, const void* hidden, uint64_t hidden_ld, const int32_t* adapter, uint32_t rows,
                                const HeadScratch& scratch, float* logits, uint64_t ld, cudaStream_t stream);
 
+// What a slice of a position's rows leaves, and what becomes of the position: maximum and sum of the target's and the drafter's
+// row, the first column that holds the maximum (where that matters).
+struct SpecPart {
+    float m_p, s_p;
+    uint32_t at_p, unused_p;
+    float m_q, s_q;
+    uint32_t at_q, unused_q;
+};
+struct SpecState {
+    float m_p, s_p;
+    uint32_t at_p, state;
+    float m_q, s_q;
+    uint32_t at_q, unused;
+};
+constexpr uint32_t kSpecPositions = 33; // words of counters a row of a handle has: 32 positions and the round's end
+inline uint32_t spec_slices(uint32_t n_vocab) { return n_vocab / 1024u + 1u < 64u ? n_vocab / 1024u + 1u : 64u; }
+
 struct SpecVerifyArgs {
     mk_spec_rows r;
     int32_t *n_kept, *next_token, *tokens;
     float* logprob;
     uint32_t* flags;
+    // the handle's: [n_seq * n_pos][slices], [n_seq * n_pos], and counters that are zero between calls: [n_seq * n_pos], [n_seq], one
+    // of the work taken, and one that stays up once a wait has run out
+    SpecPart* parts;
+    SpecState* states;
+    uint32_t *tickets, *ended, *counter, *failed;
+    uint32_t slices; // at most
 };
 cudaError_t launch_spec_verify(const SpecVerifyArgs& a, cudaStream_t stream);
 
+constexpr uint32_t kPlanMaxSeq = 8192;
 struct KvPlanArgs {
     mk_kv_pages p;
     mk_kv_plan o;

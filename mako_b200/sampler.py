@@ -405,12 +405,12 @@ class BatchSampler:
         if mask is not None:
             assert mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos and mask.stride(1) == 1
             r.mask, r.mask_ld, r.mask_drafts = mask.data_ptr(), mask.stride(0), int(mask_drafts)
-        i32 = torch.empty(n_seq * (n_pos + 3), dtype=torch.int32, device=self.device)
-        kept, nxt, flags, tokens = i32.split([n_seq, n_seq, n_seq, n_seq * n_pos])
+        kept, nxt, flags = torch.empty((3, n_seq), dtype=torch.int32, device=self.device).unbind()
+        tokens = torch.empty((n_seq, n_pos), dtype=torch.int32, device=self.device)
         logprob = torch.empty((n_seq, n_pos), dtype=torch.float32, device=self.device)
         check(lib.mk_spec_verify(self._h, C.byref(r), kept.data_ptr(), nxt.data_ptr(), tokens.data_ptr(), logprob.data_ptr(),
                                  flags.data_ptr(), _stream_ptr(self.device)))
-        return SpecVerifyResult(kept, nxt, tokens.view(n_seq, n_pos), logprob, flags)
+        return SpecVerifyResult(kept, nxt, tokens, logprob, flags)
 
     def kv_plan(self, block_table, n_pages, free_list, n_free, cache_len, n_new=None, *, page_size: int,
                 out: Optional[KvPlan] = None) -> Optional[KvPlan]:

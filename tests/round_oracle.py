@@ -29,7 +29,7 @@ def _dist(row, t, allowed):
     m = x.max()
     if m == -math.inf:
         return np.zeros_like(x)
-    if not 0 < t < math.inf or m == math.inf:
+    if not 0 < t < 1e30 or m == math.inf:
         w = np.zeros_like(x)
         w[int(x.argmax())] = 1.0
         return w
