@@ -7,7 +7,7 @@
 //
 // A tile is 128 vocabulary rows (the MMA's M, a lane of tensor memory each) by the batch's rows (its N, padded to 16). Batches of
 // few rows take two or four vocabulary tiles side by side, so that the hidden states' tile, which comes from L2 every time, is
-// read once for all of them. Warp 0 copies tiles in, warp 1 issues the MMAs, eight warps drain tensor memory.
+// read once for all of them. Three warps copy tiles in, one issues the MMAs, eight drain tensor memory.
 //
 // Precision: the tensor core's fp32 accumulator truncates, 1.0e-6 of the result for every 1024 terms, all of it towards zero
 // (measured against 64 bits). So a run of 512 terms goes into one of two accumulators and is added in registers, rounding to
@@ -27,10 +27,12 @@ constexpr uint32_t kBlockK = 64;                   // elements of the contractio
 constexpr uint32_t kRunBlocks = 8;                 // tiles that go into one accumulator
 constexpr uint32_t kTileV = 128, kGroupV = 16;     // vocabulary rows of a tile; of a CTA's share, a multiple
 constexpr uint32_t kTileBytes = kTileV * kBlockK * 2;
+constexpr uint32_t kWeightWarps = 2;                // that copy weights; before them one issues products, one copies rows
 constexpr uint32_t kDrainWarps = 8, kFirstDrain = 4, kHeadThreads = 32 * (kFirstDrain + kDrainWarps);
 constexpr uint32_t kRankStep = 16;                  // ranks that a lane holds of `up` at a time
 constexpr uint32_t kDeltas = 16;                   // columns that the adapters' part is formed for at a time
-constexpr uint32_t kMaxColumns = 256;              // of one accumulator: vocabulary tiles x rows
+constexpr uint32_t kMaxColumns = 256;              // of one of two accumulators: vocabulary tiles x rows
+constexpr uint32_t kOneColumns = 320;              // of a single one: what the draining warps have registers for
 constexpr uint32_t kMaxStages = 16;
 constexpr uint32_t kRingBytes = 190 * 1024;
 
@@ -146,7 +148,10 @@ struct HeadArgs {
     uint64_t ld;
     uint32_t rows;
     uint32_t n;            // rows of a tile, a multiple of 16
-    uint32_t side;         // vocabulary tiles side by side: side * n <= kMaxColumns
+    uint32_t side;         // vocabulary tiles side by side
+    uint32_t bufs;         // accumulators of side * n columns: two of up to 256, or one of up to 320
+    uint32_t spread;       // row tiles that CTAs side by side have at the same time
+    uint32_t turn;         // steps of the contraction that a vocabulary tile is copied for before the next one's turn: 1, 2 or 4
     uint32_t w_slots, x_slots;
 };
 
@@ -187,10 +192,18 @@ __device__ __forceinline__ bool await(HeadShared& s, uint64_t* bar, uint32_t par
     return false;
 }
 
+// A CTA's rings and its share of the vocabulary: [v_from, v_end) is copied, [v_from, v_to) is written.
+struct Share {
+    unsigned char *ring, *x_ring;
+    uint32_t x_bytes, k_blocks, v_from, v_end, v_to;
+    uint32_t t_from, t_step; // its row tiles
+};
+
 // Columns: of one accumulator that a draining thread has, half of all. Its lane is a vocabulary row.
 template <typename T, int Columns>
-__device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t v_from, uint32_t v_to)
+__device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Share& c)
 {
+    const uint32_t v_from = c.v_from, v_to = c.v_to;
     const uint32_t tid = threadIdx.x - 32u * kFirstDrain, w = tid / 32u, lane = tid & 31u, c0 = (w / 4u) * Columns;
     const uint32_t quarter = w & 3u; // of the lanes, the one that this warp may read
     const uint32_t k_blocks = (a.h.dim + kBlockK - 1) / kBlockK, runs = (k_blocks + kRunBlocks - 1) / kRunBlocks;
@@ -203,7 +216,7 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
     uint32_t buf = 0, parity = 0;
     bool alive = true;
     griddep_wait(); // for the rows' order and `inner`
-    for (uint32_t t0 = 0; t0 < a.rows; t0 += a.n) {
+    for (uint32_t t0 = c.t_from; t0 < a.rows; t0 += c.t_step) {
         named_barrier(1, kDrainWarps * 32);
         if (tid < a.n) {
             const bool real = t0 + tid < a.rows;
@@ -238,7 +251,7 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive(&s.acc_empty[buf]);
-                buf ^= 1u;
+                buf = buf + 1u == a.bufs ? 0u : buf + 1u;
                 parity ^= buf == 0;
                 // this run's part of the adapters' work, which is 16 ranks of 16 columns at a time
                 for (const uint32_t until = ((run + 1u) * units + runs - 1u) / runs; unit < until;) {
@@ -318,94 +331,104 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, uint32_t
     }
 }
 
-// A CTA's rings and its share of the vocabulary: [v_from, v_end) is copied, [v_from, v_to) is written.
-struct Share {
-    unsigned char *ring, *x_ring;
-    uint32_t x_bytes, k_blocks, v_from, v_end, v_to;
-};
-
-__device__ __forceinline__ void produce(const HeadArgs& a, HeadShared& s, const Share& c, const CUtensorMap* w_map,
-                                        const CUtensorMap* w_small, const CUtensorMap* x_map)
+// One of kWeightWarps threads that copy weights: a tile each in turn. (A thread takes about 150 cycles from one copy to the next.)
+__device__ __forceinline__ void copy_weights(const HeadArgs& a, HeadShared& s, const Share& c, const CUtensorMap* w_map,
+                                             const CUtensorMap* w_small, uint32_t mine)
 {
-    const uint64_t once = l2_evict_first(), often = l2_evict_last();
-    Place w, x;
-    bool ok = true;
-    auto copy_w = [&](uint32_t k, uint32_t v) {
-        if (!(ok = ok && await(s, &s.w_empty[w.slot], w.parity ^ 1u)))
-            return;
-        unsigned char* to = c.ring + w.slot * kTileBytes;
-        const uint32_t left = c.v_end - v;
-        if (left >= kTileV) {
-            mbar_arrive_expect_tx(&s.w_full[w.slot], kTileBytes);
-            tma_load_2d(to, w_map, (int32_t)(k * kBlockK), (int32_t)v, &s.w_full[w.slot], once);
-        } else { // the share's end, in steps of 16 rows; what lies behind them in the slot has no part
-            mbar_arrive_expect_tx(&s.w_full[w.slot], left * kBlockK * 2);
-            for (uint32_t i = 0; i < left; i += kGroupV)
-                tma_load_2d(to + i * kBlockK * 2, w_small, (int32_t)(k * kBlockK), (int32_t)(v + i), &s.w_full[w.slot], once);
-        }
-        w.next(a.w_slots);
-    };
-    auto copy_x = [&](uint32_t k, uint32_t t0) {
-        if (!(ok = ok && await(s, &s.x_empty[x.slot], x.parity ^ 1u)))
-            return;
-        mbar_arrive_expect_tx(&s.x_full[x.slot], c.x_bytes);
-        tma_load_2d(c.x_ring + x.slot * c.x_bytes, x_map, (int32_t)(k * kBlockK), (int32_t)t0, &s.x_full[x.slot], often);
-        x.next(a.x_slots);
-    };
-    // the c.ring's first weights are under way before the rows' order is waited for
-    const uint32_t ahead = min(min(a.w_slots / a.side, a.x_slots), c.k_blocks);
-    for (uint32_t k = 0; k < ahead; ++k)
-        for (uint32_t v = c.v_from; v < c.v_end && v < c.v_from + a.side * kTileV; v += kTileV)
-            copy_w(k, v);
+    const uint64_t policy = a.spread > 1 ? l2_evict_last() : l2_evict_first(); // do other CTAs read them too?
+    Place w;
+    uint32_t turn = 0;
+    for (uint32_t t0 = c.t_from; t0 < a.rows; t0 += c.t_step)
+        for (uint32_t v0 = c.v_from; v0 < c.v_end; v0 += a.side * kTileV)
+            for (uint32_t k0 = 0; k0 < c.k_blocks; k0 += a.turn)
+                for (uint32_t v = v0; v < c.v_end && v < v0 + a.side * kTileV; v += kTileV)
+                    for (uint32_t k = k0; k < c.k_blocks && k < k0 + a.turn; ++k) {
+                        if (turn == mine) {
+                            if (!await(s, &s.w_empty[w.slot], w.parity ^ 1u))
+                                return;
+                            unsigned char* to = c.ring + w.slot * kTileBytes;
+                            const uint32_t left = c.v_end - v;
+                            if (left >= kTileV) {
+                                mbar_arrive_expect_tx(&s.w_full[w.slot], kTileBytes);
+                                tma_load_2d(to, w_map, (int32_t)(k * kBlockK), (int32_t)v, &s.w_full[w.slot], policy);
+                            } else { // the share's end, in steps of 16 rows; what lies behind them in the slot has no part
+                                mbar_arrive_expect_tx(&s.w_full[w.slot], left * kBlockK * 2);
+                                for (uint32_t i = 0; i < left; i += kGroupV)
+                                    tma_load_2d(to + i * kBlockK * 2, w_small, (int32_t)(k * kBlockK), (int32_t)(v + i), &s.w_full[w.slot],
+                                                policy);
+                            }
+                        }
+                        w.next(a.w_slots);
+                        turn = turn + 1u == kWeightWarps ? 0u : turn + 1u;
+                    }
+}
+
+// And the one that copies hidden states, once their order is there.
+__device__ __forceinline__ void copy_rows(const HeadArgs& a, HeadShared& s, const Share& c, const CUtensorMap* x_map)
+{
+    const uint64_t policy = l2_evict_last();
+    Place x;
     griddep_wait();
-    for (uint32_t t0 = 0; t0 < a.rows && ok; t0 += a.n)
-        for (uint32_t v0 = c.v_from; v0 < c.v_end && ok; v0 += a.side * kTileV)
-            for (uint32_t k = 0; k < c.k_blocks && ok; ++k) {
-                copy_x(k, t0);
-                if (t0 != 0 || v0 != c.v_from || k >= ahead)
-                    for (uint32_t v = v0; v < c.v_end && v < v0 + a.side * kTileV; v += kTileV)
-                        copy_w(k, v);
+    for (uint32_t t0 = c.t_from; t0 < a.rows; t0 += c.t_step)
+        for (uint32_t v0 = c.v_from; v0 < c.v_end; v0 += a.side * kTileV)
+            for (uint32_t k0 = 0; k0 < c.k_blocks; k0 += a.turn) {
+                if (!await(s, &s.x_empty[x.slot], x.parity ^ 1u))
+                    return;
+                const uint32_t steps = min(a.turn, c.k_blocks - k0);
+                unsigned char* to = c.x_ring + x.slot * a.turn * c.x_bytes;
+                mbar_arrive_expect_tx(&s.x_full[x.slot], steps * c.x_bytes);
+                for (uint32_t i = 0; i < steps; ++i)
+                    tma_load_2d(to + i * c.x_bytes, x_map, (int32_t)((k0 + i) * kBlockK), (int32_t)t0, &s.x_full[x.slot], policy);
+                x.next(a.x_slots);
             }
 }
 
+// The one that issues products.
 template <typename T>
 __device__ __forceinline__ void issue(const HeadArgs& a, HeadShared& s, const Share& c)
 {
-                const uint32_t desc = mma_f16_desc(Type<T>::bf16, a.n);
-                Place w, x;
-                uint32_t buf = 0, parity = 0;
-                bool ok = true;
-                for (uint32_t t0 = 0; t0 < a.rows && ok; t0 += a.n)
-                    for (uint32_t v0 = c.v_from; v0 < c.v_end && ok; v0 += a.side * kTileV)
-                        for (uint32_t k = 0; k < c.k_blocks && ok; ++k) {
-                            if (k % kRunBlocks == 0) {
-                                if (!(ok = await(s, &s.acc_empty[buf], parity ^ 1u)))
-                                    break;
-                                tc_fence_after();
-                            }
-                            if (!(ok = await(s, &s.x_full[x.slot], x.parity)))
-                                break;
-                            const uint64_t b = smem_tile_desc(c.x_ring + x.slot * c.x_bytes);
-                            uint32_t g = 0;
-                            for (uint32_t v = v0; v < c.v_end && v < v0 + a.side * kTileV; v += kTileV, ++g) {
-                                if (!(ok = await(s, &s.w_full[w.slot], w.parity)))
-                                    break;
-                                tc_fence_after();
-                                const uint64_t d = smem_tile_desc(c.ring + w.slot * kTileBytes);
-    #pragma unroll
-                                for (uint32_t i = 0; i < kBlockK / 16; ++i)
-                                    mma_f16(s.tmem + buf * kMaxColumns + g * a.n, d + 2 * i, b + 2 * i, desc, k % kRunBlocks != 0 || i != 0);
-                                mma_commit(&s.w_empty[w.slot]);
-                                w.next(a.w_slots);
-                            }
-                            mma_commit(&s.x_empty[x.slot]);
-                            x.next(a.x_slots);
-                            if (k % kRunBlocks == kRunBlocks - 1 || k + 1 == c.k_blocks) {
-                                mma_commit(&s.acc_full[buf]);
-                                buf ^= 1u;
-                                parity ^= buf == 0;
-                            }
-                        }
+    const uint32_t desc = mma_f16_desc(Type<T>::bf16, a.n), tmem = s.tmem;
+    const uint64_t w_desc = smem_tile_desc(c.ring), x_desc = smem_tile_desc(c.x_ring);
+    Place w, x;
+    uint32_t buf = 0, parity = 0;
+    for (uint32_t t0 = c.t_from; t0 < a.rows; t0 += c.t_step)
+        for (uint32_t v0 = c.v_from; v0 < c.v_end; v0 += a.side * kTileV) {
+            const uint32_t tiles = min(a.side, (c.v_end - v0 + kTileV - 1u) / kTileV);
+            for (uint32_t k0 = 0; k0 < c.k_blocks; k0 += a.turn) {
+                const uint32_t steps = min(a.turn, c.k_blocks - k0);
+                uint32_t add = k0 % kRunBlocks != 0;
+                if (!add && !await(s, &s.acc_empty[buf], parity ^ 1u))
+                    return;
+                if (!await(s, &s.x_full[x.slot], x.parity))
+                    return;
+                const uint64_t b0 = x_desc + (x.slot * a.turn * c.x_bytes >> 4);
+                uint32_t d = tmem + buf * kMaxColumns;
+                for (uint32_t g = 0; g < tiles; ++g, d += a.n) {
+                    uint64_t b = b0;
+                    uint32_t more = add;
+                    for (uint32_t i = 0; i < steps; ++i, b += c.x_bytes >> 4) {
+                        if (!await(s, &s.w_full[w.slot], w.parity))
+                            return;
+                        tc_fence_after();
+                        const uint64_t t = w_desc + (w.slot * kTileBytes >> 4);
+                        mma_f16(d, t, b, desc, more);
+                        mma_f16(d, t + 2, b + 2, desc, true);
+                        mma_f16(d, t + 4, b + 4, desc, true);
+                        mma_f16(d, t + 6, b + 6, desc, true);
+                        mma_commit(&s.w_empty[w.slot]);
+                        w.next(a.w_slots);
+                        more = 1;
+                    }
+                }
+                mma_commit(&s.x_empty[x.slot]);
+                x.next(a.x_slots);
+                if ((k0 + steps) % kRunBlocks == 0 || k0 + steps == c.k_blocks) {
+                    mma_commit(&s.acc_full[buf]);
+                    buf = buf + 1u == a.bufs ? 0u : buf + 1u;
+                    parity ^= buf == 0;
+                }
+            }
+        }
 }
 
 template <typename T, int Columns>
@@ -421,8 +444,11 @@ __global__ void __launch_bounds__(kHeadThreads, 1)
     c.x_ring = c.ring + a.w_slots * kTileBytes;
     c.x_bytes = a.n * kBlockK * 2;
     c.k_blocks = (a.h.dim + kBlockK - 1) / kBlockK;
-    c.v_from = (uint32_t)((uint64_t)groups * blockIdx.x / gridDim.x) * kGroupV;
-    c.v_end = (uint32_t)((uint64_t)groups * (blockIdx.x + 1) / gridDim.x) * kGroupV;
+    const uint32_t shares = gridDim.x / a.spread, mine = blockIdx.x / a.spread;
+    c.v_from = (uint32_t)((uint64_t)groups * mine / shares) * kGroupV;
+    c.v_end = (uint32_t)((uint64_t)groups * (mine + 1u) / shares) * kGroupV;
+    c.t_from = blockIdx.x % a.spread * a.n;
+    c.t_step = a.spread * a.n;
     c.v_to = min(c.v_end, a.h.n_vocab);
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kMaxStages; ++i) {
@@ -446,13 +472,15 @@ __global__ void __launch_bounds__(kHeadThreads, 1)
     // 168 registers a thread at launch: 128 threads give up what 256 that drain take (128 x 40 + 256 x 232 = 384 x 168)
     if (warp >= kFirstDrain) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        drain<T, Columns>(a, s, c.v_from, c.v_to);
+        drain<T, Columns>(a, s, c);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (threadIdx.x == 0)
-            produce(a, s, c, &w_map, &w_small, &x_map);
-        else if (threadIdx.x == 32)
             issue<T>(a, s, c);
+        else if (threadIdx.x == 32)
+            copy_rows(a, s, c, &x_map);
+        else if (threadIdx.x == 64 || threadIdx.x == 96)
+            copy_weights(a, s, c, &w_map, &w_small, threadIdx.x / 32u - 2u);
     }
     __syncwarp();
     tc_fence_before();
@@ -461,7 +489,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1)
     if (s.failed) { // never seen: copies and products in flight end within this, and the share's logits say what happened
         for (int i = 0; i < 2000; ++i)
             __nanosleep(1000);
-        for (uint32_t t = 0; t < a.rows; ++t)
+        for (uint32_t t = 0; t < a.rows; ++t) // (of all rows: which ones were this CTA's is in what may have failed)
             for (uint32_t v = c.v_from + threadIdx.x; v < c.v_to; v += kHeadThreads)
                 a.logits[(size_t)t * a.ld + v] = __int_as_float(0x7fc00000);
         __syncthreads();
@@ -536,21 +564,35 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     a.logits = logits;
     a.ld = ld;
     a.rows = rows;
-    const uint32_t tiles = (rows + kMaxColumns - 1) / kMaxColumns;
+    // What the ring carries for a step of 64 of the contraction and 128 vocabulary rows is 16 KB of weights and, over the tiles side
+    // by side, the rows' 128 bytes each; rows by the 160 in CTAs side by side, which read the same weights at the same time, carry the
+    // least beyond 256.
+    const uint32_t tiles = rows <= kMaxColumns ? 1u : (rows + kOneColumns / 2 - 1) / (kOneColumns / 2);
     a.n = ((rows + tiles - 1) / tiles + 15u) & ~15u;
-    a.side = a.n <= kMaxColumns / 4 ? 4u : a.n <= kMaxColumns / 2 ? 2u : 1u;
+    a.side = a.n <= kMaxColumns / 4 ? 4u : a.n <= kOneColumns / 2 ? 2u : 1u;
+    a.bufs = a.side * a.n <= kMaxColumns ? 2u : 1u;
+    a.spread = tiles < 8u ? tiles : 8u;
     const uint32_t x_bytes = a.n * kBlockK * 2;
-    a.x_slots = a.w_slots = 0; // as deep a ring of steps of the contraction as fits
-    for (uint32_t x = 2, best = 0; x <= kMaxStages && x * x_bytes < kRingBytes; ++x) {
-        uint32_t w = (kRingBytes - x * x_bytes) / kTileBytes;
-        w = w > kMaxStages ? kMaxStages : w;
-        const uint32_t deep = w < x * a.side ? w : x * a.side;
-        if (deep > best) {
-            best = deep;
-            a.x_slots = x;
-            a.w_slots = w;
+    // What a step costs beside its bytes is the issuing thread's time, barriers mostly: steps in turns of four share one for the rows, and
+    // the weights come in pieces of 512 bytes a row. In turns of 1, 2, 4 a call without adapters of 129280 x 4096 took 190, 167, 163 us
+    // for one row, 197, 176, 175 for 64, 239, 209, 234 for 128 (whose rows fill the ring), 323, 310, 307 for 256.
+    a.turn = a.n <= kMaxColumns / 4 ? 4u : 2u;
+    // As deep a ring of tiles as fits: of rows two turns at least, of weights a tile for each of their warps (with fewer a warp could
+    // be two rounds of the ring ahead, and take a barrier's phase for another).
+    a.x_slots = a.w_slots = 0;
+    for (uint32_t best = 0; a.turn && !best; a.turn /= best ? 1u : 2u)
+        for (uint32_t x = 2; x <= kMaxStages && x * a.turn * x_bytes < kRingBytes; ++x) {
+            uint32_t w = (kRingBytes - x * a.turn * x_bytes) / kTileBytes;
+            w = w > kMaxStages ? kMaxStages : w;
+            const uint32_t deep = w < x * a.turn * a.side ? w : x * a.turn * a.side;
+            if (w >= kWeightWarps && deep > best) {
+                best = deep;
+                a.x_slots = x;
+                a.w_slots = w;
+            }
         }
-    }
+    if (a.w_slots < kWeightWarps || a.x_slots * a.turn * x_bytes + a.w_slots * kTileBytes > kRingBytes)
+        return cudaErrorInvalidConfiguration;
     CUtensorMap maps[3];
     constexpr bool bf16 = Type<T>::bf16;
     if (!encode(f, &maps[0], bf16, h.weight, h.dim, h.n_vocab, h.dim, kTileV) ||
@@ -562,13 +604,15 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     e = cudaGetLastError();
     if (e != cudaSuccess)
         return e;
-    const uint32_t groups = (h.n_vocab + kGroupV - 1) / kGroupV, grid = groups < 148u ? groups : 148u;
+    const uint32_t groups = (h.n_vocab + kGroupV - 1) / kGroupV, most = 148u / a.spread;
+    const uint32_t grid = (groups < most ? groups : most) * a.spread;
     const uint32_t half = (a.side * a.n + 1) / 2;
     const bool behind = h.n_adapters != 0;
     return half <= 32 ? launch_tiles<T, 32>(a, grid, behind, maps, stream)
            : half <= 64 ? launch_tiles<T, 64>(a, grid, behind, maps, stream)
            : half <= 96 ? launch_tiles<T, 96>(a, grid, behind, maps, stream)
-                        : launch_tiles<T, 128>(a, grid, behind, maps, stream);
+           : half <= 128 ? launch_tiles<T, 128>(a, grid, behind, maps, stream)
+                        : launch_tiles<T, 160>(a, grid, behind, maps, stream);
 }
 
 } // namespace
