@@ -274,6 +274,8 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Sh
                         if ((uint32_t)block < from || (uint32_t)block >= to)
                             continue;
                         uint32_t g = (c0 + block * kDeltas) / a.n, t = c0 + block * kDeltas - g * a.n, c = 0;
+                        if (s.adapter[t] < 0) // nor has a row behind it an adapter
+                            continue;
                         const uint32_t turn = (turns[block / 2] >> (block % 2 * 16)) | 1u;
                         while (c < kDeltas) {
                             const int32_t ad = s.adapter[t];
