@@ -506,11 +506,19 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
 
 cudaError_t encoder(EncodeTiled& f)
 {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q);
+    static std::atomic<void*> found{nullptr};
+    void* p = found.load(std::memory_order_relaxed);
+    if (!p) {
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q);
+        if (e != cudaSuccess)
+            return e;
+        if (!p || q != cudaDriverEntryPointSuccess)
+            return cudaErrorNotSupported;
+        found.store(p, std::memory_order_relaxed);
+    }
     f = reinterpret_cast<EncodeTiled>(p);
-    return e != cudaSuccess ? e : p && q == cudaDriverEntryPointSuccess ? cudaSuccess : cudaErrorNotSupported;
+    return cudaSuccess;
 }
 
 // A row-major matrix of 16-bit elements in boxes of 64 elements by `box` rows.
@@ -533,7 +541,8 @@ cudaError_t launch_tiles(const HeadArgs& a, uint32_t grid, bool behind_inner, co
     }();
     if (!split_fits)
         return cudaErrorInvalidKernelImage;
-    cudaError_t e = cudaFuncSetAttribute(head_kernel<T, Columns>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = set_once(done, head_kernel<T, Columns>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess)
         return e;
     cudaLaunchConfig_t c = {};

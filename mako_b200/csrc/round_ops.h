@@ -1,12 +1,27 @@
 // Host-visible declarations of the operators of a serving round around the sampler (internal to the library; the public
 // surface is include/mako_b200.h): the head with adapters, the verification of drafts against distributions, the page plan.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
 #include "../../include/mako_b200.h"
 
 namespace mk {
+
+// Sets a kernel's attribute, once on each of the first 64 devices: a call takes about a microsecond. `done`: the kernel's own.
+template <typename K>
+cudaError_t set_once(std::atomic<uint64_t>& done, K* kernel, cudaFuncAttribute attr, int value)
+{
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1u)))
+        return e;
+    e = cudaFuncSetAttribute(kernel, attr, value);
+    if (e == cudaSuccess && device < 64)
+        done.fetch_or(1ull << device, std::memory_order_relaxed);
+    return e;
+}
 
 constexpr uint32_t kHeadMaxRank = 128;
 // What a call with adapters needs of the handle, for its rows: `hidden` [rows][dim] of the matrices' type on a 16-byte boundary,

@@ -1219,7 +1219,8 @@ cudaError_t launch(SpecVerifyArgs a, cudaStream_t stream)
     slices = slices > room ? slices : room;
     slices = slices < a.slices ? slices : a.slices;
     a.slices = slices < most ? slices : most;
-    cudaError_t e = cudaFuncSetAttribute(spec_scan_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTiles * kTileBytes));
+    static std::atomic<uint64_t> scan_set{0}, draw_set{0};
+    cudaError_t e = set_once(scan_set, spec_scan_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTiles * kTileBytes));
     if (e != cudaSuccess)
         return e;
     const uint32_t work = rows * a.slices;
@@ -1234,7 +1235,7 @@ cudaError_t launch(SpecVerifyArgs a, cudaStream_t stream)
     while (size > 1 && a.r.n_vocab < size * 1024u)
         size >>= 1;
     if (size > 8) {
-        e = cudaFuncSetAttribute(spec_draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        e = set_once(draw_set, spec_draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess)
             return e;
     }

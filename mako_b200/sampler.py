@@ -355,21 +355,21 @@ class BatchSampler:
         sampler reads, [T, V] float32 (`out` where given)."""
         (rows, dim), v = hidden.shape, weight.shape[0]
         assert hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.stride(1) == 1
-        assert weight.dtype == hidden.dtype and weight.is_contiguous() and weight.shape[1] == dim
-        h = HeadC()
-        h.weight, h.n_vocab, h.dim, h.type = weight.data_ptr(), v, dim, _TYPE[hidden.dtype]
+        assert weight.is_cuda and weight.dtype == hidden.dtype and weight.is_contiguous() and weight.shape[1] == dim
+        d_ptr = u_ptr = s_ptr = n = rank = 0
         if adapter is not None:
-            assert adapter.dtype == torch.int32 and adapter.is_contiguous() and adapter.numel() == rows
+            assert adapter.is_cuda and adapter.dtype == torch.int32 and adapter.is_contiguous() and adapter.numel() == rows
             n, rank, _ = down.shape
-            assert down.dtype == up.dtype == hidden.dtype and down.is_contiguous() and up.is_contiguous()
-            assert down.shape == (n, rank, dim) and up.shape == (n, v, rank)
-            h.down, h.up, h.n_adapters, h.rank = down.data_ptr(), up.data_ptr(), n, rank
+            assert down.is_cuda and up.is_cuda and down.dtype == up.dtype == hidden.dtype
+            assert down.shape == (n, rank, dim) and up.shape == (n, v, rank) and down.is_contiguous() and up.is_contiguous()
+            d_ptr, u_ptr = down.data_ptr(), up.data_ptr()
             if scale is not None:
-                assert scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == n
-                h.scale = scale.data_ptr()
+                assert scale.is_cuda and scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == n
+                s_ptr = scale.data_ptr()
+        h = HeadC(weight.data_ptr(), d_ptr or None, u_ptr or None, s_ptr or None, v, dim, n, rank, _TYPE[hidden.dtype])
         if out is None:
             out = torch.empty((rows, v), dtype=torch.float32, device=hidden.device)
-        assert out.dtype == torch.float32 and out.shape == (rows, v) and out.stride(1) == 1
+        assert out.is_cuda and out.dtype == torch.float32 and out.shape == (rows, v) and out.stride(1) == 1
         check(lib.mk_head_logits(self._h, C.byref(h), hidden.data_ptr(), hidden.stride(0), _ptr(adapter), rows, out.data_ptr(),
                                  out.stride(0), _stream_ptr(self.device)))
         return out
@@ -383,28 +383,31 @@ class BatchSampler:
         n_seq, n_drafts = drafts.shape
         n_pos, v = n_drafts + 1, logits.shape[1]
         assert logits.is_cuda and logits.shape[0] == n_seq * n_pos and logits.stride(1) == 1
-        assert drafts.dtype == torch.int32 and drafts.is_contiguous()
-        assert u.shape == (n_seq, n_pos + 1) and u.dtype == torch.float32 and u.is_contiguous()
-        r = SpecRowsC()
-        r.logits, r.ld, r.type = logits.data_ptr(), logits.stride(0), _TYPE[logits.dtype]
-        r.n_seq, r.n_pos, r.n_vocab = n_seq, n_pos, v
-        r.drafts, r.u = drafts.data_ptr(), u.data_ptr()
+        assert drafts.is_cuda and drafts.dtype == torch.int32 and drafts.is_contiguous()
+        assert u.is_cuda and u.shape == (n_seq, n_pos + 1) and u.dtype == torch.float32 and u.is_contiguous()
+        q_ptr = q_ld = t_ptr = t_all = qt_ptr = m_ptr = m_ld = 0
         if draft_logits is not None:
-            assert draft_logits.dtype == logits.dtype and draft_logits.shape == (n_seq * n_drafts, v)
-            assert draft_logits.stride(1) == 1
-            r.draft_logits, r.draft_ld = draft_logits.data_ptr(), draft_logits.stride(0)
+            assert draft_logits.is_cuda and draft_logits.dtype == logits.dtype and draft_logits.shape == (n_seq * n_drafts, v)
+            q_ld, unit = draft_logits.stride()
+            assert unit == 1
+            q_ptr = draft_logits.data_ptr()
         if isinstance(temperature, torch.Tensor):
-            assert temperature.dtype == torch.float32 and temperature.shape == (n_seq,) and temperature.is_contiguous()
-            r.temperature = temperature.data_ptr()
+            assert temperature.is_cuda and temperature.dtype == torch.float32 and temperature.shape == (n_seq,)
+            assert temperature.is_contiguous()
+            t_ptr = temperature.data_ptr()
         else:
-            r.temperature_all = temperature
+            t_all = temperature
         if draft_temperature is not None:
-            assert draft_temperature.dtype == torch.float32 and draft_temperature.shape == (n_seq,)
-            assert draft_temperature.is_contiguous()
-            r.draft_temperature = draft_temperature.data_ptr()
+            assert draft_temperature.is_cuda and draft_temperature.dtype == torch.float32
+            assert draft_temperature.shape == (n_seq,) and draft_temperature.is_contiguous()
+            qt_ptr = draft_temperature.data_ptr()
         if mask is not None:
-            assert mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos and mask.stride(1) == 1
-            r.mask, r.mask_ld, r.mask_drafts = mask.data_ptr(), mask.stride(0), int(mask_drafts)
+            assert mask.is_cuda and mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos
+            m_ld, unit = mask.stride()
+            assert unit == 1
+            m_ptr = mask.data_ptr()
+        r = SpecRowsC(logits.data_ptr(), logits.stride(0), q_ptr or None, q_ld, _TYPE[logits.dtype], n_seq, n_pos, v,
+                      drafts.data_ptr(), u.data_ptr(), t_ptr or None, qt_ptr or None, t_all, m_ptr or None, m_ld, int(mask_drafts))
         kept, nxt, flags = torch.empty((3, n_seq), dtype=torch.int32, device=self.device).unbind()
         tokens = torch.empty((n_seq, n_pos), dtype=torch.int32, device=self.device)
         logprob = torch.empty((n_seq, n_pos), dtype=torch.float32, device=self.device)
@@ -418,26 +421,25 @@ class BatchSampler:
         block_table [S, columns], n_pages [S], free_list [P] and n_free [1] int32 are updated in place; cache_len [S] tokens are
         in the cache, n_new [S] come with the pass (None: pages above the need go back, and that is all). Fills and returns
         `out` (KvPlan.empty)."""
-        n_seq, cols = block_table.shape
-        for t in (block_table, n_pages, free_list, n_free, cache_len):
-            assert t.is_cuda and t.dtype == torch.int32
-        assert block_table.stride(1) == 1 and n_pages.is_contiguous() and cache_len.is_contiguous() and free_list.is_contiguous()
+        (n_seq, cols), (ld, unit), i32 = block_table.shape, block_table.stride(), torch.int32
+        assert block_table.dtype == n_pages.dtype == free_list.dtype == n_free.dtype == cache_len.dtype == i32 and unit == 1
+        assert block_table.is_cuda and n_pages.is_cuda and free_list.is_cuda and n_free.is_cuda and cache_len.is_cuda
+        assert n_pages.is_contiguous() and cache_len.is_contiguous() and free_list.is_contiguous()
         assert n_pages.numel() == cache_len.numel() == n_seq and n_free.numel() == 1
-        p, o = KvPagesC(), KvPlanC()
-        p.block_table, p.table_ld, p.table_cols = block_table.data_ptr(), block_table.stride(0), cols
-        p.n_pages, p.free_list, p.free_cap = n_pages.data_ptr(), free_list.data_ptr(), free_list.numel()
-        p.n_free, p.page_size = n_free.data_ptr(), page_size
+        p = KvPagesC(block_table.data_ptr(), ld, cols, n_pages.data_ptr(), free_list.data_ptr(), free_list.numel(),
+                     n_free.data_ptr(), page_size)
         if n_new is not None:
-            assert n_new.dtype == torch.int32 and n_new.is_contiguous() and n_new.numel() == n_seq and out is not None
-        if out is not None:
-            t = out.positions.numel()
-            for x, n in ((out.query_start, n_seq + 1), (out.kv_len, n_seq), (out.positions, t), (out.token_seq, t),
-                         (out.flags, n_seq)):
-                assert x.dtype == torch.int32 and x.numel() == n and x.is_contiguous()
-            assert out.slots.dtype == torch.int64 and out.slots.numel() == t and out.slots.is_contiguous()
-            o.query_start, o.kv_len, o.positions = out.query_start.data_ptr(), out.kv_len.data_ptr(), out.positions.data_ptr()
-            o.slots, o.token_seq, o.flags = out.slots.data_ptr(), out.token_seq.data_ptr(), out.flags.data_ptr()
-            o.max_tokens = t
+            assert n_new.is_cuda and n_new.dtype == i32 and n_new.is_contiguous() and n_new.numel() == n_seq and out is not None
+        if out is None:
+            o = KvPlanC()
+        else:
+            start, kv_len, pos, slots, seq, flags = out.query_start, out.kv_len, out.positions, out.slots, out.token_seq, out.flags
+            t = pos.numel()
+            assert start.numel() == n_seq + 1 and kv_len.numel() == flags.numel() == n_seq and slots.numel() == seq.numel() == t
+            assert start.dtype == kv_len.dtype == pos.dtype == seq.dtype == flags.dtype == i32 and slots.dtype == torch.int64
+            assert start.is_contiguous() and kv_len.is_contiguous() and pos.is_contiguous() and slots.is_contiguous()
+            assert seq.is_contiguous() and flags.is_contiguous() and start.is_cuda and slots.is_cuda
+            o = KvPlanC(start.data_ptr(), kv_len.data_ptr(), pos.data_ptr(), slots.data_ptr(), seq.data_ptr(), flags.data_ptr(), t)
         check(lib.mk_kv_plan_step(self._h, C.byref(p), cache_len.data_ptr(), _ptr(n_new), n_seq, C.byref(o),
                                   _stream_ptr(self.device)))
         return out
