@@ -34,7 +34,7 @@ constexpr uint32_t kScanThreads = kVerifyThreads + 64; // and a warp that copies
 constexpr uint32_t kSteps = 16;   // of the table of exp2
 constexpr uint32_t kParts = 8;   // of a warp's share of a row
 constexpr float kNear = 3e-5f;    // decisions nearer than this, relative, are taken in 64 bits
-constexpr double kSome = 1e-290;   // a weight below this is none
+constexpr double kSome = 1e-290;   // a weight below this, where the largest is about 1, is none
 constexpr float kHottest = 1e30f;  // a temperature from here on is not one
 constexpr float kInf = __builtin_huge_valf();
 
@@ -170,7 +170,7 @@ struct Row {
     __device__ void weighed(const Mass& a)
     {
         mass = a;
-        lowest = fmaxf(a.m - 693.0f * t, -3.4e38f);
+        lowest = fmaxf((a.m - base()) - 693.0f * t, -3.4e38f);
     }
     __device__ bool none() const { return mass.m == -kInf; }
     __device__ bool far() const { return !none() && !single() && !(fabsf(__fmul_rn(mass.m, scale)) < kFar); }
@@ -681,7 +681,7 @@ __device__ __forceinline__ void weights64(const Weigh<T>& row, const float (&x)[
     uint32_t n[N];
 #pragma unroll
     for (int i = 0; i < N; ++i)
-        d[i] = (double)(fmaxf(x[i], row.lowest) - row.base);
+        d[i] = (double)fmaxf(x[i] - row.base, row.lowest);
 #pragma unroll
     for (int i = 0; i < N; ++i)
         r[i] = fma(d[i], row.steps, shift);
@@ -723,7 +723,7 @@ __device__ __forceinline__ double weight_of(const Row<T>& row, uint32_t i, uint3
     const float x[1] = {row.get(i)};
     double w[1];
     weights64(Weigh<T>(row), x, w, table);
-    return w[0];
+    return w[0] > kSome ? w[0] : 0.0;
 }
 
 // x where that is above 0, else 0: no branch, no comparison of 64 bits.

@@ -66,7 +66,9 @@ def compare(sampler, c, pad=0, offset=0, **kw):
         assert tokens[i].tolist() == toks, i
         # log P: a rounding to fp32, and what rows of fp32 exponentials leave of the sum
         assert np.allclose(lp[i], logs, rtol=2.0 ** -22, atol=2e-6), (i, lp[i], logs)
-    assert sure >= 0.9 * len(want)
+    # that few are passed over: a tenth, or one of a few (of far_from_one's eight rows one has a draft of 1.7e-299 of the whole, which
+    # is less than the 1e-290 that weigh anything)
+    assert sure >= len(want) - max(1, len(want) // 10)
     return got
 
 
