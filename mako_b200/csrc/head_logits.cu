@@ -32,7 +32,7 @@ constexpr uint32_t kDrainWarps = 8, kFirstDrain = 4, kHeadThreads = 32 * (kFirst
 constexpr uint32_t kRankStep = 16;                  // ranks that a lane holds of `up` at a time
 constexpr uint32_t kDeltas = 16;                   // columns that the adapters' part is formed for at a time
 constexpr uint32_t kMaxColumns = 256;              // of one of two accumulators: vocabulary tiles x rows
-constexpr uint32_t kMaxRows = 160;                 // of a tile: twice that is one accumulator, what the draining warps have registers for
+constexpr uint32_t kPairRows = 160;                // of two tiles side by side: one accumulator, what the draining warps have registers for
 constexpr uint32_t kMaxStages = 16;
 constexpr uint32_t kRingBytes = 180 * 1024;
 
@@ -148,7 +148,7 @@ struct HeadArgs {
     uint64_t ld;
     uint32_t rows;
     uint32_t n;            // rows of a tile, a multiple of 16
-    uint32_t side;         // vocabulary tiles side by side, 4 or 2
+    uint32_t side;         // vocabulary tiles side by side: 4, 2 or 1
     uint32_t bufs;         // accumulators of side * n columns: two of up to 256, or one of up to 320
     uint32_t spread;       // row tiles that CTAs side by side have at the same time
     uint32_t turn;         // steps of the contraction that a vocabulary tile is copied for before the next one's turn: 1, 2 or 4
@@ -160,9 +160,14 @@ struct HeadShared {
     uint64_t acc_full[2], acc_empty[2];
     uint32_t tmem;
     int failed;
-    int32_t row[kMaxRows + kDeltas], adapter[kMaxRows + kDeltas]; // of the tile's columns, and none behind them
-    float4 inner[kMaxRows + kDeltas][kRankStep / 4];
-    float2 delta[kDrainWarps][kDeltas][32]; // each thread's own; kept here because registers take no running index
+    int32_t row[kMaxColumns], adapter[kMaxColumns]; // of the tile's columns
+};
+
+// And what the adapters' part needs, where a draining thread has so many vocabulary tiles.
+template <int Tiles>
+struct DrainShared {
+    float4 inner[Tiles == 2 ? kPairRows : kMaxColumns][kRankStep / 4];
+    float delta[kDrainWarps][kDeltas][32][Tiles]; // each thread's own; kept here because registers take no running index
 };
 
 // A ring's place: slot and the parity its barriers complete with next.
@@ -199,16 +204,17 @@ struct Share {
     uint32_t t_from, t_step; // its row tiles
 };
 
-// A draining thread has a lane, which is a vocabulary row, of two tiles side by side, and up to Rows of the batch's rows in either. Two,
-// because what the adapters' part costs is reading `inner`: a float4 that all lanes of a warp share takes shared memory, of which the
-// products' operands want all but 10 %, as long as 32 of them, and now serves two vocabulary rows.
-template <typename T, int Rows>
-__device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Share& c)
+// A draining thread has a lane, which is a vocabulary row, of one or two tiles side by side, and up to Rows of the batch's rows in each.
+// Two where they fit, because what the adapters' part costs is reading `inner`: a float4 that all lanes of a warp share takes shared
+// memory, of which the products' operands want all but a tenth, as long as 32 of them, and so serves two vocabulary rows (320 rows with
+// adapters of rank 64 at 151552 x 4096: 690 us, with one tile a thread 868; without adapters 435).
+template <typename T, int Tiles, int Rows>
+__device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, DrainShared<Tiles>& own, const Share& c)
 {
     const uint32_t v_from = c.v_from, v_to = c.v_to;
     const uint32_t tid = threadIdx.x - 32u * kFirstDrain, w = tid / 32u, lane = tid & 31u;
     const uint32_t quarter = w & 3u; // of the lanes, the one that this warp may read
-    // four tiles: two for each four warps; two: half of the rows for each
+    // four tiles: two for each four warps; fewer: half of the rows for each
     const uint32_t g0 = a.side == 4u ? w / 4u * 2u : 0u, m = a.side == 4u ? a.n : a.n / 2u, row0 = a.side == 4u ? 0u : w / 4u * m;
     const uint32_t k_blocks = (a.h.dim + kBlockK - 1) / kBlockK, runs = (k_blocks + kRunBlocks - 1) / kRunBlocks;
     const uint32_t steps = a.h.n_adapters ? (a.h.rank + kRankStep - 1) / kRankStep : 0u;
@@ -216,14 +222,14 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Sh
     const uint32_t units = steps * blocks;
     const uint32_t tmem = s.tmem + ((quarter * 32u) << 16) + g0 * a.n + row0;
     const T* up = static_cast<const T*>(a.h.up);
-    float acc[2][Rows];
+    float acc[Tiles][Rows];
     uint32_t buf = 0, parity = 0;
     bool alive = true;
     griddep_wait(); // for the rows' order and `inner`
     for (uint32_t t0 = c.t_from; t0 < a.rows; t0 += c.t_step) {
         named_barrier(1, kDrainWarps * 32);
-        if (tid < kMaxRows + kDeltas) {
-            const bool real = tid < a.n && t0 + tid < a.rows;
+        if (tid < a.n) {
+            const bool real = t0 + tid < a.rows;
             s.row[tid] = !real ? -1 : steps ? a.order.row[t0 + tid] : (int32_t)(t0 + tid);
             s.adapter[tid] = real && steps ? a.order.adapter[t0 + tid] : -1;
         }
@@ -235,24 +241,25 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Sh
             turns[k] = __ballot_sync(~0u, i < m && (i == 0 || s.adapter[t] != s.adapter[t - 1u]));
         }
         for (uint32_t v0 = v_from; v0 < v_to; v0 += a.side * kTileV) {
-            const uint32_t v = v0 + g0 * kTileV + quarter * 32u + lane; // in the first of the two tiles
+            const uint32_t v = v0 + g0 * kTileV + quarter * 32u + lane; // in the first of its tiles
 #pragma unroll
             for (int i = 0; i < Rows; ++i)
-                acc[0][i] = acc[1][i] = 0.0f;
+                acc[0][i] = acc[Tiles - 1][i] = 0.0f;
             uint32_t unit = 0;
             for (uint32_t run = 0; run < runs; ++run) {
                 alive = alive && await(s, &s.acc_full[buf], parity); // a warp that gave up still meets the others' barriers
                 tc_fence_after();
 #pragma unroll
-                for (int i = 0; i < Rows; i += 16) { // (columns behind the rows that are its own hold anything, and are not written)
+                for (int i = 0; i < Rows; i += 32 / Tiles) { // (columns behind the rows that are its own hold anything, and are not written)
+                    const int j = Tiles == 2 ? i : i + 16;
                     float x[2][16];
                     tmem_load16(x[0], tmem + buf * kMaxColumns + i);
-                    tmem_load16(x[1], tmem + buf * kMaxColumns + a.n + i);
+                    tmem_load16(x[1], tmem + buf * kMaxColumns + (Tiles == 2 ? a.n : 0u) + j);
                     tmem_wait(x[0], x[1]);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         acc[0][i + k] += x[0][k];
-                        acc[1][i + k] += x[1][k];
+                        acc[Tiles - 1][j + k] += x[1][k];
                     }
                 }
                 tc_fence_before();
@@ -273,7 +280,7 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Sh
                             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             if (t0 + t < a.rows && q * 4u < left)
                                 y = __ldg(reinterpret_cast<const float4*>(a.order.inner + (size_t)(t0 + t) * kHeadMaxRank + r) + q);
-                            s.inner[t][q] = y;
+                            own.inner[t][q] = y;
                         }
                         named_barrier(1, kDrainWarps * 32);
                     }
@@ -287,9 +294,9 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Sh
                         const uint32_t turn = (turns[block / 2] >> (block % 2 * 16)) | 1u, last = min(kDeltas, m - block * kDeltas);
                         while (c < last) {
                             const int32_t ad = s.adapter[t];
-                            float2 x[2][kRankStep / 2];
+                            float2 x[Tiles][kRankStep / 2];
 #pragma unroll
-                            for (int g = 0; g < 2; ++g) {
+                            for (int g = 0; g < Tiles; ++g) {
 #pragma unroll
                                 for (int i = 0; i < (int)kRankStep / 2; ++i)
                                     x[g][i] = make_float2(0.0f, 0.0f);
@@ -302,28 +309,30 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Sh
                             }
                             const uint32_t later = (turn >> c) >> 1;
                             const uint32_t end = later ? min(c + (uint32_t)__ffs(later), last) : last;
-                            const float4(*y)[kRankStep / 4] = &s.inner[t];
+                            const float4(*y)[kRankStep / 4] = &own.inner[t];
                             t += end - c;
 #pragma unroll 2
                             for (; c < end; ++c, ++y) {
-                                float2 d[2] = {}, e[2] = {};
+                                float2 d[Tiles] = {}, e[Tiles] = {};
 #pragma unroll
                                 for (int i = 0; i < (int)kRankStep / 4; ++i) {
                                     const float4 z = (*y)[i];
 #pragma unroll
-                                    for (int g = 0; g < 2; ++g) {
+                                    for (int g = 0; g < Tiles; ++g) {
                                         d[g] = fma2(x[g][2 * i], make_float2(z.x, z.y), d[g]);
                                         e[g] = fma2(x[g][2 * i + 1], make_float2(z.z, z.w), e[g]);
                                     }
                                 }
-                                s.delta[w][c][lane] = make_float2((d[0].x + e[0].x) + (d[0].y + e[0].y), (d[1].x + e[1].x) + (d[1].y + e[1].y));
+#pragma unroll
+                                for (int g = 0; g < Tiles; ++g)
+                                    own.delta[w][c][lane][g] = (d[g].x + e[g].x) + (d[g].y + e[g].y);
                             }
                         }
 #pragma unroll
                         for (int k = 0; k < (int)kDeltas; ++k) { // (behind the last row what an earlier block left)
-                            const float2 d = s.delta[w][k][lane];
-                            acc[0][block * (int)kDeltas + k] += d.x;
-                            acc[1][block * (int)kDeltas + k] += d.y;
+#pragma unroll
+                            for (int g = 0; g < Tiles; ++g)
+                                acc[g][block * (int)kDeltas + k] += own.delta[w][k][lane][g];
                         }
                     }
                 }
@@ -333,10 +342,10 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, const Sh
                 const int32_t row = (uint32_t)k < m ? s.row[row0 + k] : -1;
                 if (row >= 0) {
                     float* p = a.logits + (size_t)row * a.ld + v;
-                    if (v < v_to)
-                        p[0] = acc[0][k];
-                    if (v + kTileV < v_to)
-                        p[kTileV] = acc[1][k];
+#pragma unroll
+                    for (int g = 0; g < Tiles; ++g)
+                        if (v + g * kTileV < v_to)
+                            p[g * kTileV] = acc[g][k];
                 }
             }
         }
@@ -443,13 +452,14 @@ __device__ __forceinline__ void issue(const HeadArgs& a, HeadShared& s, const Sh
         }
 }
 
-template <typename T, int Rows>
+template <typename T, int Tiles, int Rows>
 __global__ void __launch_bounds__(kHeadThreads, 1)
     head_kernel(const HeadArgs a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap w_small,
                 const __grid_constant__ CUtensorMap x_map)
 {
     extern __shared__ unsigned char raw[];
     __shared__ HeadShared s;
+    __shared__ DrainShared<Tiles> own;
     const uint32_t warp = threadIdx.x / 32u, groups = (a.h.n_vocab + kGroupV - 1) / kGroupV;
     Share c;
     c.ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
@@ -484,7 +494,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1)
     // 168 registers a thread at launch: 128 threads give up what 256 that drain take (128 x 40 + 256 x 232 = 384 x 168)
     if (warp >= kFirstDrain) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        drain<T, Rows>(a, s, c);
+        drain<T, Tiles, Rows>(a, s, own, c);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (threadIdx.x == 0)
@@ -541,18 +551,18 @@ bool encode(EncodeTiled f, CUtensorMap* map, bool bf16, const void* base, uint64
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int Rows>
+template <typename T, int Tiles, int Rows>
 cudaError_t launch_tiles(const HeadArgs& a, uint32_t grid, bool behind_inner, const CUtensorMap* maps, cudaStream_t stream)
 {
     const size_t smem = kRingBytes + 1024;
     static const bool split_fits = [] { // the registers that the warps share out among themselves are those of the launch
         cudaFuncAttributes f;
-        return cudaFuncGetAttributes(&f, head_kernel<T, Rows>) == cudaSuccess && f.numRegs == 168;
+        return cudaFuncGetAttributes(&f, head_kernel<T, Tiles, Rows>) == cudaSuccess && f.numRegs == 168;
     }();
     if (!split_fits)
         return cudaErrorInvalidKernelImage;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = set_once(done, head_kernel<T, Rows>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = set_once(done, head_kernel<T, Tiles, Rows>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess)
         return e;
     cudaLaunchConfig_t c = {};
@@ -565,7 +575,7 @@ cudaError_t launch_tiles(const HeadArgs& a, uint32_t grid, bool behind_inner, co
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     c.attrs = attr;
     c.numAttrs = behind_inner ? 1 : 0;
-    return cudaLaunchKernelEx(&c, head_kernel<T, Rows>, a, maps[0], maps[1], maps[2]);
+    return cudaLaunchKernelEx(&c, head_kernel<T, Tiles, Rows>, a, maps[0], maps[1], maps[2]);
 }
 
 template <typename T>
@@ -588,9 +598,9 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     // What the ring carries for a step of 64 of the contraction and 128 vocabulary rows is 16 KB of weights and, over the tiles side
     // by side, the rows' 128 bytes each; rows by the 160 in CTAs side by side, which read the same weights at the same time, carry the
     // least beyond 256.
-    const uint32_t tiles = (rows + kMaxRows - 1) / kMaxRows;
+    const uint32_t tiles = rows <= kMaxColumns ? 1u : (rows + kPairRows - 1) / kPairRows;
     a.n = ((rows + tiles - 1) / tiles + 15u) & ~15u;
-    a.side = a.n <= kMaxColumns / 4 ? 4u : 2u;
+    a.side = a.n <= kMaxColumns / 4 ? 4u : a.n <= kPairRows ? 2u : 1u;
     a.bufs = a.side * a.n <= kMaxColumns ? 2u : 1u;
     a.spread = tiles < 8u ? tiles : 8u;
     const uint32_t x_bytes = a.n * kBlockK * 2;
@@ -629,11 +639,13 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     const uint32_t grid = (groups < most ? groups : most) * a.spread;
     const uint32_t half = a.side == 4u ? a.n : a.n / 2u;
     const bool behind = h.n_adapters != 0;
-    return half <= 16 ? launch_tiles<T, 16>(a, grid, behind, maps, stream)
-           : half <= 32 ? launch_tiles<T, 32>(a, grid, behind, maps, stream)
-           : half <= 48 ? launch_tiles<T, 48>(a, grid, behind, maps, stream)
-           : half <= 64 ? launch_tiles<T, 64>(a, grid, behind, maps, stream)
-                        : launch_tiles<T, 80>(a, grid, behind, maps, stream);
+    return half <= 16 ? launch_tiles<T, 2, 16>(a, grid, behind, maps, stream)
+           : half <= 32 ? launch_tiles<T, 2, 32>(a, grid, behind, maps, stream)
+           : half <= 48 ? launch_tiles<T, 2, 48>(a, grid, behind, maps, stream)
+           : half <= 64 ? launch_tiles<T, 2, 64>(a, grid, behind, maps, stream)
+           : half <= 80 ? launch_tiles<T, 2, 80>(a, grid, behind, maps, stream)
+           : half <= 96 ? launch_tiles<T, 1, 96>(a, grid, behind, maps, stream)
+                        : launch_tiles<T, 1, 128>(a, grid, behind, maps, stream);
 }
 
 } // namespace
