@@ -98,3 +98,26 @@ def test_a_handle_after_its_neighbours_calls(gpu_sampler_factory):
     for _ in range(3):
         assert torch.equal(h.sample(logits, p, u).token, first)
         assert torch.equal(h.head_logits(**c), second)
+
+
+@pytest.mark.parametrize("rows", [9, 25, 47, 64, 81, 112, 145, 160, 161, 192, 225, 256, 310])
+def test_heads_of_several_tiles_a_share(rows):
+    """Every number of vocabulary tiles and rows that a thread has, with shares of the vocabulary that fill no number of them."""
+    from mako_b200 import BatchSampler
+    head.compare(BatchSampler(60007, 512), head.make(rows, rows, 60007, 136, 40, 6, torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows", [48, 130, 230])
+def test_an_adapters_infinities_stay_its_own(gpu_sampler_factory, rows):
+    c = head.make(11, rows, 1500, 128, 24, 5, torch.bfloat16)
+    sampler = gpu_sampler_factory(129280, 512)
+    gpu = {k: x.cuda() for k, x in c.items()}
+    call = lambda: sampler.head_logits(gpu["hidden"], gpu["weight"], **{k: gpu[k] for k in ("adapter", "down", "up", "scale")}).cpu()  # noqa: E731
+    before = call().clone()
+    gpu["up"][2, 700:1100:100] = math.inf
+    gpu["up"][2, 900] = math.nan
+    after = call()
+    hit = torch.zeros(rows, 1500, dtype=torch.bool)
+    hit[(c["adapter"] == 2).nonzero(), torch.arange(700, 1100, 100)] = True
+    assert hit.any() and not after[hit].isfinite().any()
+    assert torch.equal(after[~hit], before[~hit])
