@@ -274,8 +274,9 @@ typedef struct mk_head {
  *   logits[t][v] = sum_k weight[v][k] hidden[t][k] + scale[a] sum_r up[a][v][r] (sum_k down[a][r][k] hidden[t][k]),  a = adapter[t].
  * adapter [rows] names each row's adapter, in any order; one outside [0, n_adapters) and a NULL array mean none. Products are
  * exact, sums are in fp32, the inner sums stay in fp32 between the two projections. rows is at most the handle's max_batch,
- * n_vocab at most its n_vocab, and with adapters rows * dim at most 8 * max_batch times its n_vocab; hidden_ld is a multiple of 8; columns behind n_vocab of a logits row are left as they are. No
- * row's values reach another row. Calls on one handle must not overlap (they share its scratch). */
+ * n_vocab at most its n_vocab, and with adapters rows * dim at most 8 * max_batch times its n_vocab; hidden_ld is a multiple
+ * of 8; columns behind n_vocab of a logits row are left as they are. No row's values reach another row. Calls on one handle
+ * must not overlap (they share its scratch). */
 int mk_head_logits(mk_sampler* s, const mk_head* head, const void* hidden, uint64_t hidden_ld, const int32_t* adapter,
                    uint32_t rows, float* logits, uint64_t ld, void* stream);
 
