@@ -14,7 +14,7 @@
 // Precision: the tensor core's fp32 accumulator truncates, 1.0e-6 of the result for every 1024 terms, all of it towards zero
 // (measured against 64 bits). So a run of 512 terms goes into one of two accumulators and is added in registers, rounding to
 // nearest, while the next run goes into the other. `inner` stays in fp32; its products with `up` are FMAs of the draining warps,
-// 16 ranks at a time between the runs: rows of one adapter stand side by side, so that a lane's piece of `up` is loaded once for
+// 16 or 32 ranks at a time between the runs: rows of one adapter stand side by side, so that a lane's piece of `up` is loaded once for
 // all of them. (As MMAs they would want `inner` cut to 16 bits, and one adapter's infinite weight would reach other rows as 0 x inf.)
 #include "round_ops.h"
 #include "tcgen05.cuh"
@@ -31,12 +31,13 @@ constexpr uint32_t kTileV = 128, kGroupV = 16;     // vocabulary rows of a tile;
 constexpr uint32_t kTileBytes = kTileV * kBlockK * 2;
 constexpr uint32_t kWeightWarps = 2;                // that copy weights; before them one issues products, one copies rows
 constexpr uint32_t kDrainWarps = 8, kFirstDrain = 4, kHeadThreads = 32 * (kFirstDrain + kDrainWarps);
-constexpr uint32_t kRankStep = 16;                  // ranks that a lane holds of `up` at a time
+constexpr int kRankStep = 16, kWideStep = 32;      // ranks that a lane holds of `up` at a time; where few rows leave registers for more
+constexpr uint32_t kWideRows = 96;
 constexpr uint32_t kDeltas = 16;                   // columns that the adapters' part is formed for at a time
 constexpr uint32_t kMaxColumns = 256;              // of one of two accumulators: vocabulary tiles x rows
 constexpr uint32_t kPairRows = 160;                // of two tiles side by side: one accumulator, what the draining warps have registers for
 constexpr uint32_t kMaxStages = 16;
-constexpr uint32_t kRingBytes = 180 * 1024;
+constexpr uint32_t kRingBytes = 178 * 1024;
 
 __device__ __forceinline__ float2 pair_to_float(__nv_bfloat162 x) { return __bfloat1622float2(x); }
 __device__ __forceinline__ float2 pair_to_float(__half2 x) { return __half22float2(x); }
@@ -166,9 +167,9 @@ struct HeadShared {
 };
 
 // And what the adapters' part needs, where a draining thread has so many vocabulary tiles.
-template <int Tiles>
+template <int Tiles, int Step>
 struct DrainShared {
-    float4 inner[Tiles == 2 ? kPairRows : kMaxColumns][kRankStep / 4];
+    float4 inner[Step == kWideStep ? kWideRows : Tiles == 2 ? kPairRows : kMaxColumns][Step / 4];
     float delta[kDrainWarps][kDeltas][32][Tiles]; // each thread's own; kept here because registers take no running index
 };
 
@@ -210,8 +211,8 @@ struct Share {
 // Two where they fit, because what the adapters' part costs is reading `inner`: a float4 that all lanes of a warp share takes shared
 // memory, of which the products' operands want all but a tenth, as long as 32 of them, and so serves two vocabulary rows (320 rows with
 // adapters of rank 64 at 151552 x 4096: 690 us, with one tile a thread 868; without adapters 435).
-template <typename T, int Tiles, int Rows>
-__device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, DrainShared<Tiles>& own, const Share& c)
+template <typename T, int Tiles, int Rows, int Step>
+__device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, DrainShared<Tiles, Step>& own, const Share& c)
 {
     const uint32_t v_from = c.v_from, v_to = c.v_to;
     const uint32_t tid = threadIdx.x - 32u * kFirstDrain, w = tid / 32u, lane = tid & 31u;
@@ -219,7 +220,7 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, DrainSha
     // four tiles: two for each four warps; fewer: half of the rows for each
     const uint32_t g0 = a.side == 4u ? w / 4u * 2u : 0u, m = a.side == 4u ? a.n : a.n / 2u, row0 = a.side == 4u ? 0u : w / 4u * m;
     const uint32_t k_blocks = (a.h.dim + kBlockK - 1) / kBlockK, runs = (k_blocks + kRunBlocks - 1) / kRunBlocks;
-    const uint32_t steps = a.h.n_adapters ? (a.h.rank + kRankStep - 1) / kRankStep : 0u;
+    const uint32_t steps = a.h.n_adapters ? (a.h.rank + Step - 1) / Step : 0u;
     constexpr uint32_t blocks = Rows / kDeltas;
     const uint32_t units = steps * blocks;
     const uint32_t tmem = s.tmem + ((quarter * 32u) << 16) + g0 * a.n + row0;
@@ -270,15 +271,15 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, DrainSha
                     mbar_arrive(&s.acc_empty[buf]);
                 buf = buf + 1u == a.bufs ? 0u : buf + 1u;
                 parity ^= buf == 0;
-                // this run's part of the adapters' work, which is 16 ranks of 16 rows at a time
+                // this run's part of the adapters' work, which is Step ranks of 16 rows at a time
                 for (const uint32_t until = ((run + 1u) * units + runs - 1u) / runs; unit < until;) {
-                    const uint32_t r = unit / blocks * kRankStep, left = a.h.rank - r, from = unit % blocks;
+                    const uint32_t r = unit / blocks * Step, left = a.h.rank - r, from = unit % blocks;
                     const uint32_t to = min(blocks, from + until - unit);
                     unit += to - from;
                     if (from == 0 && (steps > 1 || v0 == v_from)) {
                         named_barrier(1, kDrainWarps * 32); // the ranks before these have been used
-                        for (uint32_t i = tid; i < a.n * (kRankStep / 4); i += kDrainWarps * 32) {
-                            const uint32_t t = i / (kRankStep / 4), q = i % (kRankStep / 4);
+                        for (uint32_t i = tid; i < a.n * (Step / 4); i += kDrainWarps * 32) {
+                            const uint32_t t = i / (Step / 4), q = i % (Step / 4);
                             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             if (t0 + t < a.rows && q * 4u < left)
                                 y = __ldg(reinterpret_cast<const float4*>(a.order.inner + (size_t)(t0 + t) * kHeadMaxRank + r) + q);
@@ -296,28 +297,30 @@ __device__ __forceinline__ void drain(const HeadArgs& a, HeadShared& s, DrainSha
                         const uint32_t turn = (turns[block / 2] >> (block % 2 * 16)) | 1u, last = min(kDeltas, m - block * kDeltas);
                         while (c < last) {
                             const int32_t ad = s.adapter[t];
-                            float2 x[Tiles][kRankStep / 2];
+                            float2 x[Tiles][Step / 2];
 #pragma unroll
                             for (int g = 0; g < Tiles; ++g) {
 #pragma unroll
-                                for (int i = 0; i < (int)kRankStep / 2; ++i)
+                                for (int i = 0; i < (int)Step / 2; ++i)
                                     x[g][i] = make_float2(0.0f, 0.0f);
                                 if (ad >= 0 && v + g * kTileV < v_to) {
                                     const T* p = up + ((size_t)ad * a.h.n_vocab + v + g * kTileV) * a.h.rank + r;
                                     load8(*reinterpret_cast<float2(*)[4]>(&x[g][0]), p);
-                                    if (left > 8u)
-                                        load8(*reinterpret_cast<float2(*)[4]>(&x[g][4]), p + 8);
+#pragma unroll
+                                    for (int i = 8; i < Step; i += 8)
+                                        if (left > (uint32_t)i)
+                                            load8(*reinterpret_cast<float2(*)[4]>(&x[g][i / 2]), p + i);
                                 }
                             }
                             const uint32_t later = (turn >> c) >> 1;
                             const uint32_t end = later ? min(c + (uint32_t)__ffs(later), last) : last;
-                            const float4(*y)[kRankStep / 4] = &own.inner[t];
+                            const float4(*y)[Step / 4] = &own.inner[t];
                             t += end - c;
 #pragma unroll 2
                             for (; c < end; ++c, ++y) {
                                 float2 d[Tiles] = {}, e[Tiles] = {};
 #pragma unroll
-                                for (int i = 0; i < (int)kRankStep / 4; ++i) {
+                                for (int i = 0; i < (int)Step / 4; ++i) {
                                     const float4 z = (*y)[i];
 #pragma unroll
                                     for (int g = 0; g < Tiles; ++g) {
@@ -454,14 +457,14 @@ __device__ __forceinline__ void issue(const HeadArgs& a, HeadShared& s, const Sh
         }
 }
 
-template <typename T, int Tiles, int Rows>
+template <typename T, int Tiles, int Rows, int Step>
 __global__ void __launch_bounds__(kHeadThreads, 1)
     head_kernel(const HeadArgs a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap w_small,
                 const __grid_constant__ CUtensorMap x_map)
 {
     extern __shared__ unsigned char raw[];
     __shared__ HeadShared s;
-    __shared__ DrainShared<Tiles> own;
+    __shared__ DrainShared<Tiles, Step> own;
     const uint32_t warp = threadIdx.x / 32u, groups = (a.h.n_vocab + kGroupV - 1) / kGroupV;
     Share c;
     c.ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
@@ -496,7 +499,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1)
     // 168 registers a thread at launch: 128 threads give up what 256 that drain take (128 x 40 + 256 x 232 = 384 x 168)
     if (warp >= kFirstDrain) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        drain<T, Tiles, Rows>(a, s, own, c);
+        drain<T, Tiles, Rows, Step>(a, s, own, c);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (threadIdx.x == 0)
@@ -553,18 +556,18 @@ bool encode(EncodeTiled f, CUtensorMap* map, bool bf16, const void* base, uint64
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int Tiles, int Rows>
+template <typename T, int Tiles, int Rows, int Step>
 cudaError_t launch_tiles(const HeadArgs& a, uint32_t grid, bool behind_inner, const CUtensorMap* maps, cudaStream_t stream)
 {
     const size_t smem = kRingBytes + 1024;
     static const bool split_fits = [] { // the registers that the warps share out among themselves are those of the launch
         cudaFuncAttributes f;
-        return cudaFuncGetAttributes(&f, head_kernel<T, Tiles, Rows>) == cudaSuccess && f.numRegs == 168;
+        return cudaFuncGetAttributes(&f, head_kernel<T, Tiles, Rows, Step>) == cudaSuccess && f.numRegs == 168;
     }();
     if (!split_fits)
         return cudaErrorInvalidKernelImage;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = set_once(done, head_kernel<T, Tiles, Rows>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = set_once(done, head_kernel<T, Tiles, Rows, Step>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess)
         return e;
     cudaLaunchConfig_t c = {};
@@ -577,7 +580,7 @@ cudaError_t launch_tiles(const HeadArgs& a, uint32_t grid, bool behind_inner, co
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     c.attrs = attr;
     c.numAttrs = behind_inner ? 1 : 0;
-    return cudaLaunchKernelEx(&c, head_kernel<T, Tiles, Rows>, a, maps[0], maps[1], maps[2]);
+    return cudaLaunchKernelEx(&c, head_kernel<T, Tiles, Rows, Step>, a, maps[0], maps[1], maps[2]);
 }
 
 template <typename T>
@@ -641,13 +644,19 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     const uint32_t grid = (groups < most ? groups : most) * a.spread;
     const uint32_t half = a.side == 4u ? a.n : a.n / 2u;
     const bool behind = h.n_adapters != 0;
-    return half <= 16 ? launch_tiles<T, 2, 16>(a, grid, behind, maps, stream)
-           : half <= 32 ? launch_tiles<T, 2, 32>(a, grid, behind, maps, stream)
-           : half <= 48 ? launch_tiles<T, 2, 48>(a, grid, behind, maps, stream)
-           : half <= 64 ? launch_tiles<T, 2, 64>(a, grid, behind, maps, stream)
-           : half <= 80 ? launch_tiles<T, 2, 80>(a, grid, behind, maps, stream)
-           : half <= 96 ? launch_tiles<T, 1, 96>(a, grid, behind, maps, stream)
-                        : launch_tiles<T, 1, 128>(a, grid, behind, maps, stream);
+    // What rows of many adapters wait for is `up`, once for every adapter and step of ranks: 64 rows, 16 adapters of rank 64 at 129280 x 4096
+    // by steps of 16 420 us, of 32 308; of rank 32 223 and 213; 16 rows of rank 64 228 and 234.
+    if (h.n_adapters && h.rank > (uint32_t)kRankStep && a.n > 16u && a.n <= kWideRows)
+        return half <= 32 ? launch_tiles<T, 2, 32, kWideStep>(a, grid, behind, maps, stream)
+               : half <= 48 ? launch_tiles<T, 2, 48, kWideStep>(a, grid, behind, maps, stream)
+                            : launch_tiles<T, 2, 64, kWideStep>(a, grid, behind, maps, stream);
+    return half <= 16 ? launch_tiles<T, 2, 16, kRankStep>(a, grid, behind, maps, stream)
+           : half <= 32 ? launch_tiles<T, 2, 32, kRankStep>(a, grid, behind, maps, stream)
+           : half <= 48 ? launch_tiles<T, 2, 48, kRankStep>(a, grid, behind, maps, stream)
+           : half <= 64 ? launch_tiles<T, 2, 64, kRankStep>(a, grid, behind, maps, stream)
+           : half <= 80 ? launch_tiles<T, 2, 80, kRankStep>(a, grid, behind, maps, stream)
+           : half <= 96 ? launch_tiles<T, 1, 96, kRankStep>(a, grid, behind, maps, stream)
+                        : launch_tiles<T, 1, 128, kRankStep>(a, grid, behind, maps, stream);
 }
 
 } // namespace
