@@ -354,7 +354,8 @@ typedef struct mk_kv_plan {
  *     list holds is left alone (MK_FLAG_NO_PAGES).
  * A sequence that is left alone keeps its pages and has no tokens in the pass. Places behind the last token get position 0,
  * slot -1, sequence -1, so that a pass of max_tokens rows, captured once, runs on any plan. An n_free outside [0, free_cap] is
- * taken as the nearest of the two. Table entries are taken as they are. At most 8192 sequences. */
+ * taken as the nearest of the two. Table entries are taken as they are. At most 8192 sequences. A
+ * plan uses nothing of the handle but its device: calls may overlap, on one handle too, where their arrays are not the same. */
 int mk_kv_plan_step(mk_sampler* s, const mk_kv_pages* pages, const int32_t* cache_len, const int32_t* n_new, uint32_t n_seq,
                     const mk_kv_plan* plan, void* stream);
 

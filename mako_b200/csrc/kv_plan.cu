@@ -15,6 +15,7 @@ namespace {
 
 constexpr uint32_t kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
 constexpr uint32_t kPlanTokens = 4096, kTokenThreads = 256;
+constexpr uint32_t kSeqBytes = 3 * 4; // of shared memory: three running sums
 
 struct Sums {
     long long tokens, give, take;
@@ -225,15 +226,16 @@ __global__ void __launch_bounds__(kTokenThreads) kv_token_kernel(const KvPlanArg
 
 cudaError_t launch_kv_plan(const KvPlanArgs& a, cudaStream_t stream)
 {
-    const size_t smem = (size_t)a.n_seq * 3u * 4u;
-    if (smem > 48u * 1024u) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess)
-            return e;
-    }
+    // What a call may ask for is set once, for the most sequences there are: it belongs to the kernel, not to the call, so that one
+    // thread's call must not lower it under another's. (Without it dynamic and static shared memory have 48 KB together: 4030 sequences.)
+    static std::atomic<uint64_t> room_set{0};
+    const size_t smem = (size_t)a.n_seq * kSeqBytes;
+    cudaError_t e = set_once(room_set, kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPlanMaxSeq * kSeqBytes));
+    if (e != cudaSuccess)
+        return e;
     const bool rows = a.o.positions || a.o.slots || a.o.token_seq, here = a.o.max_tokens <= kPlanTokens;
     kv_plan_kernel<<<1, kPlanThreads, smem, stream>>>(a, rows && here);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess || !rows || here)
         return e;
     const uint32_t work = (a.o.max_tokens + kTokenThreads - 1) / kTokenThreads;
