@@ -135,15 +135,16 @@ __device__ __forceinline__ void put(uint32_t at, double a, double b)
 }
 
 // A maximum m and the sum of 2^(x scale - fl(m scale)): the product rounds once, in the FMA, so that its reference point is
-// exact; -inf and 0 where there is none. A reference point beyond kFar (logits of the type's lowest value, temperatures of next to
-// nothing) makes no sum, as it is off by more than a little itself: such a row is weighed in 64 bits.
-constexpr float kFar = 1e6f;
+// exact; -inf and 0 where there is none. A row whose reference point is beyond kFar (logits of the type's lowest value, temperatures
+// of next to nothing) is weighed in 64 bits, as that point is off by more than a little itself. A part of a row, which lies below the
+// row's own largest where that is negative, makes its sum up to kSum: parts beyond that weigh 2^-4096 at most in a row that is not far.
+constexpr float kFar = 1e6f, kSum = kFar + 4096.0f;
 struct Mass {
     float m, s;
     __device__ void add(const Mass& o, float scale)
     {
         const float top = fmaxf(m, o.m);
-        if (fabsf(__fmul_rn(top, scale)) < kFar) { // else nothing yet, or a sum that no one will use
+        if (fabsf(__fmul_rn(top, scale)) < kSum) { // else nothing yet, or a sum that no one will use
             const float mine = m > -kInf ? s * ex2_approx(__fmul_rn(m, scale) - __fmul_rn(top, scale)) : 0.0f;
             s = mine + (o.m > -kInf ? o.s * ex2_approx(__fmul_rn(o.m, scale) - __fmul_rn(top, scale)) : 0.0f);
         }
@@ -295,7 +296,7 @@ struct Scan {
         }
         const float m = fmaxf(a.m, top);
         float all = 0.0f;
-        const bool near = fabsf(__fmul_rn(m, scale)) < kFar;
+        const bool near = fabsf(__fmul_rn(m, scale)) < kSum;
         if (near) {
             const float2 by = make_float2(scale, scale), off = make_float2(-__fmul_rn(m, scale), -__fmul_rn(m, scale));
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -341,7 +342,7 @@ __device__ __forceinline__ Mass warp_merge(Mass a, float scale, uint32_t& at)
         top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     at = __reduce_min_sync(~0u, a.m == top ? at : ~0u);
     float s = 0.0f;
-    if (fabsf(__fmul_rn(top, scale)) < kFar && a.s != 0.0f)
+    if (fabsf(__fmul_rn(top, scale)) < kSum && a.s != 0.0f)
         s = a.s * ex2_approx(__fmul_rn(a.m, scale) - __fmul_rn(top, scale));
 #pragma unroll
     for (uint32_t d = 16; d; d >>= 1)

@@ -1,0 +1,52 @@
+"""Verification of drafts (mk_spec_verify) where its single-precision sums end, against the 64-bit form."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import test_gpu_spec_verify as verify
+
+pytestmark = pytest.mark.gpu
+
+
+def plain(s, d, v, logits, drafts, u, temperature, draft_logits=None, draft_temperature=None):
+    f32 = lambda x: np.asarray(x, np.float32)  # noqa: E731
+    c = {"logits": torch.from_numpy(f32(logits).reshape(s * (d + 1), v)), "drafts": np.asarray(drafts, np.int32).reshape(s, d),
+         "u": f32(u).reshape(s, d + 2), "temperature": np.broadcast_to(f32(temperature), (s,)).copy(), "mask": None, "mask_drafts": False,
+         "draft_logits": None if draft_logits is None else torch.from_numpy(f32(draft_logits).reshape(s * d, v))}
+    if draft_temperature is not None:
+        c["draft_temperature"] = np.broadcast_to(f32(draft_temperature), (s,)).copy()
+    return c
+
+
+def test_a_part_of_a_row_beyond_the_line(gpu_sampler_factory):
+    """Two columns of different threads' on the two sides of 1e6 (693147 log2 e): P is 0.622 and 0.378."""
+    row = np.full((2, 40), -np.inf, np.float32)
+    row[:, 0], row[:, 16] = -693147.0, -693147.5
+    c = plain(1, 1, 40, row, [[0]], [[0.9, 0.3, 0.5]], 1.0)
+    got = verify.compare(gpu_sampler_factory(129280, 512), c)
+    assert got.n_kept.tolist() == [0] and got.next_token.tolist() == [16]
+    c["u"][0] = 0.5
+    got = verify.compare(gpu_sampler_factory(129280, 512), c)
+    assert got.n_kept.tolist() == [1]
+
+
+@pytest.mark.parametrize("onehot", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 1e-4])
+@pytest.mark.parametrize("v", [61, 5003, 100003])
+def test_rows_on_both_sides_of_the_line(gpu_sampler_factory, v, temperature, onehot):
+    """Largest logits over T whose log2 lies just inside or just outside of 1e6, of either sign, and at 1e6 + 4096."""
+    rng = np.random.default_rng(v)
+    tops = [side * (line + off) for line in (1e6, 1e6 + 4096) for side in (-1, 1) for off in (-30.0, -1.0, -0.1, 0.1, 1.0, 30.0)]
+    s, t = len(tops), np.float32(temperature)
+    base = np.array(tops)[:, None, None] * math.log(2) * float(t)
+
+    def rows(n):
+        below = rng.exponential(4.0, (s, n, v)) * (rng.random((s, n, v)) < 0.9)
+        return (base - below * float(t)).astype(np.float32)
+
+    target, draft = rows(2), rows(1)
+    drafts = np.argmax(draft[:, 0] / t + rng.gumbel(size=(s, v)), axis=1)
+    c = plain(s, 1, v, target, drafts, rng.random((s, 3)), t, None if onehot else draft)
+    verify.compare(gpu_sampler_factory(129280, 512), c)
