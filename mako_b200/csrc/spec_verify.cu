@@ -177,13 +177,14 @@ struct Row {
     __device__ bool far() const { return !none() && !single() && !(fabsf(__fmul_rn(mass.m, scale)) < kFar); }
     __device__ float base() const { return fabsf(__fmul_rn(mass.m, scale)) < kFar ? 0.0f : mass.m; }
     __device__ double zero() const { return rint((double)(mass.m - base()) * scale64 * kSteps); }
-    // The whole weight where the step of the draw's table next to the largest weighs 1, as good as the fp32 sums are.
+    // The whole weight where the step of the draw's table next to the largest weighs 1, as good as the fp32 sums are. Those stand on
+    // fl(m scale) in units of the fp32 scale, which is off by 2^-25 of itself: 0.03 of a power of two where m scale is 1e6.
     __device__ double whole() const
     {
         if (far())
             return sum64;
-        const double d = ((double)__fmul_rn(mass.m, scale) - zero() / kSteps) * 0.6931471805599453; // |d| < 0.06
-        return (double)mass.s * (1.0 + d * (1.0 + d * (1.0 / 2.0 + d * (1.0 / 6.0 + d / 24.0))));
+        const double d = (((double)__fmul_rn(mass.m, scale) - zero() / kSteps) + (double)mass.m * (scale64 - (double)scale)) * 0.6931471805599453;
+        return (double)mass.s * (1.0 + d * (1.0 + d * (1.0 / 2.0 + d * (1.0 / 6.0 + d / 24.0)))); // |d| < 0.1
     }
     // A logit's logarithm of its part.
     __device__ float log_part(float x) const

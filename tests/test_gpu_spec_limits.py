@@ -50,3 +50,18 @@ def test_rows_on_both_sides_of_the_line(gpu_sampler_factory, v, temperature, one
     drafts = np.argmax(draft[:, 0] / t + rng.gumbel(size=(s, v)), axis=1)
     c = plain(s, 1, v, target, drafts, rng.random((s, 3)), t, None if onehot else draft)
     verify.compare(gpu_sampler_factory(129280, 512), c)
+
+
+@pytest.mark.parametrize("swap", [False, True])
+def test_a_residual_between_rows_of_far_temperatures(gpu_sampler_factory, swap):
+    """log2(e) / T as fp32 is off by 2^-25 of itself, which at a logit of 9e5 times T is 0.03 of a power of two, up for one of these
+    temperatures and down for the other. Eight columns, all alike in P; Q has more on the draft: the draft has no part in the rest."""
+    tp, tq = (2.5843542971415445e-05, 2.517000939405989e-05)[::-1 if swap else 1]
+    p = np.full((2, 8), 15.0, np.float32)
+    q = p[:1].copy()
+    q[0, 0] = np.nextafter(np.float32(15), np.float32(16))
+    us = [0.002, 0.05, 0.2, 0.4, 0.6, 0.97]
+    n = len(us)
+    c = plain(n, 1, 8, np.tile(p, (n, 1, 1)), [[0]] * n, [[0.995, x, 0.5] for x in us], tp, np.tile(q, (n, 1, 1)), tq)
+    got = verify.compare(gpu_sampler_factory(129280, 512), c)
+    assert got.n_kept.tolist() == [0] * n and got.next_token.tolist() == [1 + int(7 * x) for x in us]
