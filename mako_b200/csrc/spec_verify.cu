@@ -35,6 +35,7 @@ constexpr uint32_t kSteps = 16;   // of the table of exp2
 constexpr uint32_t kParts = 8;   // of a warp's share of a row
 constexpr float kNear = 3e-5f;    // decisions nearer than this, relative, are taken in 64 bits
 constexpr double kSome = 1e-290;   // a weight below this, where the largest is about 1, is none
+constexpr double kSteepest = 3e38; // log2(e) / T above this is none of fp32's numbers
 constexpr float kHottest = 1e30f;  // a temperature from here on is not one
 constexpr float kInf = __builtin_huge_valf();
 
@@ -166,7 +167,7 @@ struct Row {
     {
         t = v > 0.0f && v < kHottest ? v : 0.0f;
         scale64 = t > 0.0f ? 1.4426950408889634 / (double)t : 0.0;
-        scale = (float)fmin(scale64, 3e38);
+        scale = (float)fmin(scale64, kSteepest);
     }
     __device__ void weighed(const Mass& a)
     {
@@ -174,8 +175,9 @@ struct Row {
         lowest = fmaxf((a.m - base()) - 693.0f * t, -3.4e38f);
     }
     __device__ bool none() const { return mass.m == -kInf; }
-    __device__ bool far() const { return !none() && !single() && !(fabsf(__fmul_rn(mass.m, scale)) < kFar); }
-    __device__ float base() const { return fabsf(__fmul_rn(mass.m, scale)) < kFar ? 0.0f : mass.m; }
+    __device__ bool off() const { return !(fabsf(__fmul_rn(mass.m, scale)) < kFar) || scale64 > kSteepest; } // the fp32 sums are
+    __device__ bool far() const { return !none() && !single() && off(); }
+    __device__ float base() const { return off() ? mass.m : 0.0f; }
     __device__ double zero() const { return rint((double)(mass.m - base()) * scale64 * kSteps); }
     // The whole weight where the step of the draw's table next to the largest weighs 1, as good as the fp32 sums are. Those stand on
     // fl(m scale) in units of the fp32 scale, which is off by 2^-25 of itself: 0.03 of a power of two where m scale is 1e6.

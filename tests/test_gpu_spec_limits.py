@@ -65,3 +65,13 @@ def test_a_residual_between_rows_of_far_temperatures(gpu_sampler_factory, swap):
     c = plain(n, 1, 8, np.tile(p, (n, 1, 1)), [[0]] * n, [[0.995, x, 0.5] for x in us], tp, np.tile(q, (n, 1, 1)), tq)
     got = verify.compare(gpu_sampler_factory(129280, 512), c)
     assert got.n_kept.tolist() == [0] * n and got.next_token.tolist() == [1 + int(7 * x) for x in us]
+
+
+def test_temperatures_whose_inverse_passes_fp32(gpu_sampler_factory):
+    """log2(e) / T above fp32's range, and logits of that temperature's size: P is 0.622 and 0.378."""
+    row = np.full((2, 40), -1.0, np.float32)
+    row[:, 0], row[:, 16] = 0.0, -1e-39
+    c = plain(2, 1, 40, np.tile(row, (2, 1, 1)), [[0], [0]], [[0.9, 0.3, 0.5], [0.5, 0.3, 0.7]], 2e-39)
+    got = verify.compare(gpu_sampler_factory(129280, 512), c)
+    # the second one keeps its draft; the token behind it is drawn with 0.3, which is below 0.622
+    assert got.n_kept.tolist() == [0, 1] and got.next_token.tolist() == [16, 0]
