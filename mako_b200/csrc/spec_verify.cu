@@ -34,6 +34,7 @@ constexpr uint32_t kScanThreads = kVerifyThreads + 64; // and a warp that copies
 constexpr uint32_t kSteps = 16;   // of the table of exp2
 constexpr uint32_t kParts = 8;   // of a warp's share of a row
 constexpr float kNear = 3e-5f;    // decisions nearer than this, relative, are taken in 64 bits
+constexpr float kFew = 1e-30f;    // and those of probabilities of which fp32 may hold few bits or none: ex2_approx ends at 2^-126
 constexpr double kSome = 1e-290;   // a weight below this, where the largest is about 1, is none
 constexpr double kSteepest = 3e38; // log2(e) / T above this is none of fp32's numbers
 constexpr float kHottest = 1e30f;  // a temperature from here on is not one
@@ -530,7 +531,8 @@ __device__ void close_piece(const SpecVerifyArgs& a, const Tile& z, Mass mp, uin
     if (drafted) {
         const float pd = part_of(p, x, at_p, d), lhs = u * (against ? part_of(q, y, at_q, d) : 1.0f);
         const bool soft_q = against && !q.none() && !q.single();
-        if (p.far() || (soft_q && q.far()) || (((!p.none() && !p.single()) || soft_q) && fabsf(lhs - pd) <= kNear * fmaxf(lhs, pd)))
+        const float more = fmaxf(lhs, pd);
+        if (p.far() || (soft_q && q.far()) || (((!p.none() && !p.single()) || soft_q) && (fabsf(lhs - pd) <= kNear * more || more < kFew)))
             state = kOpen;
         else if (lhs < pd)
             state = kKept;

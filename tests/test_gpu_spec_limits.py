@@ -1,4 +1,5 @@
-"""Verification of drafts (mk_spec_verify) where its single-precision sums end, against the 64-bit form."""
+"""Verification of drafts (mk_spec_verify) where its single-precision sums end and where probabilities are next to nothing, against the
+64-bit form."""
 import math
 
 import numpy as np
@@ -65,6 +66,31 @@ def test_a_residual_between_rows_of_far_temperatures(gpu_sampler_factory, swap):
     c = plain(n, 1, 8, np.tile(p, (n, 1, 1)), [[0]] * n, [[0.995, x, 0.5] for x in us], tp, np.tile(q, (n, 1, 1)), tq)
     got = verify.compare(gpu_sampler_factory(129280, 512), c)
     assert got.n_kept.tolist() == [0] * n and got.next_token.tolist() == [1 + int(7 * x) for x in us]
+
+
+def test_probabilities_next_to_nothing(gpu_sampler_factory):
+    """P and u Q of 2^-120 to 2^-160, which fp32 holds in few bits or not at all: kept iff u Q is below P, by a tenth or by much."""
+    rng = np.random.default_rng(5)
+    cases = [(-127.0, -125.0, 2.0 ** -5), (-127.4, -120.0, 2.0 ** -7.3), (-130.0, -133.0, 0.5), (-140.0, -140.0, 0.99)]
+    for e in np.arange(-160.0, -100.0, 0.5):
+        for by in (0.9, 1.1, 0.5, 2.0):
+            u = rng.uniform(0.01, 0.45)
+            cases.append((e, e + math.log2(by / u), u))
+    s, v = len(cases), 4096
+    p, q = np.full((s, 2, v), -np.inf, np.float32), np.full((s, 1, v), -np.inf, np.float32)
+    for i, (ep, eq, _) in enumerate(cases):
+        n = 1 if i % 2 else v - 1  # what has the rest: one column, or all others
+        p[i, :, :n] = q[i, :, :n] = 0.0
+        p[i, 0, -1], q[i, 0, -1] = ep * math.log(2), eq * math.log(2)
+    u = np.array([[x[2], 0.5, 0.5] for x in cases], np.float32)
+    dist = lambda x: np.exp(x[:, 0, -1].astype(np.float64)) / (np.exp(x[:, 0].astype(np.float64)).sum(1))  # noqa: E731
+    lhs, rhs = u[:, 0].astype(np.float64) * dist(q), dist(p)
+    assert (np.abs(lhs - rhs) > 0.005 * rhs).all()
+    cuda = lambda x: torch.from_numpy(x).cuda()  # noqa: E731
+    got = gpu_sampler_factory(129280, 512).spec_verify(
+        cuda(p.reshape(2 * s, v)), torch.full((s, 1), v - 1, dtype=torch.int32, device="cuda"), cuda(u), 1.0,
+        draft_logits=cuda(q.reshape(s, v)))
+    assert np.array_equal(got.n_kept.cpu().numpy(), (lhs < rhs).astype(np.int32))
 
 
 def test_temperatures_whose_inverse_passes_fp32(gpu_sampler_factory):
