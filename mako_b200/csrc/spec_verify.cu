@@ -15,7 +15,7 @@
 // the 64-bit pipe (23 operations a column) and by the latency of its few steps. max(0, P - Q) wants both rows' whole weights first;
 // instead of a pass for them, the one pass forms A = sum of (p - c q) and B = sum of q over the columns where p > c q, with the
 // c = P's / Q's whole weight that the fp32 sums give, beside the exact sums, and A - (exact c - c) B is what is drawn from: only
-// columns between the two c, 1e-6 apart, are off, by as much again. The sums by CTA and warp lead to one warp's columns, which the
+// columns between the two c, 1e-6 apart, are off, by as much again (rows so alike that this matters are summed twice, see draw()). The sums by CTA and warp lead to one warp's columns, which the
 // CTA goes over once more, eight a thread. 53 us for the same sequences, 16 for a single one.
 #include "ptx.cuh"
 #include "round_ops.h"
@@ -35,6 +35,7 @@ constexpr uint32_t kSteps = 16;   // of the table of exp2
 constexpr uint32_t kParts = 8;   // of a warp's share of a row
 constexpr float kNear = 3e-5f;    // decisions nearer than this, relative, are taken in 64 bits
 constexpr float kFew = 1e-30f;    // and those of probabilities of which fp32 may hold few bits or none: ex2_approx ends at 2^-126
+constexpr double kLoose = 1e-4;    // see draw()
 constexpr double kSome = 1e-290;   // a weight below this, where the largest is about 1, is none
 constexpr double kSteepest = 3e38; // log2(e) / T above this is none of fp32's numbers
 constexpr float kHottest = 1e30f;  // a temperature from here on is not one
@@ -1020,24 +1021,33 @@ template <typename T>
 __device__ int32_t draw(Rest<T> rest, double u, Shared& s, Part& c)
 {
     const uint32_t lane = threadIdx.x & 31u;
-    const double2(*all)[2] = exchange(s, c, sweep(rest, s, c));
-    const double2 mine = lane < c.size ? all[lane][0] : make_double2(0.0, 0.0);
-    double off = 0.0; // the exact c above the one that the sums were formed with
-    if (rest.against) {
-        double2 both = lane < c.size ? all[lane][1] : make_double2(0.0, 0.0);
+    double off = 0.0, of_cta, total, before; // off: the exact c above the one that the sums were formed with
+    // The sums have the wrong sign for columns between the two c, up to |off| q of each. Rows whose p / q spread are off by the square of
+    // |off| over the rest, a few 1e-12; where all of Q lay between, it could be |off| over the rest. Above 1e-4 of that, which means
+    // rows alike to a hundredth, once more with the exact c (the second time off is 0: the whole weights do not depend on c). From 1e-6
+    // on nearly every refused draft would be summed twice: 64 sequences of four drafts 104 -> 123 us.
+    for (bool again = false;; again = true) {
+        const double2(*all)[2] = exchange(s, c, sweep(rest, s, c));
+        const double2 mine = lane < c.size ? all[lane][0] : make_double2(0.0, 0.0);
+        double2 both = make_double2(0.0, 0.0);
+        if (rest.against) {
+            if (lane < c.size)
+                both = all[lane][1];
 #pragma unroll
-        for (uint32_t d = 16; d; d >>= 1) {
-            both.x += __shfl_xor_sync(~0u, both.x, d);
-            both.y += __shfl_xor_sync(~0u, both.y, d);
+            for (uint32_t d = 16; d; d >>= 1) {
+                both.x += __shfl_xor_sync(~0u, both.x, d);
+                both.y += __shfl_xor_sync(~0u, both.y, d);
+            }
+            off = both.x / both.y - rest.c;
+            rest.c = both.x / both.y;
         }
-        off = both.x / both.y - rest.c;
-        rest.c = both.x / both.y;
-    }
-    const double of_cta = fma(-off, mine.y, mine.x);
-    double total = of_cta, before;
+        total = of_cta = fma(-off, mine.y, mine.x);
 #pragma unroll
-    for (uint32_t d = 16; d; d >>= 1)
-        total += __shfl_xor_sync(~0u, total, d);
+        for (uint32_t d = 16; d; d >>= 1)
+            total += __shfl_xor_sync(~0u, total, d);
+        if (again || fabs(off) * both.y <= kLoose * total)
+            break;
+    }
     if (!(total > kSome))
         return -1;
     const double want = u * total;

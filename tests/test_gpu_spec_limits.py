@@ -1,5 +1,5 @@
-"""Verification of drafts (mk_spec_verify) where its single-precision sums end and where probabilities are next to nothing, against the
-64-bit form."""
+"""Verification of drafts (mk_spec_verify) where its single-precision sums end and where probabilities are next to nothing or next to
+each other, against the 64-bit form."""
 import math
 
 import numpy as np
@@ -91,6 +91,19 @@ def test_probabilities_next_to_nothing(gpu_sampler_factory):
         cuda(p.reshape(2 * s, v)), torch.full((s, 1), v - 1, dtype=torch.int32, device="cuda"), cuda(u), 1.0,
         draft_logits=cuda(q.reshape(s, v)))
     assert np.array_equal(got.n_kept.cpu().numpy(), (lhs < rhs).astype(np.int32))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_residual_of_next_to_nothing(gpu_sampler_factory, seed):
+    """P and Q alike to 1e-7 in every column but the draft's, where Q has twice P's 1e-8: the rest is a few 1e-8 of the whole, spread over
+    the columns whose part is above the average change."""
+    rng = np.random.default_rng(seed)
+    s, v = 40, 1000
+    q = np.zeros((s, 1, v), np.float32)
+    p = np.concatenate([rng.uniform(0.0, 1e-7, (s, 1, v)), np.zeros((s, 1, v))], 1).astype(np.float32)
+    p[:, 0, 7], q[:, 0, 7] = math.log(1e-5), math.log(2e-5)
+    c = plain(s, 1, v, p, np.full((s, 1), 7), np.stack([np.full(s, 0.9), rng.random(s), rng.random(s)], 1), 1.0, q)
+    verify.compare(gpu_sampler_factory(129280, 512), c)
 
 
 def test_temperatures_whose_inverse_passes_fp32(gpu_sampler_factory):
