@@ -136,7 +136,7 @@ class BatchSampler:
     def __init__(self, n_vocab: int, max_batch: int, device: int = 0, cand_cap: int = 0):
         if n_vocab == 0:
             raise ValueError("sampler: empty vocabulary")
-        self.device = torch.device("cuda", device)
+        self.device, self._index = torch.device("cuda", device), device
         self._h = C.c_void_p()
         check(lib.mk_sampler_create(C.byref(self._h), device, n_vocab, max_batch))
         self.n_vocab, self.max_batch, self.cand_cap = n_vocab, max_batch, cand_cap
@@ -206,6 +206,11 @@ class BatchSampler:
             p.presence_penalty, p.frequency_penalty = params.presence_penalty, params.frequency_penalty
             p.repetition_penalty = params.repetition_penalty
         return r
+
+    def _here(self, *tensors: torch.Tensor) -> None:
+        """Refuses what lies on the host or on another device than the handle: a kernel that follows such an address faults."""
+        for t in tensors:
+            assert t.get_device() == self._index, f"a tensor on device {t.device}, the handle is on {self.device}"
 
     def _out(self, batch: int) -> SampleOutC:
         o = SampleOutC()
@@ -354,22 +359,26 @@ class BatchSampler:
         down [N, R, D], up [N, V, R] bf16 or fp16, adapter [T] int32 (-1: none), scale [N] float32. Returns the rows that the
         sampler reads, [T, V] float32 (`out` where given)."""
         (rows, dim), v = hidden.shape, weight.shape[0]
-        assert hidden.is_cuda and hidden.dtype in (torch.bfloat16, torch.float16) and hidden.stride(1) == 1
-        assert weight.is_cuda and weight.dtype == hidden.dtype and weight.is_contiguous() and weight.shape[1] == dim
+        self._here(hidden, weight)
+        assert hidden.dtype in (torch.bfloat16, torch.float16) and hidden.stride(1) == 1
+        assert weight.dtype == hidden.dtype and weight.is_contiguous() and weight.shape[1] == dim
         d_ptr = u_ptr = s_ptr = n = rank = 0
         if adapter is not None:
-            assert adapter.is_cuda and adapter.dtype == torch.int32 and adapter.is_contiguous() and adapter.numel() == rows
+            self._here(adapter, down, up)
+            assert adapter.dtype == torch.int32 and adapter.is_contiguous() and adapter.numel() == rows
             n, rank, _ = down.shape
-            assert down.is_cuda and up.is_cuda and down.dtype == up.dtype == hidden.dtype
+            assert down.dtype == up.dtype == hidden.dtype
             assert down.shape == (n, rank, dim) and up.shape == (n, v, rank) and down.is_contiguous() and up.is_contiguous()
             d_ptr, u_ptr = down.data_ptr(), up.data_ptr()
             if scale is not None:
-                assert scale.is_cuda and scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == n
+                self._here(scale)
+                assert scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == n
                 s_ptr = scale.data_ptr()
         h = HeadC(weight.data_ptr(), d_ptr or None, u_ptr or None, s_ptr or None, v, dim, n, rank, _TYPE[hidden.dtype])
         if out is None:
             out = torch.empty((rows, v), dtype=torch.float32, device=hidden.device)
-        assert out.is_cuda and out.dtype == torch.float32 and out.shape == (rows, v) and out.stride(1) == 1
+        self._here(out)
+        assert out.dtype == torch.float32 and out.shape == (rows, v) and out.stride(1) == 1
         check(lib.mk_head_logits(self._h, C.byref(h), hidden.data_ptr(), hidden.stride(0), _ptr(adapter), rows, out.data_ptr(),
                                  out.stride(0), _stream_ptr(self.device)))
         return out
@@ -382,27 +391,31 @@ class BatchSampler:
         tokens [S, n_pos], logprob [S, n_pos], flags [S]."""
         n_seq, n_drafts = drafts.shape
         n_pos, v = n_drafts + 1, logits.shape[1]
-        assert logits.is_cuda and logits.shape[0] == n_seq * n_pos and logits.stride(1) == 1
-        assert drafts.is_cuda and drafts.dtype == torch.int32 and drafts.is_contiguous()
-        assert u.is_cuda and u.shape == (n_seq, n_pos + 1) and u.dtype == torch.float32 and u.is_contiguous()
+        self._here(logits, drafts, u)
+        assert logits.shape[0] == n_seq * n_pos and logits.stride(1) == 1
+        assert drafts.dtype == torch.int32 and drafts.is_contiguous()
+        assert u.shape == (n_seq, n_pos + 1) and u.dtype == torch.float32 and u.is_contiguous()
         q_ptr = q_ld = t_ptr = t_all = qt_ptr = m_ptr = m_ld = 0
         if draft_logits is not None:
-            assert draft_logits.is_cuda and draft_logits.dtype == logits.dtype and draft_logits.shape == (n_seq * n_drafts, v)
+            self._here(draft_logits)
+            assert draft_logits.dtype == logits.dtype and draft_logits.shape == (n_seq * n_drafts, v)
             q_ld, unit = draft_logits.stride()
             assert unit == 1
             q_ptr = draft_logits.data_ptr()
         if isinstance(temperature, torch.Tensor):
-            assert temperature.is_cuda and temperature.dtype == torch.float32 and temperature.shape == (n_seq,)
-            assert temperature.is_contiguous()
+            self._here(temperature)
+            assert temperature.dtype == torch.float32 and temperature.shape == (n_seq,) and temperature.is_contiguous()
             t_ptr = temperature.data_ptr()
         else:
             t_all = temperature
         if draft_temperature is not None:
-            assert draft_temperature.is_cuda and draft_temperature.dtype == torch.float32
+            self._here(draft_temperature)
+            assert draft_temperature.dtype == torch.float32
             assert draft_temperature.shape == (n_seq,) and draft_temperature.is_contiguous()
             qt_ptr = draft_temperature.data_ptr()
         if mask is not None:
-            assert mask.is_cuda and mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos
+            self._here(mask)
+            assert mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos
             m_ld, unit = mask.stride()
             assert unit == 1
             m_ptr = mask.data_ptr()
@@ -423,22 +436,27 @@ class BatchSampler:
         `out` (KvPlan.empty)."""
         (n_seq, cols), (ld, unit), i32 = block_table.shape, block_table.stride(), torch.int32
         assert block_table.dtype == n_pages.dtype == free_list.dtype == n_free.dtype == cache_len.dtype == i32 and unit == 1
-        assert block_table.is_cuda and n_pages.is_cuda and free_list.is_cuda and n_free.is_cuda and cache_len.is_cuda
+        on = self._index  # (as _here does, in one expression: a plan's time is its host's)
+        assert block_table.get_device() == n_pages.get_device() == free_list.get_device() == n_free.get_device() == on
+        assert cache_len.get_device() == on
         assert n_pages.is_contiguous() and cache_len.is_contiguous() and free_list.is_contiguous()
         assert n_pages.numel() == cache_len.numel() == n_seq and n_free.numel() == 1
         p = KvPagesC(block_table.data_ptr(), ld, cols, n_pages.data_ptr(), free_list.data_ptr(), free_list.numel(),
                      n_free.data_ptr(), page_size)
         if n_new is not None:
-            assert n_new.is_cuda and n_new.dtype == i32 and n_new.is_contiguous() and n_new.numel() == n_seq and out is not None
+            assert n_new.get_device() == on and n_new.dtype == i32 and n_new.is_contiguous() and n_new.numel() == n_seq
+            assert out is not None
         if out is None:
             o = KvPlanC()
         else:
             start, kv_len, pos, slots, seq, flags = out.query_start, out.kv_len, out.positions, out.slots, out.token_seq, out.flags
+            assert start.get_device() == kv_len.get_device() == pos.get_device() == slots.get_device() == on
+            assert seq.get_device() == flags.get_device() == on
             t = pos.numel()
             assert start.numel() == n_seq + 1 and kv_len.numel() == flags.numel() == n_seq and slots.numel() == seq.numel() == t
             assert start.dtype == kv_len.dtype == pos.dtype == seq.dtype == flags.dtype == i32 and slots.dtype == torch.int64
             assert start.is_contiguous() and kv_len.is_contiguous() and pos.is_contiguous() and slots.is_contiguous()
-            assert seq.is_contiguous() and flags.is_contiguous() and start.is_cuda and slots.is_cuda
+            assert seq.is_contiguous() and flags.is_contiguous()
             o = KvPlanC(start.data_ptr(), kv_len.data_ptr(), pos.data_ptr(), slots.data_ptr(), seq.data_ptr(), flags.data_ptr(), t)
         check(lib.mk_kv_plan_step(self._h, C.byref(p), cache_len.data_ptr(), _ptr(n_new), n_seq, C.byref(o),
                                   _stream_ptr(self.device)))
