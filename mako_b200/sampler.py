@@ -39,6 +39,13 @@ def _first(t: torch.Tensor, b: int) -> torch.Tensor:
     return t.detach() if t.shape[0] == b else t[:b]
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """From one row to the next, of rows whose columns lie side by side (a tensor of one row, or one column, may say any stride)."""
+    (ld, unit), (n, columns) = t.stride(), t.shape
+    assert unit == 1 or columns <= 1
+    return ld if n > 1 else columns
+
+
 class Sampler:
     """One row at a time, as the reference: Sampler(params, n_vocab, seed); sample(); verify(); accept()."""
 
@@ -360,7 +367,7 @@ class BatchSampler:
         sampler reads, [T, V] float32 (`out` where given)."""
         (rows, dim), v = hidden.shape, weight.shape[0]
         self._here(hidden, weight)
-        assert hidden.dtype in (torch.bfloat16, torch.float16) and hidden.stride(1) == 1
+        assert hidden.dtype in (torch.bfloat16, torch.float16)
         assert weight.dtype == hidden.dtype and weight.is_contiguous() and weight.shape[1] == dim
         d_ptr = u_ptr = s_ptr = n = rank = 0
         if adapter is not None:
@@ -378,9 +385,9 @@ class BatchSampler:
         if out is None:
             out = torch.empty((rows, v), dtype=torch.float32, device=hidden.device)
         self._here(out)
-        assert out.dtype == torch.float32 and out.shape == (rows, v) and out.stride(1) == 1
-        check(lib.mk_head_logits(self._h, C.byref(h), hidden.data_ptr(), hidden.stride(0), _ptr(adapter), rows, out.data_ptr(),
-                                 out.stride(0), _stream_ptr(self.device)))
+        assert out.dtype == torch.float32 and out.shape == (rows, v)
+        check(lib.mk_head_logits(self._h, C.byref(h), hidden.data_ptr(), _row_stride(hidden), _ptr(adapter), rows, out.data_ptr(),
+                                 _row_stride(out), _stream_ptr(self.device)))
         return out
 
     def spec_verify(self, logits, drafts, u, temperature, *, draft_logits=None, draft_temperature=None, mask=None,
@@ -392,16 +399,14 @@ class BatchSampler:
         n_seq, n_drafts = drafts.shape
         n_pos, v = n_drafts + 1, logits.shape[1]
         self._here(logits, drafts, u)
-        assert logits.shape[0] == n_seq * n_pos and logits.stride(1) == 1
+        assert logits.shape[0] == n_seq * n_pos
         assert drafts.dtype == torch.int32 and drafts.is_contiguous()
         assert u.shape == (n_seq, n_pos + 1) and u.dtype == torch.float32 and u.is_contiguous()
         q_ptr = q_ld = t_ptr = t_all = qt_ptr = m_ptr = m_ld = 0
         if draft_logits is not None:
             self._here(draft_logits)
             assert draft_logits.dtype == logits.dtype and draft_logits.shape == (n_seq * n_drafts, v)
-            q_ld, unit = draft_logits.stride()
-            assert unit == 1
-            q_ptr = draft_logits.data_ptr()
+            q_ptr, q_ld = draft_logits.data_ptr(), _row_stride(draft_logits)
         if isinstance(temperature, torch.Tensor):
             self._here(temperature)
             assert temperature.dtype == torch.float32 and temperature.shape == (n_seq,) and temperature.is_contiguous()
@@ -416,10 +421,8 @@ class BatchSampler:
         if mask is not None:
             self._here(mask)
             assert mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos
-            m_ld, unit = mask.stride()
-            assert unit == 1
-            m_ptr = mask.data_ptr()
-        r = SpecRowsC(logits.data_ptr(), logits.stride(0), q_ptr or None, q_ld, _TYPE[logits.dtype], n_seq, n_pos, v,
+            m_ptr, m_ld = mask.data_ptr(), _row_stride(mask)
+        r = SpecRowsC(logits.data_ptr(), _row_stride(logits), q_ptr or None, q_ld, _TYPE[logits.dtype], n_seq, n_pos, v,
                       drafts.data_ptr(), u.data_ptr(), t_ptr or None, qt_ptr or None, t_all, m_ptr or None, m_ld, int(mask_drafts))
         kept, nxt, flags = torch.empty((3, n_seq), dtype=torch.int32, device=self.device).unbind()
         tokens = torch.empty((n_seq, n_pos), dtype=torch.int32, device=self.device)
@@ -434,8 +437,8 @@ class BatchSampler:
         block_table [S, columns], n_pages [S], free_list [P] and n_free [1] int32 are updated in place; cache_len [S] tokens are
         in the cache, n_new [S] come with the pass (None: pages above the need go back, and that is all). Fills and returns
         `out` (KvPlan.empty)."""
-        (n_seq, cols), (ld, unit), i32 = block_table.shape, block_table.stride(), torch.int32
-        assert block_table.dtype == n_pages.dtype == free_list.dtype == n_free.dtype == cache_len.dtype == i32 and unit == 1
+        (n_seq, cols), ld, i32 = block_table.shape, _row_stride(block_table), torch.int32
+        assert block_table.dtype == n_pages.dtype == free_list.dtype == n_free.dtype == cache_len.dtype == i32
         on = self._index  # (as _here does, in one expression: a plan's time is its host's)
         assert block_table.get_device() == n_pages.get_device() == free_list.get_device() == n_free.get_device() == on
         assert cache_len.get_device() == on
