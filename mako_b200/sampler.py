@@ -422,6 +422,7 @@ class BatchSampler:
             self._here(mask)
             assert mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == n_seq * n_pos
             m_ptr, m_ld = mask.data_ptr(), _row_stride(mask)
+            assert 32 * mask.shape[1] >= v or m_ld == mask.shape[1], "a mask narrower than its rows"  # (the library sees strides alone)
         r = SpecRowsC(logits.data_ptr(), _row_stride(logits), q_ptr or None, q_ld, _TYPE[logits.dtype], n_seq, n_pos, v,
                       drafts.data_ptr(), u.data_ptr(), t_ptr or None, qt_ptr or None, t_all, m_ptr or None, m_ld, int(mask_drafts))
         kept, nxt, flags = torch.empty((3, n_seq), dtype=torch.int32, device=self.device).unbind()

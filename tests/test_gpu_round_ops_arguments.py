@@ -42,3 +42,10 @@ def test_a_single_rows_stride_has_no_meaning(gpu_sampler_factory):
 def _plan(s, t):
     from mako_b200 import KvPlan
     return KvPlan.empty(s, t)
+
+
+def test_a_mask_narrower_than_the_rows_is_refused(gpu_sampler_factory):
+    """Also where its row stride would be wide enough: what lies behind is not its own."""
+    z = lambda *n, t=torch.float32: torch.zeros(*n, dtype=t, device="cuda")  # noqa: E731
+    with pytest.raises(AssertionError):
+        gpu_sampler_factory(129280, 512).spec_verify(z(4, 100), z(2, 1, t=torch.int32), z(2, 3), 1.0, mask=z(4, 8, t=torch.int32)[:, :3])

@@ -60,3 +60,12 @@ def test_tensors_of_another_device_or_the_host_are_refused(handle, call):
                 run()
                 pytest.fail(k)
         x.where = 0
+
+
+def test_a_mask_narrower_than_the_rows_is_refused(handle):
+    tensors, run = verify(handle)
+    run_with = lambda mask: (tensors.update(mask=mask), run())  # noqa: E731
+    with pytest.raises(AssertionError, match="narrower"):
+        run_with(on(6, 8, t=torch.int32)[:, :3])
+    with pytest.raises(MakoError, match="null argument"):  # (else the library's own check)
+        run_with(on(6, 8, t=torch.int32)[:, :4])
