@@ -492,6 +492,7 @@ __device__ void close_piece(const SpecVerifyArgs& a, const Tile& z, Mass mp, uin
     }
     if (__shfl_sync(~0u, before, 0) != a.slices - 1u)
         return;
+    __syncwarp(); // what the first lane's counting made visible to it is so to the others (a shuffle orders no memory)
     Row<T> p, q;
     heat_rows(r, z.sq, p, q);
     place_rows(r, z.sq, z.j, against, p, q);
