@@ -27,7 +27,7 @@ namespace mk {
 namespace {
 
 constexpr uint32_t kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32, kMaxCluster = 16;
-constexpr uint32_t kDrawThreads = 384, kDrawWarps = kDrawThreads / 32, kDrawCtas = 296; // two on each of 148 SMs
+constexpr uint32_t kDrawThreads = 384, kDrawWarps = kDrawThreads / 32;
 constexpr uint32_t kTileBlocks = 1024, kTileBytes = 16 * kTileBlocks, kTiles = 6; // of the ring
 constexpr uint32_t kScanCtas = 296; // two on each of 148 SMs
 constexpr uint32_t kScanThreads = kVerifyThreads + 64; // and a warp that copies, and one that closes pieces of work
@@ -1226,6 +1226,42 @@ __global__ void __launch_bounds__(kDrawThreads, 2) spec_draw_kernel(const SpecVe
     cluster_sync(); // nothing is sent to a CTA that has gone
 }
 
+// How many of the draw's clusters of a size fit on the device: fewer than its CTAs would make, as a cluster lies within a part of the
+// chip (of 296 CTAs 14 clusters of 16, 33 of 8, 71 of 4). Asked for once on each of the first 64 devices.
+template <typename T>
+cudaError_t resident_clusters(uint32_t size, uint32_t& fit)
+{
+    static std::atomic<int> known[64][kMaxCluster + 1];
+    static std::atomic<uint64_t> wide_set{0};
+    int device = 0, n = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && size > 8)
+        e = set_once(wide_set, spec_draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess)
+        return e;
+    if (device < 64 && (n = known[device][size].load(std::memory_order_relaxed)) != 0) {
+        fit = (uint32_t)n - 1u;
+        return e;
+    }
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(size);
+    c.blockDim = dim3(kDrawThreads);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    c.attrs = attr;
+    c.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&n, spec_draw_kernel<T>, &c);
+    if (e != cudaSuccess)
+        return e;
+    fit = n > 0 ? (uint32_t)n : 0u;
+    if (device < 64)
+        known[device][size].store((int)fit + 1, std::memory_order_relaxed);
+    return e;
+}
+
 template <typename T>
 cudaError_t launch(SpecVerifyArgs a, cudaStream_t stream)
 {
@@ -1236,26 +1272,28 @@ cudaError_t launch(SpecVerifyArgs a, cudaStream_t stream)
     slices = slices > room ? slices : room;
     slices = slices < a.slices ? slices : a.slices;
     a.slices = slices < most ? slices : most;
-    static std::atomic<uint64_t> scan_set{0}, draw_set{0};
+    static std::atomic<uint64_t> scan_set{0};
     cudaError_t e = set_once(scan_set, spec_scan_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTiles * kTileBytes));
     if (e != cudaSuccess)
         return e;
+    // The largest clusters of which all are resident at once: a second wave takes as long as the first (18 sequences of 129280 columns
+    // by 16 CTAs 49 us, by 8 37; 37 by 8 54, by 4 43; 74 by 4 65, by 2 57; 148 by 2 70, by one 91; 149 by 2 97, by one 90).
+    uint32_t size = kMaxCluster;
+    while (size > 1 && a.r.n_vocab < size * 1024u)
+        size >>= 1;
+    for (; size > 1; size >>= 1) {
+        uint32_t fit = 0;
+        e = resident_clusters<T>(size, fit);
+        if (e != cudaSuccess)
+            return e;
+        if (n <= fit)
+            break;
+    }
     const uint32_t work = rows * a.slices;
     spec_scan_kernel<T><<<work < kScanCtas ? work : kScanCtas, kScanThreads, kTiles * kTileBytes, stream>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess)
         return e;
-    // The largest clusters of which all are resident at once.
-    uint32_t size = kMaxCluster;
-    while (size > 1 && n * size > kDrawCtas)
-        size >>= 1;
-    while (size > 1 && a.r.n_vocab < size * 1024u)
-        size >>= 1;
-    if (size > 8) {
-        e = set_once(draw_set, spec_draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess)
-            return e;
-    }
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(n * size);
     c.blockDim = dim3(kDrawThreads);
