@@ -3,9 +3,11 @@
 // Two launches. The first brings the rows into the order of their adapters (a copy of the hidden states, a few MB at most) and
 // forms `inner`, a CTA per row. The second streams the weight matrix once past the rows: it is what bounds a decode step (1.06 GB
 // at 129280 x 4096), so every CTA has an equal share of the vocabulary, a run of columns of the logits in steps of 16, and keeps
-// as much of it on the way as shared memory holds. Measured at 129280 x 4096, bf16: 167 us for a row with an adapter of rank 16 (0.97 of
-// the rate of a copy), 202 for 64 rows with 16 of them; without adapters 171 for 64 rows, 200 for 128, 310 for 256, where what an SM
-// takes in from L2 (about 65 GB/s) bounds it; 435 for 320 rows of 151552, with adapters of rank 64 690.
+// as much of it on the way as shared memory holds. Measured at 129280 x 4096, bf16, replayed from a graph: 165 us for a row with an
+// adapter of rank 16 (0.99 of the rate of a copy), 199 for 64 rows with 16 of them; without adapters 168 for 64 rows, 200 for 128, 219 for
+// 160, 253 for 192, 304 for 256, where what an SM takes in from L2 (about 65 GB/s) bounds it, 708 for 512; 429 for 320 rows of 151552, with
+// 8 adapters of rank 64 692. (The first launch is 7 to 31 us of these, and hides nowhere: a CTA of the second has nearly all of an SM's
+// registers, so that it starts where none of the first is left.)
 //
 // A tile is 128 vocabulary rows (the MMA's M, a lane of tensor memory each) by the batch's rows (its N, padded to 16). Batches of
 // few rows take two or four vocabulary tiles side by side, so that the hidden states' tile, which comes from L2 every time, is
@@ -604,7 +606,7 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     a.rows = rows;
     // What the ring carries for a step of 64 of the contraction and 128 vocabulary rows is 16 KB of weights and, over the tiles side
     // by side, the rows' 128 bytes each; rows by the 160 in CTAs side by side, which read the same weights at the same time, carry the
-    // least beyond 256. (From 161 to 256 one tile of all rows is better: 192 rows 260 us, as two of 96 353; 256 rows 304, as two of 128 362.)
+    // least beyond 256. (From 161 to 256 one tile of all rows is better: 192 rows 253 us, as two of 96 353; 256 rows 304, as two of 128 362.)
     const uint32_t tiles = rows <= kMaxColumns ? 1u : (rows + kPairRows - 1) / kPairRows;
     a.n = ((rows + tiles - 1) / tiles + 15u) & ~15u;
     a.side = a.n <= kMaxColumns / 4 ? 4u : a.n <= kPairRows ? 2u : 1u;
@@ -612,8 +614,8 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     a.spread = tiles < 8u ? tiles : 8u;
     const uint32_t x_bytes = a.n * kBlockK * 2;
     // What a step costs beside its bytes is the issuing thread's time, barriers mostly: steps in turns of four share one for the rows, and
-    // the weights come in pieces of 512 bytes a row. In turns of 1, 2, 4 a call without adapters of 129280 x 4096 took 190, 167, 163 us
-    // for one row, 197, 176, 175 for 64, 239, 209, 234 for 128 (whose rows fill the ring), 323, 310, 307 for 256.
+    // the weights come in pieces of 512 bytes a row. In turns of 1, 2, 4 a call without adapters of 129280 x 4096 took 187, 163, 158 us
+    // for one row, 194, 169, 167 for 64, 232, 199, 230 for 128 (whose rows fill the ring), 316, 305, 304 for 256.
     a.turn = a.n <= kMaxColumns / 4 ? 4u : 2u;
     // As deep a ring of tiles as fits: of rows two turns at least, of weights a tile for each of their warps (with fewer a warp could
     // be two rounds of the ring ahead, and take a barrier's phase for another).
@@ -647,7 +649,8 @@ cudaError_t launch(const mk_head& h, const void* hidden, uint64_t hidden_ld, con
     const uint32_t half = a.side == 4u ? a.n : a.n / 2u;
     const bool behind = h.n_adapters != 0;
     // What rows of many adapters wait for is `up`, once for every adapter and step of ranks: 64 rows, 16 adapters of rank 64 at 129280 x 4096
-    // by steps of 16 420 us, of 32 308; of rank 32 223 and 213; 16 rows of rank 64 228 and 234.
+    // by steps of 16 422 us, of 32 313; of rank 32 227 and 217; 96 rows with 4 of rank 128 394 and 336; 16 rows with 4 of rank 64 193 and
+    // 194; a row with one 176 and 178. (16 rows with an adapter of rank 64 each are on the wrong side of the bound: 389 and 308.)
     if (h.n_adapters && h.rank > (uint32_t)kRankStep && a.n > 16u && a.n <= kWideRows)
         return half <= 32 ? launch_tiles<T, 2, 32, kWideStep>(a, grid, behind, maps, stream)
                : half <= 48 ? launch_tiles<T, 2, 48, kWideStep>(a, grid, behind, maps, stream)

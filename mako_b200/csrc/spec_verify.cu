@@ -8,15 +8,17 @@
 // As one cluster per sequence that walks its positions in turn, the chain of reads, exchanges and decisions took 5 us a position; as
 // a CTA per slice, the CTAs spent two thirds of their lives on starting and ending.)
 // Each thread keeps a running maximum and sum of exp2((x - max) log2(e) / T) in fp32, good to about 1e-6; a decision nearer than
-// kNear is left to the second launch. 64 sequences of four drafts, 129280 columns in fp32: 56 us for 242 MB.
+// kNear is left to the second launch. 64 sequences of four drafts, 129280 columns in fp32: 55 us for 234 MB.
 //
 // The second draws, a cluster of CTAs per sequence. In a vocabulary's running sum every token lies next to others, so weights and
-// sums are in 64 bits here: exp2 by a table of 16 steps (one row of the banks: no conflicts) and a quartic, error 4e-11; bound by
-// the 64-bit pipe (23 operations a column) and by the latency of its few steps. max(0, P - Q) wants both rows' whole weights first;
-// instead of a pass for them, the one pass forms A = sum of (p - c q) and B = sum of q over the columns where p > c q, with the
-// c = P's / Q's whole weight that the fp32 sums give, beside the exact sums, and A - (exact c - c) B is what is drawn from: only
-// columns between the two c, 1e-6 apart, are off, by as much again (rows so alike that this matters are summed twice, see draw()). The sums by CTA and warp lead to one warp's columns, which the
-// CTA goes over once more, eight a thread. 53 us for the same sequences, 16 for a single one.
+// sums are in 64 bits here: exp2 by a table of 16 steps (one row of the banks: no conflicts) and a quartic, error 4e-11. max(0, P - Q)
+// wants both rows' whole weights first; instead of a pass for them, the one pass forms A = sum of (p - c q) and B = sum of q over the
+// columns where p > c q, with the c = P's / Q's whole weight that the fp32 sums give, beside the exact sums, and A - (exact c - c) B is
+// what is drawn from: only columns between the two c, 1e-6 apart, are off, by as much again (rows so alike that this matters are summed
+// twice, see draw()). The sums by CTA and warp lead to one warp's columns, which the CTA goes over once more, eight a thread. 52 us for
+// the same sequences, 16 for a single one: neither the 64-bit pipe (23 operations a column, a quarter of its rate) nor DRAM (64 MB, 16 %)
+// bounds it, it waits: 0.45 instructions a cycle from 24 warps an SM of 80 registers, one block of 16 bytes a lane under way, and its few
+// steps one behind another.
 #include "ptx.cuh"
 #include "round_ops.h"
 
@@ -190,7 +192,8 @@ struct Row {
         const double d = (((double)__fmul_rn(mass.m, scale) - zero() / kSteps) + (double)mass.m * (scale64 - (double)scale)) * 0.6931471805599453;
         return (double)mass.s * (1.0 + d * (1.0 + d * (1.0 / 2.0 + d * (1.0 / 6.0 + d / 24.0)))); // |d| < 0.1
     }
-    // A logit's logarithm of its part.
+    // A logit's logarithm of its part. From the fp32 sums, which are off by 1e-7 as fp32 itself is for logarithms of a few units: a
+    // kept draft's whole weight in 64 bits would be a pass over its row.
     __device__ float log_part(float x) const
     {
         if (far())
