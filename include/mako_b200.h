@@ -305,8 +305,8 @@ typedef struct mk_spec_rows {
  * its temperature), or all of Q on the draft: draft j is kept iff u[s][j] Q(d) < P(d); at the first one refused the token is
  * drawn from max(0, P - Q) with u[s][j + 1]; where no draft is refused it is drawn from P of the position behind the last one
  * with that position's u[s][j]. A draw is the first token, by id, at which the running sum is above u times the whole; weights
- * and running sums of a draw are in 64 bits, and what weighs below 1e-290 of the largest weighs nothing. Where max(0, P - Q) is
- * nothing, P is drawn from.
+ * and running sums of a draw are in 64 bits, and what weighs below 1e-290 of the largest weighs nothing, nor does a column of
+ * max(0, P - Q) that has less than 2^-48 of its P, a rounding. Where max(0, P - Q) is nothing, P is drawn from.
  * NaN and masked logits weigh nothing; where the largest is +inf, its first place weighs all. A row in which nothing weighs
  * anything refuses its draft, and gives next_token -1 and MK_FLAG_NO_CANDIDATE (with MK_FLAG_ALL_MASKED where its mask allows
  * no token). Outputs, device: n_kept[n_seq], next_token[n_seq]; optional tokens[n_seq][n_pos] (the kept drafts, next_token,

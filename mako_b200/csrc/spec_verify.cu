@@ -14,8 +14,8 @@
 // sums are in 64 bits here: exp2 by a table of 16 steps (one row of the banks: no conflicts) and a quartic, error 4e-11. max(0, P - Q)
 // wants both rows' whole weights first; instead of a pass for them, the one pass forms A = sum of (p - c q) and B = sum of q over the
 // columns where p > c q, with the c = P's / Q's whole weight that the fp32 sums give, beside the exact sums, and A - (exact c - c) B is
-// what is drawn from: only columns between the two c, 1e-6 apart, are off, by as much again (rows so alike that this matters are summed
-// twice, see draw()). The sums by CTA and warp lead to one warp's columns, which the CTA goes over once more, eight a thread. 52 us for
+// what is drawn from: only columns between the two c, 1e-6 apart, are off, by as much again (rows so alike that this matters are drawn from
+// once more, see draw()). The sums by CTA and warp lead to one warp's columns, which the CTA goes over once more, eight a thread. 52 us for
 // the same sequences, 16 for a single one: neither the 64-bit pipe (23 operations a column, a quarter of its rate) nor DRAM (64 MB, 16 %)
 // bounds it, it waits: 0.45 instructions a cycle from 24 warps an SM of 80 registers, one block of 16 bytes a lane under way, and its few
 // steps one behind another.
@@ -37,7 +37,7 @@ constexpr uint32_t kSteps = 16;   // of the table of exp2
 constexpr uint32_t kParts = 8;   // of a warp's share of a row
 constexpr float kNear = 3e-5f;    // decisions nearer than this, relative, are taken in 64 bits
 constexpr float kFew = 1e-30f;    // and those of probabilities of which fp32 may hold few bits or none: ex2_approx ends at 2^-126
-constexpr double kLoose = 1e-4;    // see draw()
+constexpr double kLoose = 1e-4, kLittle = 1e-6; // see draw()
 constexpr double kSome = 1e-290;   // a weight below this, where the largest is about 1, is none
 constexpr double kSteepest = 3e38; // log2(e) / T above this is none of fp32's numbers
 constexpr float kHottest = 1e30f;  // a temperature from here on is not one
@@ -681,9 +681,9 @@ __device__ __forceinline__ double entry(uint32_t table, uint32_t i)
 }
 
 // Weights in 64 bits of columns x of the row, in units of the step next to the maximum's: 2^(k/16) from the table times a quartic
-// of the rest r, |r| <= 1/32 of a power: (r ln2)^5 / 120 = 4e-11 at most, of either sign. Step by step for all of them, so that
-// their operations stand between one another.
-template <int N, typename T>
+// of the rest r, |r| <= 1/32 of a power: (r ln2)^5 / 120 = 4e-11 at most, of either sign. Fine: two terms more, (r ln2)^7 / 5040 = 5e-16.
+// Step by step for all of them, so that their operations stand between one another.
+template <bool Fine, int N, typename T>
 __device__ __forceinline__ void weights64(const Weigh<T>& row, const float (&x)[N], double (&w)[N], uint32_t table)
 {
     constexpr double ln2 = 0.6931471805599453 / kSteps;
@@ -707,9 +707,17 @@ __device__ __forceinline__ void weights64(const Weigh<T>& row, const float (&x)[
 #pragma unroll
     for (int i = 0; i < N; ++i)
         r[i] = fma(d[i], row.steps, r[i]);
+    if (Fine) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            w[i] = fma(ln2 * ln2 * ln2 * ln2 * ln2 * ln2 / 720.0, r[i], ln2 * ln2 * ln2 * ln2 * ln2 / 120.0);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            w[i] = fma(w[i], r[i], ln2 * ln2 * ln2 * ln2 / 24.0);
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-        w[i] = fma(ln2 * ln2 * ln2 * ln2 / 24.0, r[i], ln2 * ln2 * ln2 / 6.0);
+        w[i] = fma(Fine ? w[i] : ln2 * ln2 * ln2 * ln2 / 24.0, r[i], ln2 * ln2 * ln2 / 6.0);
 #pragma unroll
     for (int i = 0; i < N; ++i)
         w[i] = fma(w[i], r[i], ln2 * ln2 / 2.0);
@@ -733,14 +741,15 @@ __device__ __forceinline__ double weight_of(const Row<T>& row, uint32_t i, uint3
 {
     const float x[1] = {row.get(i)};
     double w[1];
-    weights64(Weigh<T>(row), x, w, table);
+    weights64<false>(Weigh<T>(row), x, w, table);
     return w[0] > kSome ? w[0] : 0.0;
 }
 
-// x where that is above 0, else 0: no branch, no comparison of 64 bits.
-__device__ __forceinline__ double above(double x, double of)
+// x where d = p - c q is above 2^-48 p, else 0; no branch, no comparison of 64 bits. Less than that is what roundings leave of columns that
+// weigh the same in P and Q, and would be drawn from where little else is left.
+__device__ __forceinline__ double if_more(double x, double d, double p)
 {
-    const int keep = ~(__double2hiint(of) >> 31);
+    const int keep = __double2hiint(d) > __double2hiint(p) - (48 << 20) ? -1 : 0;
     return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
 }
 
@@ -770,7 +779,7 @@ __device__ __forceinline__ uint4 load_block(const Weigh<T>& r, int32_t i0, uint3
 }
 
 // Weights of a block's columns of both rows, and f(column's place in the block, p, q) of each. Plain: all columns count.
-template <typename T, bool Against, bool Plain, typename F>
+template <typename T, bool Against, bool Plain, bool Fine, typename F>
 __device__ __forceinline__ void each_weight(const Rest<T>& rest, int32_t i0, uint32_t n, const uint4& wp, const uint4& wq,
                                             uint32_t table, F f)
 {
@@ -812,9 +821,9 @@ __device__ __forceinline__ void each_weight(const Rest<T>& rest, int32_t i0, uin
                 u[i] = without == (uint32_t)e ? -kInf : u[i];
             q[i] = 0.0;
         }
-        weights64(rest.p, u, p, table);
+        weights64<Fine>(rest.p, u, p, table);
         if (Against)
-            weights64(rest.q, v, q, table);
+            weights64<Fine>(rest.q, v, q, table);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             f(at + i, p[i], q[i]);
@@ -836,7 +845,7 @@ struct Share {
 
 // The sums over the CTA's share of the row, by warp in s.warp, by its parts in s.upto, and of the CTA: A and B of what is drawn
 // from, whole weights.
-template <typename T, bool Against, bool Plain>
+template <typename T, bool Against, bool Plain, bool Fine>
 __device__ __noinline__ Sums sweep_rows(const Rest<T> rest, Shared& s, const Part c)
 {
     constexpr int deep = Share::kDeep;
@@ -850,8 +859,8 @@ __device__ __noinline__ Sums sweep_rows(const Rest<T> rest, Shared& s, const Par
         if (Against) {
             const double d = fma(-rest.c, q, p);
             x.q += q;
-            x.a += above(d, d);
-            x.b += above(q, d);
+            x.a += if_more(d, d, p);
+            x.b += if_more(q, d, p);
         }
     };
     auto all_lanes = [](double v) {
@@ -885,7 +894,7 @@ __device__ __noinline__ Sums sweep_rows(const Rest<T> rest, Shared& s, const Par
 #pragma unroll
         for (int i = 0; i < deep; ++i)
             if (b + lane + i * 32u < mine.b1)
-                each_weight<T, Against, Plain>(rest, k.column(b + lane + i * 32u), n, vp[i], vq[i], table, add);
+                each_weight<T, Against, Plain, Fine>(rest, k.column(b + lane + i * 32u), n, vp[i], vq[i], table, add);
         if (b + Share::kRound == next || b + Share::kRound >= mine.b1) {
             __syncwarp();
             upto = make_double2(all_lanes(Against ? x.a : x.p), Against ? all_lanes(x.b) : 0.0);
@@ -923,12 +932,12 @@ __device__ __forceinline__ bool is_plain(const Rest<T>& rest)
     return !rest.p.mask && (!rest.against || (!rest.q.mask && ((reinterpret_cast<uintptr_t>(rest.p.x) ^ reinterpret_cast<uintptr_t>(rest.q.x)) & 15u) == 0));
 }
 
-template <typename T>
+template <typename T, bool Fine>
 __device__ Sums sweep(const Rest<T>& rest, Shared& s, const Part& c)
 {
     if (is_plain(rest))
-        return rest.against ? sweep_rows<T, true, true>(rest, s, c) : sweep_rows<T, false, true>(rest, s, c);
-    return rest.against ? sweep_rows<T, true, false>(rest, s, c) : sweep_rows<T, false, false>(rest, s, c);
+        return Fine || rest.against ? sweep_rows<T, true, true, Fine>(rest, s, c) : sweep_rows<T, false, true, false>(rest, s, c);
+    return Fine || rest.against ? sweep_rows<T, true, false, Fine>(rest, s, c) : sweep_rows<T, false, false, false>(rest, s, c);
 }
 
 // Of the lanes' parts x of a whole, in order: the first lane at whose end the running sum is above `want`, the last with any part
@@ -952,7 +961,7 @@ __device__ __forceinline__ uint32_t pick(double x, double want, double start, do
 template <typename T>
 __device__ double2 whole(const Row<T>& p, const Row<T>* q, Shared& s, Part& c)
 {
-    const double2(*all)[2] = exchange(s, c, sweep(Rest<T>{Weigh<T>(p), Weigh<T>(q ? *q : p), q != nullptr, ~0u, 1.0}, s, c));
+    const double2(*all)[2] = exchange(s, c, sweep<T, false>(Rest<T>{Weigh<T>(p), Weigh<T>(q ? *q : p), q != nullptr, ~0u, 1.0}, s, c));
     double2 sum = make_double2(0.0, 0.0);
     for (uint32_t k = 0; k < c.size; ++k) {
         sum.x += all[k][1].x;
@@ -963,7 +972,7 @@ __device__ double2 whole(const Row<T>& p, const Row<T>* q, Shared& s, Part& c)
 
 // The first column of the blocks [b0, b1) at which the running sum, `before` in front of them, is above `want`; the last that weighs
 // anything where there is none. By the whole CTA, a block a thread.
-template <typename T, bool Against>
+template <typename T, bool Against, bool Fine>
 __device__ __noinline__ int32_t walk(const Rest<T> rest, uint32_t b0, uint32_t b1, double before, double want, Shared& s, const Part c)
 {
     constexpr int per = (int)Blocks<T>::per;
@@ -977,9 +986,9 @@ __device__ __noinline__ int32_t walk(const Rest<T> rest, uint32_t b0, uint32_t b
         const uint32_t b = base + threadIdx.x;
         const int32_t i0 = k.column(min(b, b1 - 1u));
         const uint4 wp = load_block(rest.p, i0, c.n, true), wq = Against ? load_block(rest.q, i0, c.n, aligned) : wp;
-        each_weight<T, Against, false>(rest, i0, c.n, wp, wq, table, [&](int e, double p, double q) {
+        each_weight<T, Against, false, Fine>(rest, i0, c.n, wp, wq, table, [&](int e, double p, double q) {
             const double d = Against ? fma(-rest.c, q, p) : p;
-            x[e] = b < b1 ? above(d, d) : 0.0;
+            x[e] = b < b1 ? if_more(d, d, p) : 0.0; // (of P alone d is p)
         });
 #pragma unroll
         for (int e = 0; e < per; ++e) {
@@ -1021,37 +1030,48 @@ __device__ __noinline__ int32_t walk(const Rest<T> rest, uint32_t b0, uint32_t b
 }
 
 // The first column at which the running sum of `rest` is above u times the whole, in every CTA; -1 where the whole is nothing.
-template <typename T>
-__device__ int32_t draw(Rest<T> rest, double u, Shared& s, Part& c)
+//
+// The sums have the wrong sign for columns between the two c, up to |off| q of each. Rows whose p / q spread are off by the square of
+// |off| over the rest, a few 1e-12; where all of Q lay between, it could be |off| over the rest. Above 1e-4 of that, which means rows
+// alike to a hundredth, or where the rest is less than 1e-6 of P, the answer is kAgain: the draw is made once more, Fine, with weights
+// of two terms more, whose sums are formed with the exact c (the second time off is 0: whole weights do not depend on c). From 1e-6 on
+// nearly every refused draft would be drawn again: 64 sequences of four drafts 104 -> 123 us.
+constexpr int32_t kAgain = -2;
+template <typename T, bool Fine>
+__device__ __forceinline__ int32_t draw(Rest<T> rest, double u, Shared& s, Part& c)
 {
     const uint32_t lane = threadIdx.x & 31u;
-    double off = 0.0, of_cta, total, before; // off: the exact c above the one that the sums were formed with
-    // The sums have the wrong sign for columns between the two c, up to |off| q of each. Rows whose p / q spread are off by the square of
-    // |off| over the rest, a few 1e-12; where all of Q lay between, it could be |off| over the rest. Above 1e-4 of that, which means
-    // rows alike to a hundredth, once more with the exact c (the second time off is 0: the whole weights do not depend on c). From 1e-6
-    // on nearly every refused draft would be summed twice: 64 sequences of four drafts 104 -> 123 us.
-    for (bool again = false;; again = true) {
-        const double2(*all)[2] = exchange(s, c, sweep(rest, s, c));
-        const double2 mine = lane < c.size ? all[lane][0] : make_double2(0.0, 0.0);
+    if (Fine) {
+        const double2(*all)[2] = exchange(s, c, sweep<T, true>(rest, s, c));
         double2 both = make_double2(0.0, 0.0);
-        if (rest.against) {
-            if (lane < c.size)
-                both = all[lane][1];
-#pragma unroll
-            for (uint32_t d = 16; d; d >>= 1) {
-                both.x += __shfl_xor_sync(~0u, both.x, d);
-                both.y += __shfl_xor_sync(~0u, both.y, d);
-            }
-            off = both.x / both.y - rest.c;
-            rest.c = both.x / both.y;
+        for (uint32_t k = 0; k < c.size; ++k) {
+            both.x += all[k][1].x;
+            both.y += all[k][1].y;
         }
-        total = of_cta = fma(-off, mine.y, mine.x);
-#pragma unroll
-        for (uint32_t d = 16; d; d >>= 1)
-            total += __shfl_xor_sync(~0u, total, d);
-        if (again || fabs(off) * both.y <= kLoose * total)
-            break;
+        rest.c = both.x / both.y;
     }
+    const double2(*all)[2] = exchange(s, c, sweep<T, Fine>(rest, s, c));
+    const double2 mine = lane < c.size ? all[lane][0] : make_double2(0.0, 0.0);
+    double off = 0.0; // the exact c above the one that the sums were formed with
+    double2 both = make_double2(0.0, 0.0);
+    if (!Fine && rest.against) {
+        if (lane < c.size)
+            both = all[lane][1];
+#pragma unroll
+        for (uint32_t d = 16; d; d >>= 1) {
+            both.x += __shfl_xor_sync(~0u, both.x, d);
+            both.y += __shfl_xor_sync(~0u, both.y, d);
+        }
+        off = both.x / both.y - rest.c;
+        rest.c = both.x / both.y;
+    }
+    const double of_cta = fma(-off, mine.y, mine.x);
+    double total = of_cta, before;
+#pragma unroll
+    for (uint32_t d = 16; d; d >>= 1)
+        total += __shfl_xor_sync(~0u, total, d);
+    if (!Fine && rest.against && !(fabs(off) * both.y <= kLoose * total && total > kLittle * both.x))
+        return kAgain;
     if (!(total > kSome))
         return -1;
     const double want = u * total;
@@ -1072,9 +1092,17 @@ __device__ int32_t draw(Rest<T> rest, double u, Shared& s, Part& c)
         if (threadIdx.x == 0)
             s.token = 0x7fffffff;
         __syncthreads();
-        found = rest.against ? walk<T, true>(rest, b0, b1, before, want, s, c) : walk<T, false>(rest, b0, b1, before, want, s, c);
+        found = Fine || rest.against ? walk<T, true, Fine>(rest, b0, b1, before, want, s, c) : walk<T, false, false>(rest, b0, b1, before, want, s, c);
     }
     return (int32_t)exchange(s, c, Sums{(double)found, 0.0, 0.0, 0.0})[owner][0].x;
+}
+
+// Out of the way of the others. The turn of the exchanges goes with the answer, so that no one has it in memory.
+template <typename T>
+__device__ __noinline__ int2 draw_fine(Rest<T> rest, double u, Shared& s, Part c)
+{
+    const int32_t token = draw<T, true>(rest, u, s, c);
+    return make_int2(token, (int32_t)c.turn);
 }
 
 template <typename T>
@@ -1183,7 +1211,12 @@ __global__ void __launch_bounds__(kDrawThreads, 2) spec_draw_kernel(const SpecVe
                     rest.without = (uint32_t)d;
                 }
                 for (bool all = false; token < 0 && !all;) { // where nothing is left of P, it is drawn from as a whole
-                    token = draw(rest, with, s, c);
+                    token = draw<T, false>(rest, with, s, c);
+                    if (token == kAgain) {
+                        const int2 fine = draw_fine(rest, with, s, c);
+                        token = fine.x;
+                        c.turn = (uint32_t)fine.y;
+                    }
                     all = !rest.against && rest.without == ~0u;
                     rest.against = false;
                     rest.without = ~0u;

@@ -114,3 +114,34 @@ def test_temperatures_whose_inverse_passes_fp32(gpu_sampler_factory):
     got = verify.compare(gpu_sampler_factory(129280, 512), c)
     # the second one keeps its draft; the token behind it is drawn with 0.3, which is below 0.622
     assert got.n_kept.tolist() == [0, 1] and got.next_token.tolist() == [16, 0]
+
+
+def test_p_and_q_alike_but_for_what_is_next_to_nothing(gpu_sampler_factory):
+    """Both rows are one token's, all but 2e-28 of P and less of Q, and the draft weighs nothing in either: what P has above Q is spread over
+    the others, however little it is; 1 - 1 is nothing."""
+    v, n = 500, 24
+    rng = np.random.default_rng(3)
+    p, q = np.full((n, 2, v), -np.inf, np.float32), np.full((n, 1, v), -np.inf, np.float32)
+    p[:, :, 33], q[:, :, 33] = rng.uniform(0.2, 0.5, (n, 1)), rng.uniform(0.2, 0.5, (n, 1))
+    p[:, :, 17], q[:, :, 17] = p[:, :, 33] - 0.085, q[:, :, 33] - 0.2
+    p[:, :, 400], q[:, :, 400] = p[:, :, 33] - 0.0855, q[:, :, 33] - 0.2
+    c = plain(n, 1, v, p, np.full((n, 1), 5), np.stack([np.full(n, 0.5), rng.random(n), rng.random(n)], 1), 0.00135, q)
+    got = verify.compare(gpu_sampler_factory(129280, 512), c)
+    assert set(got.next_token.tolist()) == {17, 400}
+
+
+def test_p_and_q_the_same_but_for_a_constant(gpu_sampler_factory):
+    """A draft that weighs nothing in either is refused; max(0, P - Q) is nothing, so P is drawn from (in 64 bits P - Q is of roundings)."""
+    v, n = 1000, 200
+    rng = np.random.default_rng(4)
+    p = np.round(rng.normal(0.0, 2.0, (n, 2, v)) * 1024) / 1024
+    p[:, :, 5] = -np.inf
+    q = p[:, :1] + rng.integers(1, 2048, (n, 1, 1)) / 512
+    u = np.stack([np.full(n, 0.5), rng.random(n), rng.random(n)], 1).astype(np.float32)
+    c = plain(n, 1, v, p, np.full((n, 1), 5), u, 0.7, q)
+    cuda = lambda x: torch.as_tensor(x).cuda()  # noqa: E731
+    got = gpu_sampler_factory(129280, 512).spec_verify(cuda(c["logits"]), cuda(c["drafts"]), cuda(c["u"]), cuda(c["temperature"]),
+                                                       draft_logits=cuda(c["draft_logits"]))
+    run = np.cumsum(np.exp(p[:, 0] / float(np.float32(0.7))), 1)
+    want = (run <= u[:, 1:2].astype(np.float64) * run[:, -1:]).sum(1)
+    assert got.n_kept.tolist() == [0] * n and got.next_token.tolist() == want.tolist()
