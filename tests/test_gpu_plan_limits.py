@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+from tests import round_oracle as oracle
 from tests import test_gpu_kv_plan as kv
 from tests.conftest import ROOT
 
@@ -65,3 +66,32 @@ def test_two_threads_of_other_sizes():
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+def test_plans_of_one_handle_side_by_side(gpu_sampler_factory):
+    """Four streams, one handle, arrays of their own: pages taken and given back, over and over."""
+    from mako_b200 import KvPlan
+    sampler, rng, work = gpu_sampler_factory(32, 1), np.random.default_rng(6), []
+    for s in (300, 1000, 4500, 64):
+        table, held, free, n_free, ln, nw = kv.make(rng, s, 16, 200, 9, 4 * s)
+        held = -(-ln // 16)
+        ids = rng.permutation(int(held.sum()) + 4 * s).astype(np.int32)
+        table[:] = -1
+        for i, at in enumerate(np.cumsum(held) - held):
+            table[i, :held[i]] = ids[at:at + held[i]]
+        free = np.concatenate([ids[held.sum():], np.full(held.sum(), -1, np.int32)])
+        d = [torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).cuda() for x in (table, held, free, [4 * s], ln)]
+        want, _ = oracle.plan(table, held.astype(np.int32), free, 4 * s, ln, nw, 16, 9 * s)
+        work.append((d, [x.clone() for x in d], torch.from_numpy(nw).cuda(), KvPlan.empty(s, 9 * s), want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(40):
+        for d, _, nw, plan, _, stream in work:
+            with torch.cuda.stream(stream):
+                sampler.kv_plan(*d, nw, page_size=16, out=plan)
+                sampler.kv_plan(*d, page_size=16)
+    torch.cuda.synchronize()
+    for d, before, _, plan, want, _ in work:
+        for x, y in zip(d, before):
+            assert torch.equal(x, y)
+        for k, x in want.items():
+            assert np.array_equal(getattr(plan, k).cpu().numpy().astype(np.int64), np.asarray(x, dtype=np.int64)), k
