@@ -16,8 +16,8 @@
 // columns where p > c q, with the c = P's / Q's whole weight that the fp32 sums give, beside the exact sums, and A - (exact c - c) B is
 // what is drawn from: only columns between the two c, 1e-6 apart, are off, by as much again (rows so alike that this matters are drawn from
 // once more, see draw()). The sums by CTA and warp lead to one warp's columns, which the CTA goes over once more, eight a thread. 52 us for
-// the same sequences, 16 for a single one: neither the 64-bit pipe (23 operations a column, a quarter of its rate) nor DRAM (64 MB, 16 %)
-// bounds it, it waits: 0.45 instructions a cycle from 24 warps an SM of 80 registers, one block of 16 bytes a lane under way, and its few
+// the same sequences, 16 for a single one: neither the 64-bit pipe (23 operations a column, a quarter of its rate) nor DRAM (65 MB, 17 %)
+// bounds it, it waits: 0.44 instructions a cycle from 24 warps an SM of 80 registers, one block of 16 bytes a lane under way, and its few
 // steps one behind another.
 #include "ptx.cuh"
 #include "round_ops.h"
