@@ -359,6 +359,110 @@ typedef struct mk_kv_plan {
 int mk_kv_plan_step(mk_sampler* s, const mk_kv_pages* pages, const int32_t* cache_len, const int32_t* n_new, uint32_t n_seq,
                     const mk_kv_plan* plan, void* stream);
 
+/* Whole distributions whose tokens' log-probabilities are wanted: rows of one type, MK_FP32, MK_BF16 or MK_FP16, that start at any
+ * element and are read in whole 16-byte blocks, as mk_rows says. */
+typedef struct mk_logprob_rows {
+    const void* logits;       /* device [rows][ld] */
+    uint64_t ld;
+    int type;
+    uint32_t rows, n_vocab;   /* n_vocab at most 2^28 */
+    const int32_t* tokens;    /* device [rows][n_given] the tokens asked for, or NULL where n_given is 0 */
+    uint32_t n_given;
+    uint32_t n_top;           /* alternatives wanted, at most 64 */
+    const float* temperature; /* device [rows], or NULL: temperature_all. Not above 1e-30, or 1e30 and more: the largest logit alone */
+    float temperature_all;
+    const uint32_t* mask;     /* device [rows][mask_ld] allowed tokens, or NULL */
+    uint64_t mask_ld;
+} mk_logprob_rows;
+
+/* With P = softmax(row / temperature) over the tokens that the mask allows: logprob[rows][n_given] = ln P of the tokens asked for
+ * (-inf where P is nothing, 0 for one outside [0, n_vocab), which names none), entropy[rows] = -sum P ln P, top_ids[rows][n_top]
+ * the likeliest tokens, the largest logit first and the lowest id among equals, with their ln P in top_logprob[rows][n_top] (-1 and
+ * -inf where there are no more). Outputs, device, each optional; flags[rows]. NaN and masked logits weigh nothing; where the largest is
+ * +inf, or the temperature selects it, its first place weighs all. A row in which nothing weighs anything has -inf throughout, entropy
+ * 0 and MK_FLAG_NO_CANDIDATE (with MK_FLAG_ALL_MASKED where its mask allows no token). Weights and sums are in fp32. A call uses
+ * nothing of the handle but its device: calls may overlap, on one handle too. */
+int mk_token_logprobs(mk_sampler* s, const mk_logprob_rows* rows, float* logprob, float* entropy, int32_t* top_ids,
+                      float* top_logprob, uint32_t* flags, void* stream);
+
+/* A paged cache of keys and values in 8 bits: e4m3 codes (a sign, four bits of exponent, three of mantissa; 0x7f and 0xff are NaN,
+ * there are no infinities), a scale for each page and head. What a code stands for times its scale is the value. A page's head is
+ * page_size rows of dim codes; strides are in bytes, multiples of 16, the same for k and v, which start on 16-byte boundaries. The
+ * pages are those of mk_kv_pages. */
+typedef struct mk_kv_cache {
+    void* k;          /* device: page p, head h, place i at k + p * page_stride + h * head_stride + i * token_stride */
+    void* v;
+    float* k_scale;   /* device [n_pages][n_heads] */
+    float* v_scale;
+    uint64_t page_stride, head_stride, token_stride;
+    uint32_t n_pages, n_heads; /* heads of keys and values */
+    uint32_t page_size, dim;   /* tokens a page; columns a head, a multiple of 16, at most 256 */
+} mk_kv_cache;
+
+/* Keys and values of a pass, and queries to be rotated with them. Rows of a token have their heads side by side, [heads][dim]; ld:
+ * elements from one token to the next, a multiple of 8; all start on 16-byte boundaries. */
+typedef struct mk_kv_rows {
+    const void *k, *v;        /* device [n_tokens][ld] */
+    uint64_t k_ld, v_ld;
+    const void* q;            /* device [n_tokens][q_ld], or NULL */
+    void* q_out;              /* device [n_tokens][q_out_ld]; may be q */
+    uint64_t q_ld, q_out_ld;
+    uint32_t n_q_heads;       /* a multiple of the cache's heads */
+    int type;                 /* MK_BF16 or MK_FP16 */
+    uint32_t n_tokens;
+    const int32_t* positions; /* device [n_tokens]; unread without a rotation */
+    const int64_t* slots;     /* device [n_tokens] page * page_size + place; one outside of the cache: the row is padding */
+} mk_kv_rows;
+
+/* Rotary positions. The first dim columns of each head of q and k turn, in pairs, by the angles position * inv_freq[i], i from 0 to
+ * dim / 2: columns i and i + dim / 2 or, interleaved, 2i and 2i + 1. What scales positions for long contexts is in inv_freq and, for
+ * the turned columns, in scale. */
+typedef struct mk_rotary {
+    const float* inv_freq;    /* device [dim / 2], or NULL: no rotation */
+    uint32_t dim;             /* a multiple of 16, at most the cache's */
+    int interleaved;
+    float scale;
+} mk_rotary;
+
+/* Puts a pass's keys, rotated, and values into the cache, at the slots that mk_kv_plan_step gave. Rows that go into one page stand side by
+ * side, at rising places without a gap, and a page has one such run a call (a plan's rows do). A run that begins at place 0 takes
+ * the page over: its scales become those of the run. One that begins behind leaves what stands before it: a scale becomes the larger of
+ * the page's and the run's, and where it has grown the older codes are brought to it. The scale of numbers up to m is the least power of
+ * two s with m <= 448 s, at least 2^-100; codes are rounded to nearest even; what is no finite number becomes NaN and has no part in
+ * m. Angles are formed in 64 bits; rotated numbers are rounded once, to 8 bits or, in q_out, to the type. Rows of padding are left as they
+ * are, in q_out as well. Uses nothing of the handle but its device. */
+int mk_kv_append(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_rows* rows, const mk_rotary* rotary, void* stream);
+
+/* A pass's queries over a paged cache. Sequence i's are rows query_start[i] to query_start[i + 1] of q, the last ones of its kv_len[i]
+ * tokens, whose pages are in row i of the block table: what mk_kv_plan_step gives, once mk_kv_append has run. */
+typedef struct mk_kv_queries {
+    const void* q;              /* device [n_tokens][q_ld], heads side by side */
+    void* out;                  /* device [n_tokens][out_ld]; not q */
+    uint64_t q_ld, out_ld;      /* elements, multiples of 8; q and out start on 16-byte boundaries */
+    uint32_t n_q_heads;         /* a multiple of the cache's heads; query head i reads key head i / (n_q_heads / n_heads) */
+    int type;                   /* MK_BF16 or MK_FP16 */
+    uint32_t n_tokens;          /* rows of q and out: none beyond is touched, whatever query_start says */
+    const int32_t* block_table; /* device [n_seq][table_ld], table_cols used */
+    uint64_t table_ld;
+    uint32_t table_cols;
+    const int32_t* query_start; /* device [n_seq + 1] */
+    const int32_t* kv_len;      /* device [n_seq]; at most table_cols pages of it are read */
+    uint32_t n_seq;             /* at most 8192 */
+    uint32_t max_new;           /* the most tokens that a sequence has in the pass, or 0: not known. Chooses kernels, nothing else */
+    float scale;                /* of a score */
+    uint32_t window;            /* a token sees so many keys, its own among them; 0: all before it and its own */
+    void* workspace;            /* device, 16-byte aligned, mk_kv_attention_bytes(); no other call's until this one has run */
+    uint64_t workspace_bytes;
+} mk_kv_queries;
+
+/* out[t][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q[t][h] . k_j), over the keys j that the token sees. Keys whose page is outside of the
+ * cache (a table entry of -1) are not there; a row that sees none is zeros. Rows of q that are no sequence's are left as they are in out.
+ * dim is 64 or 128. Products are of fp16 numbers that codes and queries become without a loss, weights are rounded to fp16 (2^-11 of
+ * each), sums and softmax in fp32. A value that is not a number makes rows that see it NaN (in its column at least), no others. Uses
+ * nothing of the handle but its device. */
+uint64_t mk_kv_attention_bytes(const mk_kv_cache* cache, const mk_kv_queries* queries);
+int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries* queries, void* stream);
+
 /* Vocab-parallel sampling, step 1 of 2 (no counterpart in the reference, which runs on one device): each shard
  * writes one record per row — its maximum, its sum of exp((l - max)/T) and its `k` best candidates (<= 64) — of
  * mk_vp_record_bytes(k) bytes. The caller all-gathers the records of all shards ([n_shards][batch] records,

@@ -4,7 +4,7 @@ The first use of any name below loads libmako_b200.so; that raises ImportError w
 has not been built (`python -m mako_b200.build`, which itself needs no built library). Nothing here computes on the
 CPU.
 """
-_SAMPLER = {"BatchSampler", "KvPlan", "SampleResult", "SpecVerifyResult", "Sampler", "SamplingParams", "check_sampling", "pack_bias", "pack_params"}
+_SAMPLER = {"BatchSampler", "KvCache", "KvPlan", "SampleResult", "SpecVerifyResult", "Sampler", "SamplingParams", "TokenLogprobs", "check_sampling", "pack_bias", "pack_params"}
 _LIB = {"MakoError", "lib", "FLAG_ALL_MASKED", "FLAG_GUARD_BAND", "FLAG_NEAR_CDF_BOUNDARY", "FLAG_NO_CANDIDATE",
         "FLAG_OVERFLOW", "FLAG_TIMEOUT", "FLAG_HISTORY_FULL", "FLAG_VP_TRUNCATED", "FLAG_PLAN_INVALID", "FLAG_NO_ROOM",
         "FLAG_NO_PAGES"}

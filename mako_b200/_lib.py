@@ -138,6 +138,89 @@ class KvPlanC(C.Structure):
     ]
 
 
+class LogprobRowsC(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("ld", C.c_uint64),
+        ("type", C.c_int),
+        ("rows", C.c_uint32),
+        ("n_vocab", C.c_uint32),
+        ("tokens", C.c_void_p),
+        ("n_given", C.c_uint32),
+        ("n_top", C.c_uint32),
+        ("temperature", C.c_void_p),
+        ("temperature_all", C.c_float),
+        ("mask", C.c_void_p),
+        ("mask_ld", C.c_uint64),
+    ]
+
+
+class KvCacheC(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("page_stride", C.c_uint64),
+        ("head_stride", C.c_uint64),
+        ("token_stride", C.c_uint64),
+        ("n_pages", C.c_uint32),
+        ("n_heads", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("dim", C.c_uint32),
+    ]
+
+
+class KvRowsC(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_ld", C.c_uint64),
+        ("v_ld", C.c_uint64),
+        ("q", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("q_ld", C.c_uint64),
+        ("q_out_ld", C.c_uint64),
+        ("n_q_heads", C.c_uint32),
+        ("type", C.c_int),
+        ("n_tokens", C.c_uint32),
+        ("positions", C.c_void_p),
+        ("slots", C.c_void_p),
+    ]
+
+
+class RotaryC(C.Structure):
+    _fields_ = [
+        ("inv_freq", C.c_void_p),
+        ("dim", C.c_uint32),
+        ("interleaved", C.c_int),
+        ("scale", C.c_float),
+    ]
+
+
+class KvQueriesC(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_ld", C.c_uint64),
+        ("out_ld", C.c_uint64),
+        ("n_q_heads", C.c_uint32),
+        ("type", C.c_int),
+        ("n_tokens", C.c_uint32),
+        ("block_table", C.c_void_p),
+        ("table_ld", C.c_uint64),
+        ("table_cols", C.c_uint32),
+        ("query_start", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("n_seq", C.c_uint32),
+        ("max_new", C.c_uint32),
+        ("scale", C.c_float),
+        ("window", C.c_uint32),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
 class MakoError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"mako_b200 error {code}: {message}")
@@ -181,6 +264,11 @@ def _load() -> C.CDLL:
     lib.mk_head_logits.argtypes = [vp, C.POINTER(HeadC), vp, C.c_uint64, vp, C.c_uint32, vp, C.c_uint64, vp]
     lib.mk_spec_verify.argtypes = [vp, C.POINTER(SpecRowsC), vp, vp, vp, vp, vp, vp]
     lib.mk_kv_plan_step.argtypes = [vp, C.POINTER(KvPagesC), vp, vp, C.c_uint32, C.POINTER(KvPlanC), vp]
+    lib.mk_token_logprobs.argtypes = [vp, C.POINTER(LogprobRowsC), vp, vp, vp, vp, vp, vp]
+    lib.mk_kv_append.argtypes = [vp, C.POINTER(KvCacheC), C.POINTER(KvRowsC), C.POINTER(RotaryC), vp]
+    lib.mk_kv_attention_bytes.restype = C.c_uint64
+    lib.mk_kv_attention_bytes.argtypes = [C.POINTER(KvCacheC), C.POINTER(KvQueriesC)]
+    lib.mk_kv_attention.argtypes = [vp, C.POINTER(KvCacheC), C.POINTER(KvQueriesC), vp]
     lib.mk_vp_record_bytes.restype = C.c_uint32
     lib.mk_vp_record_bytes.argtypes = [C.c_uint32]
     lib.mk_sampler_vp_local.argtypes = [vp, C.POINTER(RowsC), C.c_uint32, vp, vp]

@@ -777,6 +777,168 @@ int mk_kv_plan_step(mk_sampler* s, const mk_kv_pages* pages, const int32_t* cach
     return MK_OK;
 }
 
+int mk_token_logprobs(mk_sampler* s, const mk_logprob_rows* r, float* logprob, float* entropy, int32_t* top_ids, float* top_logprob,
+                      uint32_t* flags, void* stream)
+{
+    if (!s || !r)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: null argument");
+    if (r->type != MK_FP32 && r->type != MK_BF16 && r->type != MK_FP16)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: type %d is none of MK_FP32, MK_BF16, MK_FP16", r->type);
+    if (r->n_vocab == 0 || r->n_vocab > (1u << 28) || r->rows > (1u << 28) || r->n_top > mk::kLogprobMaxTop)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: n_vocab %u and rows %u (at most 2^28), n_top %u (at most %u)", r->n_vocab,
+                    r->rows, r->n_top, mk::kLogprobMaxTop);
+    if (r->ld < r->n_vocab)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: ld %llu below n_vocab %u", (unsigned long long)r->ld, r->n_vocab);
+    if (r->mask && r->mask_ld < (uint64_t)(r->n_vocab + 31) / 32)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: mask_ld %llu smaller than ceil(n_vocab/32)",
+                    (unsigned long long)r->mask_ld);
+    if (!r->temperature && !std::isfinite(r->temperature_all))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: the temperature must be finite");
+    if (r->rows == 0)
+        return MK_OK;
+    if (!r->logits || (r->n_given && logprob && !r->tokens))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: logits, and tokens where some are given, are required");
+    if (reinterpret_cast<uintptr_t>(r->logits) & (r->type == MK_FP32 ? 3u : 1u))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_token_logprobs: logits start at an element");
+    DeviceGuard g(s->device);
+    MK_CUDA(mk::launch_token_logprobs(*r, mk::LogprobOut{logprob, entropy, top_ids, top_logprob, flags}, (cudaStream_t)stream));
+    return MK_OK;
+}
+
+namespace {
+
+bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+int check_cache(const mk_kv_cache& c, const char* who)
+{
+    if (c.page_size == 0 || c.page_size > 0x7fffffffu || c.n_pages > 0x7fffffffu || c.n_heads == 0 || c.n_heads > 65535u || c.dim == 0 ||
+        (c.dim & 15u) || c.dim > 256u)
+        return fail(MK_ERR_INVALID_ARGUMENT, "%s: page_size %u, n_pages %u, n_heads %u (at most 65535), dim %u (a multiple of 16, at most 256)",
+                    who, c.page_size, c.n_pages, c.n_heads, c.dim);
+    if (((c.page_stride | c.head_stride | c.token_stride) & 15u) || c.token_stride < c.dim)
+        return fail(MK_ERR_INVALID_ARGUMENT, "%s: strides of %llu, %llu and %llu bytes: multiples of 16, a token's at least dim", who,
+                    (unsigned long long)c.page_stride, (unsigned long long)c.head_stride, (unsigned long long)c.token_stride);
+    if (c.n_pages && (!c.k || !c.v || !c.k_scale || !c.v_scale))
+        return fail(MK_ERR_INVALID_ARGUMENT, "%s: k, v, k_scale and v_scale are required", who);
+    if (off16(c.k) || off16(c.v))
+        return fail(MK_ERR_INVALID_ARGUMENT, "%s: k and v start on 16-byte boundaries", who);
+    return MK_OK;
+}
+
+} // namespace
+
+int mk_kv_append(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_rows* r, const mk_rotary* rotary, void* stream)
+{
+    if (!s || !cache || !r)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: null argument");
+    if (int rc = check_cache(*cache, "mk_kv_append"))
+        return rc;
+    if (r->type != MK_BF16 && r->type != MK_FP16)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: type %d is neither MK_BF16 nor MK_FP16", r->type);
+    const bool turns = rotary && rotary->inv_freq;
+    if (turns && (rotary->dim == 0 || (rotary->dim & 15u) || rotary->dim > cache->dim || !std::isfinite(rotary->scale)))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: a rotation of %u columns (a multiple of 16, at most %u) by a finite scale", rotary->dim,
+                    cache->dim);
+    const uint64_t kv = (uint64_t)cache->n_heads * cache->dim, qs = (uint64_t)r->n_q_heads * cache->dim;
+    if (r->k_ld < kv || r->v_ld < kv || ((r->k_ld | r->v_ld) & 7u) || r->n_tokens > 0x7fffffffu)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: n_tokens %u, k_ld %llu and v_ld %llu: multiples of 8, at least %llu", r->n_tokens,
+                    (unsigned long long)r->k_ld, (unsigned long long)r->v_ld, (unsigned long long)kv);
+    if (r->q && (!r->q_out || r->n_q_heads == 0 || r->n_q_heads % cache->n_heads || r->q_ld < qs || r->q_out_ld < qs || ((r->q_ld | r->q_out_ld) & 7u)))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: n_q_heads %u (a multiple of %u), q_ld %llu and q_out_ld %llu (multiples of 8), q_out", r->n_q_heads,
+                    cache->n_heads, (unsigned long long)r->q_ld, (unsigned long long)r->q_out_ld);
+    if (off16(r->k) || off16(r->v) || off16(r->q) || (r->q && off16(r->q_out)))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: q, k, v and q_out start on 16-byte boundaries");
+    if (r->n_tokens == 0)
+        return MK_OK;
+    if (!r->k || !r->v || !r->slots || (turns && !r->positions))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: k, v, slots and, for a rotation, positions are required");
+    DeviceGuard g(s->device);
+    mk::KvAppendArgs a;
+    a.c = *cache;
+    a.q = r->q;
+    a.k = r->k;
+    a.v = r->v;
+    a.q_out = r->q_out;
+    a.q_ld = r->q_ld;
+    a.k_ld = r->k_ld;
+    a.v_ld = r->v_ld;
+    a.q_out_ld = r->q_out_ld;
+    a.positions = r->positions;
+    a.slots = r->slots;
+    a.n_tokens = r->n_tokens;
+    a.group = r->q ? r->n_q_heads / cache->n_heads : 0u;
+    a.inv_freq = turns ? rotary->inv_freq : nullptr;
+    a.rotary = turns ? rotary->dim : 0u;
+    a.interleaved = turns && rotary->interleaved;
+    a.rotary_scale = turns ? rotary->scale : 1.0f;
+    a.tokens_each = 1;
+    MK_CUDA(mk::launch_kv_append(a, r->type, (cudaStream_t)stream));
+    return MK_OK;
+}
+
+uint64_t mk_kv_attention_bytes(const mk_kv_cache* cache, const mk_kv_queries* q)
+{
+    return cache && q ? mk::kv_attend_bytes(cache->dim) : 0;
+}
+
+int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries* q, void* stream)
+{
+    if (!s || !cache || !q)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: null argument");
+    if (int rc = check_cache(*cache, "mk_kv_attention"))
+        return rc;
+    if (q->type != MK_BF16 && q->type != MK_FP16)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: type %d is neither MK_BF16 nor MK_FP16", q->type);
+    if (cache->dim != 64u && cache->dim != 128u)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: dim %u is neither 64 nor 128", cache->dim);
+    const uint64_t width = (uint64_t)q->n_q_heads * cache->dim;
+    if (q->n_q_heads == 0 || q->n_q_heads % cache->n_heads || q->q_ld < width || q->out_ld < width || ((q->q_ld | q->out_ld) & 7u))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: n_q_heads %u (a multiple of %u), q_ld %llu and out_ld %llu (multiples of 8)", q->n_q_heads,
+                    cache->n_heads, (unsigned long long)q->q_ld, (unsigned long long)q->out_ld);
+    if ((uint64_t)q->n_tokens * (q->n_q_heads / cache->n_heads) > 0x7fffffffu || q->n_seq > mk::kPlanMaxSeq || q->table_cols > 0x7fffffffu ||
+        q->table_ld < q->table_cols)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: n_tokens %u, n_seq %u (at most %u), table_cols %u, table_ld %llu", q->n_tokens, q->n_seq,
+                    mk::kPlanMaxSeq, q->table_cols, (unsigned long long)q->table_ld);
+    if (!std::isfinite(q->scale) || q->window > 0x7fffffffu)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: the scale must be finite, window %u", q->window);
+    if (off16(q->q) || off16(q->out) || off16(q->workspace))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: q, out and workspace start on 16-byte boundaries");
+    if (q->n_seq == 0 || q->n_tokens == 0)
+        return MK_OK;
+    if (!q->q || !q->out || !q->query_start || !q->kv_len || (q->table_cols && !q->block_table))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: q, out, block_table, query_start and kv_len are required");
+    if (!q->workspace || q->workspace_bytes < mk_kv_attention_bytes(cache, q))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: a workspace of %llu bytes is required",
+                    (unsigned long long)mk_kv_attention_bytes(cache, q));
+    DeviceGuard g(s->device);
+    mk::KvAttendArgs a;
+    std::memset(&a, 0, sizeof a);
+    a.c = *cache;
+    a.q = q->q;
+    a.out = q->out;
+    a.q_ld = q->q_ld;
+    a.out_ld = q->out_ld;
+    a.block_table = q->block_table;
+    a.table_ld = q->table_ld;
+    a.table_cols = q->table_cols;
+    a.query_start = q->query_start;
+    a.kv_len = q->kv_len;
+    a.parts = static_cast<float*>(q->workspace);
+    uint32_t bits = 0;
+    while ((1ull << bits) < cache->page_size)
+        ++bits;
+    a.page_shift = 31u + bits;
+    a.page_inverse = ((1ull << a.page_shift) + cache->page_size - 1u) / cache->page_size;
+    a.n_seq = q->n_seq;
+    a.n_tokens = q->n_tokens;
+    a.max_new = q->max_new && q->max_new < q->n_tokens ? q->max_new : q->n_tokens;
+    a.group = q->n_q_heads / cache->n_heads;
+    a.window = q->window;
+    a.scale_log2 = (float)(q->scale * 1.4426950408889634);
+    MK_CUDA(mk::launch_kv_attend(a, q->type, (cudaStream_t)stream));
+    return MK_OK;
+}
+
 uint32_t mk_vp_record_bytes(uint32_t k)
 {
     return mk::vp_record_bytes(k);

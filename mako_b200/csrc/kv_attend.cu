@@ -1,0 +1,606 @@
+// Attention of few rows over a paged 8-bit cache (mk_kv_attention in include/mako_b200.h): a decode step, a speculative round. Every
+// key and value is read once for all query heads that share it, which is what bounds it.
+//
+// A unit has 16 rows (or 32): the MMA's M. A warp takes every fourth block of its CTA's keys, 4 KB of keys and values, which it copies into a ring
+// of its own in shared memory, so that warps wait for nobody until their segment ends. Codes become fp16 (exactly) on the way from shared
+// memory into registers, in the order in which the tensor core wants them: of a block's keys a lane reads 16 of a token's columns,
+// four steps of the contraction; of its values the four tokens whose weights it holds, which byte permutations put side by
+// side. Queries are fp16 too, each row times the power of two that brings its largest to about 2^12: bf16 loses nothing by it.
+// Scales of keys go into the scores, scales of values into the weights: 2^7 v_j / v p_j is what fp16 holds, v being the largest scale
+// so far, so that a weight's rounding is 2^-11 of it down to 2^-21 of the largest; sums are in fp32.
+#include "kv_cache.cuh"
+#include "kv_work.cuh"
+#include "ptx.cuh"
+
+#include <cuda_bf16.h>
+
+namespace mk {
+namespace {
+
+constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
+constexpr uint32_t kStages = 4;
+constexpr uint32_t kStageBytes = 4096 + 256; // keys and values, two scales a token
+constexpr uint32_t kRingBytes = kStages * kStageBytes;
+constexpr float kWeightUnit = 128.0f;
+
+template <uint32_t D>
+constexpr uint32_t kBlockTokens = 2048 / D;
+
+__device__ __forceinline__ void copy16(void* to, const void* from, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from, bool there)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 4u : 0u) : "memory");
+}
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <uint32_t N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pair_of(float x, float y)
+{
+    const __half2 r = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Where the 16 bytes `chunk` of a token's keys, and of its values, lie in a block: such that the lanes that read at the same time
+// (keys: two tokens' four chunks; values: every second token's same chunk) are in different banks.
+template <uint32_t D>
+__device__ __forceinline__ uint32_t key_at(uint32_t token, uint32_t chunk)
+{
+    return D == 128 ? token * 128u + ((chunk ^ ((token & 1u) << 2)) << 4) : token * 64u + (chunk << 4);
+}
+template <uint32_t D>
+__device__ __forceinline__ uint32_t value_at(uint32_t token, uint32_t chunk)
+{
+    return D == 128 ? token * 128u + ((chunk ^ (token & 7u)) << 4)
+                    : (token >> 1) * 128u + (((((token & 1u) << 2) + chunk) ^ ((token & 6u))) << 4);
+}
+
+template <uint32_t D, uint32_t MT>
+struct Shared {
+    uint64_t find[40];
+    float factor[16 * MT];               // of a row's scores
+    int32_t lo[16 * MT], hi[16 * MT];    // the keys that a row sees: [lo, hi)
+    float m[kWarps][16 * MT], l[kWarps][16 * MT];
+    uint32_t valid[kWarps][kStages];
+    uint4 q[MT * (D / 16) * 32];         // queries in the order of the MMA's registers
+};
+
+template <typename T>
+__device__ __forceinline__ float2 two(uint32_t w)
+{
+    if constexpr (std::is_same<T, __half>::value)
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// The unit's queries: a thread has 16 columns of a row.
+template <typename T, uint32_t D, uint32_t MT>
+__device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSeq& seq, const KvUnit& u)
+{
+    constexpr uint32_t chunks = D / 16;
+    for (uint32_t i = threadIdx.x; i < MT * 16u * chunks; i += kThreads) { // (whole warps: chunks divides 32)
+        const uint32_t r = i / chunks, chunk = i % chunks, row = u.row0 + r;
+        const bool real = r < u.rows;
+        uint32_t w[8] = {};
+        if (real) {
+            const uint64_t token = seq.first + row / a.group;
+            const T* p = static_cast<const T*>(a.q) + token * a.q_ld + (uint64_t)(u.head * a.group + row % a.group) * D + chunk * 16u;
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(p)), y = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+        }
+        float most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float2 x = two<T>(w[k]);
+            most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
+        }
+#pragma unroll
+        for (uint32_t d = 1; d < chunks; d <<= 1)
+            most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+        // a power of two; 1 where a row is nothing or infinite
+        const int e = (int)(__float_as_uint(most) >> 23) - 127;
+        const int up = most > 0.0f && e < 128 ? max(-100, min(100, 12 - e)) : 0;
+        const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+        uint32_t* to = reinterpret_cast<uint32_t*>(s.q) + ((r / 16u * (D / 16u) + chunk / 4u * 4u) * 32u + (r & 7u) * 4u + (chunk & 3u)) * 4u + (r >> 3 & 1u);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) { // a step of the contraction each
+            const float2 x = two<T>(w[2 * k]), y = two<T>(w[2 * k + 1]);
+            to[k * 128u] = pair_of(x.x * by, x.y * by);
+            to[k * 128u + 2u] = pair_of(y.x * by, y.y * by);
+        }
+        if (chunk == 0) {
+            const int64_t at = (int64_t)seq.len - seq.n + row / a.group; // its position
+            s.factor[r] = a.scale_log2 / by;
+            s.hi[r] = real && at >= 0 ? (int32_t)(at + 1 < seq.len ? at + 1 : seq.len) : 0;
+            s.lo[r] = a.window && at + 1 > (int64_t)a.window ? (int32_t)(at + 1 - a.window) : 0;
+        }
+    }
+}
+
+// A warp's copies of blocks of keys and values.
+template <uint32_t D>
+struct Copier {
+    static constexpr uint32_t tokens = kBlockTokens<D>, row_chunks = D / 16, rows_each = 32 / row_chunks;
+    const KvAttendArgs* a;
+    unsigned char* ring;
+    uint32_t* valid;              // a bit for each token of a stage's block: it is there
+    const int32_t* table;
+    uint32_t len, head;
+    int32_t page; // of this lane's token of the block that is next
+
+    __device__ __forceinline__ void look_up(uint32_t block)
+    {
+        const uint32_t t = block * tokens + (threadIdx.x & 31u);
+        page = (threadIdx.x & 31u) < tokens && t < len ? __ldg(table + kv_page_of(*a, t)) : -1;
+    }
+    __device__ __forceinline__ void issue(uint32_t block, uint32_t stage)
+    {
+        const uint32_t lane = threadIdx.x & 31u, t = block * tokens + lane;
+        unsigned char* to = ring + stage * kStageBytes;
+        const bool there = (uint32_t)page < a->c.n_pages;
+        const uint64_t p = there ? (uint64_t)(uint32_t)page : 0ull;
+        const uint32_t place = there ? t - kv_page_of(*a, t) * a->c.page_size : 0u;
+        const uint64_t off = p * a->c.page_stride + (uint64_t)head * a->c.head_stride + (uint64_t)place * a->c.token_stride;
+        const uint32_t mask = __ballot_sync(~0u, there);
+        float* scales = reinterpret_cast<float*>(to + 4096);
+        if (lane < tokens) {
+            const uint64_t at = p * a->c.n_heads + head;
+            copy4(scales + lane, a->c.k_scale + at, there);
+            copy4(scales + tokens + lane, a->c.v_scale + at, there);
+        }
+        if (lane == 0)
+            valid[stage] = mask;
+        const uint32_t chunk = lane % row_chunks;
+#pragma unroll
+        for (uint32_t i = 0; i < tokens / rows_each; ++i) {
+            const uint32_t r = i * rows_each + lane / row_chunks;
+            const uint64_t from = __shfl_sync(~0u, off, r) + chunk * 16u;
+            const bool ok = (mask >> r) & 1u;
+            copy16(to + key_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.k) + from, ok);
+            copy16(to + 2048 + value_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.v) + from, ok);
+        }
+    }
+};
+
+// What a warp has of a unit: rows g and g + 8 of each tile (g: its lane / 4) and, of them, 2 * D / 8 columns.
+template <uint32_t D, uint32_t MT>
+struct Running {
+    float m[MT][2], l[MT][2], o[MT][D / 8][4];
+    float unit; // the largest scale of values so far
+};
+
+// Is one of four codes NaN? And the codes without those.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
+template <uint32_t D, uint32_t MT>
+__device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>& s, const unsigned char* stage, uint32_t valid, uint32_t block, bool all_see)
+{
+    constexpr uint32_t tokens = kBlockTokens<D>, NT = tokens / 8, words = D / 32;
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, c = lane & 3u;
+    const float* scales = reinterpret_cast<const float*>(stage + 4096);
+    float t[MT][NT][4] = {};
+#pragma unroll
+    for (uint32_t h = 0; h < D / 64; ++h) {
+        uint4 w[NT];
+#pragma unroll
+        for (uint32_t n = 0; n < NT; ++n)
+            w[n] = *reinterpret_cast<const uint4*>(stage + key_at<D>(n * 8u + g, c + 4u * h));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            uint4 q[MT];
+#pragma unroll
+            for (uint32_t mt = 0; mt < MT; ++mt)
+                q[mt] = s.q[(mt * (D / 16u) + h * 4u + i) * 32u + lane];
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n) {
+                const uint32_t y = i == 0 ? w[n].x : i == 1 ? w[n].y : i == 2 ? w[n].z : w[n].w;
+                const uint32_t b0 = halves_of(y & 0xffffu), b1 = halves_of(y >> 16);
+#pragma unroll
+                for (uint32_t mt = 0; mt < MT; ++mt)
+                    mma16(t[mt][n], q[mt], b0, b1);
+            }
+        }
+    }
+    float2 vs[NT];
+    float unit = x.unit;
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n) {
+        const float2 ks = *reinterpret_cast<const float2*>(scales + n * 8u + 2u * c);
+        vs[n] = *reinterpret_cast<const float2*>(scales + tokens + n * 8u + 2u * c);
+        unit = fmaxf(unit, fmaxf(vs[n].x, vs[n].y));
+#pragma unroll
+        for (uint32_t mt = 0; mt < MT; ++mt) {
+            const float f0 = s.factor[mt * 16u + g], f1 = s.factor[mt * 16u + g + 8u];
+            t[mt][n][0] *= ks.x * f0;
+            t[mt][n][1] *= ks.y * f0;
+            t[mt][n][2] *= ks.x * f1;
+            t[mt][n][3] *= ks.y * f1;
+        }
+    }
+    unit = fmaxf(unit, __shfl_xor_sync(~0u, unit, 1));
+    unit = fmaxf(unit, __shfl_xor_sync(~0u, unit, 2));
+    auto sees = [&](uint32_t mt, uint32_t n, uint32_t e) {
+        const uint32_t j = n * 8u + 2u * c + (e & 1u), r = mt * 16u + g + (e >> 1) * 8u;
+        const int32_t key = (int32_t)(block * tokens + j);
+        return ((valid >> j) & 1u) && key >= s.lo[r] && key < s.hi[r];
+    };
+    if (!all_see) {
+#pragma unroll
+        for (uint32_t mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (!sees(mt, n, e))
+                        t[mt][n][e] = -INFINITY;
+    }
+    const float value_by = unit > 0.0f ? kWeightUnit / unit : 0.0f;
+    const float older = x.unit == unit ? 1.0f : x.unit / unit;
+    x.unit = unit;
+    uint4 p[MT][NT / 2];
+    bool changed = older != 1.0f;
+    float by[MT][2];
+#pragma unroll
+    for (uint32_t mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (uint32_t r = 0; r < 2; ++r) {
+            float m = x.m[mt][r];
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n)
+                m = fmaxf(m, fmaxf(t[mt][n][2 * r], t[mt][n][2 * r + 1]));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+            const float from = m == -INFINITY ? 0.0f : m;
+            by[mt][r] = ex2_approx(x.m[mt][r] - from);
+            changed = changed || m != x.m[mt][r];
+            x.m[mt][r] = m;
+            float l = 0.0f;
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n) {
+                const float a = ex2_approx(t[mt][n][2 * r] - from), b = ex2_approx(t[mt][n][2 * r + 1] - from);
+                l += a + b;
+                t[mt][n][2 * r] = a * (vs[n].x * value_by);
+                t[mt][n][2 * r + 1] = b * (vs[n].y * value_by);
+            }
+            x.l[mt][r] = x.l[mt][r] * by[mt][r] + l;
+            by[mt][r] *= older;
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < NT; n += 2)
+            p[mt][n / 2] = make_uint4(pair_of(t[mt][n][0], t[mt][n][1]), pair_of(t[mt][n][2], t[mt][n][3]),
+                                      pair_of(t[mt][n + 1][0], t[mt][n + 1][1]), pair_of(t[mt][n + 1][2], t[mt][n + 1][3]));
+    }
+    if (__any_sync(~0u, changed)) {
+#pragma unroll
+        for (uint32_t mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (uint32_t j = 0; j < D / 8; ++j) {
+                x.o[mt][j][0] *= by[mt][0];
+                x.o[mt][j][1] *= by[mt][0];
+                x.o[mt][j][2] *= by[mt][1];
+                x.o[mt][j][3] *= by[mt][1];
+            }
+    }
+    const unsigned char* values = stage + 2048;
+#pragma unroll
+    for (uint32_t k = 0; k < NT / 2; ++k) {
+        uint32_t w[4][words];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t token = k * 16u + 2u * c + (i & 1u) + (i >> 1) * 8u;
+            if constexpr (D == 128) {
+                const uint4 y = *reinterpret_cast<const uint4*>(values + value_at<D>(token, g));
+                w[i][0] = y.x, w[i][1] = y.y, w[i][2] = y.z, w[i][3] = y.w;
+            } else {
+                const uint2 y = *reinterpret_cast<const uint2*>(values + value_at<D>(token, g >> 1) + (g & 1u) * 8u);
+                w[i][0] = y.x, w[i][1] = y.y;
+            }
+        }
+        if (!all_see) { // a weight of nothing times NaN would be NaN: rows that see such a value are, the others are not to be
+            uint32_t bad = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+                for (uint32_t j = 0; j < words; ++j)
+                    bad |= nan_bytes(w[i][j]) ? 1u << i : 0u;
+            if (__any_sync(~0u, bad)) {
+                bad |= __shfl_xor_sync(~0u, bad, 4);
+                bad |= __shfl_xor_sync(~0u, bad, 8);
+                bad |= __shfl_xor_sync(~0u, bad, 16);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (uint32_t j = 0; j < words; ++j)
+                        w[i][j] &= ~nan_bytes(w[i][j]);
+#pragma unroll
+                    for (uint32_t mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (uint32_t r = 0; r < 2; ++r)
+                            if ((bad >> i & 1u) && sees(mt, 2u * k + (i >> 1), 2u * r + (i & 1u)))
+                                x.l[mt][r] = __int_as_float(0x7fc00000);
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < words; ++j) {
+#pragma unroll
+            for (uint32_t half = 0; half < 2; ++half) {
+                const uint32_t order = half ? 0x7362u : 0x5140u; // two tokens' codes of a column side by side
+                const uint32_t y0 = __byte_perm(w[0][j], w[1][j], order), y1 = __byte_perm(w[2][j], w[3][j], order);
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    const uint32_t b0 = halves_of(e ? y0 >> 16 : y0 & 0xffffu), b1 = halves_of(e ? y1 >> 16 : y1 & 0xffffu);
+#pragma unroll
+                    for (uint32_t mt = 0; mt < MT; ++mt)
+                        mma16(x.o[mt][4u * j + 2u * half + e], p[mt][k], b0, b1);
+                }
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float4& x)
+{
+    uint2 r;
+    if constexpr (std::is_same<T, __half>::value) {
+        r = make_uint2(pair_of(x.x, x.y), pair_of(x.z, x.w));
+    } else {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y), z = __floats2bfloat162_rn(x.z, x.w);
+        r = make_uint2(*reinterpret_cast<const uint32_t*>(&y), *reinterpret_cast<const uint32_t*>(&z));
+    }
+    *reinterpret_cast<uint2*>(p) = r;
+}
+
+// A row's place in the output.
+template <typename T, uint32_t D>
+__device__ __forceinline__ T* out_row(const KvAttendArgs& a, const KvSeq& seq, const KvUnit& u, uint32_t r)
+{
+    const uint32_t row = u.row0 + r;
+    return static_cast<T*>(a.out) + (seq.first + row / a.group) * a.out_ld + (uint64_t)(u.head * a.group + row % a.group) * D;
+}
+
+__device__ __forceinline__ float part_factor(float m, float most) { return m == -INFINITY ? 0.0f : ex2_approx(m - most); }
+__device__ __forceinline__ void add4(float4& x, const float4& y, float by)
+{
+    x.x += y.x * by;
+    x.y += y.y * by;
+    x.z += y.z * by;
+    x.w += y.w * by;
+}
+__device__ __forceinline__ float4 over(const float4& x, float l) // a row that saw nothing is zeros
+{
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    return make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
+}
+
+template <uint32_t D, uint32_t MT>
+constexpr uint32_t kPartFloats = MT * 16u * (D + 2u); // outputs, maxima, sums
+
+template <typename T, uint32_t D, uint32_t MT>
+__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(const KvAttendArgs a)
+{
+    extern __shared__ __align__(128) unsigned char raw[]; // the warps' rings; behind a segment, what they have of it
+    __shared__ Shared<D, MT> s;
+    constexpr uint32_t tile = 16u * MT, each = kBlockTokens<D>, row_floats = D + 4;
+    const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid & 31u, g = lane >> 2, c = lane & 3u;
+    griddep_launch_dependents();
+    griddep_wait();
+    uint64_t at, end, total;
+    uint32_t ctas;
+    const KvAt found = kv_find<kThreads>(a, tile, each, gridDim.x, a.blocks_least, s.find, blockIdx.x, at, end, total, ctas);
+    if (blockIdx.x >= ctas)
+        return;
+    const uint64_t begin = at;
+    uint64_t off = found.off;
+    Copier<D> copier;
+    copier.a = &a;
+    copier.ring = raw + warp * kRingBytes;
+    copier.valid = s.valid[warp];
+    for (uint32_t sq = found.seq; at < end && sq < a.n_seq; ++sq, off = 0) {
+        const KvSeq seq = kv_seq(a, sq);
+        const uint32_t per_head = kv_seq_blocks(a, seq, tile, each);
+        copier.table = a.block_table + (uint64_t)sq * a.table_ld;
+        copier.len = seq.len;
+        while (at < end && off < (uint64_t)per_head * a.c.n_heads) {
+            const KvUnit u = kv_unit(a, seq, per_head, off, tile, each);
+            const uint32_t from = u.blocks.from + u.skip, left = u.blocks.to - from;
+            const uint32_t to = end - at < left ? from + (uint32_t)(end - at) : u.blocks.to;
+            copier.head = u.head;
+            uint32_t next = from + warp;
+            copier.look_up(next);
+#pragma unroll
+            for (uint32_t i = 0; i + 1 < kStages; ++i, next += kWarps) {
+                if (next < to) {
+                    copier.issue(next, i);
+                    copier.look_up(next + kWarps);
+                }
+                copies_close();
+            }
+            load_queries<T, D, MT>(a, s, seq, u);
+            __syncthreads();
+            const uint32_t see_from = (uint32_t)s.lo[u.rows - 1u], see_to = (uint32_t)s.hi[0];
+            Running<D, MT> x;
+            x.unit = 0.0f;
+#pragma unroll
+            for (uint32_t mt = 0; mt < MT; ++mt) {
+                x.m[mt][0] = x.m[mt][1] = -INFINITY;
+                x.l[mt][0] = x.l[mt][1] = 0.0f;
+#pragma unroll
+                for (uint32_t j = 0; j < D / 8; ++j)
+                    x.o[mt][j][0] = x.o[mt][j][1] = x.o[mt][j][2] = x.o[mt][j][3] = 0.0f;
+            }
+            uint32_t stage = 0;
+            for (uint32_t block = from + warp; block < to; block += kWarps, next += kWarps) {
+                if (next < to) {
+                    copier.issue(next, stage == 0 ? kStages - 1u : stage - 1u);
+                    copier.look_up(next + kWarps);
+                }
+                copies_close();
+                copies_wait<kStages - 1>();
+                __syncwarp();
+                const uint32_t valid = s.valid[warp][stage];
+                const bool all_see = valid == (each == 32u ? ~0u : (1u << each) - 1u) && block * each >= see_from && (block + 1u) * each <= see_to;
+                add_block<D, MT>(x, s, copier.ring + stage * kStageBytes, valid, block, all_see);
+                __syncwarp();
+                stage = stage + 1u == kStages ? 0u : stage + 1u;
+            }
+            copies_wait<0>();
+            __syncthreads();
+            float* mine = reinterpret_cast<float*>(raw + warp * kRingBytes);
+#pragma unroll
+            for (uint32_t mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (uint32_t r = 0; r < 2; ++r) {
+                    float l = x.l[mt][r];
+                    l += __shfl_xor_sync(~0u, l, 1);
+                    l += __shfl_xor_sync(~0u, l, 2);
+                    const uint32_t row = mt * 16u + r * 8u + g;
+                    if (c == 0) {
+                        s.m[warp][row] = x.m[mt][r];
+                        s.l[warp][row] = l;
+                    }
+                    const float by = x.unit / kWeightUnit;
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e)
+#pragma unroll
+                        for (uint32_t j = 0; j < D / 8; j += 4)
+                            *reinterpret_cast<float4*>(mine + row * row_floats + (2u * c + e) * (D / 8) + j) =
+                                make_float4(x.o[mt][j][2 * r + e] * by, x.o[mt][j + 1][2 * r + e] * by, x.o[mt][j + 2][2 * r + e] * by,
+                                            x.o[mt][j + 3][2 * r + e] * by);
+                }
+            __syncthreads();
+            const bool whole = u.skip == 0 && to == u.blocks.to;
+            float* part = a.parts + (uint64_t)(2u * blockIdx.x + (at != begin)) * kPartFloats<D, MT>;
+            for (uint32_t i = tid; i < u.rows * (D / 4); i += kThreads) {
+                const uint32_t r = i / (D / 4), d = i % (D / 4) * 4u;
+                float most = s.m[0][r];
+#pragma unroll
+                for (uint32_t w = 1; w < kWarps; ++w)
+                    most = fmaxf(most, s.m[w][r]);
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float l = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) {
+                    const float f = part_factor(s.m[w][r], most);
+                    l += s.l[w][r] * f;
+                    add4(o, *reinterpret_cast<const float4*>(raw + w * kRingBytes + (r * row_floats + d) * 4u), f);
+                }
+                if (whole) {
+                    store4(out_row<T, D>(a, seq, u, r) + d, over(o, l));
+                } else {
+                    *reinterpret_cast<float4*>(part + r * D + d) = o;
+                    if (d == 0) {
+                        part[tile * D + r] = most;
+                        part[tile * (D + 1u) + r] = l;
+                    }
+                }
+            }
+            __syncthreads(); // before the next segment's copies, queries and limits
+            at += to - from;
+            off += to - from;
+        }
+    }
+}
+
+// Puts the units together that a cut goes through, a CTA for each cut: the first one inside a unit does it.
+template <typename T, uint32_t D, uint32_t Tile, uint32_t Each>
+__global__ void __launch_bounds__(kThreads) kv_join_kernel(const KvAttendArgs a, const uint32_t ctas_most)
+{
+    __shared__ uint64_t scratch[40];
+    griddep_wait();
+    uint64_t begin, end, total;
+    uint32_t ctas;
+    const uint32_t cta = blockIdx.x + 1u;
+    const KvAt found = kv_find<kThreads>(a, Tile, Each, ctas_most, a.blocks_least, scratch, cta, begin, end, total, ctas);
+    if (cta >= ctas)
+        return;
+    const KvSeq seq = kv_seq(a, found.seq);
+    const KvUnit u = kv_unit(a, seq, kv_seq_blocks(a, seq, Tile, Each), found.off, Tile, Each);
+    const uint64_t start = begin - u.skip, stop = start + (u.blocks.to - u.blocks.from), before = total * (cta - 1ull) / ctas;
+    if (u.skip == 0 || before > start)
+        return;
+    constexpr uint32_t floats = Tile * (D + 2u);
+    const float* first = a.parts + (uint64_t)(2u * (cta - 1u) + (before != start)) * floats;
+    uint32_t last = cta; // behind the last CTA that has a part
+    while (last < ctas && total * last / ctas < stop)
+        ++last;
+    for (uint32_t i = threadIdx.x; i < u.rows * (D / 4); i += kThreads) {
+        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4u;
+        float most = first[Tile * D + r];
+        for (uint32_t p = cta; p < last; ++p)
+            most = fmaxf(most, a.parts[(uint64_t)2u * p * floats + Tile * D + r]);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+        const float* x = first;
+        for (uint32_t p = cta;; ++p) {
+            const float f = part_factor(x[Tile * D + r], most);
+            l += x[Tile * (D + 1u) + r] * f;
+            add4(o, *reinterpret_cast<const float4*>(x + r * D + d), f);
+            if (p == last)
+                break;
+            x = a.parts + (uint64_t)2u * p * floats;
+        }
+        store4(out_row<T, D>(a, seq, u, r) + d, over(o, l));
+    }
+}
+
+constexpr uint32_t rows_ctas(uint32_t mt) { return 148u * (mt == 1 ? 3u : 2u); }
+
+template <typename T, uint32_t D, uint32_t MT>
+cudaError_t launch_rows(const KvAttendArgs& a, cudaStream_t stream)
+{
+    constexpr uint32_t smem = kWarps * kRingBytes, grid = rows_ctas(MT);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = set_once(done, kv_rows_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess)
+        return e;
+    kv_rows_kernel<T, D, MT><<<grid, kThreads, smem, stream>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess)
+        return e;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid - 1u);
+    c.blockDim = dim3(kThreads);
+    c.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = attr;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kv_join_kernel<T, D, 16u * MT, kBlockTokens<D>>, a, grid);
+}
+
+template <typename T, uint32_t D>
+cudaError_t launch(const KvAttendArgs& args, cudaStream_t stream)
+{
+    KvAttendArgs a = args;
+    a.rows_from = 1;
+    a.rows_to = 0xffffffffu;
+    a.blocks_least = 8;
+    return (uint64_t)a.max_new * a.group <= 16u ? launch_rows<T, D, 1>(a, stream) : launch_rows<T, D, 2>(a, stream);
+}
+
+} // namespace
+
+uint64_t kv_attend_bytes(uint32_t dim) { return (uint64_t)rows_ctas(2) * 2u * 32u * (dim + 2u) * 4u; }
+
+cudaError_t launch_kv_attend(const KvAttendArgs& a, int type, cudaStream_t stream)
+{
+    if (type == MK_BF16)
+        return a.c.dim == 128u ? launch<__nv_bfloat16, 128>(a, stream) : launch<__nv_bfloat16, 64>(a, stream);
+    return a.c.dim == 128u ? launch<__half, 128>(a, stream) : launch<__half, 64>(a, stream);
+}
+
+} // namespace mk

@@ -1,5 +1,6 @@
 // Host-visible declarations of the operators of a serving round around the sampler (internal to the library; the public
-// surface is include/mako_b200.h): the head with adapters, the verification of drafts against distributions, the page plan.
+// surface is include/mako_b200.h): the head with adapters, the verification of drafts against distributions, the page plan, the
+// cache behind it, the log-probabilities of tokens.
 #pragma once
 #include <atomic>
 #include <cstdint>
@@ -73,5 +74,48 @@ struct KvPlanArgs {
     uint32_t n_seq;
 };
 cudaError_t launch_kv_plan(const KvPlanArgs& a, cudaStream_t stream);
+
+constexpr uint32_t kLogprobMaxTop = 64;
+struct LogprobOut {
+    float *logprob, *entropy;
+    int32_t* top_ids;
+    float* top_logprob;
+    uint32_t* flags;
+};
+cudaError_t launch_token_logprobs(const mk_logprob_rows& r, const LogprobOut& o, cudaStream_t stream);
+
+struct KvAppendArgs {
+    mk_kv_cache c;
+    const void *q, *k, *v;
+    void* q_out;
+    uint64_t q_ld, k_ld, v_ld, q_out_ld;
+    const int32_t* positions;
+    const int64_t* slots;
+    uint32_t n_tokens, group; // query heads of a key head; 0: no queries
+    const float* inv_freq;
+    uint32_t rotary;          // columns that turn, or 0
+    bool interleaved;
+    float rotary_scale;
+    uint32_t tokens_each;     // of a CTA; the launch sets it
+};
+cudaError_t launch_kv_append(const KvAppendArgs& a, int type, cudaStream_t stream);
+
+struct KvAttendArgs {
+    mk_kv_cache c;
+    const void* q;
+    void* out;
+    uint64_t q_ld, out_ld;
+    const int32_t* block_table;
+    uint64_t table_ld;
+    const int32_t *query_start, *kv_len;
+    float* parts;
+    uint64_t page_inverse;
+    uint32_t page_shift, table_cols, n_seq, n_tokens, max_new, group, window;
+    float scale_log2;         // of a score, for exponents of two
+    // which sequences a launch takes, by their rows (tokens of the pass times group), and the least blocks of a CTA; the launch sets them
+    uint32_t rows_from, rows_to, blocks_least;
+};
+uint64_t kv_attend_bytes(uint32_t dim); // of parts
+cudaError_t launch_kv_attend(const KvAttendArgs& a, int type, cudaStream_t stream);
 
 } // namespace mk

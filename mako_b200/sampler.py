@@ -8,6 +8,7 @@ for device memory and streams only.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -15,7 +16,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import HeadC, KvPagesC, KvPlanC, RowsC, SampleOutC, SpecRowsC, check, lib
+from ._lib import (HeadC, KvCacheC, KvPagesC, KvPlanC, KvQueriesC, KvRowsC, LogprobRowsC, RotaryC, RowsC, SampleOutC, SpecRowsC, check,
+                   lib)
 from .params import SamplingParams
 
 
@@ -132,6 +134,52 @@ class KvPlan:
         i32 = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
         return cls(i32(n_seq + 1), i32(n_seq), i32(max_tokens), torch.empty(max_tokens, dtype=torch.int64, device=device),
                    i32(max_tokens), i32(n_seq))
+
+
+@dataclass
+class TokenLogprobs:
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+    flags: torch.Tensor
+
+
+@dataclass
+class KvCache:
+    """A paged cache of keys and values in 8 bits (mk_kv_cache): k and v [P, H, page, D] float8_e4m3fn or uint8 of one shape and
+    one set of strides, columns side by side (a [P, page, H, D] tensor is taken as its transpose(1, 2)); k_scale and v_scale [P, H]
+    float32. What stands in page p, head h is k[p, h] times k_scale[p, h]."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, n_pages: int, n_heads: int, page_size: int, dim: int, device="cuda") -> "KvCache":
+        codes = lambda: torch.zeros((n_pages, n_heads, page_size, dim), dtype=torch.float8_e4m3fn, device=device)  # noqa: E731
+        scales = lambda: torch.zeros((n_pages, n_heads), dtype=torch.float32, device=device)  # noqa: E731
+        return cls(codes(), codes(), scales(), scales())
+
+    def _c(self, on: int) -> KvCacheC:
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        (pages, heads, page, dim), stride = k.shape, k.stride()
+        assert k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == on, f"a cache on {k.device}, the handle is on {on}"
+        assert k.dtype == v.dtype and k.dtype in (torch.float8_e4m3fn, torch.uint8) and ks.dtype == vs.dtype == torch.float32
+        assert v.shape == k.shape and v.stride() == stride and stride[3] == 1
+        assert ks.shape == vs.shape == (pages, heads) and ks.is_contiguous() and vs.is_contiguous()
+        # (of a single page, head or place a tensor may say any stride)
+        token = stride[2] if page > 1 else dim
+        return KvCacheC(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), stride[0] if pages > 1 else 0, stride[1] if heads > 1 else 0,
+                        token, pages, heads, page, dim)
+
+
+def _heads_ld(t: torch.Tensor) -> int:
+    """From one token to the next, of a [T, H, D] tensor whose heads lie side by side."""
+    n, heads, dim = t.shape
+    ld, head, unit = t.stride()
+    assert unit == 1 and (head == dim or heads == 1)
+    return ld if n > 1 else heads * dim
 
 
 _TYPE = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
@@ -464,6 +512,90 @@ class BatchSampler:
             o = KvPlanC(start.data_ptr(), kv_len.data_ptr(), pos.data_ptr(), slots.data_ptr(), seq.data_ptr(), flags.data_ptr(), t)
         check(lib.mk_kv_plan_step(self._h, C.byref(p), cache_len.data_ptr(), _ptr(n_new), n_seq, C.byref(o),
                                   _stream_ptr(self.device)))
+        return out
+
+    def token_logprobs(self, logits, tokens, temperature=1.0, *, top: int = 0, mask=None) -> TokenLogprobs:
+        """Log-probabilities of given tokens (mk_token_logprobs): logits [T, V] float32, bf16 or fp16, tokens [T] or [T, N] int32 (a
+        negative one: none, 0), temperature a number or [T] float32, mask [T, words]. Returns logprob, of tokens' shape, entropy
+        [T], the `top` likeliest tokens of each row, the likeliest first, in top_ids [T, top] with top_logprobs [T, top], and flags [T]."""
+        rows, v = logits.shape
+        self._here(logits, tokens)
+        assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.dim() in (1, 2) and tokens.shape[0] == rows
+        given = tokens.shape[1] if tokens.dim() == 2 else 1
+        t_ptr = t_all = m_ptr = m_ld = 0
+        if isinstance(temperature, torch.Tensor):
+            self._here(temperature)
+            assert temperature.dtype == torch.float32 and temperature.shape == (rows,) and temperature.is_contiguous()
+            t_ptr = temperature.data_ptr()
+        else:
+            t_all = temperature
+        if mask is not None:
+            self._here(mask)
+            assert mask.dtype in (torch.int32, torch.uint32) and mask.shape[0] == rows
+            m_ptr, m_ld = mask.data_ptr(), _row_stride(mask)
+            assert 32 * mask.shape[1] >= v, "a mask narrower than its rows"
+        r = LogprobRowsC(logits.data_ptr(), _row_stride(logits), _TYPE[logits.dtype], rows, v, tokens.data_ptr(), given, top, t_ptr or None,
+                         t_all, m_ptr or None, m_ld)
+        f32 = lambda *n: torch.empty(n, dtype=torch.float32, device=self.device)  # noqa: E731
+        i32 = lambda *n: torch.empty(n, dtype=torch.int32, device=self.device)  # noqa: E731
+        out = TokenLogprobs(f32(*tokens.shape), f32(rows), i32(rows, top), f32(rows, top), i32(rows))
+        check(lib.mk_token_logprobs(self._h, C.byref(r), out.logprob.data_ptr(), out.entropy.data_ptr(), out.top_ids.data_ptr(),
+                                    out.top_logprobs.data_ptr(), out.flags.data_ptr(), _stream_ptr(self.device)))
+        return out
+
+    def kv_append(self, cache: KvCache, k, v, slots, *, q=None, q_out=None, positions=None, inv_freq=None, interleaved: bool = False,
+                  rotary_scale: float = 1.0):
+        """A pass's keys and values into the cache (mk_kv_append): k and v [T, H, D] bf16 or fp16 at slots [T] int64 (negative:
+        padding, left out), as kv_plan gives them. With inv_freq [R / 2] float32 the first R columns of k and of q [T, Hq, D] turn by
+        positions [T] int32 times inv_freq, columns i and i + R / 2 or, interleaved, 2i and 2i + 1, and are scaled by rotary_scale.
+        Returns q_out (rotated queries; q itself may be given), or None without q. k, v and q may be slices of one projection."""
+        tokens, heads, dim = k.shape
+        self._here(k, v, slots)
+        assert k.dtype in (torch.bfloat16, torch.float16) and v.dtype == k.dtype and v.shape == k.shape
+        assert slots.dtype == torch.int64 and slots.shape == (tokens,) and slots.is_contiguous()
+        c = cache._c(self._index)
+        assert (heads, dim) == (c.n_heads, c.dim)
+        r = KvRowsC(k.data_ptr(), v.data_ptr(), _heads_ld(k), _heads_ld(v), None, None, 0, 0, 0, _TYPE[k.dtype], tokens, None, slots.data_ptr())
+        if q is not None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+            self._here(q, q_out)
+            assert q.dtype == q_out.dtype == k.dtype and q.shape == q_out.shape and q.shape[0] == tokens and q.shape[2] == dim
+            r.q, r.q_out, r.q_ld, r.q_out_ld, r.n_q_heads = q.data_ptr(), q_out.data_ptr(), _heads_ld(q), _heads_ld(q_out), q.shape[1]
+        else:
+            assert q_out is None
+        turn = None
+        if inv_freq is not None:
+            self._here(inv_freq, positions)
+            assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.dim() == 1
+            assert positions.dtype == torch.int32 and positions.shape == (tokens,) and positions.is_contiguous()
+            r.positions = positions.data_ptr()
+            turn = C.byref(RotaryC(inv_freq.data_ptr(), 2 * inv_freq.numel(), int(interleaved), rotary_scale))
+        check(lib.mk_kv_append(self._h, C.byref(c), C.byref(r), turn, _stream_ptr(self.device)))
+        return q_out
+
+    def kv_attention(self, q, cache: KvCache, block_table, query_start, kv_len, *, max_new: int = 0, scale=None, window: int = 0,
+                     out=None) -> torch.Tensor:
+        """A pass's queries over the cache (mk_kv_attention): q [T, Hq, D] bf16 or fp16, block_table [S, columns], query_start
+        [S + 1] and kv_len [S] int32 as kv_plan gives them; max_new: the most tokens that a sequence has in this pass, where the
+        caller knows (it chooses kernels, nothing else); scale of a score, 1 / sqrt(D) by default; window: how many keys a token sees,
+        its own among them (0: all). Returns [T, Hq, D] (`out` where given); rows that are no sequence's are left as they are."""
+        (tokens, q_heads, dim), (n_seq, cols) = q.shape, block_table.shape
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        self._here(q, out, block_table, query_start, kv_len)
+        assert q.dtype in (torch.bfloat16, torch.float16) and out.dtype == q.dtype and out.shape == q.shape
+        assert block_table.dtype == query_start.dtype == kv_len.dtype == torch.int32
+        assert query_start.is_contiguous() and kv_len.is_contiguous() and query_start.numel() == n_seq + 1 and kv_len.numel() == n_seq
+        c = cache._c(self._index)
+        assert c.dim == dim
+        r = KvQueriesC(q.data_ptr(), out.data_ptr(), _heads_ld(q), _heads_ld(out), q_heads, _TYPE[q.dtype], tokens, block_table.data_ptr(),
+                       _row_stride(block_table), cols, query_start.data_ptr(), kv_len.data_ptr(), n_seq, max_new,
+                       1.0 / math.sqrt(dim) if scale is None else scale, window)
+        r.workspace_bytes = lib.mk_kv_attention_bytes(C.byref(c), C.byref(r))
+        # (of the caching allocator: a call's own, on its stream, and in a capture the graph's)
+        workspace = torch.empty(r.workspace_bytes, dtype=torch.uint8, device=self.device)
+        r.workspace = workspace.data_ptr()
+        check(lib.mk_kv_attention(self._h, C.byref(c), C.byref(r), _stream_ptr(self.device)))
         return out
 
     def vp_local(self, shard_logits, params, k: int, records: torch.Tensor, *, id_offset: int, history=None,
