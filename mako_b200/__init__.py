@@ -14,12 +14,15 @@ __all__ = sorted(_SAMPLER | _LIB | {"version", "synth"})
 def __getattr__(name):
     import importlib
     if name in _SAMPLER:
-        return getattr(importlib.import_module(".sampler", __name__), name)
-    if name in _LIB:
-        return getattr(importlib.import_module("._lib", __name__), name)
-    if name in ("synth", "sampler", "build", "_lib"):
-        return importlib.import_module("." + name, __name__)
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+        value = getattr(importlib.import_module(".sampler", __name__), name)
+    elif name in _LIB:
+        value = getattr(importlib.import_module("._lib", __name__), name)
+    elif name in ("synth", "sampler", "build", "_lib"):
+        value = importlib.import_module("." + name, __name__)
+    else:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()[name] = value  # found without this function from now on
+    return value
 
 
 def version() -> str:

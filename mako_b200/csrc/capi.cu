@@ -878,7 +878,10 @@ int mk_kv_append(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_rows* r, c
 
 uint64_t mk_kv_attention_bytes(const mk_kv_cache* cache, const mk_kv_queries* q)
 {
-    return cache && q ? mk::kv_attend_bytes(cache->dim) : 0;
+    if (!cache || !q || cache->n_heads == 0)
+        return 0;
+    const uint64_t most = q->max_new && q->max_new < q->n_tokens ? q->max_new : q->n_tokens;
+    return mk::kv_attend_bytes(cache->dim, most * (q->n_q_heads / cache->n_heads));
 }
 
 int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries* q, void* stream)

@@ -515,48 +515,101 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(cons
 }
 
 // Puts the units together that a cut goes through, a CTA for each cut: the first one inside a unit does it.
+constexpr uint32_t kJoinThreads = 256, kJoinParts = 32;
+
 template <typename T, uint32_t D, uint32_t Tile, uint32_t Each>
-__global__ void __launch_bounds__(kThreads) kv_join_kernel(const KvAttendArgs a, const uint32_t ctas_most)
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArgs a, const uint32_t ctas_most)
 {
     __shared__ uint64_t scratch[40];
+    __shared__ float s_factor[kJoinParts][16], s_by[16];
     griddep_wait();
     uint64_t begin, end, total;
     uint32_t ctas;
-    const uint32_t cta = blockIdx.x + 1u;
-    const KvAt found = kv_find<kThreads>(a, Tile, Each, ctas_most, a.blocks_least, scratch, cta, begin, end, total, ctas);
+    const uint32_t cta = blockIdx.x + 1u, tid = threadIdx.x;
+    const KvAt found = kv_find<kJoinThreads>(a, Tile, Each, ctas_most, a.blocks_least, scratch, cta, begin, end, total, ctas);
     if (cta >= ctas)
         return;
     const KvSeq seq = kv_seq(a, found.seq);
     const KvUnit u = kv_unit(a, seq, kv_seq_blocks(a, seq, Tile, Each), found.off, Tile, Each);
-    const uint64_t start = begin - u.skip, stop = start + (u.blocks.to - u.blocks.from), before = total * (cta - 1ull) / ctas;
+    const uint64_t start = begin - u.skip, stop = start + (u.blocks.to - u.blocks.from), before = kv_cut(total, ctas, cta - 1u);
     if (u.skip == 0 || before > start)
         return;
     constexpr uint32_t floats = Tile * (D + 2u);
-    const float* first = a.parts + (uint64_t)(2u * (cta - 1u) + (before != start)) * floats;
-    uint32_t last = cta; // behind the last CTA that has a part
-    while (last < ctas && total * last / ctas < stop)
-        ++last;
-    for (uint32_t i = threadIdx.x; i < u.rows * (D / 4); i += kThreads) {
-        const uint32_t r = i / (D / 4), d = i % (D / 4) * 4u;
-        float most = first[Tile * D + r];
-        for (uint32_t p = cta; p < last; ++p)
-            most = fmaxf(most, a.parts[(uint64_t)2u * p * floats + Tile * D + r]);
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
-        const float* x = first;
-        for (uint32_t p = cta;; ++p) {
-            const float f = part_factor(x[Tile * D + r], most);
-            l += x[Tile * (D + 1u) + r] * f;
-            add4(o, *reinterpret_cast<const float4*>(x + r * D + d), f);
-            if (p == last)
-                break;
-            x = a.parts + (uint64_t)2u * p * floats;
+    uint32_t parts = 1; // the first one's, and of those CTAs whose shares begin in the unit
+    while (cta + parts - 1u < ctas && kv_cut(total, ctas, cta + parts - 1u) < stop)
+        ++parts;
+    auto part = [&](uint32_t p) { return a.parts + (uint64_t)(2u * (cta - 1u + p) + (p == 0 && before != start)) * floats; };
+    for (uint32_t r0 = 0; r0 < u.rows; r0 += 16u) { // 16 rows at a time: their maxima, then what each part is worth, then the sums
+        const uint32_t rows = min(16u, u.rows - r0);
+        float4 o[16 * (D / 4) / kJoinThreads];
+#pragma unroll
+        for (uint32_t k = 0; k < 16 * (D / 4) / kJoinThreads; ++k)
+            o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f, most = -INFINITY;
+        // (a row's maximum over all parts first: by the 16 threads that share its row, through shuffles)
+        const uint32_t row = tid / 16u, lane = tid % 16u;
+        if (row < rows)
+            for (uint32_t p = lane; p < parts; p += 16u)
+                most = fmaxf(most, part(p)[Tile * D + r0 + row]);
+        __syncwarp();
+#pragma unroll
+        for (uint32_t d = 8; d; d >>= 1)
+            most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+        for (uint32_t p0 = 0; p0 < parts; p0 += kJoinParts) {
+            const uint32_t some = min(kJoinParts, parts - p0);
+            __syncthreads();
+            if (row < rows)
+                for (uint32_t p = lane; p < some; p += 16u) {
+                    const float* x = part(p0 + p) + r0 + row;
+                    const float f = part_factor(x[Tile * D], most);
+                    s_factor[p][row] = f;
+                    l += x[Tile * (D + 1u)] * f;
+                }
+            __syncthreads();
+#pragma unroll
+            for (uint32_t k = 0; k < 16 * (D / 4) / kJoinThreads; ++k) {
+                const uint32_t i = tid + k * kJoinThreads, r = i / (D / 4), d = i % (D / 4) * 4u;
+                if (r < rows) {
+#pragma unroll 4
+                    for (uint32_t p = 0; p < some; ++p)
+                        add4(o[k], *reinterpret_cast<const float4*>(part(p0 + p) + (r0 + r) * D + d), s_factor[p][r]);
+                }
+            }
         }
-        store4(out_row<T, D>(a, seq, u, r) + d, over(o, l));
+        __syncwarp();
+#pragma unroll
+        for (uint32_t d = 8; d; d >>= 1)
+            l += __shfl_xor_sync(~0u, l, d);
+        if (lane == 0 && row < rows)
+            s_by[row] = l;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < 16 * (D / 4) / kJoinThreads; ++k) {
+            const uint32_t i = tid + k * kJoinThreads, r = i / (D / 4), d = i % (D / 4) * 4u;
+            if (r < rows)
+                store4(out_row<T, D>(a, seq, u, r0 + r) + d, over(o[k], s_by[r]));
+        }
+        __syncthreads();
     }
 }
 
 constexpr uint32_t rows_ctas(uint32_t mt) { return 148u * (mt == 1 ? 3u : 2u); }
+constexpr uint64_t kv_rows_parts(uint32_t dim) { return (uint64_t)rows_ctas(2) * 2u * 32u * (dim + 2u) * 4u; } // bytes
+
+template <typename T, uint32_t D, uint32_t Tile, uint32_t Each>
+cudaError_t launch_join(const KvAttendArgs& a, uint32_t ctas, cudaStream_t stream)
+{
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(ctas - 1u);
+    c.blockDim = dim3(kJoinThreads);
+    c.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = attr;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kv_join_kernel<T, D, Tile, Each>, a, ctas);
+}
 
 template <typename T, uint32_t D, uint32_t MT>
 cudaError_t launch_rows(const KvAttendArgs& a, cudaStream_t stream)
@@ -570,37 +623,48 @@ cudaError_t launch_rows(const KvAttendArgs& a, cudaStream_t stream)
     e = cudaGetLastError();
     if (e != cudaSuccess)
         return e;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(grid - 1u);
-    c.blockDim = dim3(kThreads);
-    c.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = attr;
-    c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kv_join_kernel<T, D, 16u * MT, kBlockTokens<D>>, a, grid);
+    return launch_join<T, D, 16u * MT, kBlockTokens<D>>(a, grid, stream);
 }
 
+// Sequences of up to so many rows go through kv_rows_kernel, in a pass of others too.
+constexpr uint32_t kFewRows = 16, kSomeRows = 32;
+
 template <typename T, uint32_t D>
-cudaError_t launch(const KvAttendArgs& args, cudaStream_t stream)
+cudaError_t launch(const KvAttendArgs& args, int type, cudaStream_t stream)
 {
     KvAttendArgs a = args;
+    const uint64_t most = (uint64_t)a.max_new * a.group;
     a.rows_from = 1;
-    a.rows_to = 0xffffffffu;
+    a.rows_to = 0xffffffffu; // (max_new is what the caller says: where it is too small all the same rows are done)
     a.blocks_least = 8;
-    return (uint64_t)a.max_new * a.group <= 16u ? launch_rows<T, D, 1>(a, stream) : launch_rows<T, D, 2>(a, stream);
+    if (most <= kFewRows)
+        return launch_rows<T, D, 1>(a, stream);
+    if (most <= kSomeRows)
+        return launch_rows<T, D, 2>(a, stream);
+    a.rows_to = kFewRows;
+    cudaError_t e = a.group <= kFewRows ? launch_rows<T, D, 1>(a, stream) : cudaSuccess;
+    if (e != cudaSuccess)
+        return e;
+    a.parts = args.parts + kv_rows_parts(D) / 4u;
+    a.rows_from = kFewRows + 1u;
+    a.rows_to = 0xffffffffu;
+    a.blocks_least = 1;
+    e = launch_kv_prompt(a, type, stream);
+    return e != cudaSuccess ? e : launch_join<T, D, kPromptRows, kPromptBlock>(a, kPromptCtas, stream);
 }
 
 } // namespace
 
-uint64_t kv_attend_bytes(uint32_t dim) { return (uint64_t)rows_ctas(2) * 2u * 32u * (dim + 2u) * 4u; }
+uint64_t kv_attend_bytes(uint32_t dim, uint64_t most_rows)
+{
+    return kv_rows_parts(dim) + (most_rows > kSomeRows ? (uint64_t)kPromptCtas * 2u * kPromptRows * (dim + 2u) * 4u : 0u);
+}
 
 cudaError_t launch_kv_attend(const KvAttendArgs& a, int type, cudaStream_t stream)
 {
     if (type == MK_BF16)
-        return a.c.dim == 128u ? launch<__nv_bfloat16, 128>(a, stream) : launch<__nv_bfloat16, 64>(a, stream);
-    return a.c.dim == 128u ? launch<__half, 128>(a, stream) : launch<__half, 64>(a, stream);
+        return a.c.dim == 128u ? launch<__nv_bfloat16, 128>(a, type, stream) : launch<__nv_bfloat16, 64>(a, type, stream);
+    return a.c.dim == 128u ? launch<__half, 128>(a, type, stream) : launch<__half, 64>(a, type, stream);
 }
 
 } // namespace mk

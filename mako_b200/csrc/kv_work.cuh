@@ -52,6 +52,15 @@ __device__ __forceinline__ uint32_t kv_seq_blocks(const KvAttendArgs& a, const K
     return sum;
 }
 
+// Where share i of n of a whole begins: shares differ by one at most.
+__device__ __forceinline__ uint64_t kv_cut(uint64_t total, uint32_t n, uint32_t i)
+{
+    if (total >> 32) // (a division in 64 bits takes some hundred instructions)
+        return total / n * i + min((uint64_t)i, total % n);
+    const uint32_t each = (uint32_t)total / n, more = (uint32_t)total - each * n;
+    return (uint64_t)each * i + min(i, more);
+}
+
 struct KvAt {
     uint32_t seq;
     uint64_t off;   // blocks into the sequence
@@ -84,10 +93,11 @@ __device__ KvAt kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, uin
             front += scratch[w];
         total += scratch[w];
     }
-    const uint64_t most = (total + blocks_least - 1) / blocks_least;
-    ctas = most < ctas_most ? (uint32_t)most : ctas_most;
-    begin = ctas ? total * cta / ctas : 0;
-    end = ctas ? total * (cta + 1ull) / ctas : 0;
+    ctas = ctas_most;
+    if (total < (uint64_t)blocks_least * ctas_most)
+        ctas = ((uint32_t)total + blocks_least - 1u) / blocks_least;
+    begin = ctas ? kv_cut(total, ctas, cta) : 0;
+    end = ctas ? kv_cut(total, ctas, cta + 1u) : 0;
     uint64_t at = front + run - sum; // of this thread's first sequence
     if (cta < ctas && begin >= at && begin < at + sum)
         for (uint32_t s = s0; s < s1; ++s) {
@@ -115,7 +125,7 @@ struct KvUnit {
 __device__ __forceinline__ KvUnit kv_unit(const KvAttendArgs& a, const KvSeq& q, uint32_t seq_blocks, uint64_t off, uint32_t tile, uint32_t each)
 {
     KvUnit u;
-    u.head = (uint32_t)(off / seq_blocks);
+    u.head = off >> 32 ? (uint32_t)(off / seq_blocks) : (uint32_t)off / seq_blocks;
     u.skip = (uint32_t)(off - (uint64_t)u.head * seq_blocks);
     const uint32_t rows = q.n * a.group;
     for (u.row0 = 0;; u.row0 += tile) {

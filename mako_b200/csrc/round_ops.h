@@ -115,7 +115,9 @@ struct KvAttendArgs {
     // which sequences a launch takes, by their rows (tokens of the pass times group), and the least blocks of a CTA; the launch sets them
     uint32_t rows_from, rows_to, blocks_least;
 };
-uint64_t kv_attend_bytes(uint32_t dim); // of parts
+constexpr uint32_t kPromptCtas = 148, kPromptRows = 256, kPromptBlock = 128; // CTAs; rows of a unit; keys of a block
+uint64_t kv_attend_bytes(uint32_t dim, uint64_t most_rows); // of parts; rows: of a sequence
+cudaError_t launch_kv_prompt(const KvAttendArgs& a, int type, cudaStream_t stream);
 cudaError_t launch_kv_attend(const KvAttendArgs& a, int type, cudaStream_t stream);
 
 } // namespace mk
