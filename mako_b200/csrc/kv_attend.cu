@@ -86,7 +86,7 @@ __device__ __forceinline__ float2 two(uint32_t w)
 
 // The unit's queries: a thread has 16 columns of a row.
 template <typename T, uint32_t D, uint32_t MT>
-__device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSeq& seq, const KvUnit& u)
+__device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSegment& u)
 {
     constexpr uint32_t chunks = D / 16;
     for (uint32_t i = threadIdx.x; i < MT * 16u * chunks; i += kThreads) { // (whole warps: chunks divides 32)
@@ -94,7 +94,7 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSe
         const bool real = r < u.rows;
         uint32_t w[8] = {};
         if (real) {
-            const uint64_t token = seq.first + row / a.group;
+            const uint64_t token = u.seq.first + row / a.group;
             const T* p = static_cast<const T*>(a.q) + token * a.q_ld + (uint64_t)(u.head * a.group + row % a.group) * D + chunk * 16u;
             const uint4 x = __ldg(reinterpret_cast<const uint4*>(p)), y = __ldg(reinterpret_cast<const uint4*>(p) + 1);
             w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
@@ -120,9 +120,9 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSe
             to[k * 128u + 2u] = pair_of(y.x * by, y.y * by);
         }
         if (chunk == 0) {
-            const int64_t at = (int64_t)seq.len - seq.n + row / a.group; // its position
+            const int64_t at = (int64_t)u.seq.len - u.seq.n + row / a.group; // its position
             s.factor[r] = a.scale_log2 / by;
-            s.hi[r] = real && at >= 0 ? (int32_t)(at + 1 < seq.len ? at + 1 : seq.len) : 0;
+            s.hi[r] = real && at >= 0 ? (int32_t)(at + 1 < u.seq.len ? at + 1 : u.seq.len) : 0;
             s.lo[r] = a.window && at + 1 > (int64_t)a.window ? (int32_t)(at + 1 - a.window) : 0;
         }
     }
@@ -365,10 +365,10 @@ __device__ __forceinline__ void store4(T* p, const float4& x)
 
 // A row's place in the output.
 template <typename T, uint32_t D>
-__device__ __forceinline__ T* out_row(const KvAttendArgs& a, const KvSeq& seq, const KvUnit& u, uint32_t r)
+__device__ __forceinline__ T* out_row(const KvAttendArgs& a, const KvSegment& u, uint32_t r)
 {
     const uint32_t row = u.row0 + r;
-    return static_cast<T*>(a.out) + (seq.first + row / a.group) * a.out_ld + (uint64_t)(u.head * a.group + row % a.group) * D;
+    return static_cast<T*>(a.out) + (u.seq.first + row / a.group) * a.out_ld + (uint64_t)(u.head * a.group + row % a.group) * D;
 }
 
 __device__ __forceinline__ float part_factor(float m, float most) { return m == -INFINITY ? 0.0f : ex2_approx(m - most); }
@@ -397,120 +397,107 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(cons
     const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid & 31u, g = lane >> 2, c = lane & 3u;
     griddep_launch_dependents();
     griddep_wait();
-    uint64_t at, end, total;
-    uint32_t ctas;
-    const KvAt found = kv_find<kThreads>(a, tile, each, gridDim.x, a.blocks_least, s.find, blockIdx.x, at, end, total, ctas);
-    if (blockIdx.x >= ctas)
-        return;
-    const uint64_t begin = at;
-    uint64_t off = found.off;
+    KvWalk walk = kv_find<kThreads>(a, tile, each, gridDim.x, s.find, blockIdx.x);
     Copier<D> copier;
     copier.a = &a;
     copier.ring = raw + warp * kRingBytes;
     copier.valid = s.valid[warp];
-    for (uint32_t sq = found.seq; at < end && sq < a.n_seq; ++sq, off = 0) {
-        const KvSeq seq = kv_seq(a, sq);
-        const uint32_t per_head = kv_seq_blocks(a, seq, tile, each);
-        copier.table = a.block_table + (uint64_t)sq * a.table_ld;
-        copier.len = seq.len;
-        while (at < end && off < (uint64_t)per_head * a.c.n_heads) {
-            const KvUnit u = kv_unit(a, seq, per_head, off, tile, each);
-            const uint32_t from = u.blocks.from + u.skip, left = u.blocks.to - from;
-            const uint32_t to = end - at < left ? from + (uint32_t)(end - at) : u.blocks.to;
-            copier.head = u.head;
-            uint32_t next = from + warp;
-            copier.look_up(next);
+    KvSegment u;
+    for (bool first = true; kv_take(a, walk, u, first, tile, each); first = false) {
+        const uint32_t from = u.from, to = u.to;
+        copier.table = a.block_table + (uint64_t)u.sq * a.table_ld;
+        copier.len = u.seq.len;
+        copier.head = u.head;
+        uint32_t next = from + warp;
+        copier.look_up(next);
 #pragma unroll
-            for (uint32_t i = 0; i + 1 < kStages; ++i, next += kWarps) {
-                if (next < to) {
-                    copier.issue(next, i);
-                    copier.look_up(next + kWarps);
-                }
-                copies_close();
+        for (uint32_t i = 0; i + 1 < kStages; ++i, next += kWarps) {
+            if (next < to) {
+                copier.issue(next, i);
+                copier.look_up(next + kWarps);
             }
-            load_queries<T, D, MT>(a, s, seq, u);
-            __syncthreads();
-            const uint32_t see_from = (uint32_t)s.lo[u.rows - 1u], see_to = (uint32_t)s.hi[0];
-            Running<D, MT> x;
-            x.unit = 0.0f;
-#pragma unroll
-            for (uint32_t mt = 0; mt < MT; ++mt) {
-                x.m[mt][0] = x.m[mt][1] = -INFINITY;
-                x.l[mt][0] = x.l[mt][1] = 0.0f;
-#pragma unroll
-                for (uint32_t j = 0; j < D / 8; ++j)
-                    x.o[mt][j][0] = x.o[mt][j][1] = x.o[mt][j][2] = x.o[mt][j][3] = 0.0f;
-            }
-            uint32_t stage = 0;
-            for (uint32_t block = from + warp; block < to; block += kWarps, next += kWarps) {
-                if (next < to) {
-                    copier.issue(next, stage == 0 ? kStages - 1u : stage - 1u);
-                    copier.look_up(next + kWarps);
-                }
-                copies_close();
-                copies_wait<kStages - 1>();
-                __syncwarp();
-                const uint32_t valid = s.valid[warp][stage];
-                const bool all_see = valid == (each == 32u ? ~0u : (1u << each) - 1u) && block * each >= see_from && (block + 1u) * each <= see_to;
-                add_block<D, MT>(x, s, copier.ring + stage * kStageBytes, valid, block, all_see);
-                __syncwarp();
-                stage = stage + 1u == kStages ? 0u : stage + 1u;
-            }
-            copies_wait<0>();
-            __syncthreads();
-            float* mine = reinterpret_cast<float*>(raw + warp * kRingBytes);
-#pragma unroll
-            for (uint32_t mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (uint32_t r = 0; r < 2; ++r) {
-                    float l = x.l[mt][r];
-                    l += __shfl_xor_sync(~0u, l, 1);
-                    l += __shfl_xor_sync(~0u, l, 2);
-                    const uint32_t row = mt * 16u + r * 8u + g;
-                    if (c == 0) {
-                        s.m[warp][row] = x.m[mt][r];
-                        s.l[warp][row] = l;
-                    }
-                    const float by = x.unit / kWeightUnit;
-#pragma unroll
-                    for (uint32_t e = 0; e < 2; ++e)
-#pragma unroll
-                        for (uint32_t j = 0; j < D / 8; j += 4)
-                            *reinterpret_cast<float4*>(mine + row * row_floats + (2u * c + e) * (D / 8) + j) =
-                                make_float4(x.o[mt][j][2 * r + e] * by, x.o[mt][j + 1][2 * r + e] * by, x.o[mt][j + 2][2 * r + e] * by,
-                                            x.o[mt][j + 3][2 * r + e] * by);
-                }
-            __syncthreads();
-            const bool whole = u.skip == 0 && to == u.blocks.to;
-            float* part = a.parts + (uint64_t)(2u * blockIdx.x + (at != begin)) * kPartFloats<D, MT>;
-            for (uint32_t i = tid; i < u.rows * (D / 4); i += kThreads) {
-                const uint32_t r = i / (D / 4), d = i % (D / 4) * 4u;
-                float most = s.m[0][r];
-#pragma unroll
-                for (uint32_t w = 1; w < kWarps; ++w)
-                    most = fmaxf(most, s.m[w][r]);
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float l = 0.0f;
-#pragma unroll
-                for (uint32_t w = 0; w < kWarps; ++w) {
-                    const float f = part_factor(s.m[w][r], most);
-                    l += s.l[w][r] * f;
-                    add4(o, *reinterpret_cast<const float4*>(raw + w * kRingBytes + (r * row_floats + d) * 4u), f);
-                }
-                if (whole) {
-                    store4(out_row<T, D>(a, seq, u, r) + d, over(o, l));
-                } else {
-                    *reinterpret_cast<float4*>(part + r * D + d) = o;
-                    if (d == 0) {
-                        part[tile * D + r] = most;
-                        part[tile * (D + 1u) + r] = l;
-                    }
-                }
-            }
-            __syncthreads(); // before the next segment's copies, queries and limits
-            at += to - from;
-            off += to - from;
+            copies_close();
         }
+        load_queries<T, D, MT>(a, s, u);
+        __syncthreads();
+        const uint32_t see_from = (uint32_t)s.lo[u.rows - 1u], see_to = (uint32_t)s.hi[0];
+        Running<D, MT> x;
+        x.unit = 0.0f;
+#pragma unroll
+        for (uint32_t mt = 0; mt < MT; ++mt) {
+            x.m[mt][0] = x.m[mt][1] = -INFINITY;
+            x.l[mt][0] = x.l[mt][1] = 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < D / 8; ++j)
+                x.o[mt][j][0] = x.o[mt][j][1] = x.o[mt][j][2] = x.o[mt][j][3] = 0.0f;
+        }
+        uint32_t stage = 0;
+        for (uint32_t block = from + warp; block < to; block += kWarps, next += kWarps) {
+            if (next < to) {
+                copier.issue(next, stage == 0 ? kStages - 1u : stage - 1u);
+                copier.look_up(next + kWarps);
+            }
+            copies_close();
+            copies_wait<kStages - 1>();
+            __syncwarp();
+            const uint32_t valid = s.valid[warp][stage];
+            const bool all_see = valid == (each == 32u ? ~0u : (1u << each) - 1u) && block * each >= see_from && (block + 1u) * each <= see_to;
+            add_block<D, MT>(x, s, copier.ring + stage * kStageBytes, valid, block, all_see);
+            __syncwarp();
+            stage = stage + 1u == kStages ? 0u : stage + 1u;
+        }
+        copies_wait<0>();
+        __syncthreads();
+        float* mine = reinterpret_cast<float*>(raw + warp * kRingBytes);
+#pragma unroll
+        for (uint32_t mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (uint32_t r = 0; r < 2; ++r) {
+                float l = x.l[mt][r];
+                l += __shfl_xor_sync(~0u, l, 1);
+                l += __shfl_xor_sync(~0u, l, 2);
+                const uint32_t row = mt * 16u + r * 8u + g;
+                if (c == 0) {
+                    s.m[warp][row] = x.m[mt][r];
+                    s.l[warp][row] = l;
+                }
+                const float by = x.unit / kWeightUnit;
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e)
+#pragma unroll
+                    for (uint32_t j = 0; j < D / 8; j += 4)
+                        *reinterpret_cast<float4*>(mine + row * row_floats + (2u * c + e) * (D / 8) + j) =
+                            make_float4(x.o[mt][j][2 * r + e] * by, x.o[mt][j + 1][2 * r + e] * by, x.o[mt][j + 2][2 * r + e] * by,
+                                        x.o[mt][j + 3][2 * r + e] * by);
+            }
+        __syncthreads();
+        const bool whole = u.whole();
+        float* part = a.parts + (uint64_t)(2u * blockIdx.x + !u.first) * kPartFloats<D, MT>;
+        for (uint32_t i = tid; i < u.rows * (D / 4); i += kThreads) {
+            const uint32_t r = i / (D / 4), d = i % (D / 4) * 4u;
+            float most = s.m[0][r];
+#pragma unroll
+            for (uint32_t w = 1; w < kWarps; ++w)
+                most = fmaxf(most, s.m[w][r]);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float l = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                const float f = part_factor(s.m[w][r], most);
+                l += s.l[w][r] * f;
+                add4(o, *reinterpret_cast<const float4*>(raw + w * kRingBytes + (r * row_floats + d) * 4u), f);
+            }
+            if (whole) {
+                store4(out_row<T, D>(a, u, r) + d, over(o, l));
+            } else {
+                *reinterpret_cast<float4*>(part + r * D + d) = o;
+                if (d == 0) {
+                    part[tile * D + r] = most;
+                    part[tile * (D + 1u) + r] = l;
+                }
+            }
+        }
+        __syncthreads(); // before the next segment's copies, queries and limits
     }
 }
 
@@ -523,23 +510,23 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
     __shared__ uint64_t scratch[40];
     __shared__ float s_factor[kJoinParts][16], s_by[16];
     griddep_wait();
-    uint64_t begin, end, total;
-    uint32_t ctas;
     const uint32_t cta = blockIdx.x + 1u, tid = threadIdx.x;
-    const KvAt found = kv_find<kJoinThreads>(a, Tile, Each, ctas_most, a.blocks_least, scratch, cta, begin, end, total, ctas);
-    if (cta >= ctas)
+    KvWalk walk = kv_find<kJoinThreads>(a, Tile, Each, ctas_most, scratch, cta);
+    if (cta >= walk.ctas)
         return;
-    const KvSeq seq = kv_seq(a, found.seq);
-    const KvUnit u = kv_unit(a, seq, kv_seq_blocks(a, seq, Tile, Each), found.off, Tile, Each);
-    const uint64_t start = begin - u.skip, stop = start + (u.blocks.to - u.blocks.from), before = kv_cut(total, ctas, cta - 1u);
-    if (u.skip == 0 || before > start)
+    const uint32_t skip = walk.skip, ctas = walk.ctas;
+    const uint64_t start = walk.at - skip, before = kv_cut(walk.total, ctas, cta - 1u);
+    if (skip == 0 || before > start)
         return;
+    KvSegment u;
+    kv_take(a, walk, u, true, Tile, Each);
+    const uint64_t stop = start + (u.blocks.to - u.blocks.from);
     constexpr uint32_t floats = Tile * (D + 2u);
     uint32_t parts = 1; // the first one's, and of those CTAs whose shares begin in the unit
-    while (cta + parts - 1u < ctas && kv_cut(total, ctas, cta + parts - 1u) < stop)
+    while (cta + parts - 1u < ctas && kv_cut(walk.total, ctas, cta + parts - 1u) < stop)
         ++parts;
     auto part = [&](uint32_t p) { return a.parts + (uint64_t)(2u * (cta - 1u + p) + (p == 0 && before != start)) * floats; };
-    for (uint32_t r0 = 0; r0 < u.rows; r0 += 16u) { // 16 rows at a time: their maxima, then what each part is worth, then the sums
+    for (uint32_t r0 = 16u * blockIdx.y; r0 < u.rows; r0 += 16u * gridDim.y) { // 16 rows at a time: their maxima, then what each part is worth, then the sums
         const uint32_t rows = min(16u, u.rows - r0);
         float4 o[16 * (D / 4) / kJoinThreads];
 #pragma unroll
@@ -587,7 +574,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
         for (uint32_t k = 0; k < 16 * (D / 4) / kJoinThreads; ++k) {
             const uint32_t i = tid + k * kJoinThreads, r = i / (D / 4), d = i % (D / 4) * 4u;
             if (r < rows)
-                store4(out_row<T, D>(a, seq, u, r0 + r) + d, over(o[k], s_by[r]));
+                store4(out_row<T, D>(a, u, r0 + r) + d, over(o[k], s_by[r]));
         }
         __syncthreads();
     }
@@ -600,7 +587,7 @@ template <typename T, uint32_t D, uint32_t Tile, uint32_t Each>
 cudaError_t launch_join(const KvAttendArgs& a, uint32_t ctas, cudaStream_t stream)
 {
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(ctas - 1u);
+    c.gridDim = dim3(ctas - 1u, Tile / 16u);
     c.blockDim = dim3(kJoinThreads);
     c.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -41,6 +41,16 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t codes)
     return r;
 }
 
+// Four codes, as two pairs of fp16.
+__device__ __forceinline__ uint2 halves_of4(uint32_t codes)
+{
+    uint2 r;
+    asm("{\n\t.reg .b16 low, high;\n\tmov.b32 {low, high}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, low;\n\tcvt.rn.f16x2.e4m3x2 %1, high;\n\t}"
+        : "=r"(r.x), "=r"(r.y)
+        : "r"(codes));
+    return r;
+}
+
 // Four codes, each times a power of two.
 __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float by)
 {

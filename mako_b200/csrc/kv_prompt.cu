@@ -16,25 +16,19 @@ namespace mk {
 namespace {
 
 constexpr uint32_t kTileRows = 128, kUnitRows = 256, kBlock = 128; // rows of a tile, of a unit; keys of a block
-constexpr uint32_t kThreads = 512;
+constexpr uint32_t kThreads = 416; // of 128 registers each
 constexpr uint32_t kConvert = 256, kIssue = 384; // first thread of those that convert, and of the warp that issues
 constexpr uint32_t kSlots = 4;                   // of what softmax reads beside the scores
 constexpr float kWeightUnit = 128.0f;
 constexpr uint32_t kMixed = 8; // blocks of a segment that some rows see and others do not: at most 3 at either end
-
-struct Scale {
-    float key, value; // the value's: over the largest so far, times kWeightUnit
-};
 
 struct Shared {
     uint64_t find[40];
     uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
     uint32_t tmem;
     int failed;
-    float factor[kUnitRows];
-    int32_t lo[kUnitRows], hi[kUnitRows];
-    alignas(16) Scale scale[kSlots][kBlock];
-    uint32_t missing[kSlots][4];       // tokens whose page is not there
+    alignas(16) float key[kSlots][kBlock], value[kSlots][kBlock]; // scales; values' over the largest so far, times kWeightUnit
+    alignas(16) uint32_t missing[kSlots][4]; // tokens whose page is not there
     float older[kSlots];               // what outputs so far are worth in the block's unit
     float unit[2];                     // the largest scale of a segment's values, by its parity
     uint32_t n_mixed[2];
@@ -89,6 +83,18 @@ __device__ __forceinline__ void tmem_read32(float* x, uint32_t at)
         : "r"(at)
         : "memory");
 }
+__device__ __forceinline__ void tmem_read64(float* x, uint32_t at)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, "
+        "%56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : MK_R8(x, 0), MK_R8(x, 8), MK_R8(x, 16), MK_R8(x, 24), MK_R8(x, 32), MK_R8(x, 40), MK_R8(x, 48), MK_R8(x, 56)
+        : "r"(at)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_write32(uint32_t at, const uint32_t* x)
 {
     asm volatile(
@@ -96,6 +102,13 @@ __device__ __forceinline__ void tmem_write32(uint32_t at, const uint32_t* x)
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
         "%29, %30, %31};" ::MK_W8(x, 0),
         MK_W8(x, 8), MK_W8(x, 16), MK_W8(x, 24), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_write16(uint32_t at, const uint32_t* x)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::MK_W8(x, 0),
+        MK_W8(x, 8), "r"(at)
         : "memory");
 }
 __device__ __forceinline__ void tmem_written() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -118,11 +131,7 @@ __device__ __forceinline__ float2 two(uint32_t w)
 // Where the 16 bytes `chunk` (8 fp16 columns) of a row lie in a tile of 128 rows: 64 columns side by side, 16 KB to the next 64.
 __device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t chunk) { return (chunk >> 3) * 16384u + row * 128u + (((chunk ^ row) & 7u) << 4); }
 
-// A segment: blocks [from, to) of a unit.
-struct Segment {
-    KvSeq seq;
-    KvUnit u;
-    uint32_t sq, from, to;
+struct Segment : KvSegment {
     uint32_t see_from, see_to; // what all rows see
 };
 
@@ -138,66 +147,13 @@ struct Ring { // shared memory
 // Those that convert. What they count goes on from segment to segment.
 template <typename T, uint32_t D>
 struct Converter {
-    static constexpr uint32_t chunks = D / 16, rows_each = 128 / chunks, loads = kBlock / rows_each; // 16 codes a load
+    // a load is 16 codes: of 32 rows, 64 columns. (Eight lanes have two rows' quarters: their stores are in different banks.)
+    static constexpr uint32_t halves = D / 64, loads = kBlock / 32 * halves;
+    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return i / halves * 32u + (threadIdx.x - kConvert) / 4u; }
+    static __device__ __forceinline__ uint32_t chunk_of(uint32_t i) { return i % halves * 4u + (threadIdx.x & 3u); }
     uint32_t blocks = 0;   // so far
     uint32_t segments = 0;
     bool alive = true;
-
-    __device__ __forceinline__ void queries(const KvAttendArgs& a, Shared& s, const Ring<D>& ring, const Segment& g)
-    {
-        constexpr uint32_t lanes = D / 8; // of a row
-        const uint32_t tid = threadIdx.x - kConvert;
-        alive = alive && await(s, &s.q_empty, (segments & 1u) ^ 1u);
-        __syncwarp();
-        const uint32_t rows = g.u.rows > kTileRows ? kUnitRows : kTileRows;
-        for (uint32_t i = tid; i < rows * lanes; i += 128u) { // (whole warps: lanes is 8 or 16)
-            const uint32_t r = i / lanes, chunk = i % lanes, row = g.u.row0 + r;
-            const bool real = r < g.u.rows;
-            uint32_t w[4] = {};
-            if (real) {
-                const uint64_t token = g.seq.first + row / a.group;
-                const T* p = static_cast<const T*>(a.q) + token * a.q_ld + (uint64_t)(g.u.head * a.group + row % a.group) * D + chunk * 8u;
-                const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-            }
-            float most = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 x = two<T>(w[k]);
-                most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
-            }
-            __syncwarp();
-#pragma unroll
-            for (uint32_t d = 1; d < lanes; d <<= 1)
-                most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-            // a power of two that brings the largest to 2^12; 1 where a row is nothing or infinite
-            const int e = (int)(__float_as_uint(most) >> 23) - 127;
-            const int up = most > 0.0f && e < 128 ? max(-100, min(100, 12 - e)) : 0;
-            const float by = __uint_as_float((uint32_t)(up + 127) << 23), turned = a.scale_log2 < 0.0f ? -by : by;
-            uint32_t y[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 x = two<T>(w[k]);
-                y[k] = pair_of(x.x * turned, x.y * turned);
-            }
-            *reinterpret_cast<uint4*>(ring.q(r / kTileRows) + tile_at(r % kTileRows, chunk)) = make_uint4(y[0], y[1], y[2], y[3]);
-            if (chunk == 0) {
-                const int64_t at = (int64_t)g.seq.len - g.seq.n + row / a.group;
-                s.factor[r] = fmaxf(fabsf(a.scale_log2) / by, 1e-37f);
-                s.hi[r] = real && at >= 0 ? (int32_t)(at + 1 < g.seq.len ? at + 1 : g.seq.len) : 0;
-                s.lo[r] = a.window && at + 1 > (int64_t)a.window ? (int32_t)(at + 1 - a.window) : 0;
-            }
-        }
-        if (tid == 0)
-            s.n_mixed[segments & 1u] = 0;
-        fence_proxy_async();
-        __syncwarp();
-        named_barrier(2, 128);
-        if (tid == 0)
-            mbar_arrive(&s.q_full);
-        __syncwarp();
-        ++segments;
-    }
 
     // The place of this thread's token of a block (all ones: not there), and its scales.
     struct Place {
@@ -211,9 +167,9 @@ struct Converter {
         if (t < g.seq.len) {
             const uint32_t index = kv_page_of(a, t), page = (uint32_t)__ldg(table + index);
             if (page < a.c.n_pages) {
-                p.off = page * a.c.page_stride + (uint64_t)g.u.head * a.c.head_stride + (uint64_t)(t - index * a.c.page_size) * a.c.token_stride;
-                p.key = __ldg(a.c.k_scale + (uint64_t)page * a.c.n_heads + g.u.head);
-                p.value = __ldg(a.c.v_scale + (uint64_t)page * a.c.n_heads + g.u.head);
+                p.off = page * a.c.page_stride + (uint64_t)g.head * a.c.head_stride + (uint64_t)(t - index * a.c.page_size) * a.c.token_stride;
+                p.key = __ldg(a.c.k_scale + (uint64_t)page * a.c.n_heads + g.head);
+                p.value = __ldg(a.c.v_scale + (uint64_t)page * a.c.n_heads + g.head);
             }
         }
         return p;
@@ -221,25 +177,19 @@ struct Converter {
 
     __device__ __forceinline__ void load(uint4 (&x)[loads], const void* codes, const uint64_t* off)
     {
-        const uint32_t tid = threadIdx.x - kConvert, chunk = tid % chunks;
 #pragma unroll
         for (uint32_t i = 0; i < loads; ++i) {
-            const uint64_t from = off[i * rows_each + tid / chunks];
-            x[i] = from != ~0ull ? __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(codes) + from + chunk * 16u)) : make_uint4(0, 0, 0, 0);
+            const uint64_t from = off[row_of(i)];
+            x[i] = from != ~0ull ? __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(codes) + from + chunk_of(i) * 16u)) : make_uint4(0, 0, 0, 0);
         }
     }
     __device__ __forceinline__ void store(const uint4 (&x)[loads], unsigned char* tile)
     {
-        const uint32_t tid = threadIdx.x - kConvert, chunk = tid % chunks;
 #pragma unroll
         for (uint32_t i = 0; i < loads; ++i) {
-            const uint32_t row = i * rows_each + tid / chunks;
-            const uint4 low = make_uint4(halves_of(x[i].x & 0xffffu), halves_of(x[i].x >> 16), halves_of(x[i].y & 0xffffu), halves_of(x[i].y >> 16));
-            const uint4 high = make_uint4(halves_of(x[i].z & 0xffffu), halves_of(x[i].z >> 16), halves_of(x[i].w & 0xffffu), halves_of(x[i].w >> 16));
-            // (the upper half of a row's lanes begin with their second half: all banks)
-            const bool first = chunk < 4u;
-            *reinterpret_cast<uint4*>(tile + tile_at(row, 2u * chunk + !first)) = first ? low : high;
-            *reinterpret_cast<uint4*>(tile + tile_at(row, 2u * chunk + first)) = first ? high : low;
+            const uint2 y0 = halves_of4(x[i].x), y1 = halves_of4(x[i].y), y2 = halves_of4(x[i].z), y3 = halves_of4(x[i].w);
+            *reinterpret_cast<uint4*>(tile + tile_at(row_of(i), 2u * chunk_of(i))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+            *reinterpret_cast<uint4*>(tile + tile_at(row_of(i), 2u * chunk_of(i) + 1u)) = make_uint4(y2.x, y2.y, y3.x, y3.y);
         }
     }
 
@@ -249,7 +199,9 @@ struct Converter {
         const int32_t* table = a.block_table + (uint64_t)g.sq * a.table_ld;
         float unit = 0.0f;
         Place p = place(a, g, table, g.from);
-        queries(a, s, ring, g);
+        if (tid == 0)
+            s.n_mixed[segments & 1u] = 0; // (that of the segment before the last one has been read: its successor's softmax has begun)
+        ++segments;
         s.off[blocks & 1u][tid] = p.off;
         __syncwarp();
         named_barrier(2, 128);
@@ -271,7 +223,8 @@ struct Converter {
             named_barrier(2, 128); // (the block before has read warp_most, and this block's are there)
             const float largest = fmaxf(fmaxf(s.warp_most[0], s.warp_most[1]), fmaxf(s.warp_most[2], s.warp_most[3]));
             const float now = fmaxf(unit, largest);
-            s.scale[slot][tid] = Scale{p.key, now > 0.0f ? p.value * (kWeightUnit / now) : 0.0f};
+            s.key[slot][tid] = p.key;
+            s.value[slot][tid] = now > 0.0f ? p.value * (kWeightUnit / now) : 0.0f;
             if (lane == 0)
                 s.missing[slot][tid / 32u] = missing;
             if (tid == 0)
@@ -318,7 +271,7 @@ struct Converter {
 #pragma unroll
                     for (uint32_t i = 0; i < loads; ++i)
                         if (bad[i]) {
-                            const uint32_t row = i * rows_each + tid / chunks;
+                            const uint32_t row = row_of(i);
                             atomicOr(at + 1u + row / 32u, 1u << (row & 31u));
                             v[i].x &= ~__vcmpeq4(v[i].x & 0x7f7f7f7fu, 0x7f7f7f7fu);
                             v[i].y &= ~__vcmpeq4(v[i].y & 0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -358,7 +311,7 @@ struct Issuer {
 
     __device__ __forceinline__ void run(Shared& s, const Ring<D>& ring, const Segment& g)
     {
-        const uint32_t n = g.to - g.from, tiles = g.u.rows > kTileRows ? 2u : 1u;
+        const uint32_t n = g.to - g.from, tiles = g.rows > kTileRows ? 2u : 1u;
         const uint32_t desc = mma_f16_desc(false, D) | (1u << 16); // B is MN-major
         alive = alive && await(s, &s.q_full, segments & 1u);
         ++segments;
@@ -409,18 +362,57 @@ struct Softmax {
     uint32_t blocks = 0, segments = 0, seen = 0, outputs = 0; // blocks so far of all segments, and of this tile's
     bool alive = true;
 
-    __device__ __forceinline__ void run(const KvAttendArgs& a, Shared& s, const Segment& g, float* part)
+    __device__ __forceinline__ void run(const KvAttendArgs& a, Shared& s, const Ring<D>& ring, const Segment& g, float* part)
     {
         const uint32_t t = threadIdx.x / kTileRows, row = threadIdx.x, quarter = threadIdx.x / 32u % 4u;
         const uint32_t n = g.to - g.from, which = segments & 1u;
-        alive = alive && await(s, &s.q_full, segments & 1u);
-        ++segments;
-        const float f = s.factor[row];
-        const int32_t lo = s.lo[row], hi = s.hi[row];
-        mbar_arrive(&s.q_empty);
+        // the row's queries, times a power of two that brings the largest to 2^12 (1 where a row is nothing or infinite)
+        const uint32_t unit_row = g.row0 + row, token = unit_row / a.group, head = g.head * a.group + (unit_row - token * a.group);
+        const bool real = row < g.rows;
+        float f;
+        {
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.seq.first + token) * a.q_ld + (uint64_t)head * D);
+            uint4 q[D / 8];
+#pragma unroll
+            for (uint32_t i = 0; i < D / 8; ++i)
+                q[i] = real ? __ldg(p + i) : make_uint4(0, 0, 0, 0);
+            float top = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < D / 8; ++i) {
+                const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 x = two<T>(w[k]);
+                    top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+                }
+            }
+            const int e = (int)(__float_as_uint(top) >> 23) - 127;
+            const int up = top > 0.0f && e < 128 ? max(-100, min(100, 12 - e)) : 0;
+            const float by = __uint_as_float((uint32_t)(up + 127) << 23), turned = a.scale_log2 < 0.0f ? -by : by;
+            f = fmaxf(fabsf(a.scale_log2) / by, 1e-37f); // (not 0: a key that the row does not see has -inf times this)
+            alive = alive && await(s, &s.q_empty, (segments & 1u) ^ 1u);
+            ++segments;
+            unsigned char* tile = ring.q(t);
+#pragma unroll
+            for (uint32_t i = 0; i < D / 8; ++i) {
+                const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+                uint32_t y[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 x = two<T>(w[k]);
+                    y[k] = pair_of(x.x * turned, x.y * turned);
+                }
+                *reinterpret_cast<uint4*>(tile + tile_at(row % kTileRows, i)) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+            fence_proxy_async();
+            mbar_arrive(&s.q_full);
+        }
+        const int32_t at = (int32_t)g.seq.len - (int32_t)g.seq.n + (int32_t)token + 1; // behind its position
+        const int32_t hi = real && at > 0 ? at : 0, lo = a.window && at > (int32_t)a.window ? at - (int32_t)a.window : 0;
         const uint32_t first = blocks;
         blocks += n;
-        if (t && g.u.rows <= kTileRows)
+        __syncwarp();
+        if (t && g.rows <= kTileRows)
             return;
         const uint32_t lanes = (quarter * 32u) << 16, scores = s.tmem + lanes + t * 128u, out = s.tmem + lanes + 256u + t * 128u;
         float ref = -INFINITY, l = 0.0f;
@@ -433,32 +425,45 @@ struct Softmax {
                 return;
             }
             tc_fence_after();
-            float x[kBlock];
+            const float4 *key = reinterpret_cast<const float4*>(s.key[slot]), *value = reinterpret_cast<const float4*>(s.value[slot]);
+            const uint4 gone = *reinterpret_cast<const uint4*>(s.missing[slot]);
+            const int32_t low = lo - (int32_t)begin, high = hi - (int32_t)begin;
+            const bool some = __any_sync(~0u, (gone.x | gone.y | gone.z | gone.w) != 0 || low > 0 || high < (int32_t)kBlock);
+            // Half of a row's scores, times the keys' scales; -inf where it does not see the key. (A thread has registers for half of them: the
+            // second half is read twice, for the largest and once the first half's weights are made.)
+            auto read = [&](float (&x)[64], uint32_t half) {
+                tmem_read64(x, scores + 64u * half);
 #pragma unroll
-            for (uint32_t i = 0; i < kBlock; i += 32)
-                tmem_read32(x + i, scores + i);
-            const float4* scale = reinterpret_cast<const float4*>(s.scale[slot]);
+                for (uint32_t i = 0; i < 64; i += 4) {
+                    const float4 c = key[16u * half + i / 4];
+                    const float2 y = mul2(make_float2(x[i], x[i + 1]), make_float2(c.x, c.y)), z = mul2(make_float2(x[i + 2], x[i + 3]), make_float2(c.z, c.w));
+                    x[i] = y.x, x[i + 1] = y.y, x[i + 2] = z.x, x[i + 3] = z.y;
+                }
+                if (some) {
 #pragma unroll
-            for (uint32_t i = 0; i < kBlock; i += 2) {
-                const float4 c = scale[i / 2];
-                const float2 y = mul2(make_float2(x[i], x[i + 1]), make_float2(c.x, c.z));
-                x[i] = y.x;
-                x[i + 1] = y.y;
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const int32_t from = low - 64 * (int32_t)half - 32 * (int32_t)i, to = high - 64 * (int32_t)half - 32 * (int32_t)i;
+                        // the places [from, to) of 32
+                        const uint32_t behind = to <= 0 ? 0u : to >= 32 ? ~0u : (1u << to) - 1u;
+                        const uint32_t before = from <= 0 ? 0u : from >= 32 ? ~0u : (1u << from) - 1u;
+                        const uint32_t sees = behind & ~before & ~(half ? (i ? gone.w : gone.z) : (i ? gone.y : gone.x));
+#pragma unroll
+                        for (uint32_t k = 0; k < 32; ++k)
+                            x[32 * i + k] = (sees >> k) & 1u ? x[32 * i + k] : -INFINITY;
+                    }
+                }
+            };
+            float x[64], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int half = 1; half >= 0; --half) {
+                read(x, half);
+#pragma unroll
+                for (uint32_t i = 0; i < 64; i += 8)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        tops[k] = fmaxf(tops[k], fmaxf(x[i + k], x[i + k + 4]));
             }
-            const uint32_t gone = s.missing[slot][0] | s.missing[slot][1] | s.missing[slot][2] | s.missing[slot][3];
-            if (__any_sync(~0u, gone || lo > (int32_t)begin || hi < (int32_t)(begin + kBlock))) {
-                const int32_t low = lo - (int32_t)begin, high = hi - (int32_t)begin;
-                const uint32_t m[4] = {s.missing[slot][0], s.missing[slot][1], s.missing[slot][2], s.missing[slot][3]};
-#pragma unroll
-                for (int32_t i = 0; i < (int32_t)kBlock; ++i)
-                    if (i < low || i >= high || ((m[i / 32] >> (i % 32)) & 1u))
-                        x[i] = -INFINITY;
-            }
-            float most = x[0];
-#pragma unroll
-            for (uint32_t i = 1; i < kBlock; ++i)
-                most = fmaxf(most, x[i]);
-            most *= f;
+            const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
             const float older = s.older[slot];
             float by = older;
             if (most > ref + 8.0f || ref == -INFINITY) { // (-inf: nothing seen yet; its outputs and sum are zeros)
@@ -482,23 +487,29 @@ struct Softmax {
             }
             const float from = ref == -INFINITY ? 0.0f : ref;
             const float2 f2 = make_float2(f, f), minus = make_float2(-from, -from);
-            float2 sum = make_float2(0.0f, 0.0f);
+            float2 sum = make_float2(0.0f, 0.0f), more = sum;
 #pragma unroll
-            for (uint32_t i = 0; i < kBlock; i += 64) {
-                uint32_t w[32];
+            for (uint32_t half = 0; half < 2; ++half) {
+                if (half)
+                    read(x, 1u);
 #pragma unroll
-                for (uint32_t k = 0; k < 64; k += 2) {
-                    const float4 c = scale[(i + k) / 2];
-                    const float2 d = fma2(make_float2(x[i + k], x[i + k + 1]), f2, minus);
-                    const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y));
-                    sum.x += p.x;
-                    sum.y += p.y;
-                    const float2 y = mul2(p, make_float2(c.y, c.w));
-                    w[k / 2] = pair_of(y.x, y.y);
+                for (uint32_t i0 = 0; i0 < 64; i0 += 32) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (uint32_t i = i0; i < i0 + 32; i += 4) {
+                        const float4 c = value[16u * half + i / 4];
+                        const float2 d = fma2(make_float2(x[i], x[i + 1]), f2, minus), e = fma2(make_float2(x[i + 2], x[i + 3]), f2, minus);
+                        const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y)), q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                        sum = add2(sum, p);
+                        more = add2(more, q);
+                        const float2 y = mul2(p, make_float2(c.x, c.y)), z = mul2(q, make_float2(c.z, c.w));
+                        w[(i - i0) / 2] = pair_of(y.x, y.y);
+                        w[(i - i0) / 2 + 1] = pair_of(z.x, z.y);
+                    }
+                    tmem_write16(scores + 32u * half + i0 / 2, w); // (over the first half's scores, which have been read)
                 }
-                tmem_write32(scores + i / 2, w);
             }
-            l += sum.x + sum.y;
+            l += (sum.x + sum.y) + (more.x + more.y);
             __syncwarp();
             tmem_written();
             tc_fence_before();
@@ -524,10 +535,8 @@ struct Softmax {
             }
         }
         __syncwarp();
-        const bool real = row < g.u.rows;
         const float worth = s.unit[which] / kWeightUnit;
-        const uint32_t r = g.u.row0 + row;
-        T* to = static_cast<T*>(a.out) + (g.seq.first + r / a.group) * a.out_ld + (uint64_t)(g.u.head * a.group + r % a.group) * D;
+        T* to = static_cast<T*>(a.out) + (g.seq.first + token) * a.out_ld + (uint64_t)head * D;
         const float by = part ? worth : l == 0.0f ? 0.0f : worth / l;
 #pragma unroll 1
         for (uint32_t i = 0; i < D; i += 32) {
@@ -572,8 +581,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     ring.base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
     const uint32_t tid = threadIdx.x, warp = tid / 32u;
     if (tid == 0) {
-        mbar_init(&s.q_full, 1);
-        mbar_init(&s.q_empty, 1u + 2u * kTileRows);
+        mbar_init(&s.q_full, kUnitRows);
+        mbar_init(&s.q_empty, 1);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&s.k_full[i], 1);
             mbar_init(&s.k_empty[i], 1);
@@ -590,46 +599,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         tmem_alloc_all(&s.tmem);
     griddep_launch_dependents();
     griddep_wait();
-    uint64_t begin, end, total;
-    uint32_t ctas;
     tc_fence_before();
-    const KvAt found = kv_find<kThreads>(a, kUnitRows, kBlock, gridDim.x, a.blocks_least, s.find, blockIdx.x, begin, end, total, ctas);
+    const KvWalk found = kv_find<kThreads>(a, kUnitRows, kBlock, gridDim.x, s.find, blockIdx.x);
     tc_fence_after();
     // each of them goes through the CTA's segments
     auto segments = [&](auto&& role) {
-        uint64_t at = begin, off = found.off;
-        for (uint32_t sq = found.seq; at < end && sq < a.n_seq; ++sq, off = 0) {
-            Segment g;
-            g.sq = sq;
-            g.seq = kv_seq(a, sq);
-            const uint32_t per_head = kv_seq_blocks(a, g.seq, kUnitRows, kBlock);
-            while (at < end && off < (uint64_t)per_head * a.c.n_heads) {
-                g.u = kv_unit(a, g.seq, per_head, off, kUnitRows, kBlock);
-                g.from = g.u.blocks.from + g.u.skip;
-                g.to = end - at < g.u.blocks.to - g.from ? g.from + (uint32_t)(end - at) : g.u.blocks.to;
-                const int64_t back = (int64_t)g.seq.len - g.seq.n, top = back + g.u.row0 / a.group + 1, last = back + (g.u.row0 + g.u.rows - 1u) / a.group + 1;
-                g.see_to = top < 0 ? 0u : top < g.seq.len ? (uint32_t)top : g.seq.len;
-                g.see_from = a.window && last > (int64_t)a.window ? (uint32_t)(last - a.window) : 0u;
-                const bool whole = g.u.skip == 0 && g.to == g.u.blocks.to;
-                float* part = whole ? nullptr : a.parts + (uint64_t)(2u * blockIdx.x + (at != begin)) * (kUnitRows * (D + 2u));
-                role(g, part);
-                at += g.to - g.from;
-                off += g.to - g.from;
-            }
+        KvWalk walk = found;
+        Segment g;
+        for (bool first = true; kv_take(a, walk, g, first, kUnitRows, kBlock); first = false) {
+            const int32_t back = (int32_t)g.seq.len - (int32_t)g.seq.n;
+            const int32_t top = back + (int32_t)(g.row0 / a.group) + 1, last = back + (int32_t)((g.row0 + g.rows - 1u) / a.group) + 1;
+            g.see_to = top < 0 ? 0u : (uint32_t)top;
+            g.see_from = a.window && last > (int32_t)a.window ? (uint32_t)last - a.window : 0u;
+            role(g, g.whole() ? nullptr : a.parts + (uint64_t)(2u * blockIdx.x + !first) * (kUnitRows * (D + 2u)));
         }
     };
-    // 128 registers a thread at launch: 256 x 184 + 128 x 104 + 128 x 40 = 512 x 128
-    if (blockIdx.x < ctas) {
+    if (blockIdx.x < found.ctas) {
         if (tid < kConvert) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
             Softmax<T, D> x;
-            segments([&](const Segment& g, float* part) { x.run(a, s, g, part); });
+            segments([&](const Segment& g, float* part) { x.run(a, s, ring, g, part); });
         } else if (tid < kIssue) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
             Converter<T, D> x;
             segments([&](const Segment& g, float*) { x.run(a, s, ring, g); });
         } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
             if (tid == kIssue) {
                 Issuer<D> x;
                 segments([&](const Segment& g, float*) {
@@ -660,12 +652,6 @@ template <typename T, uint32_t D>
 cudaError_t launch(const KvAttendArgs& a, cudaStream_t stream)
 {
     constexpr uint32_t smem = 6u * Ring<D>::tile_bytes + 1024u;
-    static const bool split_fits = [] { // the registers that the warps share out among themselves are those of the launch
-        cudaFuncAttributes f;
-        return cudaFuncGetAttributes(&f, kv_prompt_kernel<T, D>) == cudaSuccess && f.numRegs == 128;
-    }();
-    if (!split_fits)
-        return cudaErrorInvalidKernelImage;
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = set_once(done, kv_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess)

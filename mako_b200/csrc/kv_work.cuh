@@ -30,24 +30,47 @@ struct KvBlocks {
 
 __device__ __forceinline__ KvBlocks kv_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t row0, uint32_t rows, uint32_t each)
 {
-    const int64_t back = (int64_t)q.len - q.n; // the position of the pass's first token
-    const int64_t end = back + (row0 + rows - 1u) / a.group + 1;
-    const uint32_t hi = end < 0 ? 0u : end > q.len ? q.len : (uint32_t)end;
-    const int64_t begin = a.window ? back + row0 / a.group - (int64_t)a.window + 1 : 0;
-    const uint32_t lo = begin < 0 ? 0u : (uint32_t)begin, from = lo / each, to = (hi + each - 1u) / each;
+    const int32_t back = (int32_t)q.len - (int32_t)q.n;                     // the position of the pass's first token
+    const int32_t end = back + (int32_t)((row0 + rows - 1u) / a.group) + 1; // (at most len)
+    const int32_t first = back + (int32_t)(row0 / a.group) + 1;
+    const uint32_t lo = a.window && first > (int32_t)a.window ? (uint32_t)first - a.window : 0u;
+    const uint32_t from = lo / each, to = end < 0 ? 0u : ((uint32_t)end + each - 1u) / each;
     return KvBlocks{from, to > from ? to : from + 1u};
 }
 
-// Of a sequence: blocks of one key head, all of its tiles of rows together. 0 for a sequence that is not this launch's.
-__device__ __forceinline__ uint32_t kv_seq_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t tile, uint32_t each)
+// A sequence's rows, or 0 where it is not this launch's.
+__device__ __forceinline__ uint32_t kv_rows(const KvAttendArgs& a, const KvSeq& q)
 {
     const uint32_t rows = q.n * a.group;
-    if (rows < a.rows_from || rows > a.rows_to)
+    return rows < a.rows_from || rows > a.rows_to ? 0u : rows;
+}
+
+__device__ __forceinline__ uint32_t kv_tile_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t rows, uint32_t row0, uint32_t tile, uint32_t each)
+{
+    if (row0 >= rows)
         return 0;
-    uint32_t sum = 0;
-    for (uint32_t r = 0; r < rows; r += tile) {
-        const KvBlocks b = kv_blocks(a, q, r, min(tile, rows - r), each);
-        sum += b.to - b.from;
+    const KvBlocks b = kv_blocks(a, q, row0, min(tile, rows - row0), each);
+    return b.to - b.from;
+}
+
+// Of each lane's sequence: blocks of one key head, all of its tiles of rows together. A sequence of many tiles (a prompt) is counted by the
+// warp. By whole warps.
+__device__ __forceinline__ uint32_t kv_seq_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t rows, uint32_t tile, uint32_t each)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t sum = kv_tile_blocks(a, q, rows, 0, tile, each);
+    uint32_t many = __ballot_sync(~0u, rows > tile);
+    while (many) {
+        const int i = __ffs(many) - 1;
+        many &= many - 1u;
+        const KvSeq other{0u, __shfl_sync(~0u, q.n, i), __shfl_sync(~0u, q.len, i)};
+        const uint32_t its = __shfl_sync(~0u, rows, i);
+        uint32_t x = 0;
+        for (uint32_t r = lane * tile; r < its; r += 32u * tile)
+            x += kv_tile_blocks(a, other, its, r, tile, each);
+        __syncwarp();
+        x = __reduce_add_sync(~0u, x);
+        sum = lane == (uint32_t)i ? x : sum;
     }
     return sum;
 }
@@ -61,21 +84,27 @@ __device__ __forceinline__ uint64_t kv_cut(uint64_t total, uint32_t n, uint32_t 
     return (uint64_t)each * i + min(i, more);
 }
 
-struct KvAt {
-    uint32_t seq;
-    uint64_t off;   // blocks into the sequence
+// A CTA's share of all blocks, [at, end), and the unit that it begins in, `skip` blocks behind the unit's first. take() gives one segment
+// after the other.
+struct KvWalk {
+    uint64_t at, end, total;
+    uint32_t ctas; // that have a share
+    uint32_t sq, head, row0, skip;
 };
 
-// Where the block `at` of all lies, and how many there are, by all Threads of a CTA; scratch: Threads + 8 words of 8 bytes.
+// By all Threads of a CTA; scratch: 40 words of 8 bytes.
 template <uint32_t Threads>
-__device__ KvAt kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, uint32_t ctas_most, uint32_t blocks_least, uint64_t* scratch,
-                        uint32_t cta, uint64_t& begin, uint64_t& end, uint64_t& total, uint32_t& ctas)
+__device__ KvWalk kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, uint32_t ctas_most, uint64_t* scratch, uint32_t cta)
 {
     const uint32_t tid = threadIdx.x, lane = tid & 31u, mine = (a.n_seq + Threads - 1) / Threads;
-    const uint32_t s0 = min(tid * mine, a.n_seq), s1 = min(s0 + mine, a.n_seq);
+    auto of = [&](uint32_t k) -> uint64_t { // blocks of this thread's sequence k, all heads
+        const uint32_t s = tid * mine + k;
+        const KvSeq q = s < a.n_seq ? kv_seq(a, s) : KvSeq{0, 0, 0};
+        return (uint64_t)kv_seq_blocks(a, q, s < a.n_seq ? kv_rows(a, q) : 0u, tile, each) * a.c.n_heads;
+    };
     uint64_t sum = 0;
-    for (uint32_t s = s0; s < s1; ++s)
-        sum += (uint64_t)kv_seq_blocks(a, kv_seq(a, s), tile, each) * a.c.n_heads;
+    for (uint32_t k = 0; k < mine; ++k)
+        sum += of(k);
     uint64_t run = sum;
 #pragma unroll
     for (uint32_t d = 1; d < 32; d <<= 1) {
@@ -86,56 +115,108 @@ __device__ KvAt kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, uin
     if (lane == 31u)
         scratch[tid / 32u] = run;
     __syncthreads();
+    KvWalk w;
     uint64_t front = 0;
-    total = 0;
-    for (uint32_t w = 0; w < Threads / 32u; ++w) {
-        if (w < tid / 32u)
-            front += scratch[w];
-        total += scratch[w];
+    w.total = 0;
+    for (uint32_t i = 0; i < Threads / 32u; ++i) {
+        front += i < tid / 32u ? scratch[i] : 0ull;
+        w.total += scratch[i];
     }
-    ctas = ctas_most;
-    if (total < (uint64_t)blocks_least * ctas_most)
-        ctas = ((uint32_t)total + blocks_least - 1u) / blocks_least;
-    begin = ctas ? kv_cut(total, ctas, cta) : 0;
-    end = ctas ? kv_cut(total, ctas, cta + 1u) : 0;
+    w.ctas = ctas_most;
+    if (w.total < (uint64_t)a.blocks_least * ctas_most)
+        w.ctas = ((uint32_t)w.total + a.blocks_least - 1u) / a.blocks_least;
+    const bool has = cta < w.ctas;
+    w.at = has ? kv_cut(w.total, w.ctas, cta) : 0;
+    w.end = has ? kv_cut(w.total, w.ctas, cta + 1u) : 0;
     uint64_t at = front + run - sum; // of this thread's first sequence
-    if (cta < ctas && begin >= at && begin < at + sum)
-        for (uint32_t s = s0; s < s1; ++s) {
-            const uint64_t has = (uint64_t)kv_seq_blocks(a, kv_seq(a, s), tile, each) * a.c.n_heads;
-            if (begin < at + has) {
-                scratch[32] = s;
-                scratch[33] = begin - at;
-                break;
+    if (__any_sync(~0u, has && w.at >= at && w.at < at + sum)) {
+        for (uint32_t k = 0; k < mine; ++k) {
+            const uint64_t n = mine == 1u ? sum : of(k);
+            if (has && w.at >= at && w.at < at + n) {
+                scratch[32] = tid * mine + k;
+                scratch[33] = w.at - at;
+                scratch[34] = n;
             }
-            at += has;
+            at += n;
         }
+    }
     __syncthreads();
-    const KvAt found{(uint32_t)scratch[32], scratch[33]};
+    if (has && tid < 32u) { // the head and, 32 at a time, the tile
+        const uint32_t s = (uint32_t)scratch[32];
+        const uint64_t off = scratch[33], all = scratch[34];
+        const KvSeq q = kv_seq(a, s);
+        const uint32_t rows = kv_rows(a, q), per_head = all >> 32 ? (uint32_t)(all / a.c.n_heads) : (uint32_t)all / a.c.n_heads;
+        const uint32_t head = off >> 32 ? (uint32_t)(off / per_head) : (uint32_t)off / per_head;
+        uint32_t left = (uint32_t)(off - (uint64_t)head * per_head);
+        for (uint32_t r0 = 0; r0 < rows; r0 += 32u * tile) {
+            const uint32_t r = r0 + lane * tile, n = kv_tile_blocks(a, q, rows, r, tile, each);
+            uint32_t upto = n;
+#pragma unroll
+            for (uint32_t d = 1; d < 32; d <<= 1) {
+                const uint32_t y = __shfl_up_sync(~0u, upto, d);
+                upto += lane >= d ? y : 0u;
+            }
+            if (left < upto && left >= upto - n) {
+                scratch[35] = head;
+                scratch[36] = r;
+                scratch[37] = left - (upto - n);
+            }
+            const uint32_t these = __shfl_sync(~0u, upto, 31);
+            if (left < these)
+                break;
+            left -= these;
+        }
+    }
     __syncthreads();
-    return found;
+    w.sq = (uint32_t)scratch[32];
+    w.head = (uint32_t)scratch[35];
+    w.row0 = (uint32_t)scratch[36];
+    w.skip = (uint32_t)scratch[37];
+    return w;
 }
 
-// A unit and what of it begins at `off` of a sequence.
-struct KvUnit {
-    uint32_t head, row0, rows;
-    KvBlocks blocks;      // all of its blocks
-    uint32_t skip;        // that come before `off`
+// A unit, and the blocks [from, to) of it that a CTA has.
+struct KvSegment {
+    KvSeq seq;
+    KvBlocks blocks; // all of the unit's
+    uint32_t sq, head, row0, rows, from, to;
+    bool first;      // the CTA's first one
+    __device__ __forceinline__ bool whole() const { return from == blocks.from && to == blocks.to; }
 };
 
-__device__ __forceinline__ KvUnit kv_unit(const KvAttendArgs& a, const KvSeq& q, uint32_t seq_blocks, uint64_t off, uint32_t tile, uint32_t each)
+// The walk's next segment; false behind the last. `g` is the one before, w.at the share's begin at the first call.
+__device__ __forceinline__ bool kv_take(const KvAttendArgs& a, KvWalk& w, KvSegment& g, bool first, uint32_t tile, uint32_t each)
 {
-    KvUnit u;
-    u.head = off >> 32 ? (uint32_t)(off / seq_blocks) : (uint32_t)off / seq_blocks;
-    u.skip = (uint32_t)(off - (uint64_t)u.head * seq_blocks);
-    const uint32_t rows = q.n * a.group;
-    for (u.row0 = 0;; u.row0 += tile) {
-        u.rows = min(tile, rows - u.row0);
-        u.blocks = kv_blocks(a, q, u.row0, u.rows, each);
-        const uint32_t has = u.blocks.to - u.blocks.from;
-        if (u.skip < has)
-            return u;
-        u.skip -= has;
+    if (w.at >= w.end)
+        return false;
+    if (first || w.row0 == 0) { // (a sequence begins, or a head)
+        g.seq = kv_seq(a, w.sq);
+        while (kv_rows(a, g.seq) == 0) {
+            if (++w.sq >= a.n_seq) // (not while lengths stay as they were)
+                return false;
+            g.seq = kv_seq(a, w.sq);
+        }
     }
+    const uint32_t rows = g.seq.n * a.group;
+    g.first = first;
+    g.sq = w.sq;
+    g.head = w.head;
+    g.row0 = w.row0;
+    g.rows = min(tile, rows - w.row0);
+    g.blocks = kv_blocks(a, g.seq, g.row0, g.rows, each);
+    g.from = g.blocks.from + w.skip;
+    g.to = w.end - w.at < g.blocks.to - g.from ? g.from + (uint32_t)(w.end - w.at) : g.blocks.to;
+    w.at += g.to - g.from;
+    w.skip = 0;
+    w.row0 += tile;
+    if (w.row0 >= rows) {
+        w.row0 = 0;
+        if (++w.head == a.c.n_heads) {
+            w.head = 0;
+            ++w.sq;
+        }
+    }
+    return true;
 }
 
 // Quotients by the page size: x / page for any x below 2^31 (inverse: 2^(31 + shift) / page, rounded up, shift: ceil(log2(page))).

@@ -186,17 +186,6 @@ __device__ __forceinline__ uint32_t read_block(const Columns& c, uint32_t b, uin
     return there;
 }
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-    unsigned long long ra, rb, rd;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
-    float2 d;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
-    return d;
-}
-
 // A thread's logits of a tile. Those below `least`, -inf, NaN and what is masked are taken for it, before they become floats where two
 // of them are in a word: they weigh nothing then, and nothing times their exponent is not NaN, as long as the largest is far
 // enough above, and exponents are of a size at which a shift is rounded by less than 2^6 (reachable() below says whether they are; if not the
