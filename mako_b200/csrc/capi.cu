@@ -927,15 +927,18 @@ int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries
     a.query_start = q->query_start;
     a.kv_len = q->kv_len;
     a.parts = static_cast<float*>(q->workspace);
-    uint32_t bits = 0;
-    while ((1ull << bits) < cache->page_size)
-        ++bits;
-    a.page_shift = 31u + bits;
-    a.page_inverse = ((1ull << a.page_shift) + cache->page_size - 1u) / cache->page_size;
     a.n_seq = q->n_seq;
     a.n_tokens = q->n_tokens;
     a.max_new = q->max_new && q->max_new < q->n_tokens ? q->max_new : q->n_tokens;
     a.group = q->n_q_heads / cache->n_heads;
+    auto inverse = [](uint32_t n, uint64_t& by, uint32_t& shift) {
+        shift = 31u;
+        while ((1ull << (shift - 31u)) < n)
+            ++shift;
+        by = ((1ull << shift) + n - 1u) / n;
+    };
+    inverse(cache->page_size, a.page_inverse, a.page_shift);
+    inverse(a.group, a.group_inverse, a.group_shift);
     a.window = q->window;
     a.scale_log2 = (float)(q->scale * 1.4426950408889634);
     MK_CUDA(mk::launch_kv_attend(a, q->type, (cudaStream_t)stream));

@@ -92,10 +92,10 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSe
     for (uint32_t i = threadIdx.x; i < MT * 16u * chunks; i += kThreads) { // (whole warps: chunks divides 32)
         const uint32_t r = i / chunks, chunk = i % chunks, row = u.row0 + r;
         const bool real = r < u.rows;
+        const uint32_t token = kv_token_of(a, row);
         uint32_t w[8] = {};
         if (real) {
-            const uint64_t token = u.seq.first + row / a.group;
-            const T* p = static_cast<const T*>(a.q) + token * a.q_ld + (uint64_t)(u.head * a.group + row % a.group) * D + chunk * 16u;
+            const T* p = static_cast<const T*>(a.q) + (u.seq.first + token) * a.q_ld + (uint64_t)(u.head * a.group + row - token * a.group) * D + chunk * 16u;
             const uint4 x = __ldg(reinterpret_cast<const uint4*>(p)), y = __ldg(reinterpret_cast<const uint4*>(p) + 1);
             w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
         }
@@ -120,7 +120,7 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSe
             to[k * 128u + 2u] = pair_of(y.x * by, y.y * by);
         }
         if (chunk == 0) {
-            const int64_t at = (int64_t)u.seq.len - u.seq.n + row / a.group; // its position
+            const int64_t at = (int64_t)u.seq.len - u.seq.n + token; // its position
             s.factor[r] = a.scale_log2 / by;
             s.hi[r] = real && at >= 0 ? (int32_t)(at + 1 < u.seq.len ? at + 1 : u.seq.len) : 0;
             s.lo[r] = a.window && at + 1 > (int64_t)a.window ? (int32_t)(at + 1 - a.window) : 0;
@@ -128,7 +128,7 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSe
     }
 }
 
-// A warp's copies of blocks of keys and values.
+// A warp's copies of blocks of keys and values. 16 tokens are looked up at a time where pages are a multiple of that, else each by itself.
 template <uint32_t D>
 struct Copier {
     static constexpr uint32_t tokens = kBlockTokens<D>, row_chunks = D / 16, rows_each = 32 / row_chunks;
@@ -137,7 +137,8 @@ struct Copier {
     uint32_t* valid;              // a bit for each token of a stage's block: it is there
     const int32_t* table;
     uint32_t len, head;
-    int32_t page; // of this lane's token of the block that is next
+    bool wide;                    // is a page a multiple of 16 tokens?
+    int32_t page;                 // of this lane's token of the block that is next
 
     __device__ __forceinline__ void look_up(uint32_t block)
     {
@@ -149,26 +150,46 @@ struct Copier {
         const uint32_t lane = threadIdx.x & 31u, t = block * tokens + lane;
         unsigned char* to = ring + stage * kStageBytes;
         const bool there = (uint32_t)page < a->c.n_pages;
-        const uint64_t p = there ? (uint64_t)(uint32_t)page : 0ull;
-        const uint32_t place = there ? t - kv_page_of(*a, t) * a->c.page_size : 0u;
-        const uint64_t off = p * a->c.page_stride + (uint64_t)head * a->c.head_stride + (uint64_t)place * a->c.token_stride;
+        const uint32_t p = there ? (uint32_t)page : 0u;
         const uint32_t mask = __ballot_sync(~0u, there);
         float* scales = reinterpret_cast<float*>(to + 4096);
         if (lane < tokens) {
-            const uint64_t at = p * a->c.n_heads + head;
+            const uint64_t at = (uint64_t)p * a->c.n_heads + head;
             copy4(scales + lane, a->c.k_scale + at, there);
             copy4(scales + tokens + lane, a->c.v_scale + at, there);
         }
         if (lane == 0)
             valid[stage] = mask;
-        const uint32_t chunk = lane % row_chunks;
+        const uint32_t chunk = lane % row_chunks, row = lane / row_chunks;
+        const uint64_t stride = a->c.token_stride;
+        if (wide) {
 #pragma unroll
-        for (uint32_t i = 0; i < tokens / rows_each; ++i) {
-            const uint32_t r = i * rows_each + lane / row_chunks;
-            const uint64_t from = __shfl_sync(~0u, off, r) + chunk * 16u;
-            const bool ok = (mask >> r) & 1u;
-            copy16(to + key_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.k) + from, ok);
-            copy16(to + 2048 + value_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.v) + from, ok);
+            for (uint32_t h = 0; h < tokens / 16u; ++h) { // a page's part
+                const uint32_t first = block * tokens + 16u * h, its = __shfl_sync(~0u, p, 16u * h);
+                const uint64_t base = (uint64_t)its * a->c.page_stride + (uint64_t)head * a->c.head_stride + chunk * 16u +
+                                      (uint64_t)(first - kv_page_of(*a, first) * a->c.page_size + row) * stride;
+                const unsigned char *k = static_cast<const unsigned char*>(a->c.k) + base, *v = static_cast<const unsigned char*>(a->c.v) + base;
+#pragma unroll
+                for (uint32_t i = 0; i < 16u / rows_each; ++i) {
+                    const uint32_t r = 16u * h + i * rows_each + row;
+                    const bool ok = (mask >> r) & 1u;
+                    copy16(to + key_at<D>(r, chunk), k, ok);
+                    copy16(to + 2048 + value_at<D>(r, chunk), v, ok);
+                    k += rows_each * stride;
+                    v += rows_each * stride;
+                }
+            }
+        } else {
+            const uint32_t place = there ? t - kv_page_of(*a, t) * a->c.page_size : 0u;
+            const uint64_t off = (uint64_t)p * a->c.page_stride + (uint64_t)head * a->c.head_stride + (uint64_t)place * stride;
+#pragma unroll
+            for (uint32_t i = 0; i < tokens / rows_each; ++i) {
+                const uint32_t r = i * rows_each + row;
+                const uint64_t from = __shfl_sync(~0u, off, r) + chunk * 16u;
+                const bool ok = (mask >> r) & 1u;
+                copy16(to + key_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.k) + from, ok);
+                copy16(to + 2048 + value_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.v) + from, ok);
+            }
         }
     }
 };
@@ -177,7 +198,8 @@ struct Copier {
 template <uint32_t D, uint32_t MT>
 struct Running {
     float m[MT][2], l[MT][2], o[MT][D / 8][4];
-    float unit; // the largest scale of values so far
+    float factor[MT][2];
+    float unit, value_by; // the largest scale of values so far, and what makes weights of it
 };
 
 // Is one of four codes NaN? And the codes without those.
@@ -205,10 +227,10 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) {
                 const uint32_t y = i == 0 ? w[n].x : i == 1 ? w[n].y : i == 2 ? w[n].z : w[n].w;
-                const uint32_t b0 = halves_of(y & 0xffffu), b1 = halves_of(y >> 16);
+                const uint2 b = halves_of4(y);
 #pragma unroll
                 for (uint32_t mt = 0; mt < MT; ++mt)
-                    mma16(t[mt][n], q[mt], b0, b1);
+                    mma16(t[mt][n], q[mt], b.x, b.y);
             }
         }
     }
@@ -221,11 +243,10 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
         unit = fmaxf(unit, fmaxf(vs[n].x, vs[n].y));
 #pragma unroll
         for (uint32_t mt = 0; mt < MT; ++mt) {
-            const float f0 = s.factor[mt * 16u + g], f1 = s.factor[mt * 16u + g + 8u];
-            t[mt][n][0] *= ks.x * f0;
-            t[mt][n][1] *= ks.y * f0;
-            t[mt][n][2] *= ks.x * f1;
-            t[mt][n][3] *= ks.y * f1;
+            t[mt][n][0] *= ks.x * x.factor[mt][0];
+            t[mt][n][1] *= ks.y * x.factor[mt][0];
+            t[mt][n][2] *= ks.x * x.factor[mt][1];
+            t[mt][n][3] *= ks.y * x.factor[mt][1];
         }
     }
     unit = fmaxf(unit, __shfl_xor_sync(~0u, unit, 1));
@@ -245,9 +266,12 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
                     if (!sees(mt, n, e))
                         t[mt][n][e] = -INFINITY;
     }
-    const float value_by = unit > 0.0f ? kWeightUnit / unit : 0.0f;
-    const float older = x.unit == unit ? 1.0f : x.unit / unit;
-    x.unit = unit;
+    float older = 1.0f;
+    if (unit > x.unit) { // (in all lanes)
+        older = x.unit / unit;
+        x.unit = unit;
+        x.value_by = kWeightUnit / unit;
+    }
     uint4 p[MT][NT / 2];
     bool changed = older != 1.0f;
     float by[MT][2];
@@ -270,8 +294,8 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
             for (uint32_t n = 0; n < NT; ++n) {
                 const float a = ex2_approx(t[mt][n][2 * r] - from), b = ex2_approx(t[mt][n][2 * r + 1] - from);
                 l += a + b;
-                t[mt][n][2 * r] = a * (vs[n].x * value_by);
-                t[mt][n][2 * r + 1] = b * (vs[n].y * value_by);
+                t[mt][n][2 * r] = a * (vs[n].x * x.value_by);
+                t[mt][n][2 * r + 1] = b * (vs[n].y * x.value_by);
             }
             x.l[mt][r] = x.l[mt][r] * by[mt][r] + l;
             by[mt][r] *= older;
@@ -337,13 +361,11 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
 #pragma unroll
             for (uint32_t half = 0; half < 2; ++half) {
                 const uint32_t order = half ? 0x7362u : 0x5140u; // two tokens' codes of a column side by side
-                const uint32_t y0 = __byte_perm(w[0][j], w[1][j], order), y1 = __byte_perm(w[2][j], w[3][j], order);
+                const uint2 b0 = halves_of4(__byte_perm(w[0][j], w[1][j], order)), b1 = halves_of4(__byte_perm(w[2][j], w[3][j], order));
 #pragma unroll
-                for (uint32_t e = 0; e < 2; ++e) {
-                    const uint32_t b0 = halves_of(e ? y0 >> 16 : y0 & 0xffffu), b1 = halves_of(e ? y1 >> 16 : y1 & 0xffffu);
-#pragma unroll
-                    for (uint32_t mt = 0; mt < MT; ++mt)
-                        mma16(x.o[mt][4u * j + 2u * half + e], p[mt][k], b0, b1);
+                for (uint32_t mt = 0; mt < MT; ++mt) {
+                    mma16(x.o[mt][4u * j + 2u * half], p[mt][k], b0.x, b1.x);
+                    mma16(x.o[mt][4u * j + 2u * half + 1u], p[mt][k], b0.y, b1.y);
                 }
             }
         }
@@ -368,7 +390,8 @@ template <typename T, uint32_t D>
 __device__ __forceinline__ T* out_row(const KvAttendArgs& a, const KvSegment& u, uint32_t r)
 {
     const uint32_t row = u.row0 + r;
-    return static_cast<T*>(a.out) + (u.seq.first + row / a.group) * a.out_ld + (uint64_t)(u.head * a.group + row % a.group) * D;
+    const uint32_t token = kv_token_of(a, row);
+    return static_cast<T*>(a.out) + (u.seq.first + token) * a.out_ld + (uint64_t)(u.head * a.group + row - token * a.group) * D;
 }
 
 __device__ __forceinline__ float part_factor(float m, float most) { return m == -INFINITY ? 0.0f : ex2_approx(m - most); }
@@ -402,6 +425,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(cons
     copier.a = &a;
     copier.ring = raw + warp * kRingBytes;
     copier.valid = s.valid[warp];
+    copier.wide = a.c.page_size % 16u == 0;
     KvSegment u;
     for (bool first = true; kv_take(a, walk, u, first, tile, each); first = false) {
         const uint32_t from = u.from, to = u.to;
@@ -422,9 +446,11 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(cons
         __syncthreads();
         const uint32_t see_from = (uint32_t)s.lo[u.rows - 1u], see_to = (uint32_t)s.hi[0];
         Running<D, MT> x;
-        x.unit = 0.0f;
+        x.unit = x.value_by = 0.0f;
 #pragma unroll
         for (uint32_t mt = 0; mt < MT; ++mt) {
+            x.factor[mt][0] = s.factor[mt * 16u + g];
+            x.factor[mt][1] = s.factor[mt * 16u + g + 8u];
             x.m[mt][0] = x.m[mt][1] = -INFINITY;
             x.l[mt][0] = x.l[mt][1] = 0.0f;
 #pragma unroll
@@ -509,9 +535,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
 {
     __shared__ uint64_t scratch[40];
     __shared__ float s_factor[kJoinParts][16], s_by[16];
-    griddep_wait();
     const uint32_t cta = blockIdx.x + 1u, tid = threadIdx.x;
-    KvWalk walk = kv_find<kJoinThreads>(a, Tile, Each, ctas_most, scratch, cta);
+    KvWalk walk = kv_find<kJoinThreads>(a, Tile, Each, ctas_most, scratch, cta); // (from what was there before the units were begun)
+    griddep_wait(); // (by those that have nothing to do too: what follows waits for this launch)
     if (cta >= walk.ctas)
         return;
     const uint32_t skip = walk.skip, ctas = walk.ctas;
@@ -525,6 +551,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
     uint32_t parts = 1; // the first one's, and of those CTAs whose shares begin in the unit
     while (cta + parts - 1u < ctas && kv_cut(walk.total, ctas, cta + parts - 1u) < stop)
         ++parts;
+    auto join_row = [](uint32_t i) { return Tile > 32 ? i % 16u : i / (D / 4); };
+    auto join_column = [](uint32_t i) { return (Tile > 32 ? i / 16u : i % (D / 4)) * 4u; };
     auto part = [&](uint32_t p) { return a.parts + (uint64_t)(2u * (cta - 1u + p) + (p == 0 && before != start)) * floats; };
     for (uint32_t r0 = 16u * blockIdx.y; r0 < u.rows; r0 += 16u * gridDim.y) { // 16 rows at a time: their maxima, then what each part is worth, then the sums
         const uint32_t rows = min(16u, u.rows - r0);
@@ -555,11 +583,20 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
             __syncthreads();
 #pragma unroll
             for (uint32_t k = 0; k < 16 * (D / 4) / kJoinThreads; ++k) {
-                const uint32_t i = tid + k * kJoinThreads, r = i / (D / 4), d = i % (D / 4) * 4u;
+                const uint32_t i = tid + k * kJoinThreads, r = join_row(i), d = join_column(i);
                 if (r < rows) {
 #pragma unroll 4
-                    for (uint32_t p = 0; p < some; ++p)
-                        add4(o[k], *reinterpret_cast<const float4*>(part(p0 + p) + (r0 + r) * D + d), s_factor[p][r]);
+                    for (uint32_t p = 0; p < some; ++p) {
+                        const float* x = part(p0 + p);
+                        float4 y;
+                        if constexpr (Tile > 32) { // columns, as the threads that have a row each write them
+                            x += d * Tile + r0 + r;
+                            y = make_float4(x[0], x[Tile], x[2 * Tile], x[3 * Tile]);
+                        } else {
+                            y = *reinterpret_cast<const float4*>(x + (r0 + r) * D + d);
+                        }
+                        add4(o[k], y, s_factor[p][r]);
+                    }
                 }
             }
         }
@@ -572,7 +609,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
         __syncthreads();
 #pragma unroll
         for (uint32_t k = 0; k < 16 * (D / 4) / kJoinThreads; ++k) {
-            const uint32_t i = tid + k * kJoinThreads, r = i / (D / 4), d = i % (D / 4) * 4u;
+            const uint32_t i = tid + k * kJoinThreads, r = join_row(i), d = join_column(i);
             if (r < rows)
                 store4(out_row<T, D>(a, u, r0 + r) + d, over(o[k], s_by[r]));
         }

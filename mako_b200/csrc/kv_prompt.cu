@@ -367,7 +367,7 @@ struct Softmax {
         const uint32_t t = threadIdx.x / kTileRows, row = threadIdx.x, quarter = threadIdx.x / 32u % 4u;
         const uint32_t n = g.to - g.from, which = segments & 1u;
         // the row's queries, times a power of two that brings the largest to 2^12 (1 where a row is nothing or infinite)
-        const uint32_t unit_row = g.row0 + row, token = unit_row / a.group, head = g.head * a.group + (unit_row - token * a.group);
+        const uint32_t unit_row = g.row0 + row, token = kv_token_of(a, unit_row), head = g.head * a.group + (unit_row - token * a.group);
         const bool real = row < g.rows;
         float f;
         {
@@ -544,8 +544,8 @@ struct Softmax {
             tmem_read32(y, out + i);
             if (real && part) {
 #pragma unroll
-                for (uint32_t k = 0; k < 32; k += 4)
-                    *reinterpret_cast<float4*>(part + row * D + i + k) = make_float4(y[k] * by, y[k + 1] * by, y[k + 2] * by, y[k + 3] * by);
+                for (uint32_t k = 0; k < 32; ++k)
+                    part[(i + k) * kUnitRows + row] = y[k] * by; // (by column: lanes are rows)
             } else if (real) {
 #pragma unroll
                 for (uint32_t k = 0; k < 32; k += 8) {
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         Segment g;
         for (bool first = true; kv_take(a, walk, g, first, kUnitRows, kBlock); first = false) {
             const int32_t back = (int32_t)g.seq.len - (int32_t)g.seq.n;
-            const int32_t top = back + (int32_t)(g.row0 / a.group) + 1, last = back + (int32_t)((g.row0 + g.rows - 1u) / a.group) + 1;
+            const int32_t top = back + (int32_t)kv_token_of(a, g.row0) + 1, last = back + (int32_t)kv_token_of(a, g.row0 + g.rows - 1u) + 1;
             g.see_to = top < 0 ? 0u : (uint32_t)top;
             g.see_from = a.window && last > (int32_t)a.window ? (uint32_t)last - a.window : 0u;
             role(g, g.whole() ? nullptr : a.parts + (uint64_t)(2u * blockIdx.x + !first) * (kUnitRows * (D + 2u)));

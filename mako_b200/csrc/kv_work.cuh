@@ -8,6 +8,10 @@
 
 namespace mk {
 
+// Quotients of any x below 2^31 by the page size and the group: inverses are 2^(31 + b) / n, rounded up, 2^b being at least n.
+__device__ __forceinline__ uint32_t kv_page_of(const KvAttendArgs& a, uint32_t x) { return (uint32_t)(((uint64_t)x * a.page_inverse) >> a.page_shift); }
+__device__ __forceinline__ uint32_t kv_token_of(const KvAttendArgs& a, uint32_t row) { return (uint32_t)(((uint64_t)row * a.group_inverse) >> a.group_shift); }
+
 struct KvSeq {
     uint32_t first, n; // rows of the pass that are this sequence's tokens
     uint32_t len;      // keys
@@ -31,8 +35,8 @@ struct KvBlocks {
 __device__ __forceinline__ KvBlocks kv_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t row0, uint32_t rows, uint32_t each)
 {
     const int32_t back = (int32_t)q.len - (int32_t)q.n;                     // the position of the pass's first token
-    const int32_t end = back + (int32_t)((row0 + rows - 1u) / a.group) + 1; // (at most len)
-    const int32_t first = back + (int32_t)(row0 / a.group) + 1;
+    const int32_t end = back + (int32_t)(kv_token_of(a, row0 + rows - 1u)) + 1; // (at most len)
+    const int32_t first = back + (int32_t)kv_token_of(a, row0) + 1;
     const uint32_t lo = a.window && first > (int32_t)a.window ? (uint32_t)first - a.window : 0u;
     const uint32_t from = lo / each, to = end < 0 ? 0u : ((uint32_t)end + each - 1u) / each;
     return KvBlocks{from, to > from ? to : from + 1u};
@@ -218,8 +222,5 @@ __device__ __forceinline__ bool kv_take(const KvAttendArgs& a, KvWalk& w, KvSegm
     }
     return true;
 }
-
-// Quotients by the page size: x / page for any x below 2^31 (inverse: 2^(31 + shift) / page, rounded up, shift: ceil(log2(page))).
-__device__ __forceinline__ uint32_t kv_page_of(const KvAttendArgs& a, uint32_t x) { return (uint32_t)(((uint64_t)x * a.page_inverse) >> a.page_shift); }
 
 } // namespace mk

@@ -109,8 +109,8 @@ struct KvAttendArgs {
     uint64_t table_ld;
     const int32_t *query_start, *kv_len;
     float* parts;
-    uint64_t page_inverse;
-    uint32_t page_shift, table_cols, n_seq, n_tokens, max_new, group, window;
+    uint64_t page_inverse, group_inverse;
+    uint32_t page_shift, group_shift, table_cols, n_seq, n_tokens, max_new, group, window;
     float scale_log2;         // of a score, for exponents of two
     // which sequences a launch takes, by their rows (tokens of the pass times group), and the least blocks of a CTA; the launch sets them
     uint32_t rows_from, rows_to, blocks_least;
