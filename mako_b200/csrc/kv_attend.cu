@@ -18,13 +18,14 @@ namespace mk {
 namespace {
 
 constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
-constexpr uint32_t kStages = 4;
-constexpr uint32_t kStageBytes = 4096 + 256; // keys and values, two scales a token
-constexpr uint32_t kRingBytes = kStages * kStageBytes;
+constexpr uint32_t kStages = 2;
+constexpr uint32_t kTile = 16, kBlockTokens = 32; // rows of a unit, keys of a block
 constexpr float kWeightUnit = 128.0f;
 
 template <uint32_t D>
-constexpr uint32_t kBlockTokens = 2048 / D;
+constexpr uint32_t kStageBytes = 2 * kBlockTokens * (D + 4); // keys and values, two scales a token
+template <uint32_t D>
+constexpr uint32_t kRingBytes = kStages * kStageBytes<D>;
 
 __device__ __forceinline__ void copy16(void* to, const void* from, bool there)
 {
@@ -65,14 +66,14 @@ __device__ __forceinline__ uint32_t value_at(uint32_t token, uint32_t chunk)
                     : (token >> 1) * 128u + (((((token & 1u) << 2) + chunk) ^ ((token & 6u))) << 4);
 }
 
-template <uint32_t D, uint32_t MT>
+template <uint32_t D>
 struct Shared {
     uint64_t find[40];
-    float factor[16 * MT];               // of a row's scores
-    int32_t lo[16 * MT], hi[16 * MT];    // the keys that a row sees: [lo, hi)
-    float m[kWarps][16 * MT], l[kWarps][16 * MT];
+    float factor[kTile];               // of a row's scores
+    int32_t lo[kTile], hi[kTile];    // the keys that a row sees: [lo, hi)
+    float m[kWarps][kTile], l[kWarps][kTile];
     uint32_t valid[kWarps][kStages];
-    uint4 q[MT * (D / 16) * 32];         // queries in the order of the MMA's registers
+    uint4 q[D / 16 * 32];         // queries in the order of the MMA's registers
 };
 
 template <typename T>
@@ -85,11 +86,11 @@ __device__ __forceinline__ float2 two(uint32_t w)
 }
 
 // The unit's queries: a thread has 16 columns of a row.
-template <typename T, uint32_t D, uint32_t MT>
-__device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSegment& u)
+template <typename T, uint32_t D>
+__device__ void load_queries(const KvAttendArgs& a, Shared<D>& s, const KvSegment& u)
 {
     constexpr uint32_t chunks = D / 16;
-    for (uint32_t i = threadIdx.x; i < MT * 16u * chunks; i += kThreads) { // (whole warps: chunks divides 32)
+    for (uint32_t i = threadIdx.x; i < kTile * chunks; i += kThreads) { // (whole warps: chunks divides 32)
         const uint32_t r = i / chunks, chunk = i % chunks, row = u.row0 + r;
         const bool real = r < u.rows;
         const uint32_t token = kv_token_of(a, row);
@@ -112,7 +113,7 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSe
         const int e = (int)(__float_as_uint(most) >> 23) - 127;
         const int up = most > 0.0f && e < 128 ? max(-100, min(100, 12 - e)) : 0;
         const float by = __uint_as_float((uint32_t)(up + 127) << 23);
-        uint32_t* to = reinterpret_cast<uint32_t*>(s.q) + ((r / 16u * (D / 16u) + chunk / 4u * 4u) * 32u + (r & 7u) * 4u + (chunk & 3u)) * 4u + (r >> 3 & 1u);
+        uint32_t* to = reinterpret_cast<uint32_t*>(s.q) + (chunk / 4u * 128u + (r & 7u) * 4u + (chunk & 3u)) * 4u + (r >> 3);
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) { // a step of the contraction each
             const float2 x = two<T>(w[2 * k]), y = two<T>(w[2 * k + 1]);
@@ -131,33 +132,31 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D, MT>& s, const KvSe
 // A warp's copies of blocks of keys and values. 16 tokens are looked up at a time where pages are a multiple of that, else each by itself.
 template <uint32_t D>
 struct Copier {
-    static constexpr uint32_t tokens = kBlockTokens<D>, row_chunks = D / 16, rows_each = 32 / row_chunks;
+    static constexpr uint32_t tokens = kBlockTokens, row_chunks = D / 16, rows_each = 32 / row_chunks;
     const KvAttendArgs* a;
     unsigned char* ring;
     uint32_t* valid;              // a bit for each token of a stage's block: it is there
     const int32_t* table;
     uint32_t len, head;
     bool wide;                    // is a page a multiple of 16 tokens?
-    int32_t page;                 // of this lane's token of the block that is next
 
-    __device__ __forceinline__ void look_up(uint32_t block)
+    // The page of this lane's token of a block, early: what it is good for is issued when it is there.
+    __device__ __forceinline__ int32_t look_up(uint32_t block) const
     {
         const uint32_t t = block * tokens + (threadIdx.x & 31u);
-        page = (threadIdx.x & 31u) < tokens && t < len ? __ldg(table + kv_page_of(*a, t)) : -1;
+        return t < len ? __ldg(table + kv_page_of(*a, t)) : -1;
     }
-    __device__ __forceinline__ void issue(uint32_t block, uint32_t stage)
+    __device__ __forceinline__ void issue(uint32_t block, uint32_t stage, int32_t page) const
     {
         const uint32_t lane = threadIdx.x & 31u, t = block * tokens + lane;
-        unsigned char* to = ring + stage * kStageBytes;
+        unsigned char* to = ring + stage * kStageBytes<D>;
         const bool there = (uint32_t)page < a->c.n_pages;
         const uint32_t p = there ? (uint32_t)page : 0u;
         const uint32_t mask = __ballot_sync(~0u, there);
-        float* scales = reinterpret_cast<float*>(to + 4096);
-        if (lane < tokens) {
-            const uint64_t at = (uint64_t)p * a->c.n_heads + head;
-            copy4(scales + lane, a->c.k_scale + at, there);
-            copy4(scales + tokens + lane, a->c.v_scale + at, there);
-        }
+        float* scales = reinterpret_cast<float*>(to + 2 * tokens * D);
+        const uint64_t at = (uint64_t)p * a->c.n_heads + head;
+        copy4(scales + lane, a->c.k_scale + at, there);
+        copy4(scales + tokens + lane, a->c.v_scale + at, there);
         if (lane == 0)
             valid[stage] = mask;
         const uint32_t chunk = lane % row_chunks, row = lane / row_chunks;
@@ -174,7 +173,7 @@ struct Copier {
                     const uint32_t r = 16u * h + i * rows_each + row;
                     const bool ok = (mask >> r) & 1u;
                     copy16(to + key_at<D>(r, chunk), k, ok);
-                    copy16(to + 2048 + value_at<D>(r, chunk), v, ok);
+                    copy16(to + tokens * D + value_at<D>(r, chunk), v, ok);
                     k += rows_each * stride;
                     v += rows_each * stride;
                 }
@@ -188,30 +187,30 @@ struct Copier {
                 const uint64_t from = __shfl_sync(~0u, off, r) + chunk * 16u;
                 const bool ok = (mask >> r) & 1u;
                 copy16(to + key_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.k) + from, ok);
-                copy16(to + 2048 + value_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.v) + from, ok);
+                copy16(to + tokens * D + value_at<D>(r, chunk), static_cast<const unsigned char*>(a->c.v) + from, ok);
             }
         }
     }
 };
 
 // What a warp has of a unit: rows g and g + 8 of each tile (g: its lane / 4) and, of them, 2 * D / 8 columns.
-template <uint32_t D, uint32_t MT>
+template <uint32_t D>
 struct Running {
-    float m[MT][2], l[MT][2], o[MT][D / 8][4];
-    float factor[MT][2];
+    float m[2], l[2], o[D / 8][4];
+    float factor[2];
     float unit, value_by; // the largest scale of values so far, and what makes weights of it
 };
 
 // Is one of four codes NaN? And the codes without those.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
-template <uint32_t D, uint32_t MT>
-__device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>& s, const unsigned char* stage, uint32_t valid, uint32_t block, bool all_see)
+template <uint32_t D>
+__device__ __forceinline__ void add_block(Running<D>& x, const Shared<D>& s, const unsigned char* stage, uint32_t valid, uint32_t block, bool all_see)
 {
-    constexpr uint32_t tokens = kBlockTokens<D>, NT = tokens / 8, words = D / 32;
+    constexpr uint32_t tokens = kBlockTokens, NT = tokens / 8, words = D / 32;
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, c = lane & 3u;
-    const float* scales = reinterpret_cast<const float*>(stage + 4096);
-    float t[MT][NT][4] = {};
+    const float* scales = reinterpret_cast<const float*>(stage + 2 * tokens * D);
+    float t[NT][4] = {};
 #pragma unroll
     for (uint32_t h = 0; h < D / 64; ++h) {
         uint4 w[NT];
@@ -220,17 +219,11 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
             w[n] = *reinterpret_cast<const uint4*>(stage + key_at<D>(n * 8u + g, c + 4u * h));
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            uint4 q[MT];
-#pragma unroll
-            for (uint32_t mt = 0; mt < MT; ++mt)
-                q[mt] = s.q[(mt * (D / 16u) + h * 4u + i) * 32u + lane];
+            const uint4 q = s.q[(h * 4u + i) * 32u + lane];
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) {
-                const uint32_t y = i == 0 ? w[n].x : i == 1 ? w[n].y : i == 2 ? w[n].z : w[n].w;
-                const uint2 b = halves_of4(y);
-#pragma unroll
-                for (uint32_t mt = 0; mt < MT; ++mt)
-                    mma16(t[mt][n], q[mt], b.x, b.y);
+                const uint2 b = halves_of4(i == 0 ? w[n].x : i == 1 ? w[n].y : i == 2 ? w[n].z : w[n].w);
+                mma16(t[n], q, b.x, b.y);
             }
         }
     }
@@ -241,30 +234,25 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
         const float2 ks = *reinterpret_cast<const float2*>(scales + n * 8u + 2u * c);
         vs[n] = *reinterpret_cast<const float2*>(scales + tokens + n * 8u + 2u * c);
         unit = fmaxf(unit, fmaxf(vs[n].x, vs[n].y));
-#pragma unroll
-        for (uint32_t mt = 0; mt < MT; ++mt) {
-            t[mt][n][0] *= ks.x * x.factor[mt][0];
-            t[mt][n][1] *= ks.y * x.factor[mt][0];
-            t[mt][n][2] *= ks.x * x.factor[mt][1];
-            t[mt][n][3] *= ks.y * x.factor[mt][1];
-        }
+        t[n][0] *= ks.x * x.factor[0];
+        t[n][1] *= ks.y * x.factor[0];
+        t[n][2] *= ks.x * x.factor[1];
+        t[n][3] *= ks.y * x.factor[1];
     }
     unit = fmaxf(unit, __shfl_xor_sync(~0u, unit, 1));
     unit = fmaxf(unit, __shfl_xor_sync(~0u, unit, 2));
-    auto sees = [&](uint32_t mt, uint32_t n, uint32_t e) {
-        const uint32_t j = n * 8u + 2u * c + (e & 1u), r = mt * 16u + g + (e >> 1) * 8u;
+    auto sees = [&](uint32_t n, uint32_t e) {
+        const uint32_t j = n * 8u + 2u * c + (e & 1u), r = g + (e >> 1) * 8u;
         const int32_t key = (int32_t)(block * tokens + j);
         return ((valid >> j) & 1u) && key >= s.lo[r] && key < s.hi[r];
     };
     if (!all_see) {
 #pragma unroll
-        for (uint32_t mt = 0; mt < MT; ++mt)
+        for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
-            for (uint32_t n = 0; n < NT; ++n)
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e)
-                    if (!sees(mt, n, e))
-                        t[mt][n][e] = -INFINITY;
+            for (uint32_t e = 0; e < 4; ++e)
+                if (!sees(n, e))
+                    t[n][e] = -INFINITY;
     }
     float older = 1.0f;
     if (unit > x.unit) { // (in all lanes)
@@ -272,51 +260,45 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
         x.unit = unit;
         x.value_by = kWeightUnit / unit;
     }
-    uint4 p[MT][NT / 2];
+    uint4 p[NT / 2];
     bool changed = older != 1.0f;
-    float by[MT][2];
+    float by[2];
 #pragma unroll
-    for (uint32_t mt = 0; mt < MT; ++mt) {
+    for (uint32_t r = 0; r < 2; ++r) {
+        float m = x.m[r];
 #pragma unroll
-        for (uint32_t r = 0; r < 2; ++r) {
-            float m = x.m[mt][r];
+        for (uint32_t n = 0; n < NT; ++n)
+            m = fmaxf(m, fmaxf(t[n][2 * r], t[n][2 * r + 1]));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+        const float from = m == -INFINITY ? 0.0f : m;
+        by[r] = ex2_approx(x.m[r] - from);
+        changed = changed || m != x.m[r];
+        x.m[r] = m;
+        float l = 0.0f;
 #pragma unroll
-            for (uint32_t n = 0; n < NT; ++n)
-                m = fmaxf(m, fmaxf(t[mt][n][2 * r], t[mt][n][2 * r + 1]));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
-            const float from = m == -INFINITY ? 0.0f : m;
-            by[mt][r] = ex2_approx(x.m[mt][r] - from);
-            changed = changed || m != x.m[mt][r];
-            x.m[mt][r] = m;
-            float l = 0.0f;
-#pragma unroll
-            for (uint32_t n = 0; n < NT; ++n) {
-                const float a = ex2_approx(t[mt][n][2 * r] - from), b = ex2_approx(t[mt][n][2 * r + 1] - from);
-                l += a + b;
-                t[mt][n][2 * r] = a * (vs[n].x * x.value_by);
-                t[mt][n][2 * r + 1] = b * (vs[n].y * x.value_by);
-            }
-            x.l[mt][r] = x.l[mt][r] * by[mt][r] + l;
-            by[mt][r] *= older;
+        for (uint32_t n = 0; n < NT; ++n) {
+            const float a = ex2_approx(t[n][2 * r] - from), b = ex2_approx(t[n][2 * r + 1] - from);
+            l += a + b;
+            t[n][2 * r] = a * (vs[n].x * x.value_by);
+            t[n][2 * r + 1] = b * (vs[n].y * x.value_by);
         }
-#pragma unroll
-        for (uint32_t n = 0; n < NT; n += 2)
-            p[mt][n / 2] = make_uint4(pair_of(t[mt][n][0], t[mt][n][1]), pair_of(t[mt][n][2], t[mt][n][3]),
-                                      pair_of(t[mt][n + 1][0], t[mt][n + 1][1]), pair_of(t[mt][n + 1][2], t[mt][n + 1][3]));
+        x.l[r] = x.l[r] * by[r] + l;
+        by[r] *= older;
     }
+#pragma unroll
+    for (uint32_t n = 0; n < NT; n += 2)
+        p[n / 2] = make_uint4(pair_of(t[n][0], t[n][1]), pair_of(t[n][2], t[n][3]), pair_of(t[n + 1][0], t[n + 1][1]), pair_of(t[n + 1][2], t[n + 1][3]));
     if (__any_sync(~0u, changed)) {
 #pragma unroll
-        for (uint32_t mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (uint32_t j = 0; j < D / 8; ++j) {
-                x.o[mt][j][0] *= by[mt][0];
-                x.o[mt][j][1] *= by[mt][0];
-                x.o[mt][j][2] *= by[mt][1];
-                x.o[mt][j][3] *= by[mt][1];
-            }
+        for (uint32_t j = 0; j < D / 8; ++j) {
+            x.o[j][0] *= by[0];
+            x.o[j][1] *= by[0];
+            x.o[j][2] *= by[1];
+            x.o[j][3] *= by[1];
+        }
     }
-    const unsigned char* values = stage + 2048;
+    const unsigned char* values = stage + tokens * D;
 #pragma unroll
     for (uint32_t k = 0; k < NT / 2; ++k) {
         uint32_t w[4][words];
@@ -348,11 +330,9 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
                     for (uint32_t j = 0; j < words; ++j)
                         w[i][j] &= ~nan_bytes(w[i][j]);
 #pragma unroll
-                    for (uint32_t mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (uint32_t r = 0; r < 2; ++r)
-                            if ((bad >> i & 1u) && sees(mt, 2u * k + (i >> 1), 2u * r + (i & 1u)))
-                                x.l[mt][r] = __int_as_float(0x7fc00000);
+                    for (uint32_t r = 0; r < 2; ++r)
+                        if ((bad >> i & 1u) && sees(2u * k + (i >> 1), 2u * r + (i & 1u)))
+                            x.l[r] = __int_as_float(0x7fc00000);
                 }
             }
         }
@@ -362,11 +342,8 @@ __device__ __forceinline__ void add_block(Running<D, MT>& x, const Shared<D, MT>
             for (uint32_t half = 0; half < 2; ++half) {
                 const uint32_t order = half ? 0x7362u : 0x5140u; // two tokens' codes of a column side by side
                 const uint2 b0 = halves_of4(__byte_perm(w[0][j], w[1][j], order)), b1 = halves_of4(__byte_perm(w[2][j], w[3][j], order));
-#pragma unroll
-                for (uint32_t mt = 0; mt < MT; ++mt) {
-                    mma16(x.o[mt][4u * j + 2u * half], p[mt][k], b0.x, b1.x);
-                    mma16(x.o[mt][4u * j + 2u * half + 1u], p[mt][k], b0.y, b1.y);
-                }
+                mma16(x.o[4u * j + 2u * half], p[k], b0.x, b1.x);
+                mma16(x.o[4u * j + 2u * half + 1u], p[k], b0.y, b1.y);
             }
         }
     }
@@ -408,22 +385,22 @@ __device__ __forceinline__ float4 over(const float4& x, float l) // a row that s
     return make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
 }
 
-template <uint32_t D, uint32_t MT>
-constexpr uint32_t kPartFloats = MT * 16u * (D + 2u); // outputs, maxima, sums
+template <uint32_t D>
+constexpr uint32_t kPartFloats = kTile * (D + 2u); // outputs, maxima, sums
 
-template <typename T, uint32_t D, uint32_t MT>
-__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(const KvAttendArgs a)
+template <typename T, uint32_t D>
+__global__ void __launch_bounds__(kThreads, 3) kv_rows_kernel(const KvAttendArgs a)
 {
     extern __shared__ __align__(128) unsigned char raw[]; // the warps' rings; behind a segment, what they have of it
-    __shared__ Shared<D, MT> s;
-    constexpr uint32_t tile = 16u * MT, each = kBlockTokens<D>, row_floats = D + 4;
+    __shared__ Shared<D> s;
+    constexpr uint32_t tile = kTile, each = kBlockTokens, row_floats = D + 4;
     const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid & 31u, g = lane >> 2, c = lane & 3u;
     griddep_launch_dependents();
     griddep_wait();
     KvWalk walk = kv_find<kThreads>(a, tile, each, gridDim.x, s.find, blockIdx.x);
     Copier<D> copier;
     copier.a = &a;
-    copier.ring = raw + warp * kRingBytes;
+    copier.ring = raw + warp * kRingBytes<D>;
     copier.valid = s.valid[warp];
     copier.wide = a.c.page_size % 16u == 0;
     KvSegment u;
@@ -433,72 +410,70 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(cons
         copier.len = u.seq.len;
         copier.head = u.head;
         uint32_t next = from + warp;
-        copier.look_up(next);
+        int32_t pages[kStages];
+#pragma unroll
+        for (uint32_t i = 0; i < kStages; ++i)
+            pages[i] = next + i * kWarps < to ? copier.look_up(next + i * kWarps) : -1;
 #pragma unroll
         for (uint32_t i = 0; i + 1 < kStages; ++i, next += kWarps) {
-            if (next < to) {
-                copier.issue(next, i);
-                copier.look_up(next + kWarps);
-            }
+            if (next < to)
+                copier.issue(next, i, pages[i]);
             copies_close();
         }
-        load_queries<T, D, MT>(a, s, u);
+        int32_t page = pages[kStages - 1];
+        load_queries<T, D>(a, s, u);
         __syncthreads();
         const uint32_t see_from = (uint32_t)s.lo[u.rows - 1u], see_to = (uint32_t)s.hi[0];
-        Running<D, MT> x;
+        Running<D> x;
         x.unit = x.value_by = 0.0f;
 #pragma unroll
-        for (uint32_t mt = 0; mt < MT; ++mt) {
-            x.factor[mt][0] = s.factor[mt * 16u + g];
-            x.factor[mt][1] = s.factor[mt * 16u + g + 8u];
-            x.m[mt][0] = x.m[mt][1] = -INFINITY;
-            x.l[mt][0] = x.l[mt][1] = 0.0f;
-#pragma unroll
-            for (uint32_t j = 0; j < D / 8; ++j)
-                x.o[mt][j][0] = x.o[mt][j][1] = x.o[mt][j][2] = x.o[mt][j][3] = 0.0f;
+        for (uint32_t r = 0; r < 2; ++r) {
+            x.factor[r] = s.factor[g + 8u * r];
+            x.m[r] = -INFINITY;
+            x.l[r] = 0.0f;
         }
+#pragma unroll
+        for (uint32_t j = 0; j < D / 8; ++j)
+            x.o[j][0] = x.o[j][1] = x.o[j][2] = x.o[j][3] = 0.0f;
         uint32_t stage = 0;
         for (uint32_t block = from + warp; block < to; block += kWarps, next += kWarps) {
             if (next < to) {
-                copier.issue(next, stage == 0 ? kStages - 1u : stage - 1u);
-                copier.look_up(next + kWarps);
+                copier.issue(next, stage == 0 ? kStages - 1u : stage - 1u, page);
+                page = copier.look_up(next + kWarps);
             }
             copies_close();
             copies_wait<kStages - 1>();
             __syncwarp();
             const uint32_t valid = s.valid[warp][stage];
-            const bool all_see = valid == (each == 32u ? ~0u : (1u << each) - 1u) && block * each >= see_from && (block + 1u) * each <= see_to;
-            add_block<D, MT>(x, s, copier.ring + stage * kStageBytes, valid, block, all_see);
+            const bool all_see = valid == ~0u && block * each >= see_from && (block + 1u) * each <= see_to;
+            add_block<D>(x, s, copier.ring + stage * kStageBytes<D>, valid, block, all_see);
             __syncwarp();
             stage = stage + 1u == kStages ? 0u : stage + 1u;
         }
         copies_wait<0>();
         __syncthreads();
-        float* mine = reinterpret_cast<float*>(raw + warp * kRingBytes);
+        float* mine = reinterpret_cast<float*>(raw + warp * kRingBytes<D>);
+        const float worth = x.unit / kWeightUnit;
 #pragma unroll
-        for (uint32_t mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (uint32_t r = 0; r < 2; ++r) {
-                float l = x.l[mt][r];
-                l += __shfl_xor_sync(~0u, l, 1);
-                l += __shfl_xor_sync(~0u, l, 2);
-                const uint32_t row = mt * 16u + r * 8u + g;
-                if (c == 0) {
-                    s.m[warp][row] = x.m[mt][r];
-                    s.l[warp][row] = l;
-                }
-                const float by = x.unit / kWeightUnit;
-#pragma unroll
-                for (uint32_t e = 0; e < 2; ++e)
-#pragma unroll
-                    for (uint32_t j = 0; j < D / 8; j += 4)
-                        *reinterpret_cast<float4*>(mine + row * row_floats + (2u * c + e) * (D / 8) + j) =
-                            make_float4(x.o[mt][j][2 * r + e] * by, x.o[mt][j + 1][2 * r + e] * by, x.o[mt][j + 2][2 * r + e] * by,
-                                        x.o[mt][j + 3][2 * r + e] * by);
+        for (uint32_t r = 0; r < 2; ++r) {
+            float l = x.l[r];
+            l += __shfl_xor_sync(~0u, l, 1);
+            l += __shfl_xor_sync(~0u, l, 2);
+            const uint32_t row = r * 8u + g;
+            if (c == 0) {
+                s.m[warp][row] = x.m[r];
+                s.l[warp][row] = l;
             }
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e)
+#pragma unroll
+                for (uint32_t j = 0; j < D / 8; j += 4)
+                    *reinterpret_cast<float4*>(mine + row * row_floats + (2u * c + e) * (D / 8) + j) =
+                        make_float4(x.o[j][2 * r + e] * worth, x.o[j + 1][2 * r + e] * worth, x.o[j + 2][2 * r + e] * worth, x.o[j + 3][2 * r + e] * worth);
+        }
         __syncthreads();
         const bool whole = u.whole();
-        float* part = a.parts + (uint64_t)(2u * blockIdx.x + !u.first) * kPartFloats<D, MT>;
+        float* part = a.parts + (uint64_t)(2u * blockIdx.x + !u.first) * kPartFloats<D>;
         for (uint32_t i = tid; i < u.rows * (D / 4); i += kThreads) {
             const uint32_t r = i / (D / 4), d = i % (D / 4) * 4u;
             float most = s.m[0][r];
@@ -511,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) kv_rows_kernel(cons
             for (uint32_t w = 0; w < kWarps; ++w) {
                 const float f = part_factor(s.m[w][r], most);
                 l += s.l[w][r] * f;
-                add4(o, *reinterpret_cast<const float4*>(raw + w * kRingBytes + (r * row_floats + d) * 4u), f);
+                add4(o, *reinterpret_cast<const float4*>(raw + w * kRingBytes<D> + (r * row_floats + d) * 4u), f);
             }
             if (whole) {
                 store4(out_row<T, D>(a, u, r) + d, over(o, l));
@@ -617,8 +592,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
     }
 }
 
-constexpr uint32_t rows_ctas(uint32_t mt) { return 148u * (mt == 1 ? 3u : 2u); }
-constexpr uint64_t kv_rows_parts(uint32_t dim) { return (uint64_t)rows_ctas(2) * 2u * 32u * (dim + 2u) * 4u; } // bytes
+constexpr uint32_t kRowsCtas = 148u * 3u; // all of which run at the same time
+constexpr uint64_t kv_rows_parts(uint32_t dim) { return (uint64_t)kRowsCtas * 2u * kTile * (dim + 2u) * 4u; } // bytes
 
 template <typename T, uint32_t D, uint32_t Tile, uint32_t Each>
 cudaError_t launch_join(const KvAttendArgs& a, uint32_t ctas, cudaStream_t stream)
@@ -635,39 +610,34 @@ cudaError_t launch_join(const KvAttendArgs& a, uint32_t ctas, cudaStream_t strea
     return cudaLaunchKernelEx(&c, kv_join_kernel<T, D, Tile, Each>, a, ctas);
 }
 
-template <typename T, uint32_t D, uint32_t MT>
+template <typename T, uint32_t D>
 cudaError_t launch_rows(const KvAttendArgs& a, cudaStream_t stream)
 {
-    constexpr uint32_t smem = kWarps * kRingBytes, grid = rows_ctas(MT);
+    constexpr uint32_t smem = kWarps * kRingBytes<D>, grid = kRowsCtas;
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = set_once(done, kv_rows_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = set_once(done, kv_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess)
         return e;
-    kv_rows_kernel<T, D, MT><<<grid, kThreads, smem, stream>>>(a);
+    kv_rows_kernel<T, D><<<grid, kThreads, smem, stream>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess)
         return e;
-    return launch_join<T, D, 16u * MT, kBlockTokens<D>>(a, grid, stream);
+    return launch_join<T, D, kTile, kBlockTokens>(a, grid, stream);
 }
 
-// Sequences of up to so many rows go through kv_rows_kernel, in a pass of others too.
-constexpr uint32_t kFewRows = 16, kSomeRows = 32;
+// Sequences of up to so many rows go through kv_rows_kernel, in a pass with longer ones too.
+constexpr uint32_t kFewRows = 64;
 
 template <typename T, uint32_t D>
 cudaError_t launch(const KvAttendArgs& args, int type, cudaStream_t stream)
 {
     KvAttendArgs a = args;
-    const uint64_t most = (uint64_t)a.max_new * a.group;
+    const bool few = (uint64_t)a.max_new * a.group <= kFewRows;
     a.rows_from = 1;
-    a.rows_to = 0xffffffffu; // (max_new is what the caller says: where it is too small all the same rows are done)
-    a.blocks_least = 8;
-    if (most <= kFewRows)
-        return launch_rows<T, D, 1>(a, stream);
-    if (most <= kSomeRows)
-        return launch_rows<T, D, 2>(a, stream);
-    a.rows_to = kFewRows;
-    cudaError_t e = a.group <= kFewRows ? launch_rows<T, D, 1>(a, stream) : cudaSuccess;
-    if (e != cudaSuccess)
+    a.rows_to = few ? 0xffffffffu : kFewRows; // (max_new is what the caller says: where it is too small all the same rows are done)
+    a.blocks_least = 4;
+    cudaError_t e = launch_rows<T, D>(a, stream);
+    if (e != cudaSuccess || few)
         return e;
     a.parts = args.parts + kv_rows_parts(D) / 4u;
     a.rows_from = kFewRows + 1u;
@@ -681,7 +651,7 @@ cudaError_t launch(const KvAttendArgs& args, int type, cudaStream_t stream)
 
 uint64_t kv_attend_bytes(uint32_t dim, uint64_t most_rows)
 {
-    return kv_rows_parts(dim) + (most_rows > kSomeRows ? (uint64_t)kPromptCtas * 2u * kPromptRows * (dim + 2u) * 4u : 0u);
+    return kv_rows_parts(dim) + (most_rows > kFewRows ? (uint64_t)kPromptCtas * 2u * kPromptRows * (dim + 2u) * 4u : 0u);
 }
 
 cudaError_t launch_kv_attend(const KvAttendArgs& a, int type, cudaStream_t stream)
