@@ -58,6 +58,7 @@ struct Shared {
     Key list[kListCap];
     Key best[kLogprobMaxTop]; // in order; in the first CTA of a cluster everybody's
     Sums<float> warp[kWarps];
+    uint4 handed[kWarps][kTileVecs];
     float warp_most[kWarps];
     alignas(16) float largest[kThreads];
     Key ranked[kRankMax];
@@ -325,24 +326,16 @@ __device__ __forceinline__ void rank_by_warp(const Key* list, uint32_t n, uint32
     __syncwarp();
 }
 
-// Puts a block's logits above the line, or on it, into the list, as long as it has room.
+// Puts a block's logits above the line into the list.
 template <typename T>
-__device__ __forceinline__ void put(Shared& s, const Columns& c, uint32_t b, const uint32_t (&w)[4], float line, bool also)
+__device__ __forceinline__ void put(Shared& s, const Columns& c, uint32_t b, const uint32_t (&w)[4], float line)
 {
     constexpr uint32_t each = Words<T>::each;
-    uint32_t x0 = w[0], x1 = w[1], x2 = w[2], x3 = w[3];
-#pragma unroll 1
-    for (uint32_t i = 0; i < 4u * each; i += each) {
 #pragma unroll
-        for (uint32_t j = 0; j < each; ++j) {
-            const float x = Words<T>::value(x0, j);
-            if (x > line || (also && x == line && x > -INFINITY)) {
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < kListCap)
-                    s.list[at] = make_key(x, b * 4u * each - c.before + i + j);
-            }
-        }
-        x0 = x1, x1 = x2, x2 = x3;
+    for (uint32_t i = 0; i < 4u * each; ++i) {
+        const float x = Words<T>::value(w[i / each], i % each);
+        if (x > line)
+            s.list[atomicAdd(&s.n, 1u)] = make_key(x, b * 4u * each - c.before + i);
     }
 }
 
@@ -473,21 +466,26 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_kernel(const mk_logprob_r
         }
         const float line = key_to_float(line_key);
         // (the line may be a number of this list's own that came behind an equal one: those on it go in as well)
-        if (__any_sync(~0u, here >= line && here > -INFINITY)) {
-#pragma unroll 1
-            for (uint32_t j = 0; j < kTileVecs; ++j) { // (rolled up: it is rare, and instructions are fetched anew each time)
-                uint32_t x[4];
+        // A thread that has such a logit is rare: its blocks are handed to the warp, an element or less to each lane.
+        uint32_t who = __ballot_sync(~0u, here >= line && here > -INFINITY);
+        while (who) {
+            const uint32_t from = __ffs(who) - 1;
+            who &= who - 1u;
+            if (lane == from) {
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    x[i] = w[0][i];
-#pragma unroll
-                    for (uint32_t m = 1; m < kTileVecs; ++m)
-                        x[i] = j == m ? w[m][i] : x[i];
-                }
-                if (Words<T>::largest(Words<T>::larger(Words<T>::larger(x[0], x[1]), Words<T>::larger(x[2], x[3]))) >= line)
-                    put<T>(s, c, b0 + j * kThreads + tid, x, line, true);
-                __syncwarp();
+                for (uint32_t j = 0; j < kTileVecs; ++j)
+                    s.handed[tid / 32u][j] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
             }
+            __syncwarp();
+            if (lane < kTileVecs * N) {
+                const float x = (float)reinterpret_cast<const T*>(s.handed[tid / 32u])[lane];
+                if (x >= line && x > -INFINITY) {
+                    const uint32_t at = atomicAdd(&s.n, 1u);
+                    if (at < kListCap)
+                        s.list[at] = make_key(x, (b0 + lane / N * kThreads + tid - lane + from) * N - c.before + lane % N);
+                }
+            }
+            __syncwarp();
         }
         most = fmaxf(most, here);
         add<T, kTileVecs>(sums, w, scale, here);
@@ -522,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_kernel(const mk_logprob_r
             if (b < c.to) {
                 uint32_t w[4];
                 read_block<T, Mask>(c, b, w);
-                put<T>(s, c, b, w, line, false); // an equal one comes behind k that are as large
+                put<T>(s, c, b, w, line); // (an equal one comes behind k that are as large; a piece has room)
             }
             __syncthreads();
             const uint32_t now = s.n;
