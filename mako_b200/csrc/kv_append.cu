@@ -19,7 +19,7 @@ namespace mk {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kHeadsEach = 2;    // key heads of a CTA
+constexpr uint32_t kHeadsEach = 2;    // key heads of a CTA, which share the angles
 constexpr uint32_t kAngles = 4096;    // (cosine, sine) pairs kept for a run's tokens: 32 KB
 
 template <typename T>
@@ -124,6 +124,9 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
         const int64_t x = a.slots[t];
         return x < 0 || x >= n_slots ? -1 : x;
     };
+    // A thread has the same columns of all its rows. (Threads that make no whole row of items have none.)
+    const uint32_t j = tid % items, step = kThreads / items, row0 = tid / items < step ? tid / items : ~0u >> 1;
+    const Item turned = item_of(a, j);
     const uint32_t t_end = min(a.n_tokens, (blockIdx.x + 1u) * a.tokens_each);
     for (uint32_t t0 = blockIdx.x * a.tokens_each; t0 < t_end; ++t0) {
         const int64_t slot = slot_of(t0);
@@ -148,6 +151,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
         __syncthreads();
         const uint32_t len = s_len;
         const uint32_t chunk = half ? min(len, kAngles / half) : len; // tokens whose angles are kept at a time
+        uint32_t largest[2 * kHeadsEach] = {}; // of keys and values, by head
         for (int pass = 0; pass < 2; ++pass) {
             for (uint32_t i0 = 0; i0 < len; i0 += chunk) {
                 const uint32_t n = min(chunk, len - i0);
@@ -164,9 +168,9 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
                     __syncthreads();
                 }
                 // rows of a token: keys and values of these heads and, the first time, the queries that go with them
-                const uint32_t rows = 2u * heads + (pass == 0 ? heads * a.group : 0u);
-                for (uint32_t i = tid; i < n * rows * items; i += kThreads) {
-                    const uint32_t j = i % items, row = i / items % rows, t = i / items / rows;
+                const uint32_t rows = 2u * heads + (pass == 0 ? heads * a.group : 0u), all = n * rows;
+                uint32_t t = row0 / rows, row = row0 - t * rows;
+                for (uint32_t i = row0; i < all; i += step) {
                     const uint64_t token = t0 + i0 + t;
                     const bool query = row >= 2u * heads, value = !query && row >= heads;
                     const uint32_t head = query ? row - 2u * heads : value ? row - heads : row; // among the CTA's
@@ -175,32 +179,45 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
                         p = static_cast<const T*>(a.q) + token * a.q_ld + (uint64_t)(h0 * a.group + head) * a.c.dim;
                     else
                         p = static_cast<const T*>(value ? a.v : a.k) + token * (value ? a.v_ld : a.k_ld) + (uint64_t)(h0 + head) * a.c.dim;
-                    Item at = item_of(a, j);
-                    if (value)
-                        at = Item{16u * j, 16u * j + 8u, 0u, false};
+                    const Item at = value ? Item{16u * j, 16u * j + 8u, 0u, false} : turned;
                     float x[8], y[8];
                     load8f(x, p + at.a);
                     load8f(y, p + at.b);
                     if (at.turns)
                         turn(x, y, cs + t * half + at.freq, a.interleaved);
+                    const uint32_t which = value ? kHeadsEach + head : head;
                     if (query) {
                         T* to = static_cast<T*>(a.q_out) + token * a.q_out_ld + (uint64_t)(h0 * a.group + head) * a.c.dim;
                         store8f(to + at.a, x);
                         store8f(to + at.b, y);
                     } else if (pass == 0) {
-                        atomicMax(&s_most[value ? kHeadsEach + head : head], largest8(y, largest8(x, 0u)));
+                        const uint32_t m = largest8(y, largest8(x, 0u));
+#pragma unroll
+                        for (uint32_t k = 0; k < 2u * kHeadsEach; ++k)
+                            largest[k] = which == k ? max(largest[k], m) : largest[k];
                     } else {
-                        const uint32_t which = value ? kHeadsEach + head : head;
                         const float by = 1.0f / s_scale[which]; // a power of two
                         uint8_t* to = static_cast<uint8_t*>(value ? a.c.v : a.c.k) + page * a.c.page_stride + (uint64_t)(h0 + head) * a.c.head_stride +
                                       (uint64_t)(place + i0 + t) * a.c.token_stride;
                         *reinterpret_cast<uint2*>(to + at.a) = make_uint2(codes4(x, 0, by), codes4(x, 4, by));
                         *reinterpret_cast<uint2*>(to + at.b) = make_uint2(codes4(y, 0, by), codes4(y, 4, by));
                     }
+                    row += step;
+                    while (row >= rows) {
+                        row -= rows;
+                        ++t;
+                    }
                 }
             }
             if (pass)
                 break;
+            __syncwarp();
+#pragma unroll
+            for (uint32_t k = 0; k < 2u * kHeadsEach; ++k) {
+                const uint32_t m = __reduce_max_sync(~0u, largest[k]);
+                if (tid % 32u == 0 && m)
+                    atomicMax(&s_most[k], m);
+            }
             __syncthreads();
             if (tid < 2u * kHeadsEach && tid % kHeadsEach < heads) {
                 const bool value = tid >= kHeadsEach;
