@@ -16,8 +16,8 @@ namespace mk {
 namespace {
 
 constexpr uint32_t kTileRows = 128, kUnitRows = 256, kBlock = 128; // rows of a tile, of a unit; keys of a block
-constexpr uint32_t kThreads = 416; // of 128 registers each
-constexpr uint32_t kConvert = 256, kIssue = 384; // first thread of those that convert, and of the warp that issues
+constexpr uint32_t kThreads = 672;
+constexpr uint32_t kConvert = 512, kIssue = 640; // first thread of those that convert, and of the warp that issues
 constexpr uint32_t kSlots = 4;                   // of what softmax reads beside the scores
 constexpr float kWeightUnit = 128.0f;
 constexpr uint32_t kMixed = 8; // blocks of a segment that some rows see and others do not: at most 3 at either end
@@ -35,6 +35,7 @@ struct Shared {
     uint32_t mixed[2][kMixed][5];      // a block and which of its values are NaN
     uint64_t off[2][kBlock];
     float warp_most[4];
+    float top[2][kUnitRows], most[2][kUnitRows], sum[2][kUnitRows]; // what the two threads of a row tell one another
 };
 
 __device__ __forceinline__ bool await(Shared& s, uint64_t* bar, uint32_t parity)
@@ -80,18 +81,6 @@ __device__ __forceinline__ void tmem_read32(float* x, uint32_t at)
         "%29, %30, %31}, [%32];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
         : MK_R8(x, 0), MK_R8(x, 8), MK_R8(x, 16), MK_R8(x, 24)
-        : "r"(at)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_read64(float* x, uint32_t at)
-{
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
-        "%29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, "
-        "%56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : MK_R8(x, 0), MK_R8(x, 8), MK_R8(x, 16), MK_R8(x, 24), MK_R8(x, 32), MK_R8(x, 40), MK_R8(x, 48), MK_R8(x, 56)
         : "r"(at)
         : "memory");
 }
@@ -148,48 +137,69 @@ struct Ring { // shared memory
 template <typename T, uint32_t D>
 struct Converter {
     // a load is 16 codes: of 32 rows, 64 columns. (Eight lanes have two rows' quarters: their stores are in different banks.)
-    static constexpr uint32_t halves = D / 64, loads = kBlock / 32 * halves;
-    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return i / halves * 32u + (threadIdx.x - kConvert) / 4u; }
+    // Half of a tile at a time, so that three halves under way fit into registers.
+    static constexpr uint32_t halves = D / 64, loads = kBlock / 64 * halves;
+    static __device__ __forceinline__ uint32_t row_of(uint32_t part, uint32_t i) { return 64u * part + i / halves * 32u + (threadIdx.x - kConvert) / 4u; }
     static __device__ __forceinline__ uint32_t chunk_of(uint32_t i) { return i % halves * 4u + (threadIdx.x & 3u); }
     uint32_t blocks = 0;   // so far
     uint32_t segments = 0;
     bool alive = true;
 
-    // The place of this thread's token of a block (all ones: not there), and its scales.
+    // The page of this thread's token of a block (all ones: not there), two blocks ahead; the token's place in it and its scales, one ahead:
+    // each is there when the next one is read with it.
+    __device__ __forceinline__ uint32_t look_up(const KvAttendArgs& a, const Segment& g, const int32_t* table, uint32_t block)
+    {
+        const uint32_t t = block * kBlock + (threadIdx.x - kConvert);
+        return block < g.to && t < g.seq.len ? (uint32_t)__ldg(table + kv_page_of(a, t)) : ~0u;
+    }
     struct Place {
         uint64_t off;
         float key, value;
     };
-    __device__ __forceinline__ Place place(const KvAttendArgs& a, const Segment& g, const int32_t* table, uint32_t block)
+    __device__ __forceinline__ Place place(const KvAttendArgs& a, const Segment& g, uint32_t page, uint32_t block)
     {
-        const uint32_t t = block * kBlock + (threadIdx.x - kConvert);
         Place p{~0ull, 0.0f, 0.0f};
-        if (t < g.seq.len) {
-            const uint32_t index = kv_page_of(a, t), page = (uint32_t)__ldg(table + index);
-            if (page < a.c.n_pages) {
-                p.off = page * a.c.page_stride + (uint64_t)g.head * a.c.head_stride + (uint64_t)(t - index * a.c.page_size) * a.c.token_stride;
-                p.key = __ldg(a.c.k_scale + (uint64_t)page * a.c.n_heads + g.head);
-                p.value = __ldg(a.c.v_scale + (uint64_t)page * a.c.n_heads + g.head);
-            }
+        if (page < a.c.n_pages) {
+            const uint32_t t = block * kBlock + (threadIdx.x - kConvert), in_page = t - kv_page_of(a, t) * a.c.page_size;
+            p.off = page * a.c.page_stride + (uint64_t)g.head * a.c.head_stride + (uint64_t)in_page * a.c.token_stride;
+            p.key = __ldg(a.c.k_scale + (uint64_t)page * a.c.n_heads + g.head);
+            p.value = __ldg(a.c.v_scale + (uint64_t)page * a.c.n_heads + g.head);
         }
         return p;
     }
 
-    __device__ __forceinline__ void load(uint4 (&x)[loads], const void* codes, const uint64_t* off)
+    __device__ __forceinline__ void load(uint4 (&x)[loads], const void* codes, const uint64_t* off, uint32_t part)
     {
 #pragma unroll
         for (uint32_t i = 0; i < loads; ++i) {
-            const uint64_t from = off[row_of(i)];
+            const uint64_t from = off[row_of(part, i)];
             x[i] = from != ~0ull ? __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(codes) + from + chunk_of(i) * 16u)) : make_uint4(0, 0, 0, 0);
         }
     }
-    __device__ __forceinline__ void store(const uint4 (&x)[loads], unsigned char* tile)
+    __device__ __forceinline__ void store(const uint4 (&x)[loads], unsigned char* tile, uint32_t part)
     {
 #pragma unroll
         for (uint32_t i = 0; i < loads; ++i) {
             const uint2 y0 = halves_of4(x[i].x), y1 = halves_of4(x[i].y), y2 = halves_of4(x[i].z), y3 = halves_of4(x[i].w);
-            *reinterpret_cast<uint4*>(tile + tile_at(row_of(i), 2u * chunk_of(i))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
-            *reinterpret_cast<uint4*>(tile + tile_at(row_of(i), 2u * chunk_of(i) + 1u)) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+            *reinterpret_cast<uint4*>(tile + tile_at(row_of(part, i), 2u * chunk_of(i))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+            *reinterpret_cast<uint4*>(tile + tile_at(row_of(part, i), 2u * chunk_of(i) + 1u)) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+        }
+    }
+    // Takes values that are NaN out, and says whose they are.
+    __device__ __forceinline__ void take_out(uint4 (&x)[loads], uint32_t part, uint32_t* whose)
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < loads; ++i) {
+            uint32_t* w[4] = {&x[i].x, &x[i].y, &x[i].z, &x[i].w};
+            uint32_t bad = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t nan = __vcmpeq4(*w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                *w[k] &= ~nan;
+                bad |= nan;
+            }
+            if (bad)
+                atomicOr(whose + row_of(part, i) / 32u, 1u << (row_of(part, i) & 31u));
         }
     }
 
@@ -198,18 +208,24 @@ struct Converter {
         const uint32_t tid = threadIdx.x - kConvert, lane = tid & 31u;
         const int32_t* table = a.block_table + (uint64_t)g.sq * a.table_ld;
         float unit = 0.0f;
-        Place p = place(a, g, table, g.from);
+        Place p = place(a, g, look_up(a, g, table, g.from), g.from);
+        uint32_t page = look_up(a, g, table, g.from + 1u);
         if (tid == 0)
             s.n_mixed[segments & 1u] = 0; // (that of the segment before the last one has been read: its successor's softmax has begun)
         ++segments;
         s.off[blocks & 1u][tid] = p.off;
         __syncwarp();
         named_barrier(2, 128);
-        uint4 k[loads], v[loads];
-        load(k, a.c.k, s.off[blocks & 1u]);
+        uint4 k0[loads], k1[loads], v[loads];
+        load(k0, a.c.k, s.off[blocks & 1u], 0);
+        load(k1, a.c.k, s.off[blocks & 1u], 1);
         for (uint32_t b = g.from; b < g.to; ++b, ++blocks) {
             const uint32_t stage = blocks & 1u, parity = (blocks >> 1) & 1u, slot = blocks % kSlots;
-            load(v, a.c.v, s.off[stage]);
+            load(v, a.c.v, s.off[stage], 0);
+            const bool more = b + 1u < g.to;
+            const Place next = place(a, g, page, b + 1u);
+            page = look_up(a, g, table, b + 2u);
+            s.off[stage ^ 1u][tid] = next.off;
             // what the softmax wants to know of the block
             float most = p.off != ~0ull ? p.value : 0.0f;
 #pragma unroll
@@ -230,14 +246,12 @@ struct Converter {
             if (tid == 0)
                 s.older[slot] = now > 0.0f ? unit / now : 1.0f;
             unit = now;
-            store(k, ring.k(stage));
-            const bool more = b + 1u < g.to;
-            if (more) {
-                p = place(a, g, table, b + 1u);
-                s.off[stage ^ 1u][tid] = p.off;
-            } else if (tid == 0) {
+            store(k0, ring.k(stage), 0);
+            load(k0, a.c.v, s.off[stage], 1); // the second half of the values takes the keys' registers
+            store(k1, ring.k(stage), 1);
+            if (!more && tid == 0)
                 s.unit[(segments - 1u) & 1u] = unit;
-            }
+            p = next;
             fence_proxy_async();
             __syncwarp();
             named_barrier(2, 128);
@@ -245,18 +259,8 @@ struct Converter {
                 mbar_arrive(&s.k_full[stage]);
             __syncwarp();
             if (more)
-                load(k, a.c.k, s.off[stage ^ 1u]);
+                load(k1, a.c.k, s.off[stage ^ 1u], 1);
             if (b * kBlock < g.see_from || (b + 1u) * kBlock > g.see_to) { // some rows see what others do not
-                uint32_t bad[loads], any = 0;
-#pragma unroll
-                for (uint32_t i = 0; i < loads; ++i) {
-                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                    bad[i] = 0;
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j)
-                        bad[i] |= __vcmpeq4(w[j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                    any |= bad[i];
-                }
                 const uint32_t which = s.n_mixed[(segments - 1u) & 1u];
                 uint32_t* at = s.mixed[(segments - 1u) & 1u][which < kMixed ? which : kMixed - 1u];
                 __syncwarp();
@@ -267,21 +271,16 @@ struct Converter {
                     s.n_mixed[(segments - 1u) & 1u] = which < kMixed ? which + 1u : kMixed;
                 __syncwarp();
                 named_barrier(2, 128);
-                if (any)
-#pragma unroll
-                    for (uint32_t i = 0; i < loads; ++i)
-                        if (bad[i]) {
-                            const uint32_t row = row_of(i);
-                            atomicOr(at + 1u + row / 32u, 1u << (row & 31u));
-                            v[i].x &= ~__vcmpeq4(v[i].x & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                            v[i].y &= ~__vcmpeq4(v[i].y & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                            v[i].z &= ~__vcmpeq4(v[i].z & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                            v[i].w &= ~__vcmpeq4(v[i].w & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                        }
+                take_out(v, 0, at + 1);
+                take_out(k0, 1, at + 1);
+                __syncwarp();
             }
             alive = alive && await(s, &s.v_empty[stage], parity ^ 1u);
             __syncwarp();
-            store(v, ring.v(stage));
+            store(v, ring.v(stage), 0);
+            store(k0, ring.v(stage), 1);
+            if (more)
+                load(k0, a.c.k, s.off[stage ^ 1u], 0);
             fence_proxy_async();
             __syncwarp();
             named_barrier(2, 128);
@@ -336,7 +335,7 @@ struct Issuer {
                 const uint64_t b = smem_rows_desc(ring.v(stage), 16384u);
 #pragma unroll
                 for (uint32_t k = 0; k < kBlock / 16; ++k)
-                    mma_weights(s.tmem + 256u + t * 128u, s.tmem + t * 128u + k * 8u, b + k * (2048u >> 4), desc, j || k);
+                    mma_weights(s.tmem + 256u + t * 128u, s.tmem + t * 128u + k / 4u * 64u + k % 4u * 8u, b + k * (2048u >> 4), desc, j || k);
                 if (j + 1u < n) {
                     if (t == 0 && !(alive = await(s, &s.k_full[next & 1u], (next >> 1) & 1u)))
                         return;
@@ -356,29 +355,34 @@ struct Issuer {
     }
 };
 
-// Those that turn scores into weights: a row each.
-template <typename T, uint32_t D>
+// Those that turn scores into weights: two threads a row, of half of a block's keys, and of a row's columns, each. They are in different
+// warps (a warp has access to 32 rows of tensor memory), so that four warps of each scheduler have scores under way. Group: keys, side by
+// side, that have one scale: 16 where pages are a multiple of that, else 1. Reading a scale for each key from shared memory takes as much of
+// it as the products' operands do.
+template <typename T, uint32_t D, uint32_t Group>
 struct Softmax {
     uint32_t blocks = 0, segments = 0, seen = 0, outputs = 0; // blocks so far of all segments, and of this tile's
     bool alive = true;
 
     __device__ __forceinline__ void run(const KvAttendArgs& a, Shared& s, const Ring<D>& ring, const Segment& g, float* part)
     {
-        const uint32_t t = threadIdx.x / kTileRows, row = threadIdx.x, quarter = threadIdx.x / 32u % 4u;
+        constexpr uint32_t columns = D / 2;
+        const uint32_t warp = threadIdx.x / 32u, t = warp / 8u, half = warp / 4u % 2u, quarter = warp % 4u;
+        const uint32_t row = t * kTileRows + quarter * 32u + (threadIdx.x & 31u), pair = 3u + t * 4u + quarter;
         const uint32_t n = g.to - g.from, which = segments & 1u;
         // the row's queries, times a power of two that brings the largest to 2^12 (1 where a row is nothing or infinite)
         const uint32_t unit_row = g.row0 + row, token = kv_token_of(a, unit_row), head = g.head * a.group + (unit_row - token * a.group);
         const bool real = row < g.rows;
         float f;
         {
-            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.seq.first + token) * a.q_ld + (uint64_t)head * D);
-            uint4 q[D / 8];
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.seq.first + token) * a.q_ld + (uint64_t)head * D + half * columns);
+            uint4 q[columns / 8];
 #pragma unroll
-            for (uint32_t i = 0; i < D / 8; ++i)
+            for (uint32_t i = 0; i < columns / 8; ++i)
                 q[i] = real ? __ldg(p + i) : make_uint4(0, 0, 0, 0);
             float top = 0.0f;
 #pragma unroll
-            for (uint32_t i = 0; i < D / 8; ++i) {
+            for (uint32_t i = 0; i < columns / 8; ++i) {
                 const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -386,6 +390,10 @@ struct Softmax {
                     top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
                 }
             }
+            s.top[half][row] = top;
+            __syncwarp();
+            named_barrier(pair, 64);
+            top = fmaxf(top, s.top[half ^ 1u][row]);
             const int e = (int)(__float_as_uint(top) >> 23) - 127;
             const int up = top > 0.0f && e < 128 ? max(-100, min(100, 12 - e)) : 0;
             const float by = __uint_as_float((uint32_t)(up + 127) << 23), turned = a.scale_log2 < 0.0f ? -by : by;
@@ -394,7 +402,7 @@ struct Softmax {
             ++segments;
             unsigned char* tile = ring.q(t);
 #pragma unroll
-            for (uint32_t i = 0; i < D / 8; ++i) {
+            for (uint32_t i = 0; i < columns / 8; ++i) {
                 const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
                 uint32_t y[4];
 #pragma unroll
@@ -402,7 +410,7 @@ struct Softmax {
                     const float2 x = two<T>(w[k]);
                     y[k] = pair_of(x.x * turned, x.y * turned);
                 }
-                *reinterpret_cast<uint4*>(tile + tile_at(row % kTileRows, i)) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(tile + tile_at(row % kTileRows, half * (columns / 8) + i)) = make_uint4(y[0], y[1], y[2], y[3]);
             }
             fence_proxy_async();
             mbar_arrive(&s.q_full);
@@ -414,56 +422,59 @@ struct Softmax {
         __syncwarp();
         if (t && g.rows <= kTileRows)
             return;
-        const uint32_t lanes = (quarter * 32u) << 16, scores = s.tmem + lanes + t * 128u, out = s.tmem + lanes + 256u + t * 128u;
+        const uint32_t lanes = (quarter * 32u) << 16, scores = s.tmem + lanes + t * 128u + half * 64u, out = s.tmem + lanes + 256u + t * 128u + half * columns;
         float ref = -INFINITY, l = 0.0f;
         for (uint32_t j = 0; j < n; ++j, ++seen) {
             const uint32_t slot = (first + j) % kSlots, begin = (g.from + j) * kBlock;
             alive = alive && await(s, &s.s_full[t], seen & 1u);
-            __syncwarp();
-            if (__any_sync(~0u, !alive)) { // (others of the CTA wait for nothing of this warp any more either)
-                alive = false;
-                return;
-            }
+            __syncwarp(); // (a warp that gave up goes on: its row's other thread meets it at barriers)
             tc_fence_after();
-            const float4 *key = reinterpret_cast<const float4*>(s.key[slot]), *value = reinterpret_cast<const float4*>(s.value[slot]);
-            const uint4 gone = *reinterpret_cast<const uint4*>(s.missing[slot]);
-            const int32_t low = lo - (int32_t)begin, high = hi - (int32_t)begin;
-            const bool some = __any_sync(~0u, (gone.x | gone.y | gone.z | gone.w) != 0 || low > 0 || high < (int32_t)kBlock);
-            // Half of a row's scores, times the keys' scales; -inf where it does not see the key. (A thread has registers for half of them: the
-            // second half is read twice, for the largest and once the first half's weights are made.)
-            auto read = [&](float (&x)[64], uint32_t half) {
-                tmem_read64(x, scores + 64u * half);
+            const float *key = s.key[slot] + 64u * half, *value = s.value[slot] + 64u * half;
+            const uint2 gone = *reinterpret_cast<const uint2*>(&s.missing[slot][2u * half]);
+            const int32_t low = lo - (int32_t)(begin + 64u * half), high = hi - (int32_t)(begin + 64u * half);
+            const bool some = __any_sync(~0u, (gone.x | gone.y) != 0 || low > 0 || high < 64);
+            // 32 of the row's scores, times the keys' scales where those are not taken in with f; -inf where it does not see the key. (They are
+            // read twice, for the largest first: registers for them are not worth having half as many warps.)
+            auto read = [&](float (&x)[32], uint32_t i) {
+                tmem_read32(x, scores + 32u * i);
+                if constexpr (Group == 1) {
 #pragma unroll
-                for (uint32_t i = 0; i < 64; i += 4) {
-                    const float4 c = key[16u * half + i / 4];
-                    const float2 y = mul2(make_float2(x[i], x[i + 1]), make_float2(c.x, c.y)), z = mul2(make_float2(x[i + 2], x[i + 3]), make_float2(c.z, c.w));
-                    x[i] = y.x, x[i + 1] = y.y, x[i + 2] = z.x, x[i + 3] = z.y;
-                }
-                if (some) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 2; ++i) {
-                        const int32_t from = low - 64 * (int32_t)half - 32 * (int32_t)i, to = high - 64 * (int32_t)half - 32 * (int32_t)i;
-                        // the places [from, to) of 32
-                        const uint32_t behind = to <= 0 ? 0u : to >= 32 ? ~0u : (1u << to) - 1u;
-                        const uint32_t before = from <= 0 ? 0u : from >= 32 ? ~0u : (1u << from) - 1u;
-                        const uint32_t sees = behind & ~before & ~(half ? (i ? gone.w : gone.z) : (i ? gone.y : gone.x));
-#pragma unroll
-                        for (uint32_t k = 0; k < 32; ++k)
-                            x[32 * i + k] = (sees >> k) & 1u ? x[32 * i + k] : -INFINITY;
+                    for (uint32_t k = 0; k < 32; k += 4) {
+                        const float4 c = reinterpret_cast<const float4*>(key)[8u * i + k / 4];
+                        const float2 y = mul2(make_float2(x[k], x[k + 1]), make_float2(c.x, c.y)), z = mul2(make_float2(x[k + 2], x[k + 3]), make_float2(c.z, c.w));
+                        x[k] = y.x, x[k + 1] = y.y, x[k + 2] = z.x, x[k + 3] = z.y;
                     }
                 }
+                if (some) {
+                    const int32_t from = low - 32 * (int32_t)i, to = high - 32 * (int32_t)i;
+                    // the places [from, to) of 32
+                    const uint32_t behind = to <= 0 ? 0u : to >= 32 ? ~0u : (1u << to) - 1u, before = from <= 0 ? 0u : from >= 32 ? ~0u : (1u << from) - 1u;
+                    const uint32_t sees = behind & ~before & ~(i ? gone.y : gone.x);
+#pragma unroll
+                    for (uint32_t k = 0; k < 32; ++k)
+                        x[k] = (sees >> k) & 1u ? x[k] : -INFINITY;
+                }
             };
-            float x[64], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // what makes exponents of 16 scores (not 0, as f)
+            auto factor = [&](uint32_t i) { return Group == 1 ? f : fmaxf(f * key[i], 1e-37f); };
+            float most = -INFINITY;
 #pragma unroll
-            for (int half = 1; half >= 0; --half) {
-                read(x, half);
+            for (uint32_t i = 0; i < 2; ++i) {
+                float x[32];
+                read(x, i);
 #pragma unroll
-                for (uint32_t i = 0; i < 64; i += 8)
+                for (uint32_t k = 0; k < 32; k += 16) {
+                    float tops[4];
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)
-                        tops[k] = fmaxf(tops[k], fmaxf(x[i + k], x[i + k + 4]));
+                    for (uint32_t m = 0; m < 4; ++m)
+                        tops[m] = fmaxf(fmaxf(x[k + m], x[k + m + 4]), fmaxf(x[k + m + 8], x[k + m + 12]));
+                    most = fmaxf(most, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * factor(32u * i + k));
+                }
             }
-            const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * f;
+            s.most[half][row] = most;
+            __syncwarp();
+            named_barrier(pair, 64);
+            most = fmaxf(most, s.most[half ^ 1u][row]);
             const float older = s.older[slot];
             float by = older;
             if (most > ref + 8.0f || ref == -INFINITY) { // (-inf: nothing seen yet; its outputs and sum are zeros)
@@ -475,7 +486,7 @@ struct Softmax {
             __syncwarp();
             if (j && __any_sync(~0u, by != 1.0f)) {
 #pragma unroll 1
-                for (uint32_t i = 0; i < D; i += 32) {
+                for (uint32_t i = 0; i < columns; i += 32) {
                     float y[32];
                     tmem_read32(y, out + i);
                     uint32_t z[32];
@@ -486,28 +497,28 @@ struct Softmax {
                 }
             }
             const float from = ref == -INFINITY ? 0.0f : ref;
-            const float2 f2 = make_float2(f, f), minus = make_float2(-from, -from);
+            const float2 minus = make_float2(-from, -from);
             float2 sum = make_float2(0.0f, 0.0f), more = sum;
 #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {
-                if (half)
-                    read(x, 1u);
+            for (uint32_t i = 0; i < 2; ++i) {
+                float x[32];
+                read(x, i);
+                uint32_t w[16];
 #pragma unroll
-                for (uint32_t i0 = 0; i0 < 64; i0 += 32) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (uint32_t i = i0; i < i0 + 32; i += 4) {
-                        const float4 c = value[16u * half + i / 4];
-                        const float2 d = fma2(make_float2(x[i], x[i + 1]), f2, minus), e = fma2(make_float2(x[i + 2], x[i + 3]), f2, minus);
-                        const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y)), q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                        sum = add2(sum, p);
-                        more = add2(more, q);
-                        const float2 y = mul2(p, make_float2(c.x, c.y)), z = mul2(q, make_float2(c.z, c.w));
-                        w[(i - i0) / 2] = pair_of(y.x, y.y);
-                        w[(i - i0) / 2 + 1] = pair_of(z.x, z.y);
-                    }
-                    tmem_write16(scores + 32u * half + i0 / 2, w); // (over the first half's scores, which have been read)
+                for (uint32_t k = 0; k < 32; k += 4) {
+                    const float by_f = factor(32u * i + k / 16u * 16u);
+                    const float4 c = Group == 1 ? reinterpret_cast<const float4*>(value)[8u * i + k / 4] : make_float4(value[32u * i + k / 16u * 16u], 0.0f, 0.0f, 0.0f);
+                    const float2 c0 = Group == 1 ? make_float2(c.x, c.y) : make_float2(c.x, c.x), c1 = Group == 1 ? make_float2(c.z, c.w) : c0;
+                    const float2 f2 = make_float2(by_f, by_f);
+                    const float2 d = fma2(make_float2(x[k], x[k + 1]), f2, minus), e = fma2(make_float2(x[k + 2], x[k + 3]), f2, minus);
+                    const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y)), q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                    sum = add2(sum, p);
+                    more = add2(more, q);
+                    const float2 y = mul2(p, c0), z = mul2(q, c1);
+                    w[k / 2] = pair_of(y.x, y.y);
+                    w[k / 2 + 1] = pair_of(z.x, z.y);
                 }
+                tmem_write16(scores + 16u * i, w); // (over scores of this thread's that have been read twice)
             }
             l += (sum.x + sum.y) + (more.x + more.y);
             __syncwarp();
@@ -519,33 +530,33 @@ struct Softmax {
         alive = alive && await(s, &s.o_full[t], outputs & 1u);
         ++outputs;
         __syncwarp();
-        if (__any_sync(~0u, !alive)) {
-            alive = false;
-            return;
-        }
         tc_fence_after();
+        s.sum[half][row] = l;
+        __syncwarp();
+        named_barrier(pair, 64);
+        l = half ? s.sum[0][row] + l : l + s.sum[1][row]; // (in the same order in both)
         for (uint32_t i = 0; i < s.n_mixed[which]; ++i) { // values that are NaN, of blocks that not all rows see
             const uint32_t* b = s.mixed[which][i];
+            if (!(b[1] | b[2] | b[3] | b[4]))
+                continue;
             for (uint32_t k = 0; k < kBlock; ++k) {
-                const int32_t key = (int32_t)(b[0] * kBlock + k);
-                if (!b[1] && !b[2] && !b[3] && !b[4])
-                    break;
-                if (((b[1 + k / 32u] >> (k & 31u)) & 1u) && key >= lo && key < hi)
+                const int32_t at_key = (int32_t)(b[0] * kBlock + k);
+                if (((b[1 + k / 32u] >> (k & 31u)) & 1u) && at_key >= lo && at_key < hi)
                     l = __int_as_float(0x7fc00000);
             }
         }
         __syncwarp();
         const float worth = s.unit[which] / kWeightUnit;
-        T* to = static_cast<T*>(a.out) + (g.seq.first + token) * a.out_ld + (uint64_t)head * D;
+        T* to = static_cast<T*>(a.out) + (g.seq.first + token) * a.out_ld + (uint64_t)head * D + half * columns;
         const float by = part ? worth : l == 0.0f ? 0.0f : worth / l;
 #pragma unroll 1
-        for (uint32_t i = 0; i < D; i += 32) {
+        for (uint32_t i = 0; i < columns; i += 32) {
             float y[32];
             tmem_read32(y, out + i);
             if (real && part) {
 #pragma unroll
                 for (uint32_t k = 0; k < 32; ++k)
-                    part[(i + k) * kUnitRows + row] = y[k] * by; // (by column: lanes are rows)
+                    part[(half * columns + i + k) * kUnitRows + row] = y[k] * by; // (by column: lanes are rows)
             } else if (real) {
 #pragma unroll
                 for (uint32_t k = 0; k < 32; k += 8) {
@@ -565,14 +576,15 @@ struct Softmax {
             __syncwarp();
         }
         tc_fence_before();
-        if (real && part) {
+        if (real && part && half == 0) {
             part[kUnitRows * D + row] = ref;
             part[kUnitRows * (D + 1u) + row] = l;
         }
+        __syncwarp();
     }
 };
 
-template <typename T, uint32_t D>
+template <typename T, uint32_t D, uint32_t Group>
 __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendArgs a)
 {
     extern __shared__ unsigned char raw[];
@@ -581,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     ring.base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
     const uint32_t tid = threadIdx.x, warp = tid / 32u;
     if (tid == 0) {
-        mbar_init(&s.q_full, kUnitRows);
+        mbar_init(&s.q_full, 2u * kUnitRows);
         mbar_init(&s.q_empty, 1);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&s.k_full[i], 1);
@@ -589,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             mbar_init(&s.v_full[i], 1);
             mbar_init(&s.v_empty[i], 1);
             mbar_init(&s.s_full[i], 1);
-            mbar_init(&s.p_full[i], kTileRows);
+            mbar_init(&s.p_full[i], 2u * kTileRows);
             mbar_init(&s.o_full[i], 1);
         }
         s.failed = 0;
@@ -616,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
     };
     if (blockIdx.x < found.ctas) {
         if (tid < kConvert) {
-            Softmax<T, D> x;
+            Softmax<T, D, Group> x;
             segments([&](const Segment& g, float* part) { x.run(a, s, ring, g, part); });
         } else if (tid < kIssue) {
             Converter<T, D> x;
@@ -648,16 +660,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         tmem_free_all(s.tmem);
 }
 
-template <typename T, uint32_t D>
+template <typename T, uint32_t D, uint32_t Group>
 cudaError_t launch(const KvAttendArgs& a, cudaStream_t stream)
 {
     constexpr uint32_t smem = 6u * Ring<D>::tile_bytes + 1024u;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = set_once(done, kv_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = set_once(done, kv_prompt_kernel<T, D, Group>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess)
         return e;
-    kv_prompt_kernel<T, D><<<kPromptCtas, kThreads, smem, stream>>>(a);
+    kv_prompt_kernel<T, D, Group><<<kPromptCtas, kThreads, smem, stream>>>(a);
     return cudaGetLastError();
+}
+
+template <typename T, uint32_t D>
+cudaError_t launch_group(const KvAttendArgs& a, cudaStream_t stream)
+{
+    return a.c.page_size % 16u ? launch<T, D, 1>(a, stream) : launch<T, D, 16>(a, stream);
 }
 
 } // namespace
@@ -665,8 +683,8 @@ cudaError_t launch(const KvAttendArgs& a, cudaStream_t stream)
 cudaError_t launch_kv_prompt(const KvAttendArgs& a, int type, cudaStream_t stream)
 {
     if (type == MK_BF16)
-        return a.c.dim == 128u ? launch<__nv_bfloat16, 128>(a, stream) : launch<__nv_bfloat16, 64>(a, stream);
-    return a.c.dim == 128u ? launch<__half, 128>(a, stream) : launch<__half, 64>(a, stream);
+        return a.c.dim == 128u ? launch_group<__nv_bfloat16, 128>(a, stream) : launch_group<__nv_bfloat16, 64>(a, stream);
+    return a.c.dim == 128u ? launch_group<__half, 128>(a, stream) : launch_group<__half, 64>(a, stream);
 }
 
 } // namespace mk
