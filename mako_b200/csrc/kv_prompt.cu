@@ -131,15 +131,16 @@ struct Ring { // shared memory
     __device__ __forceinline__ unsigned char* q(uint32_t t) const { return base + t * tile_bytes; }
     __device__ __forceinline__ unsigned char* k(uint32_t i) const { return base + (2u + i) * tile_bytes; }
     __device__ __forceinline__ unsigned char* v(uint32_t i) const { return base + (4u + i) * tile_bytes; }
+    __device__ __forceinline__ uint4* wait() const { return reinterpret_cast<uint4*>(base + 6u * tile_bytes); } // a block's codes
+    static constexpr uint32_t bytes = 6u * tile_bytes + kBlock * D;
 };
 
 // Those that convert. What they count goes on from segment to segment.
 template <typename T, uint32_t D>
 struct Converter {
     // a load is 16 codes: of 32 rows, 64 columns. (Eight lanes have two rows' quarters: their stores are in different banks.)
-    // Half of a tile at a time, so that three halves under way fit into registers.
-    static constexpr uint32_t halves = D / 64, loads = kBlock / 64 * halves;
-    static __device__ __forceinline__ uint32_t row_of(uint32_t part, uint32_t i) { return 64u * part + i / halves * 32u + (threadIdx.x - kConvert) / 4u; }
+    static constexpr uint32_t halves = D / 64, loads = kBlock / 32 * halves;
+    static __device__ __forceinline__ uint32_t row_of(uint32_t i) { return i / halves * 32u + (threadIdx.x - kConvert) / 4u; }
     static __device__ __forceinline__ uint32_t chunk_of(uint32_t i) { return i % halves * 4u + (threadIdx.x & 3u); }
     uint32_t blocks = 0;   // so far
     uint32_t segments = 0;
@@ -168,25 +169,36 @@ struct Converter {
         return p;
     }
 
-    __device__ __forceinline__ void load(uint4 (&x)[loads], const void* codes, const uint64_t* off, uint32_t part)
+    // A block's values wait in registers and its keys in shared memory, each thread's own, until the block before is done with: a read that L2
+    // does not answer takes 3000 cycles, as long as turning a block into fp16.
+    __device__ __forceinline__ void load(uint4 (&x)[loads], const void* codes, const uint64_t* off)
     {
 #pragma unroll
         for (uint32_t i = 0; i < loads; ++i) {
-            const uint64_t from = off[row_of(part, i)];
+            const uint64_t from = off[row_of(i)];
             x[i] = from != ~0ull ? __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(codes) + from + chunk_of(i) * 16u)) : make_uint4(0, 0, 0, 0);
         }
     }
-    __device__ __forceinline__ void store(const uint4 (&x)[loads], unsigned char* tile, uint32_t part)
+    __device__ __forceinline__ void copy(uint4* wait, const void* codes, const uint64_t* off)
     {
 #pragma unroll
         for (uint32_t i = 0; i < loads; ++i) {
-            const uint2 y0 = halves_of4(x[i].x), y1 = halves_of4(x[i].y), y2 = halves_of4(x[i].z), y3 = halves_of4(x[i].w);
-            *reinterpret_cast<uint4*>(tile + tile_at(row_of(part, i), 2u * chunk_of(i))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
-            *reinterpret_cast<uint4*>(tile + tile_at(row_of(part, i), 2u * chunk_of(i) + 1u)) = make_uint4(y2.x, y2.y, y3.x, y3.y);
+            const uint64_t from = off[row_of(i)];
+            const unsigned char* p = static_cast<const unsigned char*>(codes) + (from != ~0ull ? from + chunk_of(i) * 16u : 0ull);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(wait + i * 128u + threadIdx.x - kConvert)), "l"(p),
+                         "r"(from != ~0ull ? 16u : 0u)
+                         : "memory");
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void store(const uint4& x, unsigned char* tile, uint32_t i)
+    {
+        const uint2 y0 = halves_of4(x.x), y1 = halves_of4(x.y), y2 = halves_of4(x.z), y3 = halves_of4(x.w);
+        *reinterpret_cast<uint4*>(tile + tile_at(row_of(i), 2u * chunk_of(i))) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        *reinterpret_cast<uint4*>(tile + tile_at(row_of(i), 2u * chunk_of(i) + 1u)) = make_uint4(y2.x, y2.y, y3.x, y3.y);
     }
     // Takes values that are NaN out, and says whose they are.
-    __device__ __forceinline__ void take_out(uint4 (&x)[loads], uint32_t part, uint32_t* whose)
+    __device__ __forceinline__ void take_out(uint4 (&x)[loads], uint32_t* whose)
     {
 #pragma unroll
         for (uint32_t i = 0; i < loads; ++i) {
@@ -199,7 +211,7 @@ struct Converter {
                 bad |= nan;
             }
             if (bad)
-                atomicOr(whose + row_of(part, i) / 32u, 1u << (row_of(part, i) & 31u));
+                atomicOr(whose + row_of(i) / 32u, 1u << (row_of(i) & 31u));
         }
     }
 
@@ -216,12 +228,12 @@ struct Converter {
         s.off[blocks & 1u][tid] = p.off;
         __syncwarp();
         named_barrier(2, 128);
-        uint4 k0[loads], k1[loads], v[loads];
-        load(k0, a.c.k, s.off[blocks & 1u], 0);
-        load(k1, a.c.k, s.off[blocks & 1u], 1);
+        uint4* keys = ring.wait();
+        uint4 v[loads];
+        copy(keys, a.c.k, s.off[blocks & 1u]);
+        load(v, a.c.v, s.off[blocks & 1u]);
         for (uint32_t b = g.from; b < g.to; ++b, ++blocks) {
             const uint32_t stage = blocks & 1u, parity = (blocks >> 1) & 1u, slot = blocks % kSlots;
-            load(v, a.c.v, s.off[stage], 0);
             const bool more = b + 1u < g.to;
             const Place next = place(a, g, page, b + 1u);
             page = look_up(a, g, table, b + 2u);
@@ -246,9 +258,10 @@ struct Converter {
             if (tid == 0)
                 s.older[slot] = now > 0.0f ? unit / now : 1.0f;
             unit = now;
-            store(k0, ring.k(stage), 0);
-            load(k0, a.c.v, s.off[stage], 1); // the second half of the values takes the keys' registers
-            store(k1, ring.k(stage), 1);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+            for (uint32_t i = 0; i < loads; ++i)
+                store(keys[i * 128u + tid], ring.k(stage), i);
             if (!more && tid == 0)
                 s.unit[(segments - 1u) & 1u] = unit;
             p = next;
@@ -259,7 +272,7 @@ struct Converter {
                 mbar_arrive(&s.k_full[stage]);
             __syncwarp();
             if (more)
-                load(k1, a.c.k, s.off[stage ^ 1u], 1);
+                copy(keys, a.c.k, s.off[stage ^ 1u]);
             if (b * kBlock < g.see_from || (b + 1u) * kBlock > g.see_to) { // some rows see what others do not
                 const uint32_t which = s.n_mixed[(segments - 1u) & 1u];
                 uint32_t* at = s.mixed[(segments - 1u) & 1u][which < kMixed ? which : kMixed - 1u];
@@ -271,16 +284,16 @@ struct Converter {
                     s.n_mixed[(segments - 1u) & 1u] = which < kMixed ? which + 1u : kMixed;
                 __syncwarp();
                 named_barrier(2, 128);
-                take_out(v, 0, at + 1);
-                take_out(k0, 1, at + 1);
+                take_out(v, at + 1);
                 __syncwarp();
             }
             alive = alive && await(s, &s.v_empty[stage], parity ^ 1u);
             __syncwarp();
-            store(v, ring.v(stage), 0);
-            store(k0, ring.v(stage), 1);
+#pragma unroll
+            for (uint32_t i = 0; i < loads; ++i)
+                store(v[i], ring.v(stage), i);
             if (more)
-                load(k0, a.c.k, s.off[stage ^ 1u], 0);
+                load(v, a.c.v, s.off[stage ^ 1u]);
             fence_proxy_async();
             __syncwarp();
             named_barrier(2, 128);
@@ -663,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
 template <typename T, uint32_t D, uint32_t Group>
 cudaError_t launch(const KvAttendArgs& a, cudaStream_t stream)
 {
-    constexpr uint32_t smem = 6u * Ring<D>::tile_bytes + 1024u;
+    constexpr uint32_t smem = Ring<D>::bytes + 1024u;
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = set_once(done, kv_prompt_kernel<T, D, Group>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess)
