@@ -599,7 +599,7 @@ template <typename T, uint32_t D, uint32_t Tile, uint32_t Each>
 cudaError_t launch_join(const KvAttendArgs& a, uint32_t ctas, cudaStream_t stream)
 {
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(ctas - 1u, Tile / 16u);
+    c.gridDim = dim3(ctas - 1u, Tile > 64u ? Tile / 64u : 1u); // (all of which run at the same time)
     c.blockDim = dim3(kJoinThreads);
     c.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -99,6 +99,29 @@ def test_long_axis_is_split(sampler, q_heads, dim):
     check(sampler, *make(rng, [3000, 40, 5001, 7, 1200], [1, 1, 2, 1, 3], 2, q_heads, dim, 16, "fp16"))
 
 
+@pytest.mark.parametrize("dim,page,window", [(128, 16, 0), (64, 64, 1000), (128, 40, 0), (64, 7, 333)])
+def test_long_prompts(sampler, dim, page, window):
+    """Chunks over long contexts, whose units many CTAs share, beside single tokens and short ones; pages that are a multiple of 16 and not."""
+    rng = np.random.default_rng(dim + page)
+    check(sampler, *make(rng, [3000, 40, 1700, 129, 900], [300, 1, 130, 129, 17], 2, 10, dim, page, "bf16"), window=window)
+    check(sampler, *make(rng, [2600], [65], 1, 4, dim, page, "fp16"), window=window)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 1e-30])
+@pytest.mark.parametrize("new", [1, 40])
+def test_scales_of_scores(sampler, scale, new):
+    rng = np.random.default_rng(21)
+    check(sampler, *make(rng, [300, 77], [new, new], 2, 8, 128, 16, "bf16"), scale=scale)
+
+
+@pytest.mark.parametrize("rows", [16, 17, 63, 64, 65, 128, 129, 256, 257])
+def test_rows_around_the_tiles(sampler, rows):
+    """A key head's rows, at the borders of tiles, units and kernels, as tokens and as heads."""
+    rng = np.random.default_rng(rows)
+    check(sampler, *make(rng, [rows + 40, 3, rows], [rows, 1, rows], 1, 1, 64, 16, "bf16"))
+    check(sampler, *make(rng, [150, 1, 33], [1, 1, 1], 1, rows, 64, 16, "fp16"))
+
+
 def test_many_sequences(sampler):
     rng = np.random.default_rng(8)
     n = 700
