@@ -386,7 +386,7 @@ int mk_token_logprobs(mk_sampler* s, const mk_logprob_rows* rows, float* logprob
                       float* top_logprob, uint32_t* flags, void* stream);
 
 /* A paged cache of keys and values in 8 bits: e4m3 codes (a sign, four bits of exponent, three of mantissa; 0x7f and 0xff are NaN,
- * there are no infinities), a scale for each page and head. What a code stands for times its scale is the value. A page's head is
+ * there are no infinities), a scale for each page and head, 0 or more. What a code stands for times its scale is the value. A page's head is
  * page_size rows of dim codes; strides are in bytes, multiples of 16, the same for k and v, which start on 16-byte boundaries. The
  * pages are those of mk_kv_pages. */
 typedef struct mk_kv_cache {

@@ -8,6 +8,10 @@
 //
 // Angles are formed and brought into [-pi, pi] in 64 bits (position x frequency in 32 bits is off by 0.06 rad at a million), their sine and
 // cosine in 32.
+//
+// 64 tokens of a decode step take 6.5 us from a graph, 8 key heads of 128 with 32 query heads; chunks of some 7000 tokens 69, where
+// reading and writing once would take 21: instructions bound it, of angles (a third) and of roundings. Two heads a CTA: with one 85 us, whose angles
+// are formed eight times, with four 85, too few CTAs.
 #include "kv_cache.cuh"
 #include "ptx.cuh"
 #include "round_ops.h"

@@ -1,13 +1,22 @@
 // Attention of few rows over a paged 8-bit cache (mk_kv_attention in include/mako_b200.h): a decode step, a speculative round. Every
-// key and value is read once for all query heads that share it, which is what bounds it.
+// key and value is read once for 16 rows, tokens of the pass times query heads that share the key head, and from L2 for 16 more. HBM bounds
+// it where contexts are long (64 sequences of up to 16384 keys, 8 key heads of 128, 4 query heads each: 195 us, 5.5 TB/s or 0.84 of the rate of a
+// copy; two of 131072 with groups of 8: 102 us, 0.80), latency where they are short (one sequence of 2048: 14.5 us from a graph, of which the
+// search for a CTA's share is 1.6, the chain from page to product 2, the join 5).
 //
-// A unit has 16 rows (or 32): the MMA's M. A warp takes every fourth block of its CTA's keys, 4 KB of keys and values, which it copies into a ring
-// of its own in shared memory, so that warps wait for nobody until their segment ends. Codes become fp16 (exactly) on the way from shared
-// memory into registers, in the order in which the tensor core wants them: of a block's keys a lane reads 16 of a token's columns,
-// four steps of the contraction; of its values the four tokens whose weights it holds, which byte permutations put side by
-// side. Queries are fp16 too, each row times the power of two that brings its largest to about 2^12: bf16 loses nothing by it.
-// Scales of keys go into the scores, scales of values into the weights: 2^7 v_j / v p_j is what fp16 holds, v being the largest scale
-// so far, so that a weight's rounding is 2^-11 of it down to 2^-21 of the largest; sums are in fp32.
+// A unit has 16 rows: the MMA's M. A warp takes every fourth block of its CTA's keys, 32 keys and values (8 KB at 128 columns), which it
+// copies into a ring of its own in shared memory, so that warps wait for nobody until their segment ends; three CTAs of four warps an SM,
+// two blocks each, have 98 KB under way. (With blocks of 16 keys, four deep, 214 us: 1.3 times the instructions. With two CTAs and three
+// blocks 218: too few warps for the chain of product, exponential, product. Two tiles of rows that share what is read had 32 rows take 113 us
+// where two units take 129, but 24 rows 194 against 163.)
+// mma.sync, not tcgen05: 16 rows are an eighth of that one's M, and a product's operands would have to go through shared memory as fp16, which
+// is four times the bytes that the cache's codes are there. The tensor pipe is busy for 0.27 of the time.
+//
+// Codes become fp16 (exactly) on the way from shared memory into registers, in the order in which the tensor core wants them: of a block's
+// keys a lane reads 16 of a token's columns, four steps of the contraction; of its values the four tokens whose weights it holds, which
+// byte permutations put side by side. Queries are fp16 too, each row times the power of two that brings its largest to about 2^12: bf16 loses
+// nothing by it. Scales of keys go into the scores, scales of values into the weights: 2^7 v_j / v p_j is what fp16 holds, v being the
+// largest scale so far, so that a weight's rounding is 2^-11 of it down to 2^-21 of the largest; sums are in fp32.
 #include "kv_cache.cuh"
 #include "kv_work.cuh"
 #include "ptx.cuh"
@@ -564,7 +573,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
                     for (uint32_t p = 0; p < some; ++p) {
                         const float* x = part(p0 + p);
                         float4 y;
-                        if constexpr (Tile > 32) { // columns, as the threads that have a row each write them
+                        if constexpr (Tile > 32) { // by column, as kv_prompt_kernel writes them
                             x += d * Tile + r0 + r;
                             y = make_float4(x[0], x[Tile], x[2 * Tile], x[3 * Tile]);
                         } else {
@@ -625,7 +634,9 @@ cudaError_t launch_rows(const KvAttendArgs& a, cudaStream_t stream)
     return launch_join<T, D, kTile, kBlockTokens>(a, grid, stream);
 }
 
-// Sequences of up to so many rows go through kv_rows_kernel, in a pass with longer ones too.
+// Sequences of up to so many rows go through kv_rows_kernel, in a pass with longer ones too: it takes the time of as many tiles of 16, a unit of
+// kv_prompt_kernel that of 256 rows. 64 sequences of 8192 keys, 8 key heads of 128, by the one and by the other: 48 rows 491 and 931 us, 64 rows
+// 649 and 922; 96 rows 934 and 777.
 constexpr uint32_t kFewRows = 64;
 
 template <typename T, uint32_t D>

@@ -6,10 +6,15 @@
 // s being c times the largest x so far, rounded: a shift that is a little off is as good as another as long as it is the same one
 // everywhere, so that what the rounding of a large c x takes away does not reach the results.
 //
-// Alternatives: an x above `line` goes into a list of (x, id) in shared memory. The line is a lower bound of the k-th largest x that the
-// CTA has seen: of the threads' largest ones in the first tile, then of the list's entries after 2, 4, 8, ... tiles, so that a row in
+// Alternatives: an x on or above `line` goes into a list of (x, id) in shared memory. The line is a lower bound of the k-th largest x that the
+// CTA has seen: of groups of threads' largest in the first tile, then of the list's entries after 1, 2, 4, 8, ... tiles, so that a row in
 // no particular order has about k log2(tiles) entries. A row whose list runs over (an ascending one) is read again, in pieces of
 // which each fits.
+//
+// A CTA per row; where rows are few a cluster of up to 16 of them, whose parts are put into the first one's shared memory. Instructions bound it
+// beside HBM: 2048 rows of 151552 bf16 logits take 134 us (4.6 TB/s, 0.70 of the rate of a copy; 118 if nothing were ever put into a list),
+// a row of 129280 fp32 logits 12.5 from a graph, 137 masked rows of 50257 fp16 27. 16-bit logits are compared two at a time before they become
+// floats; weights and sums are formed two at a time. (Five CTAs an SM, 48 registers: with four 143 us, with six 137.)
 #include "ptx.cuh"
 #include "round_ops.h"
 

@@ -99,7 +99,8 @@ def check(sampler, cache, qkv, heads, q_heads, slots, positions, rotary, interle
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("heads,q_heads,dim,rotary,page", [(1, 1, 64, 64, 16), (2, 8, 128, 128, 16), (3, 3, 64, 16, 7), (5, 10, 128, 64, 1),
-                                                           (2, 0, 16, 16, 5), (1, 2, 256, 256, 24), (4, 28, 64, 0, 128), (8, 8, 128, 32, 64)])
+                                                           (2, 0, 16, 16, 5), (1, 2, 256, 256, 24), (4, 28, 64, 0, 128), (8, 8, 128, 32, 64),
+                                                           (3, 6, 48, 32, 16), (1, 3, 80, 80, 20), (5, 5, 240, 16, 9)])
 def test_runs(sampler, kind, interleaved, heads, q_heads, dim, rotary, page):
     rng = np.random.default_rng(heads * 1000 + dim + page)
     slots = runs_of(rng, 400 if page == 1 else 60, page, [(0, 1), (page - 1, 1), (page // 2, 3), (0, 2 * page), (page // 3, 40), (0, page), (page - 1, page + 2)])
