@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv_rows_kernel(const KvAttendArgs
         }
         __syncthreads();
         const bool whole = u.whole();
-        float* part = a.parts + (uint64_t)(2u * blockIdx.x + !u.first) * kPartFloats<D>;
+        float* part = a.parts + (uint64_t)u.place(blockIdx.x) * kPartFloats<D>;
         for (uint32_t i = tid; i < u.rows * (D / 4); i += kThreads) {
             const uint32_t r = i / (D / 4), d = i % (D / 4) * 4u;
             float most = s.m[0][r];
@@ -525,19 +525,24 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
     if (cta >= walk.ctas)
         return;
     const uint32_t skip = walk.skip, ctas = walk.ctas;
-    const uint64_t start = walk.at - skip, before = kv_cut(walk.total, ctas, cta - 1u);
-    if (skip == 0 || before > start)
+    const uint64_t start = walk.at - skip;
+    if (skip == 0 || kv_cut(walk.total, ctas, cta - 1u) > start)
         return;
     KvSegment u;
+    u.from = u.to = 0;
+    u.blocks = KvBlocks{0, 0};
     kv_take(a, walk, u, true, Tile, Each);
-    const uint64_t stop = start + (u.blocks.to - u.blocks.from);
+    const uint32_t blocks = u.blocks.to - u.blocks.from;
+    if (skip >= blocks || u.from != u.blocks.from + skip) // the cut is behind the unit's blocks (and what was taken is another one's)
+        return;
+    const uint64_t stop = start + blocks;
     constexpr uint32_t floats = Tile * (D + 2u);
-    uint32_t parts = 1; // the first one's, and of those CTAs whose shares begin in the unit
+    uint32_t parts = 1; // of the CTA that began the unit, and of those whose shares begin inside
     while (cta + parts - 1u < ctas && kv_cut(walk.total, ctas, cta + parts - 1u) < stop)
         ++parts;
     auto join_row = [](uint32_t i) { return Tile > 32 ? i % 16u : i / (D / 4); };
     auto join_column = [](uint32_t i) { return (Tile > 32 ? i / 16u : i % (D / 4)) * 4u; };
-    auto part = [&](uint32_t p) { return a.parts + (uint64_t)(2u * (cta - 1u + p) + (p == 0 && before != start)) * floats; };
+    auto part = [&](uint32_t p) { return a.parts + (uint64_t)(2u * (cta - 1u + p) + (p == 0)) * floats; };
     for (uint32_t r0 = 16u * blockIdx.y; r0 < u.rows; r0 += 16u * gridDim.y) { // 16 rows at a time: their maxima, then what each part is worth, then the sums
         const uint32_t rows = min(16u, u.rows - r0);
         float4 o[16 * (D / 4) / kJoinThreads];
@@ -646,13 +651,15 @@ cudaError_t launch(const KvAttendArgs& args, int type, cudaStream_t stream)
     const bool few = (uint64_t)a.max_new * a.group <= kFewRows;
     a.rows_from = 1;
     a.rows_to = few ? 0xffffffffu : kFewRows; // (max_new is what the caller says: where it is too small all the same rows are done)
-    a.blocks_least = 4;
+    a.unit_cost = 8; // (4: 187 us where 8 takes 183 and 12 184; 37 sequences of up to 6000, 27, 25, 25)
+    a.blocks_least = 8;
     cudaError_t e = launch_rows<T, D>(a, stream);
     if (e != cudaSuccess || few)
         return e;
     a.parts = args.parts + kv_rows_parts(D) / 4u;
     a.rows_from = kFewRows + 1u;
     a.rows_to = 0xffffffffu;
+    a.unit_cost = 4;
     a.blocks_least = 1;
     e = launch_kv_prompt(a, type, stream);
     return e != cudaSuccess ? e : launch_join<T, D, kPromptRows, kPromptBlock>(a, kPromptCtas, stream);

@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
             const int32_t top = back + (int32_t)kv_token_of(a, g.row0) + 1, last = back + (int32_t)kv_token_of(a, g.row0 + g.rows - 1u) + 1;
             g.see_to = top < 0 ? 0u : (uint32_t)top;
             g.see_from = a.window && last > (int32_t)a.window ? (uint32_t)last - a.window : 0u;
-            role(g, g.whole() ? nullptr : a.parts + (uint64_t)(2u * blockIdx.x + !first) * (kUnitRows * (D + 2u)));
+            role(g, g.whole() ? nullptr : a.parts + (uint64_t)g.place(blockIdx.x) * (kUnitRows * (D + 2u)));
         }
     };
     if (blockIdx.x < found.ctas) {

@@ -1,8 +1,9 @@
 // How the attention over a paged cache is dealt out to CTAs. A unit is a sequence, a key head and a tile of rows, where a row is a query
 // head of the group that shares the key head, at a token of the pass (row = token * group + head): they read the same keys. Its
-// work is counted in blocks of keys. All units' blocks, one behind the other, are cut into equal shares, so that long and short
-// sequences, prompts and single tokens, few and many of them all fill the device; a unit that a cut goes through is put together from
-// its parts by a second launch. Lengths are known on the device alone, so every CTA forms the sums by itself.
+// work is counted in blocks of keys, and unit_cost of them for what a unit costs whatever its length (queries, the first reads, its end). All
+// units' work, one behind the other, is cut into equal shares, so that long and short sequences, prompts and single tokens, few and many of
+// them all fill the device; a unit that a cut goes through is put together from its parts by a second launch. (Without unit_cost one CTA had
+// the eight units of a sequence of 50 keys among 37 of up to 6000, and the others waited for it: 46 us.) Lengths are known on the device alone, so every CTA forms the sums by itself.
 #pragma once
 #include "round_ops.h"
 
@@ -49,21 +50,25 @@ __device__ __forceinline__ uint32_t kv_rows(const KvAttendArgs& a, const KvSeq& 
     return rows < a.rows_from || rows > a.rows_to ? 0u : rows;
 }
 
+// A unit's work.
 __device__ __forceinline__ uint32_t kv_tile_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t rows, uint32_t row0, uint32_t tile, uint32_t each)
 {
     if (row0 >= rows)
         return 0;
     const KvBlocks b = kv_blocks(a, q, row0, min(tile, rows - row0), each);
-    return b.to - b.from;
+    return b.to - b.from + a.unit_cost;
 }
 
-// Of each lane's sequence: blocks of one key head, all of its tiles of rows together. A sequence of many tiles (a prompt) is counted by the
+// Of each lane's sequence: the work of one key head, all of its tiles of rows together. A sequence of many tiles (a prompt) is counted by the
 // warp. By whole warps.
 __device__ __forceinline__ uint32_t kv_seq_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t rows, uint32_t tile, uint32_t each)
 {
+    constexpr uint32_t few = 4; // tiles that a lane counts by itself
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t sum = kv_tile_blocks(a, q, rows, 0, tile, each);
-    uint32_t many = __ballot_sync(~0u, rows > tile);
+    uint32_t sum = 0;
+    for (uint32_t i = 0; i < few; ++i)
+        sum += kv_tile_blocks(a, q, rows, i * tile, tile, each);
+    uint32_t many = __ballot_sync(~0u, rows > few * tile);
     while (many) {
         const int i = __ffs(many) - 1;
         many &= many - 1u;
@@ -88,8 +93,8 @@ __device__ __forceinline__ uint64_t kv_cut(uint64_t total, uint32_t n, uint32_t 
     return (uint64_t)each * i + min(i, more);
 }
 
-// A CTA's share of all blocks, [at, end), and the unit that it begins in, `skip` blocks behind the unit's first. take() gives one segment
-// after the other.
+// A CTA's share of all work, [at, end), and the unit that it begins in, `skip` behind the unit's begin. kv_take gives one segment after the
+// other. A unit's blocks come first, what else it costs behind them.
 struct KvWalk {
     uint64_t at, end, total;
     uint32_t ctas; // that have a share
@@ -184,43 +189,48 @@ struct KvSegment {
     KvSeq seq;
     KvBlocks blocks; // all of the unit's
     uint32_t sq, head, row0, rows, from, to;
-    bool first;      // the CTA's first one
     __device__ __forceinline__ bool whole() const { return from == blocks.from && to == blocks.to; }
+    // Where a part of a unit goes. A CTA has two places: for a unit that another one began, and for one that it begins.
+    __device__ __forceinline__ uint32_t place(uint32_t cta) const { return 2u * cta + (from == blocks.from); }
 };
 
-// The walk's next segment; false behind the last. `g` is the one before, w.at the share's begin at the first call.
+// The walk's next segment; false behind the last. `g` is the one before.
 __device__ __forceinline__ bool kv_take(const KvAttendArgs& a, KvWalk& w, KvSegment& g, bool first, uint32_t tile, uint32_t each)
 {
-    if (w.at >= w.end)
-        return false;
-    if (first || w.row0 == 0) { // (a sequence begins, or a head)
-        g.seq = kv_seq(a, w.sq);
-        while (kv_rows(a, g.seq) == 0) {
-            if (++w.sq >= a.n_seq) // (not while lengths stay as they were)
-                return false;
+    while (w.at < w.end) {
+        if (first || w.row0 == 0) { // (a sequence begins, or a head)
             g.seq = kv_seq(a, w.sq);
+            while (kv_rows(a, g.seq) == 0) {
+                if (++w.sq >= a.n_seq) // (not while lengths stay as they were)
+                    return false;
+                g.seq = kv_seq(a, w.sq);
+            }
+            first = false;
         }
-    }
-    const uint32_t rows = g.seq.n * a.group;
-    g.first = first;
-    g.sq = w.sq;
-    g.head = w.head;
-    g.row0 = w.row0;
-    g.rows = min(tile, rows - w.row0);
-    g.blocks = kv_blocks(a, g.seq, g.row0, g.rows, each);
-    g.from = g.blocks.from + w.skip;
-    g.to = w.end - w.at < g.blocks.to - g.from ? g.from + (uint32_t)(w.end - w.at) : g.blocks.to;
-    w.at += g.to - g.from;
-    w.skip = 0;
-    w.row0 += tile;
-    if (w.row0 >= rows) {
-        w.row0 = 0;
-        if (++w.head == a.c.n_heads) {
-            w.head = 0;
-            ++w.sq;
+        const uint32_t rows = g.seq.n * a.group;
+        g.sq = w.sq;
+        g.head = w.head;
+        g.row0 = w.row0;
+        g.rows = min(tile, rows - w.row0);
+        g.blocks = kv_blocks(a, g.seq, g.row0, g.rows, each);
+        const uint32_t n = g.blocks.to - g.blocks.from, all = n + a.unit_cost;
+        const uint32_t upto = w.end - w.at < all - w.skip ? w.skip + (uint32_t)(w.end - w.at) : all;
+        g.from = g.blocks.from + min(w.skip, n);
+        g.to = g.blocks.from + min(upto, n);
+        w.at += upto - w.skip;
+        w.skip = 0;
+        w.row0 += tile;
+        if (w.row0 >= rows) {
+            w.row0 = 0;
+            if (++w.head == a.c.n_heads) {
+                w.head = 0;
+                ++w.sq;
+            }
         }
+        if (g.from < g.to)
+            return true;
     }
-    return true;
+    return false;
 }
 
 } // namespace mk

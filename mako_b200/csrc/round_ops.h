@@ -112,8 +112,9 @@ struct KvAttendArgs {
     uint64_t page_inverse, group_inverse;
     uint32_t page_shift, group_shift, table_cols, n_seq, n_tokens, max_new, group, window;
     float scale_log2;         // of a score, for exponents of two
-    // which sequences a launch takes, by their rows (tokens of the pass times group), and the least blocks of a CTA; the launch sets them
-    uint32_t rows_from, rows_to, blocks_least;
+    // which sequences a launch takes, by their rows (tokens of the pass times group), the least blocks of a CTA, and how many of them a unit
+    // costs beside its own; the launch sets them
+    uint32_t rows_from, rows_to, blocks_least, unit_cost;
 };
 constexpr uint32_t kPromptCtas = 148, kPromptRows = 256, kPromptBlock = 128; // CTAs; rows of a unit; keys of a block
 uint64_t kv_attend_bytes(uint32_t dim, uint64_t most_rows); // of parts; rows: of a sequence
