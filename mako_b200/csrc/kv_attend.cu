@@ -1,16 +1,16 @@
 // Attention of few rows over a paged 8-bit cache (mk_kv_attention in include/mako_b200.h): a decode step, a speculative round. Every
 // key and value is read once for 16 rows, tokens of the pass times query heads that share the key head, and from L2 for 16 more. HBM bounds
-// it where contexts are long (64 sequences of up to 16384 keys, 8 key heads of 128, 4 query heads each: 195 us, 5.5 TB/s or 0.84 of the rate of a
-// copy; two of 131072 with groups of 8: 102 us, 0.80), latency where they are short (one sequence of 2048: 14.5 us from a graph, of which the
+// it where contexts are long (64 sequences of up to 16384 keys, 8 key heads of 128, 4 query heads each: 183 us for 987 MB, 5.4 TB/s or 0.82 of the
+// rate of a copy; two of 131072 with groups of 8: 103 us, 0.80), latency where they are short (one sequence of 2048: 14.5 us from a graph, of which the
 // search for a CTA's share is 1.6, the chain from page to product 2, the join 5).
 //
 // A unit has 16 rows: the MMA's M. A warp takes every fourth block of its CTA's keys, 32 keys and values (8 KB at 128 columns), which it
 // copies into a ring of its own in shared memory, so that warps wait for nobody until their segment ends; three CTAs of four warps an SM,
-// two blocks each, have 98 KB under way. (With blocks of 16 keys, four deep, 214 us: 1.3 times the instructions. With two CTAs and three
-// blocks 218: too few warps for the chain of product, exponential, product. Two tiles of rows that share what is read had 32 rows take 113 us
+// two blocks each, have 98 KB under way. (When it took 195 us: with blocks of 16 keys, four deep, 214, 1.3 times the instructions; with two CTAs
+// and three blocks 218, too few warps for the chain of product, exponential, product. Two tiles of rows that share what is read had 32 rows take 113 us
 // where two units take 129, but 24 rows 194 against 163.)
 // mma.sync, not tcgen05: 16 rows are an eighth of that one's M, and a product's operands would have to go through shared memory as fp16, which
-// is four times the bytes that the cache's codes are there. The tensor pipe is busy for 0.27 of the time.
+// is four times the bytes that the cache's codes are there. The tensor pipe is busy for 0.35 of the time.
 //
 // Codes become fp16 (exactly) on the way from shared memory into registers, in the order in which the tensor core wants them: of a block's
 // keys a lane reads 16 of a token's columns, four steps of the contraction; of its values the four tokens whose weights it holds, which
@@ -659,7 +659,7 @@ cudaError_t launch(const KvAttendArgs& args, int type, cudaStream_t stream)
     a.parts = args.parts + kv_rows_parts(D) / 4u;
     a.rows_from = kFewRows + 1u;
     a.rows_to = 0xffffffffu;
-    a.unit_cost = 4;
+    a.unit_cost = 4; // (0: 1418 us where 4 takes 1400 and 8 1405; chunks of 400 beside 21 single tokens, 99, 79, 83)
     a.blocks_least = 1;
     e = launch_kv_prompt(a, type, stream);
     return e != cudaSuccess ? e : launch_join<T, D, kPromptRows, kPromptBlock>(a, kPromptCtas, stream);

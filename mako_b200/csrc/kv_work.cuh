@@ -3,7 +3,8 @@
 // work is counted in blocks of keys, and unit_cost of them for what a unit costs whatever its length (queries, the first reads, its end). All
 // units' work, one behind the other, is cut into equal shares, so that long and short sequences, prompts and single tokens, few and many of
 // them all fill the device; a unit that a cut goes through is put together from its parts by a second launch. (Without unit_cost one CTA had
-// the eight units of a sequence of 50 keys among 37 of up to 6000, and the others waited for it: 46 us.) Lengths are known on the device alone, so every CTA forms the sums by itself.
+// the eight units of a sequence of 50 keys among 37 of up to 6000, and the others waited for it: 36 us
+// where it takes 25.) Lengths are known on the device alone, so every CTA forms the sums by itself.
 #pragma once
 #include "round_ops.h"
 

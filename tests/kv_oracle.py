@@ -101,9 +101,8 @@ def append(values, scales, x, slots, page):
 def attention(q, k, v, table, query_start, kv_len, page, scale, window, out_type):
     """q [T, Hq, D], k and v [P, H, page, D] float64 on the CPU (torch). Returns ({token: out [Hq, D]}, {token: bound [Hq, D]}): what of a
     kernel's roundings a result may have. Products are exact; a score's sum of D terms loses up to an ulp of its largest partial sum
-    each term, 2^-23; weights are rounded to fp16, whose significand has 11 bits, so by up to 2^-11 of each (half a step, eps / 2; it read
-    2^-12 here, half of that), and made by an exponential of 2^-22; sums over n keys lose 2^-23 of what
-    they hold in each of n / 16 steps and some joins."""
+    each term, 2^-23; weights are rounded to fp16, whose significand has 11 bits, so by up to 2^-11 of each (half a step, eps / 2),
+    and made by an exponential of 2^-22; sums over n keys lose 2^-23 of what they hold in each of n / 16 steps and some joins."""
     heads, dim = q.shape[1], q.shape[2]
     kv_heads = k.shape[1]
     group = heads // kv_heads

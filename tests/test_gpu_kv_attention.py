@@ -256,11 +256,12 @@ def test_streams_graphs_and_two_calls_at_once(sampler):
         torch.cuda.synchronize()
 
 
-def test_pages_far_into_a_cache(sampler):
+@pytest.mark.parametrize("new", [3, 40])
+def test_pages_far_into_a_cache(sampler, new):
     """Offsets beyond 32 bits: 5.1 GB of keys and as many of values."""
     from mako_b200 import KvCache
     rng = np.random.default_rng(17)
-    small, q, table, start, kv_len = make(rng, [100, 41], [1, 3], 1, 4, 128, 16, "bf16")
+    small, q, table, start, kv_len = make(rng, [100, 41], [1, new], 1, 4, 128, 16, "bf16")
     want = check(sampler, small, q, table, start, kv_len)
     pages = 2_500_000
     codes = lambda: torch.empty(pages, 1, 16, 128, dtype=torch.uint8, device="cuda").view(oracle.E4M3)  # noqa: E731
@@ -272,5 +273,5 @@ def test_pages_far_into_a_cache(sampler):
     for x, y in ((big.k_scale, small.k_scale), (big.v_scale, small.v_scale)):
         for i in range(small.k.shape[0]):
             x[i * 200_000 + 50_000] = y[i]
-    got = sampler.kv_attention(q, big, *(torch.from_numpy(x).cuda() for x in (far, start, kv_len)), max_new=3, out=torch.full_like(q, 7.0))
+    got = sampler.kv_attention(q, big, *(torch.from_numpy(x).cuda() for x in (far, start, kv_len)), max_new=new, out=torch.full_like(q, 7.0))
     assert torch.equal(got, want)
