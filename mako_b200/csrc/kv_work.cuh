@@ -62,11 +62,11 @@ __device__ __forceinline__ uint32_t kv_tile_blocks(const KvAttendArgs& a, const 
 
 // Of each lane's sequence: the work of one key head, all of its tiles of rows together. A sequence of many tiles (a prompt) is counted by the
 // warp. By whole warps.
-__device__ __forceinline__ uint32_t kv_seq_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t rows, uint32_t tile, uint32_t each)
+__device__ __forceinline__ uint64_t kv_seq_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t rows, uint32_t tile, uint32_t each)
 {
     constexpr uint32_t few = 4; // tiles that a lane counts by itself
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t sum = 0;
+    uint64_t sum = 0;
     for (uint32_t i = 0; i < few; ++i)
         sum += kv_tile_blocks(a, q, rows, i * tile, tile, each);
     uint32_t many = __ballot_sync(~0u, rows > few * tile);
@@ -75,11 +75,11 @@ __device__ __forceinline__ uint32_t kv_seq_blocks(const KvAttendArgs& a, const K
         many &= many - 1u;
         const KvSeq other{0u, __shfl_sync(~0u, q.n, i), __shfl_sync(~0u, q.len, i)};
         const uint32_t its = __shfl_sync(~0u, rows, i);
-        uint32_t x = 0;
+        uint64_t x = 0;
         for (uint32_t r = lane * tile; r < its; r += 32u * tile)
             x += kv_tile_blocks(a, other, its, r, tile, each);
         __syncwarp();
-        x = __reduce_add_sync(~0u, x);
+        x = ((uint64_t)__reduce_add_sync(~0u, (uint32_t)(x >> 26)) << 26) + __reduce_add_sync(~0u, (uint32_t)x & 0x3ffffffu); // (x below 2^53)
         sum = lane == (uint32_t)i ? x : sum;
     }
     return sum;
@@ -110,7 +110,7 @@ __device__ KvWalk kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, u
     auto of = [&](uint32_t k) -> uint64_t { // blocks of this thread's sequence k, all heads
         const uint32_t s = tid * mine + k;
         const KvSeq q = s < a.n_seq ? kv_seq(a, s) : KvSeq{0, 0, 0};
-        return (uint64_t)kv_seq_blocks(a, q, s < a.n_seq ? kv_rows(a, q) : 0u, tile, each) * a.c.n_heads;
+        return kv_seq_blocks(a, q, s < a.n_seq ? kv_rows(a, q) : 0u, tile, each) * a.c.n_heads;
     };
     uint64_t sum = 0;
     for (uint32_t k = 0; k < mine; ++k)
@@ -155,9 +155,10 @@ __device__ KvWalk kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, u
         const uint32_t s = (uint32_t)scratch[32];
         const uint64_t off = scratch[33], all = scratch[34];
         const KvSeq q = kv_seq(a, s);
-        const uint32_t rows = kv_rows(a, q), per_head = all >> 32 ? (uint32_t)(all / a.c.n_heads) : (uint32_t)all / a.c.n_heads;
-        const uint32_t head = off >> 32 ? (uint32_t)(off / per_head) : (uint32_t)off / per_head;
-        uint32_t left = (uint32_t)(off - (uint64_t)head * per_head);
+        const uint32_t rows = kv_rows(a, q);
+        const uint64_t per_head = all >> 32 ? all / a.c.n_heads : (uint32_t)all / a.c.n_heads;
+        const uint32_t head = all >> 32 ? (uint32_t)(off / per_head) : (uint32_t)off / (uint32_t)per_head;
+        uint64_t left = off - head * per_head;
         for (uint32_t r0 = 0; r0 < rows; r0 += 32u * tile) {
             const uint32_t r = r0 + lane * tile, n = kv_tile_blocks(a, q, rows, r, tile, each);
             uint32_t upto = n;
@@ -169,7 +170,7 @@ __device__ KvWalk kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, u
             if (left < upto && left >= upto - n) {
                 scratch[35] = head;
                 scratch[36] = r;
-                scratch[37] = left - (upto - n);
+                scratch[37] = left - (upto - n); // (32 tiles' work is below 2^32)
             }
             const uint32_t these = __shfl_sync(~0u, upto, 31);
             if (left < these)
