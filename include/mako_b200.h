@@ -396,7 +396,7 @@ typedef struct mk_kv_cache {
     float* v_scale;
     uint64_t page_stride, head_stride, token_stride;
     uint32_t n_pages, n_heads; /* heads of keys and values */
-    uint32_t page_size, dim;   /* tokens a page; columns a head, a multiple of 16, at most 256 */
+    uint32_t page_size, dim;   /* tokens a page, at most 2^24; columns a head, a multiple of 16, at most 256 */
 } mk_kv_cache;
 
 /* Keys and values of a pass, and queries to be rotated with them. Rows of a token have their heads side by side, [heads][dim]; ld:

@@ -24,6 +24,7 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kHeadsEach = 2;    // key heads of a CTA, which share the angles
+constexpr uint32_t kTokens = 65536;   // of a run without a rotation at a time, so that its rows' count stays within 31 bits
 constexpr uint32_t kAngles = 4096;    // (cosine, sine) pairs kept for a run's tokens: 32 KB
 
 template <typename T>
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
             }
         __syncthreads();
         const uint32_t len = s_len;
-        const uint32_t chunk = half ? min(len, kAngles / half) : len; // tokens whose angles are kept at a time
+        const uint32_t chunk = min(len, half ? kAngles / half : kTokens); // tokens whose angles are kept at a time
         uint32_t largest[2 * kHeadsEach] = {}; // of keys and values, by head
         for (int pass = 0; pass < 2; ++pass) {
             for (uint32_t i0 = 0; i0 < len; i0 += chunk) {

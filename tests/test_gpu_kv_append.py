@@ -168,6 +168,16 @@ def test_long_passes(sampler, tokens):
     check(sampler, cache, x, 2, 2, np.arange(tokens, dtype=np.int64) + 11, np.arange(tokens), 128)
 
 
+@pytest.mark.parametrize("rotary", [0, 16])
+def test_a_page_as_long_as_a_sequence(sampler, rotary):
+    rng = np.random.default_rng(6)
+    page, tokens = 70000, 66000
+    cache = cache_of(rng, 2, 1, page, 16)
+    x = torch.from_numpy(rng.normal(0, 1, (tokens, 4, 16)).astype(np.float32)).to(torch.float16).cuda()
+    x[-1] *= 9.0  # the scales are the last row's
+    check(sampler, cache, x, 1, 2, np.arange(tokens, dtype=np.int64) + page + 3000, np.arange(tokens), rotary)
+
+
 def test_a_cache_whose_heads_stand_side_by_side(sampler):
     """[P, page, H, D] seen as its transpose, and both kinds in one allocation."""
     from mako_b200 import KvCache
