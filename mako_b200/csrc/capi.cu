@@ -811,9 +811,9 @@ bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; 
 
 int check_cache(const mk_kv_cache& c, const char* who)
 {
-    if (c.page_size == 0 || c.page_size > 0x7fffffffu || c.n_pages > 0x7fffffffu || c.n_heads == 0 || c.n_heads > 65535u || c.dim == 0 ||
+    if (c.page_size == 0 || c.page_size > (1u << 24) || c.n_pages > 0x7fffffffu || c.n_heads == 0 || c.n_heads > 65535u || c.dim == 0 ||
         (c.dim & 15u) || c.dim > 256u)
-        return fail(MK_ERR_INVALID_ARGUMENT, "%s: page_size %u, n_pages %u, n_heads %u (at most 65535), dim %u (a multiple of 16, at most 256)",
+        return fail(MK_ERR_INVALID_ARGUMENT, "%s: page_size %u (at most 2^24), n_pages %u, n_heads %u (at most 65535), dim %u (a multiple of 16, at most 256)",
                     who, c.page_size, c.n_pages, c.n_heads, c.dim);
     if (((c.page_stride | c.head_stride | c.token_stride) & 15u) || c.token_stride < c.dim)
         return fail(MK_ERR_INVALID_ARGUMENT, "%s: strides of %llu, %llu and %llu bytes: multiples of 16, a token's at least dim", who,
@@ -913,6 +913,8 @@ int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries
     if (!q->workspace || q->workspace_bytes < mk_kv_attention_bytes(cache, q))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: a workspace of %llu bytes is required",
                     (unsigned long long)mk_kv_attention_bytes(cache, q));
+    if (q->out == q->q)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: out is q, which CTAs read until the last one is done");
     DeviceGuard g(s->device);
     mk::KvAttendArgs a;
     std::memset(&a, 0, sizeof a);

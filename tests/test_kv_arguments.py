@@ -102,7 +102,7 @@ def test_the_library_refuses_rows_of_logits():
 
 
 CACHE = dict(k=AT, v=AT, k_scale=AT, v_scale=AT, page_stride=2 * 16 * 64, head_stride=16 * 64, token_stride=64, n_pages=4, n_heads=2, page_size=16, dim=64)
-BAD_CACHES = [(dict(page_size=0), "page_size"), (dict(n_heads=0), "n_heads"), (dict(n_heads=65536), "n_heads"), (dict(dim=0), "dim"), (dict(dim=72), "dim"),
+BAD_CACHES = [(dict(page_size=(1 << 24) + 1), "page_size"), (dict(page_size=0), "page_size"), (dict(n_heads=0), "n_heads"), (dict(n_heads=65536), "n_heads"), (dict(dim=0), "dim"), (dict(dim=72), "dim"),
               (dict(dim=272, token_stride=272), "dim"), (dict(n_pages=1 << 31), "n_pages"), (dict(page_size=1 << 31), "page_size"),
               (dict(page_stride=8), "strides"), (dict(head_stride=1000), "strides"), (dict(token_stride=48), "strides"), (dict(token_stride=72), "strides"),
               (dict(k=None), "required"), (dict(v_scale=None), "required"), (dict(k=AT + 8), "16-byte"), (dict(v=AT + 4), "16-byte")]
@@ -143,4 +143,5 @@ def test_the_library_refuses_attention():
                      (dict(workspace=None), "workspace"), (dict(workspace_bytes=1000), "workspace"), (dict(n_tokens=(1 << 30) + 1), "n_tokens")]:
         refused(call(**kw), what)
     assert call(n_seq=0) == 0 and call(n_tokens=0) == 0
+    refused(call(), "out is q")
     refused(lib.mk_kv_attention(None, None, None, None), "null")
