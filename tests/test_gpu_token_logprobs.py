@@ -52,6 +52,15 @@ def test_rows(sampler, kind, rows, vocab, top):
     check(sampler, x, tokens, 0.7, top)
 
 
+@pytest.mark.parametrize("given", [0, 33, 300, 1000])
+@pytest.mark.parametrize("rows", [2, 500])
+def test_many_tokens_of_a_row(sampler, rows, given):
+    rng = np.random.default_rng(given)
+    x = torch.from_numpy(rng.normal(0, 3, (rows, 9001)).astype(np.float32)).to(torch.bfloat16).cuda()
+    tokens = torch.from_numpy(rng.integers(-1, 9001, (rows, given)).astype(np.int32)).cuda()
+    check(sampler, x, tokens, 1.3, 5, rng.random((rows, 9001)) < 0.6)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_masks_and_temperatures_of_the_rows(sampler, kind):
     rng = np.random.default_rng(3)
