@@ -7,7 +7,7 @@
 // dividing by a scale is exact.
 //
 // Angles are formed and brought into [-pi, pi] in 64 bits (position x frequency in 32 bits is off by 0.06 rad at a million), their sine and
-// cosine in 32.
+// cosine in 32, with what an angle loses by its own rounding added.
 //
 // 64 tokens of a decode step take 6.5 us from a graph, 8 key heads of 128 with 32 query heads; chunks of some 7000 tokens 69, where
 // reading and writing once would take 21: instructions bound it, of angles (a third) and of roundings. Two heads a CTA: with one 85 us, whose angles
@@ -166,9 +166,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
                         const uint32_t t = i / half, f = i - t * half;
                         const double x = (double)a.positions[t0 + i0 + t] * (double)__ldg(a.inv_freq + f);
                         const double whole = rint(x * 0.15915494309189533577);
+                        const double left = fma(whole, -6.28318530717958647693, x);
+                        const float angle = (float)left, rest = (float)(left - angle); // (up to 2^-23 at pi)
                         float sine, cosine;
-                        sincosf((float)fma(whole, -6.28318530717958647693, x), &sine, &cosine);
-                        cs[i] = make_float2(cosine * a.rotary_scale, sine * a.rotary_scale);
+                        sincosf(angle, &sine, &cosine);
+                        cs[i] = make_float2(fmaf(-sine, rest, cosine) * a.rotary_scale, fmaf(cosine, rest, sine) * a.rotary_scale);
                     }
                     __syncthreads();
                 }
