@@ -29,6 +29,11 @@ constexpr uint32_t kConvert = 512, kIssue = 640; // first thread of those that c
 constexpr uint32_t kSlots = 4;                   // of what softmax reads beside the scores
 constexpr float kWeightUnit = 128.0f;
 constexpr uint32_t kMixed = 8; // blocks of a segment that some rows see and others do not: at most 3 at either end
+// Places for what a segment's softmax reads at its end, by the segment's number. Those that convert wait for products alone, and a segment may
+// be one block long: at the end of a segment s - 1 they know that the scores of the block two before its last are done. With segments s - 3
+// and s - 2 in front of it that block is of s - 3 at least, whose scores wait for all of its queries (q_full), and there every thread of the
+// softmax arrives behind its segment s - 4. (With two places a short segment's outputs got the unit of the one after the next.)
+constexpr uint32_t kHeld = 4;
 
 struct Shared {
     uint64_t find[40];
@@ -38,9 +43,9 @@ struct Shared {
     alignas(16) float key[kSlots][kBlock], value[kSlots][kBlock]; // scales; values' over the largest so far, times kWeightUnit
     alignas(16) uint32_t missing[kSlots][4]; // tokens whose page is not there
     float older[kSlots];               // what outputs so far are worth in the block's unit
-    float unit[2];                     // the largest scale of a segment's values, by its parity
-    uint32_t n_mixed[2];
-    uint32_t mixed[2][kMixed][5];      // a block and which of its values are NaN
+    float unit[kHeld];                 // the largest scale of a segment's values
+    uint32_t n_mixed[kHeld];
+    uint32_t mixed[kHeld][kMixed][5];  // a block and which of its values are NaN
     uint64_t off[2][kBlock];
     float warp_most[4];
     float top[2][kUnitRows], most[2][kUnitRows], sum[2][kUnitRows]; // what the two threads of a row tell one another
@@ -225,14 +230,13 @@ struct Converter {
 
     __device__ __forceinline__ void run(const KvAttendArgs& a, Shared& s, const Ring<D>& ring, const Segment& g)
     {
-        const uint32_t tid = threadIdx.x - kConvert, lane = tid & 31u;
+        const uint32_t tid = threadIdx.x - kConvert, lane = tid & 31u, held = segments++ % kHeld;
         const int32_t* table = a.block_table + (uint64_t)g.sq * a.table_ld;
         float unit = 0.0f;
         Place p = place(a, g, look_up(a, g, table, g.from), g.from);
         uint32_t page = look_up(a, g, table, g.from + 1u);
         if (tid == 0)
-            s.n_mixed[segments & 1u] = 0; // (that of the segment before the last one has been read: its successor's softmax has begun)
-        ++segments;
+            s.n_mixed[held] = 0; // (see kHeld)
         s.off[blocks & 1u][tid] = p.off;
         __syncwarp();
         named_barrier(2, 128);
@@ -271,7 +275,7 @@ struct Converter {
             for (uint32_t i = 0; i < loads; ++i)
                 store(keys[i * 128u + tid], ring.k(stage), i);
             if (!more && tid == 0)
-                s.unit[(segments - 1u) & 1u] = unit;
+                s.unit[held] = unit;
             p = next;
             fence_proxy_async();
             __syncwarp();
@@ -282,14 +286,14 @@ struct Converter {
             if (more)
                 copy(keys, a.c.k, s.off[stage ^ 1u]);
             if (b * kBlock < g.see_from || (b + 1u) * kBlock > g.see_to) { // some rows see what others do not
-                const uint32_t which = s.n_mixed[(segments - 1u) & 1u];
-                uint32_t* at = s.mixed[(segments - 1u) & 1u][which < kMixed ? which : kMixed - 1u];
+                const uint32_t which = s.n_mixed[held];
+                uint32_t* at = s.mixed[held][which < kMixed ? which : kMixed - 1u];
                 __syncwarp();
                 named_barrier(2, 128);
                 if (tid < 5u)
                     at[tid] = tid ? 0u : b;
                 if (tid == 0)
-                    s.n_mixed[(segments - 1u) & 1u] = which < kMixed ? which + 1u : kMixed;
+                    s.n_mixed[held] = which < kMixed ? which + 1u : kMixed;
                 __syncwarp();
                 named_barrier(2, 128);
                 take_out(v, at + 1);
@@ -390,7 +394,7 @@ struct Softmax {
         constexpr uint32_t columns = D / 2;
         const uint32_t warp = threadIdx.x / 32u, t = warp / 8u, half = warp / 4u % 2u, quarter = warp % 4u;
         const uint32_t row = t * kTileRows + quarter * 32u + (threadIdx.x & 31u), pair = 3u + t * 4u + quarter;
-        const uint32_t n = g.to - g.from, which = segments & 1u;
+        const uint32_t n = g.to - g.from, which = segments % kHeld;
         // the row's queries, times a power of two that brings the largest to 2^12 (1 where a row is nothing or infinite)
         const uint32_t unit_row = g.row0 + row, token = kv_token_of(a, unit_row), head = g.head * a.group + (unit_row - token * a.group);
         const bool real = row < g.rows;
