@@ -386,7 +386,7 @@ int mk_token_logprobs(mk_sampler* s, const mk_logprob_rows* rows, float* logprob
                       float* top_logprob, uint32_t* flags, void* stream);
 
 /* A paged cache of keys and values in 8 bits: e4m3 codes (a sign, four bits of exponent, three of mantissa; 0x7f and 0xff are NaN,
- * there are no infinities), a scale for each page and head, 0 or more. What a code stands for times its scale is the value. A page's head is
+ * there are no infinities), a scale for each page and head, 0 or more, finite. What a code stands for times its scale is the value. A page's head is
  * page_size rows of dim codes; strides are in bytes, multiples of 16, the same for k and v, which start on 16-byte boundaries. The
  * pages are those of mk_kv_pages. */
 typedef struct mk_kv_cache {
@@ -457,9 +457,10 @@ typedef struct mk_kv_queries {
 
 /* out[t][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q[t][h] . k_j), over the keys j that the token sees. Keys whose page is outside of the
  * cache (a table entry of -1) are not there; a row that sees none is zeros. Rows of q that are no sequence's are left as they are in out.
- * dim is 64 or 128. Products are of fp16 numbers that codes and queries become without a loss, weights are rounded to fp16 (2^-11 of
- * each), sums and softmax in fp32. A value that is not a number makes rows that see it NaN (in its column at least), no others. Uses
- * nothing of the handle but its device. */
+ * dim is 64 or 128. Products are of fp16 numbers that codes and queries become without a loss; weights p_j s_j, s_j the scale of value j, are
+ * rounded to fp16 in a unit of the row's own, by 2^-11 of each down to 2^-21 of the row's largest, by 2^-32 of that one below (a key whose
+ * p_j is under 2^-100 of the row's largest may count for less); sums and softmax in fp32. A value that is not a number makes rows that see it
+ * NaN (in its column at least), no others. Uses nothing of the handle but its device. */
 uint64_t mk_kv_attention_bytes(const mk_kv_cache* cache, const mk_kv_queries* queries);
 int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries* queries, void* stream);
 

@@ -15,8 +15,8 @@
 // Codes become fp16 (exactly) on the way from shared memory into registers, in the order in which the tensor core wants them: of a block's
 // keys a lane reads 16 of a token's columns, four steps of the contraction; of its values the four tokens whose weights it holds, which
 // byte permutations put side by side. Queries are fp16 too, each row times the power of two that brings its largest to about 2^12: bf16 loses
-// nothing by it. Scales of keys go into the scores, scales of values into the weights: 2^7 v_j / v p_j is what fp16 holds, v being the
-// largest scale so far, so that a weight's rounding is 2^-11 of it down to 2^-21 of the largest; sums are in fp32.
+// nothing by it. Scales of keys go into the scores, scales of values into the weights, which fp16 holds in a unit of the row's own (kv_unit in
+// kv_work.cuh); sums are in fp32.
 #include "kv_cache.cuh"
 #include "kv_work.cuh"
 #include "ptx.cuh"
@@ -29,7 +29,6 @@ namespace {
 constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
 constexpr uint32_t kStages = 2;
 constexpr uint32_t kTile = 16, kBlockTokens = 32; // rows of a unit, keys of a block
-constexpr float kWeightUnit = 128.0f;
 
 template <uint32_t D>
 constexpr uint32_t kStageBytes = 2 * kBlockTokens * (D + 4); // keys and values, two scales a token
@@ -207,7 +206,7 @@ template <uint32_t D>
 struct Running {
     float m[2], l[2], o[D / 8][4];
     float factor[2];
-    float unit, value_by; // the largest scale of values so far, and what makes weights of it
+    float unit[2]; // see kv_unit
 };
 
 // Is one of four codes NaN? And the codes without those.
@@ -237,19 +236,19 @@ __device__ __forceinline__ void add_block(Running<D>& x, const Shared<D>& s, con
         }
     }
     float2 vs[NT];
-    float unit = x.unit;
+    float v_most = 0.0f;
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n) {
         const float2 ks = *reinterpret_cast<const float2*>(scales + n * 8u + 2u * c);
         vs[n] = *reinterpret_cast<const float2*>(scales + tokens + n * 8u + 2u * c);
-        unit = fmaxf(unit, fmaxf(vs[n].x, vs[n].y));
+        v_most = fmaxf(v_most, fmaxf(vs[n].x, vs[n].y));
         t[n][0] *= ks.x * x.factor[0];
         t[n][1] *= ks.y * x.factor[0];
         t[n][2] *= ks.x * x.factor[1];
         t[n][3] *= ks.y * x.factor[1];
     }
-    unit = fmaxf(unit, __shfl_xor_sync(~0u, unit, 1));
-    unit = fmaxf(unit, __shfl_xor_sync(~0u, unit, 2));
+    v_most = fmaxf(v_most, __shfl_xor_sync(~0u, v_most, 1));
+    v_most = fmaxf(v_most, __shfl_xor_sync(~0u, v_most, 2));
     auto sees = [&](uint32_t n, uint32_t e) {
         const uint32_t j = n * 8u + 2u * c + (e & 1u), r = g + (e >> 1) * 8u;
         const int32_t key = (int32_t)(block * tokens + j);
@@ -263,49 +262,63 @@ __device__ __forceinline__ void add_block(Running<D>& x, const Shared<D>& s, con
                 if (!sees(n, e))
                     t[n][e] = -INFINITY;
     }
-    float older = 1.0f;
-    if (unit > x.unit) { // (in all lanes)
-        older = x.unit / unit;
-        x.unit = unit;
-        x.value_by = kWeightUnit / unit;
-    }
-    uint4 p[NT / 2];
-    bool changed = older != 1.0f;
-    float by[2];
+    float from[2];
+    bool grows = false; // may a row's unit have to grow? By the largest scale of all these keys, seen or not: whether it does is looked up below
+    const float v_log = __log2f(v_most);
 #pragma unroll
     for (uint32_t r = 0; r < 2; ++r) {
-        float m = x.m[r];
+        float most = -INFINITY;
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n)
-            m = fmaxf(m, fmaxf(t[n][2 * r], t[n][2 * r + 1]));
-        m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
-        const float from = m == -INFINITY ? 0.0f : m;
-        by[r] = ex2_approx(x.m[r] - from);
-        changed = changed || m != x.m[r];
+            most = fmaxf(most, fmaxf(t[n][2 * r], t[n][2 * r + 1]));
+        most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
+        const float m = fmaxf(x.m[r], most);
+        from[r] = m == -INFINITY ? 0.0f : m;
+        const float by = ex2_approx(x.m[r] - from[r]);
         x.m[r] = m;
         float l = 0.0f;
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) {
-            const float a = ex2_approx(t[n][2 * r] - from), b = ex2_approx(t[n][2 * r + 1] - from);
+            const float a = ex2_approx(t[n][2 * r] - from[r]), b = ex2_approx(t[n][2 * r + 1] - from[r]);
             l += a + b;
-            t[n][2 * r] = a * (vs[n].x * x.value_by);
-            t[n][2 * r + 1] = b * (vs[n].y * x.value_by);
+            const float2 w = mul2(make_float2(a, b), vs[n]);
+            t[n][2 * r] = w.x;
+            t[n][2 * r + 1] = w.y;
         }
-        x.l[r] = x.l[r] * by[r] + l;
-        by[r] *= older;
+        x.l[r] = x.l[r] * by + l;
+        grows = grows || kv_unit(x.unit[r], most + v_log, from[r]) != x.unit[r];
     }
+    if (__any_sync(~0u, grows)) {
+        float older[2]; // what outputs so far are worth
 #pragma unroll
-    for (uint32_t n = 0; n < NT; n += 2)
-        p[n / 2] = make_uint4(pair_of(t[n][0], t[n][1]), pair_of(t[n][2], t[n][3]), pair_of(t[n + 1][0], t[n + 1][1]), pair_of(t[n + 1][2], t[n + 1][3]));
-    if (__any_sync(~0u, changed)) {
+        for (uint32_t r = 0; r < 2; ++r) {
+            float top = 0.0f;
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n)
+                top = fmaxf(top, fmaxf(t[n][2 * r], t[n][2 * r + 1]));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            const float unit = kv_unit(x.unit[r], from[r] + __log2f(top), from[r]);
+            older[r] = unit == x.unit[r] ? 1.0f : kv_worth(x.unit[r], unit);
+            x.unit[r] = unit;
+        }
 #pragma unroll
         for (uint32_t j = 0; j < D / 8; ++j) {
-            x.o[j][0] *= by[0];
-            x.o[j][1] *= by[0];
-            x.o[j][2] *= by[1];
-            x.o[j][3] *= by[1];
+            x.o[j][0] *= older[0];
+            x.o[j][1] *= older[0];
+            x.o[j][2] *= older[1];
+            x.o[j][3] *= older[1];
         }
+    }
+    uint4 p[NT / 2];
+    const float e0 = ex2_approx(from[0] - x.unit[0]), e1 = ex2_approx(from[1] - x.unit[1]);
+    const float2 by0 = make_float2(e0, e0), by1 = make_float2(e1, e1);
+#pragma unroll
+    for (uint32_t n = 0; n < NT; n += 2) {
+        const float2 w0 = mul2(make_float2(t[n][0], t[n][1]), by0), w1 = mul2(make_float2(t[n][2], t[n][3]), by1);
+        const float2 w2 = mul2(make_float2(t[n + 1][0], t[n + 1][1]), by0), w3 = mul2(make_float2(t[n + 1][2], t[n + 1][3]), by1);
+        p[n / 2] = make_uint4(pair_of(w0.x, w0.y), pair_of(w1.x, w1.y), pair_of(w2.x, w2.y), pair_of(w3.x, w3.y));
     }
     const unsigned char* values = stage + tokens * D;
 #pragma unroll
@@ -434,10 +447,10 @@ __global__ void __launch_bounds__(kThreads, 3) kv_rows_kernel(const KvAttendArgs
         __syncthreads();
         const uint32_t see_from = (uint32_t)s.lo[u.rows - 1u], see_to = (uint32_t)s.hi[0];
         Running<D> x;
-        x.unit = x.value_by = 0.0f;
 #pragma unroll
         for (uint32_t r = 0; r < 2; ++r) {
             x.factor[r] = s.factor[g + 8u * r];
+            x.unit[r] = INFINITY;
             x.m[r] = -INFINITY;
             x.l[r] = 0.0f;
         }
@@ -462,9 +475,9 @@ __global__ void __launch_bounds__(kThreads, 3) kv_rows_kernel(const KvAttendArgs
         copies_wait<0>();
         __syncthreads();
         float* mine = reinterpret_cast<float*>(raw + warp * kRingBytes<D>);
-        const float worth = x.unit / kWeightUnit;
 #pragma unroll
         for (uint32_t r = 0; r < 2; ++r) {
+            const float worth = kv_worth(x.unit[r], x.m[r]);
             float l = x.l[r];
             l += __shfl_xor_sync(~0u, l, 1);
             l += __shfl_xor_sync(~0u, l, 2);

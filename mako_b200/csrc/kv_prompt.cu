@@ -7,8 +7,8 @@
 // A unit has 256 rows, two tiles of the MMA's M, that take turns: while one tile's scores become weights, the tensor core works for the
 // other. One warp issues; eight a tile (two threads a row) turn scores into weights; four turn the cache's codes into fp16, K-major for the
 // keys, the same bytes read as MN-major for the values. Scores and outputs are in tensor memory; weights take the scores' place, as the A
-// operand of the second product. An output is multiplied only where a row's maximum has grown by more than 2^8, or the largest scale of
-// values. Rounding is that of kv_attend.cu: queries, codes exactly, weights to fp16.
+// operand of the second product. A sum is multiplied only where a row's maximum has grown by more than 2^8, outputs where the row's largest weight
+// has (kv_unit in kv_work.cuh). Rounding is that of kv_attend.cu: queries, codes exactly, weights to fp16.
 //
 // What it came from: a thread a row with its 128 scores in registers 2058 us (registers are shared by 12 warps then), half of them at a time
 // 1650; two threads a row did not help until a scale for each key was no longer read for each (shared memory: 52 % to 35 %; 1580); pages looked
@@ -27,7 +27,6 @@ constexpr uint32_t kTileRows = 128, kUnitRows = 256, kBlock = 128; // rows of a 
 constexpr uint32_t kThreads = 672;
 constexpr uint32_t kConvert = 512, kIssue = 640; // first thread of those that convert, and of the warp that issues
 constexpr uint32_t kSlots = 4;                   // of what softmax reads beside the scores
-constexpr float kWeightUnit = 128.0f;
 constexpr uint32_t kMixed = 8; // blocks of a segment that some rows see and others do not: at most 3 at either end
 // Places for what a segment's softmax reads at its end, by the segment's number. Those that convert wait for products alone, and a segment may
 // be one block long: at the end of a segment s - 1 they know that the scores of the block two before its last are done. With segments s - 3
@@ -40,14 +39,12 @@ struct Shared {
     uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
     uint32_t tmem;
     int failed;
-    alignas(16) float key[kSlots][kBlock], value[kSlots][kBlock]; // scales; values' over the largest so far, times kWeightUnit
+    alignas(16) float key[kSlots][kBlock], value[kSlots][kBlock], value_log[kSlots][kBlock]; // scales; log2 of values'
+    float2 log_range[kSlots][kBlock / 16]; // of 16 of them: the largest and the smallest
     alignas(16) uint32_t missing[kSlots][4]; // tokens whose page is not there
-    float older[kSlots];               // what outputs so far are worth in the block's unit
-    float unit[kHeld];                 // the largest scale of a segment's values
     uint32_t n_mixed[kHeld];
     uint32_t mixed[kHeld][kMixed][5];  // a block and which of its values are NaN
     uint64_t off[2][kBlock];
-    float warp_most[4];
     float top[2][kUnitRows], most[2][kUnitRows], sum[2][kUnitRows]; // what the two threads of a row tell one another
 };
 
@@ -232,7 +229,6 @@ struct Converter {
     {
         const uint32_t tid = threadIdx.x - kConvert, lane = tid & 31u, held = segments++ % kHeld;
         const int32_t* table = a.block_table + (uint64_t)g.sq * a.table_ld;
-        float unit = 0.0f;
         Place p = place(a, g, look_up(a, g, table, g.from), g.from);
         uint32_t page = look_up(a, g, table, g.from + 1u);
         if (tid == 0)
@@ -251,31 +247,27 @@ struct Converter {
             page = look_up(a, g, table, b + 2u);
             s.off[stage ^ 1u][tid] = next.off;
             // what the softmax wants to know of the block
-            float most = p.off != ~0ull ? p.value : 0.0f;
-#pragma unroll
-            for (uint32_t d = 16; d; d >>= 1)
-                most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-            if (lane == 0)
-                s.warp_most[tid / 32u] = most;
             const uint32_t missing = __ballot_sync(~0u, p.off == ~0ull && b * kBlock + tid < g.seq.len);
             alive = alive && await(s, &s.k_empty[stage], parity ^ 1u);
             __syncwarp(); // (barriers want whole warps)
-            named_barrier(2, 128); // (the block before has read warp_most, and this block's are there)
-            const float largest = fmaxf(fmaxf(s.warp_most[0], s.warp_most[1]), fmaxf(s.warp_most[2], s.warp_most[3]));
-            const float now = fmaxf(unit, largest);
             s.key[slot][tid] = p.key;
-            s.value[slot][tid] = now > 0.0f ? p.value * (kWeightUnit / now) : 0.0f;
+            s.value[slot][tid] = p.value;
+            const float value_log = __log2f(p.value);
+            s.value_log[slot][tid] = value_log;
+            if (a.c.page_size % 16u) { // (else 16 have one)
+                float2 range = p.off != ~0ull ? make_float2(value_log, value_log) : make_float2(-INFINITY, INFINITY);
+#pragma unroll
+                for (uint32_t d = 8; d; d >>= 1)
+                    range = make_float2(fmaxf(range.x, __shfl_xor_sync(~0u, range.x, d)), fminf(range.y, __shfl_xor_sync(~0u, range.y, d)));
+                if (tid % 16u == 0)
+                    s.log_range[slot][tid / 16u] = range;
+            }
             if (lane == 0)
                 s.missing[slot][tid / 32u] = missing;
-            if (tid == 0)
-                s.older[slot] = now > 0.0f ? unit / now : 1.0f;
-            unit = now;
             asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
             for (uint32_t i = 0; i < loads; ++i)
                 store(keys[i * 128u + tid], ring.k(stage), i);
-            if (!more && tid == 0)
-                s.unit[held] = unit;
             p = next;
             fence_proxy_async();
             __syncwarp();
@@ -448,13 +440,13 @@ struct Softmax {
         if (t && g.rows <= kTileRows)
             return;
         const uint32_t lanes = (quarter * 32u) << 16, scores = s.tmem + lanes + t * 128u + half * 64u, out = s.tmem + lanes + 256u + t * 128u + half * columns;
-        float ref = -INFINITY, l = 0.0f;
+        float ref = -INFINITY, unit = INFINITY, l = 0.0f;
         for (uint32_t j = 0; j < n; ++j, ++seen) {
             const uint32_t slot = (first + j) % kSlots, begin = (g.from + j) * kBlock;
             alive = alive && await(s, &s.s_full[t], seen & 1u);
             __syncwarp(); // (a warp that gave up goes on: its row's other thread meets it at barriers)
             tc_fence_after();
-            const float *key = s.key[slot] + 64u * half, *value = s.value[slot] + 64u * half;
+            const float *key = s.key[slot] + 64u * half, *value = s.value[slot] + 64u * half, *value_log = s.value_log[slot] + 64u * half;
             const uint2 gone = *reinterpret_cast<const uint2*>(&s.missing[slot][2u * half]);
             const int32_t low = lo - (int32_t)(begin + 64u * half), high = hi - (int32_t)(begin + 64u * half);
             const bool some = __any_sync(~0u, (gone.x | gone.y) != 0 || low > 0 || high < 64);
@@ -482,7 +474,7 @@ struct Softmax {
             };
             // what makes exponents of 16 scores (not 0, as f)
             auto factor = [&](uint32_t i) { return Group == 1 ? f : fmaxf(f * key[i], 1e-37f); };
-            float most = -INFINITY;
+            float most = -INFINITY, peak = -INFINITY; // log2 of the largest p and of the largest weight
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) {
                 float x[32];
@@ -493,21 +485,36 @@ struct Softmax {
 #pragma unroll
                     for (uint32_t m = 0; m < 4; ++m)
                         tops[m] = fmaxf(fmaxf(x[k + m], x[k + m + 4]), fmaxf(x[k + m + 8], x[k + m + 12]));
-                    most = fmaxf(most, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * factor(32u * i + k));
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * factor(32u * i + k);
+                    most = fmaxf(most, top);
+                    const float2 range = Group == 1 ? s.log_range[slot][4u * half + 2u * i + k / 16u] : make_float2(value_log[32u * i + k], 0.0f);
+                    if (Group != 1 || range.x - range.y <= kHighSlack) {
+                        peak = fmaxf(peak, top + range.x);
+                    } else { // scales that are far from one another: each by itself
+#pragma unroll
+                        for (uint32_t m = 0; m < 16; m += 4) {
+                            const float4 c = reinterpret_cast<const float4*>(value_log)[8u * i + (k + m) / 4];
+                            const float2 f2 = make_float2(f, f);
+                            const float2 y = fma2(make_float2(x[k + m], x[k + m + 1]), f2, make_float2(c.x, c.y));
+                            const float2 z = fma2(make_float2(x[k + m + 2], x[k + m + 3]), f2, make_float2(c.z, c.w));
+                            peak = fmaxf(peak, fmaxf(fmaxf(y.x, y.y), fmaxf(z.x, z.y)));
+                        }
+                    }
                 }
             }
             s.most[half][row] = most;
+            s.top[half][row] = peak;
             __syncwarp();
             named_barrier(pair, 64);
             most = fmaxf(most, s.most[half ^ 1u][row]);
-            const float older = s.older[slot];
-            float by = older;
+            peak = fmaxf(peak, s.top[half ^ 1u][row]);
             if (most > ref + 8.0f || ref == -INFINITY) { // (-inf: nothing seen yet; its outputs and sum are zeros)
                 const float to = most > ref ? most : ref;
-                by = ref == -INFINITY ? (to == -INFINITY ? older : 0.0f) : older * ex2_approx(ref - to);
                 l *= ref == -INFINITY ? 1.0f : ex2_approx(ref - to);
                 ref = to;
             }
+            const float now = kv_unit(unit, peak, ref), by = now == unit ? 1.0f : kv_worth(unit, now);
+            unit = now;
             __syncwarp();
             if (j && __any_sync(~0u, by != 1.0f)) {
 #pragma unroll 1
@@ -523,6 +530,7 @@ struct Softmax {
             }
             const float from = ref == -INFINITY ? 0.0f : ref;
             const float2 minus = make_float2(-from, -from);
+            const float each_is = ex2_approx(from - unit); // (0 where there is no weight yet)
             float2 sum = make_float2(0.0f, 0.0f), more = sum;
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) {
@@ -532,14 +540,19 @@ struct Softmax {
 #pragma unroll
                 for (uint32_t k = 0; k < 32; k += 4) {
                     const float by_f = factor(32u * i + k / 16u * 16u);
-                    const float4 c = Group == 1 ? reinterpret_cast<const float4*>(value)[8u * i + k / 4] : make_float4(value[32u * i + k / 16u * 16u], 0.0f, 0.0f, 0.0f);
+                    // what makes a weight of p. (Where 16 have one, at most 2^127: above, p is below 2^-112 of the largest, and not to become NaN where it is 0.)
+                    const float4 c = Group == 1 ? reinterpret_cast<const float4*>(value)[8u * i + k / 4] : make_float4(fminf(value[32u * i + k / 16u * 16u] * each_is, 0x1p127f), 0.0f, 0.0f, 0.0f);
                     const float2 c0 = Group == 1 ? make_float2(c.x, c.y) : make_float2(c.x, c.x), c1 = Group == 1 ? make_float2(c.z, c.w) : c0;
                     const float2 f2 = make_float2(by_f, by_f);
                     const float2 d = fma2(make_float2(x[k], x[k + 1]), f2, minus), e = fma2(make_float2(x[k + 2], x[k + 3]), f2, minus);
                     const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y)), q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
                     sum = add2(sum, p);
                     more = add2(more, q);
-                    const float2 y = mul2(p, c0), z = mul2(q, c1);
+                    float2 y = mul2(p, c0), z = mul2(q, c1);
+                    if constexpr (Group == 1) {
+                        y = mul2(y, make_float2(each_is, each_is));
+                        z = mul2(z, make_float2(each_is, each_is));
+                    }
                     w[k / 2] = pair_of(y.x, y.y);
                     w[k / 2 + 1] = pair_of(z.x, z.y);
                 }
@@ -571,7 +584,7 @@ struct Softmax {
             }
         }
         __syncwarp();
-        const float worth = s.unit[which] / kWeightUnit;
+        const float worth = kv_worth(unit, ref);
         T* to = static_cast<T*>(a.out) + (g.seq.first + token) * a.out_ld + (uint64_t)head * D + half * columns;
         const float by = part ? worth : l == 0.0f ? 0.0f : worth / l;
 #pragma unroll 1

@@ -6,6 +6,7 @@
 // the eight units of a sequence of 50 keys among 37 of up to 6000, and the others waited for it: 36 us
 // where it takes 25.) Lengths are known on the device alone, so every CTA forms the sums by itself.
 #pragma once
+#include "ptx.cuh"
 #include "round_ops.h"
 
 namespace mk {
@@ -93,6 +94,20 @@ __device__ __forceinline__ uint64_t kv_cut(uint64_t total, uint32_t n, uint32_t 
     const uint32_t each = (uint32_t)total / n, more = (uint32_t)total - each * n;
     return (uint64_t)each * i + min(i, more);
 }
+
+// What a row's weights p_j v_j (v_j: the scale of key j's values) are held in, as fp16: a weight of 1 is 2^unit, where exponents of p are those
+// of its scores. Whatever the row does not see, and whatever scales there are elsewhere, has no part in it: its largest weight so far is from 2^7 to
+// 2^15, so that one is rounded by 2^-11 of it down to 2^-21 of the largest. `high`: log2 of the largest weight of a block (-inf: none), too large by
+// kHighSlack at most; `ref`: that of p = 1, which a unit is at most 2^126 below, so that what it is multiplied by is a number. +inf: no weight yet.
+constexpr float kHighSlack = 3.0f;
+__device__ __forceinline__ float kv_unit(float unit, float high, float ref)
+{
+    if (high > unit + 15.0f || (unit == INFINITY && high > -INFINITY))
+        unit = high - (7.0f + kHighSlack);
+    return fmaxf(unit, ref - 126.0f);
+}
+// What outputs in one unit are worth in another.
+__device__ __forceinline__ float kv_worth(float unit, float in) { return unit == INFINITY ? 0.0f : ex2_approx(unit - in); }
 
 // A CTA's share of all work, [at, end), and the unit that it begins in, `skip` behind the unit's begin. kv_take gives one segment after the
 // other. A unit's blocks come first, what else it costs behind them.
