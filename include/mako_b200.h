@@ -457,7 +457,8 @@ typedef struct mk_kv_queries {
 
 /* out[t][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q[t][h] . k_j), over the keys j that the token sees. Keys whose page is outside of the
  * cache (a table entry of -1) are not there; a row that sees none is zeros. Rows of q that are no sequence's are left as they are in out.
- * dim is 64 or 128. Products are of fp16 numbers that codes and queries become without a loss; weights p_j s_j, s_j the scale of value j, are
+ * dim is 64 or 128. Products are of fp16 numbers, which codes become without a loss, and queries, each row times a power of two: its numbers down
+ * to 2^-26 of its largest (from 2^-88 up) without a loss, below off by 2^-37 of it; weights p_j s_j, s_j the scale of value j, are
  * rounded to fp16 in a unit of the row's own, by 2^-11 of each down to 2^-21 of the row's largest, by 2^-32 of that one below (a key whose
  * p_j is under 2^-100 of the row's largest may count for less); sums and softmax in fp32. A value that is not a number makes rows that see it
  * NaN (in its column at least), no others. Uses nothing of the handle but its device. */

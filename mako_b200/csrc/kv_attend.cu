@@ -15,7 +15,7 @@
 // Codes become fp16 (exactly) on the way from shared memory into registers, in the order in which the tensor core wants them: of a block's
 // keys a lane reads 16 of a token's columns, four steps of the contraction; of its values the four tokens whose weights it holds, which
 // byte permutations put side by side. Queries are fp16 too, each row times the power of two that brings its largest to about 2^12: bf16 loses
-// nothing by it. Scales of keys go into the scores, scales of values into the weights, which fp16 holds in a unit of the row's own (kv_unit in
+// nothing by it down to 2^-29 of that one. Scales of keys go into the scores, scales of values into the weights, which fp16 holds in a unit of the row's own (kv_unit in
 // kv_work.cuh); sums are in fp32.
 #include "kv_cache.cuh"
 #include "kv_work.cuh"
@@ -117,9 +117,9 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D>& s, const KvSegmen
 #pragma unroll
         for (uint32_t d = 1; d < chunks; d <<= 1)
             most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-        // a power of two; 1 where a row is nothing or infinite
+        // a power of two, from 2^-115; 1 where a row is nothing or infinite
         const int e = (int)(__float_as_uint(most) >> 23) - 127;
-        const int up = most > 0.0f && e < 128 ? max(-100, min(100, 12 - e)) : 0;
+        const int up = most > 0.0f && e < 128 ? min(100, 12 - e) : 0;
         const float by = __uint_as_float((uint32_t)(up + 127) << 23);
         uint32_t* to = reinterpret_cast<uint32_t*>(s.q) + (chunk / 4u * 128u + (r & 7u) * 4u + (chunk & 3u)) * 4u + (r >> 3);
 #pragma unroll

@@ -412,7 +412,7 @@ struct Softmax {
             named_barrier(pair, 64);
             top = fmaxf(top, s.top[half ^ 1u][row]);
             const int e = (int)(__float_as_uint(top) >> 23) - 127;
-            const int up = top > 0.0f && e < 128 ? max(-100, min(100, 12 - e)) : 0;
+            const int up = top > 0.0f && e < 128 ? min(100, 12 - e) : 0;
             const float by = __uint_as_float((uint32_t)(up + 127) << 23), turned = a.scale_log2 < 0.0f ? -by : by;
             f = fmaxf(fabsf(a.scale_log2) / by, 1e-37f); // (not 0: a key that the row does not see has -inf times this)
             alive = alive && await(s, &s.q_empty, (segments & 1u) ^ 1u);

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_kv_attention import make, sampler  # noqa: F401
+from tests.test_gpu_kv_attention import check as check_at, make, sampler  # noqa: F401
 from tests import kv_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -97,3 +97,18 @@ def test_the_smallest_and_largest_scales(sampler, new, page, scale):  # noqa: F8
     assert scale == -140 or (out[:int(start[-1])] != 0).any(2).all()
     cache.v_scale[::2] = 2.0 ** (scale + 9 if scale < 0 else scale - 100)
     check(sampler, cache, q, table, start, lens)
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("up,of_scale", [(114, False), (117, False), (120, True), (124, False), (-85, False)])
+def test_the_largest_and_smallest_queries(sampler, new, page, up, of_scale):  # noqa: F811
+    """Rows up to the type's largest numbers, with keys or a scale of scores that make scores of their products."""
+    rng = np.random.default_rng(up + 200)
+    cache, q, table, start, lens = make(rng, [150, 61], [new, new], 2, 8, 128, page, "bf16")
+    q.clamp_(-7.0, 7.0)  # 7 * 2^124 is a number
+    q[1:, ::3] *= 2.0 ** -20
+    q *= 2.0 ** up
+    if not of_scale:
+        cache.k_scale *= 2.0 ** (-up if up < 116 else -116)
+    check_at(sampler, cache, q, table, start, lens, scale=2.0 ** (-up) / math.sqrt(128) if of_scale else 2.0 ** min(0, 116 - up) / math.sqrt(128))
