@@ -446,7 +446,7 @@ typedef struct mk_kv_queries {
     uint64_t table_ld;
     uint32_t table_cols;
     const int32_t* query_start; /* device [n_seq + 1] */
-    const int32_t* kv_len;      /* device [n_seq]; at most table_cols pages of it are read */
+    const int32_t* kv_len;      /* device [n_seq]; of tokens beyond table_cols pages there are no keys */
     uint32_t n_seq;             /* at most 8192 */
     uint32_t max_new;           /* the most tokens that a sequence has in the pass, or 0: not known. Chooses kernels, nothing else */
     float scale;                /* of a score */

@@ -131,7 +131,7 @@ __device__ void load_queries(const KvAttendArgs& a, Shared<D>& s, const KvSegmen
         if (chunk == 0) {
             const int64_t at = (int64_t)u.seq.len - u.seq.n + token; // its position
             s.factor[r] = a.scale_log2 / by;
-            s.hi[r] = real && at >= 0 ? (int32_t)(at + 1 < u.seq.len ? at + 1 : u.seq.len) : 0;
+            s.hi[r] = real && at >= 0 ? (int32_t)(at + 1 < u.seq.keys ? at + 1 : u.seq.keys) : 0;
             s.lo[r] = a.window && at + 1 > (int64_t)a.window ? (int32_t)(at + 1 - a.window) : 0;
         }
     }
@@ -145,14 +145,14 @@ struct Copier {
     unsigned char* ring;
     uint32_t* valid;              // a bit for each token of a stage's block: it is there
     const int32_t* table;
-    uint32_t len, head;
+    uint32_t keys, head;
     bool wide;                    // is a page a multiple of 16 tokens?
 
     // The page of this lane's token of a block, early: what it is good for is issued when it is there.
     __device__ __forceinline__ int32_t look_up(uint32_t block) const
     {
         const uint32_t t = block * tokens + (threadIdx.x & 31u);
-        return t < len ? __ldg(table + kv_page_of(*a, t)) : -1;
+        return t < keys ? __ldg(table + kv_page_of(*a, t)) : -1;
     }
     __device__ __forceinline__ void issue(uint32_t block, uint32_t stage, int32_t page) const
     {
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv_rows_kernel(const KvAttendArgs
     for (bool first = true; kv_take(a, walk, u, first, tile, each); first = false) {
         const uint32_t from = u.from, to = u.to;
         copier.table = a.block_table + (uint64_t)u.sq * a.table_ld;
-        copier.len = u.seq.len;
+        copier.keys = u.seq.keys;
         copier.head = u.head;
         uint32_t next = from + warp;
         int32_t pages[kStages];

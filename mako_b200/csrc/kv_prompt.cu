@@ -161,7 +161,7 @@ struct Converter {
     __device__ __forceinline__ uint32_t look_up(const KvAttendArgs& a, const Segment& g, const int32_t* table, uint32_t block)
     {
         const uint32_t t = block * kBlock + (threadIdx.x - kConvert);
-        return block < g.to && t < g.seq.len ? (uint32_t)__ldg(table + kv_page_of(a, t)) : ~0u;
+        return block < g.to && t < g.seq.keys ? (uint32_t)__ldg(table + kv_page_of(a, t)) : ~0u;
     }
     struct Place {
         uint64_t off;
@@ -247,7 +247,7 @@ struct Converter {
             page = look_up(a, g, table, b + 2u);
             s.off[stage ^ 1u][tid] = next.off;
             // what the softmax wants to know of the block
-            const uint32_t missing = __ballot_sync(~0u, p.off == ~0ull && b * kBlock + tid < g.seq.len);
+            const uint32_t missing = __ballot_sync(~0u, p.off == ~0ull && b * kBlock + tid < g.seq.keys);
             alive = alive && await(s, &s.k_empty[stage], parity ^ 1u);
             __syncwarp(); // (barriers want whole warps)
             s.key[slot][tid] = p.key;
@@ -433,7 +433,7 @@ struct Softmax {
             mbar_arrive(&s.q_full);
         }
         const int32_t at = (int32_t)g.seq.len - (int32_t)g.seq.n + (int32_t)token + 1; // behind its position
-        const int32_t hi = real && at > 0 ? at : 0, lo = a.window && at > (int32_t)a.window ? at - (int32_t)a.window : 0;
+        const int32_t hi = real && at > 0 ? min(at, (int32_t)g.seq.keys) : 0, lo = a.window && at > (int32_t)a.window ? at - (int32_t)a.window : 0;
         const uint32_t first = blocks;
         blocks += n;
         __syncwarp();
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const KvAttendAr
         for (bool first = true; kv_take(a, walk, g, first, kUnitRows, kBlock); first = false) {
             const int32_t back = (int32_t)g.seq.len - (int32_t)g.seq.n;
             const int32_t top = back + (int32_t)kv_token_of(a, g.row0) + 1, last = back + (int32_t)kv_token_of(a, g.row0 + g.rows - 1u) + 1;
-            g.see_to = top < 0 ? 0u : (uint32_t)top;
+            g.see_to = top < 0 ? 0u : min((uint32_t)top, g.seq.keys);
             g.see_from = a.window && last > (int32_t)a.window ? (uint32_t)last - a.window : 0u;
             role(g, g.whole() ? nullptr : a.parts + (uint64_t)g.place(blockIdx.x) * (kUnitRows * (D + 2u)));
         }

@@ -17,7 +17,8 @@ __device__ __forceinline__ uint32_t kv_token_of(const KvAttendArgs& a, uint32_t 
 
 struct KvSeq {
     uint32_t first, n; // rows of the pass that are this sequence's tokens
-    uint32_t len;      // keys
+    uint32_t len;      // tokens, the last n of which are the rows'
+    uint32_t keys;     // of them that the block table has columns for
 };
 
 __device__ __forceinline__ KvSeq kv_seq(const KvAttendArgs& a, uint32_t s)
@@ -26,8 +27,8 @@ __device__ __forceinline__ KvSeq kv_seq(const KvAttendArgs& a, uint32_t s)
     int64_t from = __ldg(a.query_start + s), to = __ldg(a.query_start + s + 1), len = __ldg(a.kv_len + s);
     from = from < 0 ? 0 : from > most ? most : from;
     to = to < from ? from : to > most ? most : to;
-    len = len < 0 ? 0 : len > held ? held : len;
-    return KvSeq{(uint32_t)from, (uint32_t)(to - from), (uint32_t)len};
+    len = len < 0 ? 0 : len;
+    return KvSeq{(uint32_t)from, (uint32_t)(to - from), (uint32_t)len, (uint32_t)(len > held ? held : len)};
 }
 
 // The blocks of `each` keys that a tile of rows has to look at: [from, to), at least one, so that a tile that sees nothing is a unit too.
@@ -38,7 +39,7 @@ struct KvBlocks {
 __device__ __forceinline__ KvBlocks kv_blocks(const KvAttendArgs& a, const KvSeq& q, uint32_t row0, uint32_t rows, uint32_t each)
 {
     const int32_t back = (int32_t)q.len - (int32_t)q.n;                     // the position of the pass's first token
-    const int32_t end = back + (int32_t)(kv_token_of(a, row0 + rows - 1u)) + 1; // (at most len)
+    const int32_t end = min(back + (int32_t)(kv_token_of(a, row0 + rows - 1u)) + 1, (int32_t)q.keys);
     const int32_t first = back + (int32_t)kv_token_of(a, row0) + 1;
     const uint32_t lo = a.window && first > (int32_t)a.window ? (uint32_t)first - a.window : 0u;
     const uint32_t from = lo / each, to = end < 0 ? 0u : ((uint32_t)end + each - 1u) / each;
@@ -74,7 +75,7 @@ __device__ __forceinline__ uint64_t kv_seq_blocks(const KvAttendArgs& a, const K
     while (many) {
         const int i = __ffs(many) - 1;
         many &= many - 1u;
-        const KvSeq other{0u, __shfl_sync(~0u, q.n, i), __shfl_sync(~0u, q.len, i)};
+        const KvSeq other{0u, __shfl_sync(~0u, q.n, i), __shfl_sync(~0u, q.len, i), __shfl_sync(~0u, q.keys, i)};
         const uint32_t its = __shfl_sync(~0u, rows, i);
         uint64_t x = 0;
         for (uint32_t r = lane * tile; r < its; r += 32u * tile)
@@ -124,7 +125,7 @@ __device__ KvWalk kv_find(const KvAttendArgs& a, uint32_t tile, uint32_t each, u
     const uint32_t tid = threadIdx.x, lane = tid & 31u, mine = (a.n_seq + Threads - 1) / Threads;
     auto of = [&](uint32_t k) -> uint64_t { // blocks of this thread's sequence k, all heads
         const uint32_t s = tid * mine + k;
-        const KvSeq q = s < a.n_seq ? kv_seq(a, s) : KvSeq{0, 0, 0};
+        const KvSeq q = s < a.n_seq ? kv_seq(a, s) : KvSeq{0, 0, 0, 0};
         return kv_seq_blocks(a, q, s < a.n_seq ? kv_rows(a, q) : 0u, tile, each) * a.c.n_heads;
     };
     uint64_t sum = 0;
