@@ -428,9 +428,9 @@ typedef struct mk_rotary {
  * side, at rising places without a gap, and a page has one such run a call (a plan's rows do). A run that begins at place 0 takes
  * the page over: its scales become those of the run. One that begins behind leaves what stands before it: a scale becomes the larger of
  * the page's and the run's, and where it has grown the older codes are brought to it. The scale of numbers up to m is the least power of
- * two s with m <= 448 s, at least 2^-100; codes are rounded to nearest even; what is no finite number becomes NaN and has no part in
- * m. Angles are formed in 64 bits; rotated numbers are rounded once, to 8 bits or, in q_out, to the type. Rows of padding are left as they
- * are, in q_out as well. Uses nothing of the handle but its device. */
+ * two s with m <= 448 s, at least 2^-100; codes are rounded to nearest even (of a quotient in fp32, where a page's own larger scale is no
+ * power of two); what is no finite number becomes NaN and has no part in m. Angles are formed in 64 bits; rotated numbers are rounded once,
+ * to 8 bits or, in q_out, to the type. Rows of padding are left as they are, in q_out as well. Uses nothing of the handle but its device. */
 int mk_kv_append(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_rows* rows, const mk_rotary* rotary, void* stream);
 
 /* A pass's queries over a paged cache. Sequence i's are rows query_start[i] to query_start[i + 1] of q, the last ones of its kv_len[i]

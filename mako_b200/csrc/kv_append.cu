@@ -4,7 +4,7 @@
 // the heads: the rows' angles once, then for every head the largest key and value, the page's new scales, the codes. A scale is a
 // power of two, so that a page whose scale grows (a later token is larger than all before) has its older codes multiplied by a power of
 // two, which changes nothing but what becomes subnormal: a token's code does not depend on how often the scale has grown since, and
-// dividing by a scale is exact.
+// dividing by a scale is exact. (A page's scale that somebody else has put there may be another number: quotients are rounded to fp32 then.)
 //
 // Angles are formed and brought into [-pi, pi] in 64 bits (position x frequency in 32 bits is off by 0.06 rad at a million), their sine and
 // cosine in 32, with what an angle loses by its own rounding added.
@@ -203,7 +203,16 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
                         for (uint32_t k = 0; k < 2u * kHeadsEach; ++k)
                             largest[k] = which == k ? max(largest[k], m) : largest[k];
                     } else {
-                        const float by = 1.0f / s_scale[which]; // a power of two
+                        const float scale = s_scale[which];
+                        float by = 1.0f / scale;
+                        if (__float_as_uint(scale) & 0x7fffffu) { // a page's own, no power of two (the inverse is rounded): quotients
+                            by = 1.0f;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                x[i] = __fdiv_rn(x[i], scale);
+                                y[i] = __fdiv_rn(y[i], scale);
+                            }
+                        }
                         uint8_t* to = static_cast<uint8_t*>(value ? a.c.v : a.c.k) + page * a.c.page_stride + (uint64_t)(h0 + head) * a.c.head_stride +
                                       (uint64_t)(place + i0 + t) * a.c.token_stride;
                         *reinterpret_cast<uint2*>(to + at.a) = make_uint2(codes4(x, 0, by), codes4(x, 4, by));
