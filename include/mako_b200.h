@@ -407,7 +407,7 @@ typedef struct mk_kv_rows {
     const void* q;            /* device [n_tokens][q_ld], or NULL */
     void* q_out;              /* device [n_tokens][q_out_ld]; may be q */
     uint64_t q_ld, q_out_ld;
-    uint32_t n_q_heads;       /* a multiple of the cache's heads */
+    uint32_t n_q_heads;       /* a multiple of the cache's heads, at most 8192 times */
     int type;                 /* MK_BF16 or MK_FP16 */
     uint32_t n_tokens;
     const int32_t* positions; /* device [n_tokens]; unread without a rotation */

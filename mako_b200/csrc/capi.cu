@@ -846,6 +846,8 @@ int mk_kv_append(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_rows* r, c
     if (r->q && (!r->q_out || r->n_q_heads == 0 || r->n_q_heads % cache->n_heads || r->q_ld < qs || r->q_out_ld < qs || ((r->q_ld | r->q_out_ld) & 7u)))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: n_q_heads %u (a multiple of %u), q_ld %llu and q_out_ld %llu (multiples of 8), q_out", r->n_q_heads,
                     cache->n_heads, (unsigned long long)r->q_ld, (unsigned long long)r->q_out_ld);
+    if (r->q && r->n_q_heads / cache->n_heads > mk::kAppendMaxGroup)
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: n_q_heads %u: at most %u of a key head", r->n_q_heads, mk::kAppendMaxGroup);
     if (off16(r->k) || off16(r->v) || off16(r->q) || (r->q && off16(r->q_out)))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: q, k, v and q_out start on 16-byte boundaries");
     if (r->n_tokens == 0)

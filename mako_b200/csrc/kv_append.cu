@@ -25,6 +25,7 @@ namespace {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kHeadsEach = 2;    // key heads of a CTA, which share the angles
 constexpr uint32_t kTokens = 65536;   // of a run without a rotation at a time, so that its rows' count stays within 31 bits
+static_assert((uint64_t)kTokens * kHeadsEach * (2u + kAppendMaxGroup) + kThreads < (1ull << 31), "rows are counted in 31 bits");
 constexpr uint32_t kAngles = 4096;    // (cosine, sine) pairs kept for a run's tokens: 32 KB
 
 template <typename T>

@@ -84,6 +84,7 @@ struct LogprobOut {
 };
 cudaError_t launch_token_logprobs(const mk_logprob_rows& r, const LogprobOut& o, cudaStream_t stream);
 
+constexpr uint32_t kAppendMaxGroup = 8192; // query heads of a key head: 65536 tokens' rows of two key heads are counted in 31 bits
 struct KvAppendArgs {
     mk_kv_cache c;
     const void *q, *k, *v;
