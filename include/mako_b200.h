@@ -405,7 +405,7 @@ typedef struct mk_kv_rows {
     const void *k, *v;        /* device [n_tokens][ld] */
     uint64_t k_ld, v_ld;
     const void* q;            /* device [n_tokens][q_ld], or NULL */
-    void* q_out;              /* device [n_tokens][q_out_ld]; may be q */
+    void* q_out;              /* device [n_tokens][q_out_ld]; may be q, else apart from q; apart from k and v */
     uint64_t q_ld, q_out_ld;
     uint32_t n_q_heads;       /* a multiple of the cache's heads, at most 8192 times */
     int type;                 /* MK_BF16 or MK_FP16 */
@@ -437,7 +437,7 @@ int mk_kv_append(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_rows* rows
  * tokens, whose pages are in row i of the block table: what mk_kv_plan_step gives, once mk_kv_append has run. */
 typedef struct mk_kv_queries {
     const void* q;              /* device [n_tokens][q_ld], heads side by side */
-    void* out;                  /* device [n_tokens][out_ld]; not q */
+    void* out;                  /* device [n_tokens][out_ld]; apart from q */
     uint64_t q_ld, out_ld;      /* elements, multiples of 8; q and out start on 16-byte boundaries */
     uint32_t n_q_heads;         /* a multiple of the cache's heads; query head i reads key head i / (n_q_heads / n_heads) */
     int type;                   /* MK_BF16 or MK_FP16 */

@@ -809,6 +809,24 @@ namespace {
 
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
+// n rows of 16-bit numbers, ld apart, the first `width` of each.
+struct Rows16 {
+    const void* at;
+    uint64_t ld, width;
+};
+
+// Have two sets of n rows a number in common? Of rows that are as far apart in both, exactly; of others, where their extents meet.
+bool meet(const Rows16& a, const Rows16& b, uint64_t n)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    if (x + 2 * ((n - 1) * a.ld + a.width) <= y || y + 2 * ((n - 1) * b.ld + b.width) <= x)
+        return false;
+    if (a.ld != b.ld)
+        return true;
+    const uint64_t step = 2 * a.ld, off = y >= x ? (y - x) % step : (step - (x - y) % step) % step; // from a row of a to one of b behind it
+    return off < 2 * a.width || step - off < 2 * b.width;
+}
+
 int check_cache(const mk_kv_cache& c, const char* who)
 {
     if (c.page_size == 0 || c.page_size > (1u << 24) || c.n_pages > 0x7fffffffu || c.n_heads == 0 || c.n_heads > 65535u || c.dim == 0 ||
@@ -854,6 +872,13 @@ int mk_kv_append(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_rows* r, c
         return MK_OK;
     if (!r->k || !r->v || !r->slots || (turns && !r->positions))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: k, v, slots and, for a rotation, positions are required");
+    if (r->q) {
+        const Rows16 out{r->q_out, r->q_out_ld, qs};
+        const bool in_place = r->q == r->q_out && r->q_ld == r->q_out_ld;
+        if ((!in_place && meet(out, Rows16{r->q, r->q_ld, qs}, r->n_tokens)) || meet(out, Rows16{r->k, r->k_ld, kv}, r->n_tokens) ||
+            meet(out, Rows16{r->v, r->v_ld, kv}, r->n_tokens))
+            return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_append: q_out overlaps k, v or, not being it, q");
+    }
     DeviceGuard g(s->device);
     mk::KvAppendArgs a;
     a.c = *cache;
@@ -915,8 +940,8 @@ int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries
     if (!q->workspace || q->workspace_bytes < mk_kv_attention_bytes(cache, q))
         return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: a workspace of %llu bytes is required",
                     (unsigned long long)mk_kv_attention_bytes(cache, q));
-    if (q->out == q->q)
-        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: out is q, which CTAs read until the last one is done");
+    if (meet(Rows16{q->q, q->q_ld, width}, Rows16{q->out, q->out_ld, width}, q->n_tokens))
+        return fail(MK_ERR_INVALID_ARGUMENT, "mk_kv_attention: out is q or overlaps it, which CTAs read until the last one is done");
     DeviceGuard g(s->device);
     mk::KvAttendArgs a;
     std::memset(&a, 0, sizeof a);
