@@ -40,7 +40,7 @@ struct Shared {
     uint32_t tmem;
     int failed;
     alignas(16) float key[kSlots][kBlock], value[kSlots][kBlock], value_log[kSlots][kBlock]; // scales; log2 of values'
-    float2 log_range[kSlots][kBlock / 16]; // of 16 of them: the largest and the smallest
+    float2 log_range[kSlots][kBlock / 32]; // of 32 of them: the largest and the smallest
     alignas(16) uint32_t missing[kSlots][4]; // tokens whose page is not there
     uint32_t n_mixed[kHeld];
     uint32_t mixed[kHeld][kMixed][5];  // a block and which of its values are NaN
@@ -252,15 +252,12 @@ struct Converter {
             __syncwarp(); // (barriers want whole warps)
             s.key[slot][tid] = p.key;
             s.value[slot][tid] = p.value;
-            const float value_log = __log2f(p.value);
-            s.value_log[slot][tid] = value_log;
-            if (a.c.page_size % 16u) { // (else 16 have one)
-                float2 range = p.off != ~0ull ? make_float2(value_log, value_log) : make_float2(-INFINITY, INFINITY);
-#pragma unroll
-                for (uint32_t d = 8; d; d >>= 1)
-                    range = make_float2(fmaxf(range.x, __shfl_xor_sync(~0u, range.x, d)), fminf(range.y, __shfl_xor_sync(~0u, range.y, d)));
-                if (tid % 16u == 0)
-                    s.log_range[slot][tid / 16u] = range;
+            s.value_log[slot][tid] = __log2f(p.value);
+            if (a.c.page_size % 16u) { // (else 16 have one. Scales are not below 0: as bits they are in the order of numbers)
+                const uint32_t most = __reduce_max_sync(~0u, p.off != ~0ull ? __float_as_uint(p.value) : 0u);
+                const uint32_t least = __reduce_min_sync(~0u, p.off != ~0ull ? __float_as_uint(p.value) : 0x7f800000u);
+                if (lane == 0)
+                    s.log_range[slot][tid / 32u] = make_float2(__log2f(__uint_as_float(most)), __log2f(__uint_as_float(least)));
             }
             if (lane == 0)
                 s.missing[slot][tid / 32u] = missing;
@@ -487,17 +484,23 @@ struct Softmax {
                         tops[m] = fmaxf(fmaxf(x[k + m], x[k + m + 4]), fmaxf(x[k + m + 8], x[k + m + 12]));
                     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * factor(32u * i + k);
                     most = fmaxf(most, top);
-                    const float2 range = Group == 1 ? s.log_range[slot][4u * half + 2u * i + k / 16u] : make_float2(value_log[32u * i + k], 0.0f);
-                    if (Group != 1 || range.x - range.y <= kHighSlack) {
-                        peak = fmaxf(peak, top + range.x);
-                    } else { // scales that are far from one another: each by itself
+                    peak = fmaxf(peak, top + (Group == 1 ? s.log_range[slot][2u * half + i].x : value_log[32u * i + k]));
+                }
+            }
+            if constexpr (Group == 1) { // where scales are far from one another and the unit may have to grow: each by itself
+                const float2 first = s.log_range[slot][2u * half], second = s.log_range[slot][2u * half + 1u];
+                const bool far = !(first.x - first.y <= kHighSlack) || !(second.x - second.y <= kHighSlack); // (in all lanes)
+                if (far && __any_sync(~0u, peak > unit + 15.0f || unit == INFINITY)) {
+                    peak = -INFINITY;
+#pragma unroll 1
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        float x[32];
+                        read(x, i);
 #pragma unroll
-                        for (uint32_t m = 0; m < 16; m += 4) {
-                            const float4 c = reinterpret_cast<const float4*>(value_log)[8u * i + (k + m) / 4];
-                            const float2 f2 = make_float2(f, f);
-                            const float2 y = fma2(make_float2(x[k + m], x[k + m + 1]), f2, make_float2(c.x, c.y));
-                            const float2 z = fma2(make_float2(x[k + m + 2], x[k + m + 3]), f2, make_float2(c.z, c.w));
-                            peak = fmaxf(peak, fmaxf(fmaxf(y.x, y.y), fmaxf(z.x, z.y)));
+                        for (uint32_t k = 0; k < 32; k += 2) {
+                            const float2 c = reinterpret_cast<const float2*>(value_log)[16u * i + k / 2];
+                            const float2 y = fma2(make_float2(x[k], x[k + 1]), make_float2(f, f), c);
+                            peak = fmaxf(peak, fmaxf(y.x, y.y));
                         }
                     }
                 }
@@ -529,36 +532,44 @@ struct Softmax {
                 }
             }
             const float from = ref == -INFINITY ? 0.0f : ref;
-            const float2 minus = make_float2(-from, -from);
-            const float each_is = ex2_approx(from - unit); // (0 where there is no weight yet)
+            // Exponents are relative to the unit where that is near the largest p's, so that a weight is p times a scale; else to the largest p, and a
+            // weight is multiplied once more. (Near: no sum of p passes fp32, and p of 2^-100 of the largest are numbers.)
+            const bool near = __all_sync(~0u, (from - unit >= -26.0f && from - unit <= 60.0f) || ref == -INFINITY);
+            const float base = near && ref != -INFINITY ? unit : from;
+            const float2 minus = make_float2(-base, -base);
             float2 sum = make_float2(0.0f, 0.0f), more = sum;
+            auto weigh = [&](auto once_more, float each_is) {
 #pragma unroll
-            for (uint32_t i = 0; i < 2; ++i) {
-                float x[32];
-                read(x, i);
-                uint32_t w[16];
+                for (uint32_t i = 0; i < 2; ++i) {
+                    float x[32];
+                    read(x, i);
+                    uint32_t w[16];
 #pragma unroll
-                for (uint32_t k = 0; k < 32; k += 4) {
-                    const float by_f = factor(32u * i + k / 16u * 16u);
-                    // what makes a weight of p. (Where 16 have one, at most 2^127: above, p is below 2^-112 of the largest, and not to become NaN where it is 0.)
-                    const float4 c = Group == 1 ? reinterpret_cast<const float4*>(value)[8u * i + k / 4] : make_float4(fminf(value[32u * i + k / 16u * 16u] * each_is, 0x1p127f), 0.0f, 0.0f, 0.0f);
-                    const float2 c0 = Group == 1 ? make_float2(c.x, c.y) : make_float2(c.x, c.x), c1 = Group == 1 ? make_float2(c.z, c.w) : c0;
-                    const float2 f2 = make_float2(by_f, by_f);
-                    const float2 d = fma2(make_float2(x[k], x[k + 1]), f2, minus), e = fma2(make_float2(x[k + 2], x[k + 3]), f2, minus);
-                    const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y)), q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                    sum = add2(sum, p);
-                    more = add2(more, q);
-                    float2 y = mul2(p, c0), z = mul2(q, c1);
-                    if constexpr (Group == 1) {
-                        y = mul2(y, make_float2(each_is, each_is));
-                        z = mul2(z, make_float2(each_is, each_is));
+                    for (uint32_t k = 0; k < 32; k += 4) {
+                        const float by_f = factor(32u * i + k / 16u * 16u);
+                        const float4 c = Group == 1 ? reinterpret_cast<const float4*>(value)[8u * i + k / 4] : make_float4(value[32u * i + k / 16u * 16u], 0.0f, 0.0f, 0.0f);
+                        const float2 c0 = Group == 1 ? make_float2(c.x, c.y) : make_float2(c.x, c.x), c1 = Group == 1 ? make_float2(c.z, c.w) : c0;
+                        const float2 f2 = make_float2(by_f, by_f);
+                        const float2 d = fma2(make_float2(x[k], x[k + 1]), f2, minus), e = fma2(make_float2(x[k + 2], x[k + 3]), f2, minus);
+                        const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y)), q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                        sum = add2(sum, p);
+                        more = add2(more, q);
+                        float2 y = mul2(p, c0), z = mul2(q, c1);
+                        if constexpr (decltype(once_more)::value) {
+                            y = mul2(y, make_float2(each_is, each_is));
+                            z = mul2(z, make_float2(each_is, each_is));
+                        }
+                        w[k / 2] = pair_of(y.x, y.y);
+                        w[k / 2 + 1] = pair_of(z.x, z.y);
                     }
-                    w[k / 2] = pair_of(y.x, y.y);
-                    w[k / 2 + 1] = pair_of(z.x, z.y);
+                    tmem_write16(scores + 16u * i, w); // (over scores of this thread's that have been read twice)
                 }
-                tmem_write16(scores + 16u * i, w); // (over scores of this thread's that have been read twice)
-            }
-            l += (sum.x + sum.y) + (more.x + more.y);
+            };
+            if (near)
+                weigh(std::false_type{}, 1.0f);
+            else
+                weigh(std::true_type{}, ex2_approx(from - unit)); // (0 where there is no weight yet)
+            l += ((sum.x + sum.y) + (more.x + more.y)) * ex2_approx(base - from);
             __syncwarp();
             tmem_written();
             tc_fence_before();
