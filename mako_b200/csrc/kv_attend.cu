@@ -1,7 +1,7 @@
 // Attention of few rows over a paged 8-bit cache (mk_kv_attention in include/mako_b200.h): a decode step, a speculative round. Every
 // key and value is read once for 16 rows, tokens of the pass times query heads that share the key head, and from L2 for 16 more. HBM bounds
 // it where contexts are long (64 sequences of up to 16384 keys, 8 key heads of 128, 4 query heads each: 183 us for 987 MB, 5.4 TB/s or 0.82 of the
-// rate of a copy; two of 131072 with groups of 8: 103 us, 0.80), latency where they are short (one sequence of 2048: 14.5 us from a graph, of which the
+// rate of a copy; two of 131072 with groups of 8: 107 us, 0.77), latency where they are short (one sequence of 2048: 14.5 us from a graph, of which the
 // search for a CTA's share is 1.6, the chain from page to product 2, the join 5).
 //
 // A unit has 16 rows: the MMA's M. A warp takes every fourth block of its CTA's keys, 32 keys and values (8 KB at 128 columns), which it
@@ -653,8 +653,8 @@ cudaError_t launch_rows(const KvAttendArgs& a, cudaStream_t stream)
 }
 
 // Sequences of up to so many rows go through kv_rows_kernel, in a pass with longer ones too: it takes the time of as many tiles of 16, a unit of
-// kv_prompt_kernel that of 256 rows. 64 sequences of 8192 keys, 8 key heads of 128, by the one and by the other: 48 rows 491 and 931 us, 64 rows
-// 649 and 922; 96 rows 934 and 777.
+// kv_prompt_kernel that of 256 rows. 64 sequences of 8192 keys, 8 key heads of 128, by the one and by the other: 48 rows 551 and 730 us, 64 rows
+// 762 and 726; 96 rows 1134 and 731.
 constexpr uint32_t kFewRows = 64;
 
 template <typename T, uint32_t D>
@@ -672,7 +672,7 @@ cudaError_t launch(const KvAttendArgs& args, int type, cudaStream_t stream)
     a.parts = args.parts + kv_rows_parts(D) / 4u;
     a.rows_from = kFewRows + 1u;
     a.rows_to = 0xffffffffu;
-    a.unit_cost = 4; // (0: 1418 us where 4 takes 1400 and 8 1405; chunks of 400 beside 21 single tokens, 99, 79, 83)
+    a.unit_cost = 4; // (0: 1303 us where 4 takes 1295 and 8 1297; chunks of 400 beside 21 single tokens, 121, 95, 97)
     a.blocks_least = 1;
     e = launch_kv_prompt(a, type, stream);
     return e != cudaSuccess ? e : launch_join<T, D, kPromptRows, kPromptBlock>(a, kPromptCtas, stream);

@@ -1,8 +1,8 @@
 // Attention of many rows over a paged 8-bit cache (mk_kv_attention in include/mako_b200.h): prompts' chunks. The tensor core's work is 2048 cycles
-// for a block of 128 keys past 256 rows of 128 columns, as much as its exponentials take; a block takes about 5500 (4 chunks of 2048
-// tokens at the end of 8192, 32 query heads on 8: 1400 us, 690 TFLOP/s, 0.41 of the measured rate of a matrix product). What it waits for
-// is the chain of a tile's turn: scores out of tensor memory, their largest, exponentials, weights back (2500 cycles), two products and their
-// signals (2000), with 2800 of conversion beside it; shared memory is a third busy.
+// for a block of 128 keys past 256 rows of 128 columns, as much as its exponentials take; a block takes about 5100 (4 chunks of 2048
+// tokens at the end of 8192, 32 query heads on 8: 1295 us, 743 TFLOP/s, 0.45 of the measured rate of a matrix product). What it waits for
+// is the chain of a tile's turn: scores out of tensor memory, their largest, exponentials, weights back, two products and their signals, with
+// the conversion beside it; shared memory is two fifths busy.
 //
 // A unit has 256 rows, two tiles of the MMA's M, that take turns: while one tile's scores become weights, the tensor core works for the
 // other. One warp issues; eight a tile (two threads a row) turn scores into weights; four turn the cache's codes into fp16, K-major for the
@@ -13,7 +13,8 @@
 // What it came from: a thread a row with its 128 scores in registers 2058 us (registers are shared by 12 warps then), half of them at a time
 // 1650; two threads a row did not help until a scale for each key was no longer read for each (shared memory: 52 % to 35 %; 1580); pages looked
 // up two blocks ahead 1448; a block's codes read a block ahead 1361 (1358 to
-// 1420 from one device to another).
+// 1420 from one device to another); units of the rows' own in place of the converters' common one, which had them wait for one another, 1410 -> 1295.
+// Pages that are no multiple of 16 tokens: 1654 (of 24 tokens; 1580 with the common unit).
 #include "kv_cache.cuh"
 #include "kv_work.cuh"
 #include "tcgen05.cuh"

@@ -13,7 +13,7 @@
 //
 // A CTA per row; where rows are few a cluster of up to 16 of them, whose parts are put into the first one's shared memory. Instructions bound it
 // beside HBM: 2048 rows of 151552 bf16 logits take 134 us (4.6 TB/s, 0.70 of the rate of a copy; 118 if nothing were ever put into a list),
-// a row of 129280 fp32 logits 12.5 from a graph, 137 masked rows of 50257 fp16 27. 16-bit logits are compared two at a time before they become
+// a row of 129280 fp32 logits 10.4 from a graph, 137 masked rows of 50257 fp16 27. 16-bit logits are compared two at a time before they become
 // floats; weights and sums are formed two at a time. (Five CTAs an SM, 48 registers: with four 143 us, with six 137.)
 #include "ptx.cuh"
 #include "round_ops.h"
