@@ -946,6 +946,10 @@ int mk_kv_attention(mk_sampler* s, const mk_kv_cache* cache, const mk_kv_queries
     mk::KvAttendArgs a;
     std::memset(&a, 0, sizeof a);
     a.c = *cache;
+    if (a.c.n_pages == 0) { // its pointers may be null: copies of no bytes start somewhere all the same
+        a.c.k = a.c.v = q->workspace;
+        a.c.k_scale = a.c.v_scale = static_cast<float*>(q->workspace);
+    }
     a.q = q->q;
     a.out = q->out;
     a.q_ld = q->q_ld;

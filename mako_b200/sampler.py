@@ -577,7 +577,7 @@ class BatchSampler:
         """A pass's queries over the cache (mk_kv_attention): q [T, Hq, D] bf16 or fp16, block_table [S, columns], query_start
         [S + 1] and kv_len [S] int32 as kv_plan gives them; max_new: the most tokens that a sequence has in this pass, where the
         caller knows (it chooses kernels, nothing else); scale of a score, 1 / sqrt(D) by default; window: how many keys a token sees,
-        its own among them (0: all). Returns [T, Hq, D] (`out` where given); rows that are no sequence's are left as they are."""
+        its own among them (0: all). Returns [T, Hq, D] (`out` where given, apart from q); rows that are no sequence's are left as they are."""
         (tokens, q_heads, dim), (n_seq, cols) = q.shape, block_table.shape
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

@@ -52,3 +52,17 @@ def test_lengths_beyond_all_pages(sampler):  # noqa: F811
         held = int((table[of] >= 0).sum()) * 16
         want, bound = oracle.attention(q[t:t + 1].double().cpu(), k, v, table[of:of + 1], [0, 1], [held], 16, 1 / math.sqrt(128), 0, q.dtype)
         assert ((out[t] - want[0]).abs() <= bound[0]).all(), t
+
+
+@pytest.mark.parametrize("new", [1, 90])
+def test_a_cache_without_pages(sampler, new):  # noqa: F811
+    """Whatever the table says, no page is there: zeros."""
+    from mako_b200 import KvCache
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for page, dim in ((16, 128), (24, 64)):
+        q = torch.randn(new + 2, 4, dim, device="cuda").half()
+        out = sampler.kv_attention(q, KvCache.empty(0, 2, page, dim), i32(0, 1, 2, 3, -1, 5).view(1, 6), i32(0, new), i32(90), max_new=new, out=torch.full_like(q, 7.0))
+        assert (out[:new] == 0).all() and (out[new:] == 7).all()
+        k = torch.randn(3, 2, dim, device="cuda").half()
+        sampler.kv_append(KvCache.empty(0, 2, page, dim), k, k.clone(), torch.tensor([-1, 0, 5], device="cuda"))
+    torch.cuda.synchronize()
